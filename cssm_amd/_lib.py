@@ -47,8 +47,15 @@ class GdnGateParams(ctypes.Structure):
     ]
 
 
+class TokenRows(ctypes.Structure):
+    """cssm_token_rows (include/cssm_amd.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_longlong), ("row_stride", ctypes.c_longlong)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_F = ctypes.c_float
+_Z = ctypes.c_size_t
 _LL = ctypes.c_longlong
 
 # name -> (restype, argtypes); every symbol declared in include/cssm_amd.h
@@ -158,6 +165,18 @@ SIGNATURES = {
     "cssm_stem_conv_supported": (_I, [_LL, _I, _I, _I, _I]),
     "cssm_stem_conv": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _P, _P, ctypes.c_float, _I, _P, _P]),
     "cssm_layer_norm": (_I, [_P, _I, _LL, _I, ctypes.c_float, _P, _P, _I, _I, _P, _P]),
+    "cssm_token_scan_chunks": (_I, [_I]),
+    "cssm_token_scan_workspace_size": (_Z, [_I, _I, _I, _I]),
+    "cssm_token_scan": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _Z, _P]),
+    "cssm_token_scan_bwd": (_I, [_P, _P, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P,
+                                 _P, _P, _P, _P, _Z, _P]),
+    "cssm_token_scan_step": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "cssm_rms_norm": (_I, [_P, _P, _I, _LL, _I, _P, _F, _P, _P, _P, _P]),
+    "cssm_rms_norm_bwd_workspace_size": (_Z, [_LL, _I]),
+    "cssm_rms_norm_bwd": (_I, [_P, _P, _P, _I, _LL, _I, _P, _F, _P, _P, _P, _Z, _P]),
+    "cssm_quantize_rows": (_I, [_P, _I, _LL, _I, _P, _P, _P]),
+    "cssm_quantize_weight": (_I, [_P, _I, _I, _P, _P, _P]),
+    "cssm_scaled_matmul": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I, _P, _I, _P]),
     "cssm_block_residual": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                                            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                            ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),

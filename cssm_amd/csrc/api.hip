@@ -1192,3 +1192,206 @@ int cssm_proj_in_noalloc(const void* x, int in_dtype, int F, int HW, int K, int 
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- token sequences
+
+namespace {
+
+using cssm::TokenRows;
+using cssm::TokenScan;
+
+TokenRows rows_of(const cssm_token_rows* r) {
+  return r ? TokenRows{r->data, r->batch_stride, r->row_stride} : TokenRows{nullptr, 0, 0};
+}
+bool has(const cssm_token_rows* r) { return r && r->data; }
+
+size_t elem_size(int dtype) { return dtype == CSSM_F32 ? 4 : 2; }
+
+// what the forward and the adjoint check alike; 0 or the failing status
+int token_scan_check(const char* who, int dtype, int B, int T, int C, const float* kappa, const float* bias,
+                     const int* offsets, int nseq) {
+  if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
+  if (B < 0 || T < 0 || C < 0) return fail(CSSM_ERR_SHAPE, "%s: B=%d T=%d C=%d", who, B, T, C);
+  if (offsets && (B != 1 || nseq < 0)) return fail(CSSM_ERR_SHAPE, "%s: packed rows need B = 1 (B=%d nseq=%d)", who, B, nseq);
+  if (!kappa || !bias) return fail(CSSM_ERR_NULL, "%s: kappa and bias must be non-null", who);
+  // workgroups of a launch (at least 16 channels x 128 rows each)
+  if ((long long)B * cssm_token_scan_chunks(T) * ((C + 15) / 16) > 0x7fffffffLL)
+    return fail(CSSM_ERR_UNSUPPORTED, "%s: B=%d T=%d C=%d is too large for one launch", who, B, T, C);
+  return CSSM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cssm_token_scan_chunks(int T) { return cssm::token_scan_chunks(T); }
+
+size_t cssm_token_scan_workspace_size(int B, int T, int C, int backward) {
+  if (B <= 0 || C <= 0 || T < 0) return 0;
+  const size_t n = size_t(cssm::token_scan_chunks(T)), values = size_t(B) * n * size_t(C) * sizeof(float);
+  if (!backward) return n > 1 ? 2 * values : 0;
+  return (n > 1 ? 3 : 0) * values + 2 * values;   // maps and entering gradients, the tiles' sums
+}
+
+int cssm_token_scan(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int dtype, int B,
+                    int T, int C, const float* kappa, const float* bias, const float* h0, const int* offsets, int nseq,
+                    void* y, int zero_tail, float* h_out, float* states, void* kept, void* kept_scales, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  const char* who = "cssm_token_scan";
+  if (const int st = token_scan_check(who, dtype, B, T, C, kappa, bias, offsets, nseq)) return st;
+  if (B == 0 || C == 0 || (offsets && nseq == 0 && T == 0)) return ok();
+  if (T > 0 && (!has(x) || !has(delta) || !y)) return fail(CSSM_ERR_NULL, "%s: x, delta and y must be non-null", who);
+  if (z && !z->data && T > 0) return fail(CSSM_ERR_NULL, "%s: z rows without data", who);
+  if (!kept != !kept_scales) return fail(CSSM_ERR_NULL, "%s: kept and kept_scales go together", who);
+  const int n = cssm::token_scan_chunks(T);
+  if ((n > 1 || kept) && !states) return fail(CSSM_ERR_NULL, "%s: states must be non-null for T=%d", who, T);
+  const size_t need = cssm_token_scan_workspace_size(B, T, C, 0);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned(workspace, 8)) return fail(CSSM_ERR_ALIGN, "%s: workspace must be 8-byte aligned", who);
+  TokenScan a = {};
+  a.x = rows_of(x), a.delta = rows_of(delta), a.z = rows_of(z);
+  a.gated = z != nullptr;
+  a.kappa = kappa, a.bias = bias, a.h0 = h0, a.offsets = offsets, a.nseq = nseq, a.B = B, a.T = T, a.C = C;
+  a.y = y, a.zero_tail = zero_tail, a.h_out = h_out, a.states = states;
+  a.maps = static_cast<float*>(workspace);
+  a.kept = static_cast<uint8_t*>(kept), a.kept_scales = static_cast<uint8_t*>(kept_scales);
+  return hip_status(cssm::launch_token_scan(a, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int cssm_token_scan_bwd(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int gated,
+                        const cssm_token_rows* dy, int dtype, int B, int T, int C, const float* kappa, const float* bias,
+                        const float* h0, const int* offsets, int nseq, const float* states, const void* kept,
+                        const void* kept_scales, const float* dh, void* dx, void* ddelta, void* dz, float* dkappa,
+                        float* dbias, float* dh0, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "cssm_token_scan_bwd";
+  if (const int st = token_scan_check(who, dtype, B, T, C, kappa, bias, offsets, nseq)) return st;
+  if (C == 0) return ok();
+  if (B == 0) return fail(CSSM_ERR_SHAPE, "%s: B must be positive", who);
+  if (!kept != !kept_scales) return fail(CSSM_ERR_NULL, "%s: kept and kept_scales go together", who);
+  if (!dkappa || !dbias || !states) return fail(CSSM_ERR_NULL, "%s: dkappa, dbias and states must be non-null", who);
+  if (T > 0) {
+    if (!has(dy) || !dx || !ddelta || (gated && !dz))
+      return fail(CSSM_ERR_NULL, "%s: dy, dx, ddelta and, with a gate, dz must be non-null", who);
+    if (!kept && (!has(x) || !has(delta) || (gated && !has(z))))
+      return fail(CSSM_ERR_NULL, "%s: x, delta and, with a gate, z must be non-null unless kept", who);
+  }
+  const size_t need = cssm_token_scan_workspace_size(B, T, C, 1);
+  if (!workspace || workspace_bytes < need)
+    return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned(workspace, 8)) return fail(CSSM_ERR_ALIGN, "%s: workspace must be 8-byte aligned", who);
+  TokenScan a = {};
+  if (!kept) a.x = rows_of(x), a.delta = rows_of(delta), a.z = gated ? rows_of(z) : rows_of(nullptr);
+  a.dy = rows_of(dy);
+  a.gated = gated != 0;
+  a.kappa = kappa, a.bias = bias, a.h0 = h0, a.offsets = offsets, a.nseq = nseq, a.B = B, a.T = T, a.C = C;
+  a.states = const_cast<float*>(states);
+  a.kept = static_cast<uint8_t*>(const_cast<void*>(kept));
+  a.kept_scales = static_cast<uint8_t*>(const_cast<void*>(kept_scales));
+  a.dh = dh, a.dx = dx, a.ddelta = ddelta, a.dz = gated ? dz : nullptr;
+  a.dkappa = dkappa, a.dbias = dbias, a.dh0 = dh0;
+  const size_t values = size_t(B) * size_t(cssm::token_scan_chunks(T)) * size_t(C);
+  a.parts = static_cast<float*>(workspace);
+  a.maps = a.parts + 2 * values;
+  a.enter = a.maps + 2 * values;
+  return hip_status(cssm::launch_token_scan_bwd(a, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int cssm_token_scan_step(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int dtype, int B,
+                         int C, const float* kappa, const float* bias, const float* state, void* y, float* state_out,
+                         void* stream) {
+  const char* who = "cssm_token_scan_step";
+  if (const int st = token_scan_check(who, dtype, B, 1, C, kappa, bias, nullptr, 0)) return st;
+  if (B == 0 || C == 0) return ok();
+  if (!has(x) || !has(delta) || (z && !z->data) || !state || !y || !state_out)
+    return fail(CSSM_ERR_NULL, "%s: x, delta, state, y and state_out must be non-null", who);
+  TokenScan a = {};
+  a.x = rows_of(x), a.delta = rows_of(delta), a.z = rows_of(z);
+  a.gated = z != nullptr;
+  a.kappa = kappa, a.bias = bias, a.h0 = state, a.B = B, a.T = 1, a.C = C, a.y = y, a.h_out = state_out;
+  return hip_status(cssm::launch_token_scan_step(a, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+// ---------------------------------------------------------------- norm of rows, 8-bit operands and their product
+
+int cssm_rms_norm(const void* x, const void* residual, int dtype, long long M, int C, const float* weight, float eps,
+                  void* s_out, void* y, void* scales, void* stream) {
+  const char* who = "cssm_rms_norm";
+  if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
+  if (M < 0 || C < 0 || M > 0x7fffffffLL) return fail(CSSM_ERR_SHAPE, "%s: M=%lld C=%d", who, M, C);
+  if (M == 0 || C == 0) return ok();
+  if (!x || !weight || !y) return fail(CSSM_ERR_NULL, "%s: x, weight and y must be non-null", who);
+  if (!residual != !s_out) return fail(CSSM_ERR_NULL, "%s: residual and s_out go together", who);
+  if (!(eps >= 0.0f)) return fail(CSSM_ERR_ARG, "%s: eps=%g", who, double(eps));
+  if (!aligned(x, elem_size(dtype)) || !aligned(residual, elem_size(dtype)) || !aligned(weight, 4))
+    return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
+  cssm::RmsNorm a = {};
+  a.x = x, a.res = residual, a.M = M, a.C = C, a.w = weight, a.eps = eps, a.s = s_out, a.y = y;
+  a.scales = static_cast<uint8_t*>(scales);
+  return hip_status(cssm::launch_rms_norm(a, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+size_t cssm_rms_norm_bwd_workspace_size(long long M, int C) {
+  return M <= 0 || C <= 0 ? 0 : cssm::rms_norm_bwd_workspace(M, C);
+}
+
+int cssm_rms_norm_bwd(const void* dy, const void* ds, const void* s, int dtype, long long M, int C, const float* weight,
+                      float eps, void* dx, float* dweight, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "cssm_rms_norm_bwd";
+  if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
+  if (M <= 0 || C <= 0 || M > 0x7fffffffLL) return fail(CSSM_ERR_SHAPE, "%s: M=%lld C=%d must be positive", who, M, C);
+  if (!dy || !s || !weight || !dx || !dweight)
+    return fail(CSSM_ERR_NULL, "%s: dy, s, weight, dx and dweight must be non-null", who);
+  if (!(eps >= 0.0f)) return fail(CSSM_ERR_ARG, "%s: eps=%g", who, double(eps));
+  const size_t need = cssm_rms_norm_bwd_workspace_size(M, C);
+  if (!workspace || workspace_bytes < need)
+    return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned(workspace, 4)) return fail(CSSM_ERR_ALIGN, "%s: workspace must be 4-byte aligned", who);
+  cssm::RmsNorm a = {};
+  a.dy = dy, a.ds = ds, a.x = s, a.M = M, a.C = C, a.w = weight, a.eps = eps, a.dx = dx, a.dw = dweight;
+  a.rstds = static_cast<float*>(workspace);
+  a.parts = a.rstds + M;
+  return hip_status(cssm::launch_rms_norm_bwd(a, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+int cssm_quantize_rows(const void* x, int dtype, long long M, int K, void* q, void* scales, void* stream) {
+  const char* who = "cssm_quantize_rows";
+  if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
+  if (M < 0 || K < 0 || M * ((K + 127) / 128) > 0x1ffffffffLL) return fail(CSSM_ERR_SHAPE, "%s: M=%lld K=%d", who, M, K);
+  if (M == 0 || K == 0) return ok();
+  if (!x || !q || !scales) return fail(CSSM_ERR_NULL, "%s: x, q and scales must be non-null", who);
+  return hip_status(cssm::launch_quantize_rows(x, dtype, M, K, static_cast<uint8_t*>(q), static_cast<uint8_t*>(scales),
+                                               static_cast<hipStream_t>(stream)),
+                    who);
+}
+
+int cssm_quantize_weight(const float* kernel, int K, int N, void* q, void* scales, void* stream) {
+  const char* who = "cssm_quantize_weight";
+  if (K <= 0 || N <= 0) return fail(CSSM_ERR_SHAPE, "%s: K=%d N=%d must be positive", who, K, N);
+  if (!kernel || !q || !scales) return fail(CSSM_ERR_NULL, "%s: kernel, q and scales must be non-null", who);
+  return hip_status(cssm::launch_quantize_weight(kernel, K, N, static_cast<uint8_t*>(q), static_cast<uint8_t*>(scales),
+                                                 static_cast<hipStream_t>(stream)),
+                    who);
+}
+
+int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const void* w_scales, int M, int N, int K,
+                       const float* bias, int act, void* out, int out_dtype, void* stream) {
+  const char* who = "cssm_scaled_matmul";
+  if (out_dtype != CSSM_F32 && out_dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: out_dtype=%d", who, out_dtype);
+  if (act < 0 || act > 2) return fail(CSSM_ERR_ARG, "%s: act=%d", who, act);
+  if (M < 0 || N <= 0 || K <= 0) return fail(CSSM_ERR_SHAPE, "%s: M=%d N=%d K=%d", who, M, N, K);
+  if (K % 16) return fail(CSSM_ERR_UNSUPPORTED, "%s: K=%d is not a multiple of 16", who, K);
+  if (M == 0) return ok();
+  if (!a || !a_scales || !w || !w_scales || !out)
+    return fail(CSSM_ERR_NULL, "%s: a, w, their scales and out must be non-null", who);
+  if (!aligned(a, 16) || !aligned(w, 16)) return fail(CSSM_ERR_ALIGN, "%s: a and w must be 16-byte aligned", who);
+  if (!aligned(out, elem_size(out_dtype)) || !aligned(bias, 4))
+    return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
+  cssm::Product8 p = {};
+  p.a = static_cast<const uint8_t*>(a), p.sa = static_cast<const uint8_t*>(a_scales);
+  p.w = static_cast<const uint8_t*>(w), p.sw = static_cast<const uint8_t*>(w_scales);
+  p.M = M, p.N = N, p.K = K, p.bias = bias, p.act = act, p.out = out;
+  return hip_status(cssm::launch_product8(p, out_dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+}  // extern "C"

@@ -299,4 +299,80 @@ hipError_t launch_layer_norm(const void* x, int dtype, long long M, int C, float
 hipError_t launch_block_residual(const void* res, int T_res, const void* y, int T_y, int dtype, int B, int T_out,
                                  int H, int W, int C, int act, void* out, hipStream_t s);
 
+// ---- token sequences (token_scan.hip)
+struct TokenRows {         // rows of a (B, T, C) tensor: element strides of a batch and of a row, channels side by side
+  const void* p;
+  long long batch, row;
+};
+constexpr int kTokenTile = 128;
+struct TokenScan {
+  TokenRows x, delta, z, dy;
+  int gated;               // z is there
+  const float* kappa;
+  const float* bias;
+  const float* h0;         // (n, C) or null: zeros
+  const int* offsets;      // packed rows (B = 1): nseq + 1 starts; null: n = B sequences of T rows
+  int nseq, B, T, C;
+  void* y;                 // (B, T, C)
+  int zero_tail;           // packed: write zeros to the rows of y behind the last sequence
+  float* h_out;            // (n, C) or null
+  float* states;           // (B, chunks, C): the state before every 128th row
+  float* maps;             // (B, chunks, C, 2)
+  uint8_t* kept;           // (3 or 2, B, T, C) e4m3 of x, delta, z; null: not kept (forward) / not read (adjoint)
+  uint8_t* kept_scales;    // (3 or 2, B, ceil(T / 8), ceil(C / 16)) exponents
+  // adjoint
+  const float* dh;         // (n, C) or null: zeros
+  float* enter;            // (B, chunks, C)
+  float* parts;            // (B, chunks, C, 2)
+  void* dx;
+  void* ddelta;
+  void* dz;
+  float* dkappa;
+  float* dbias;
+  float* dh0;              // (n, C) or null
+};
+int token_scan_chunks(int T);
+hipError_t launch_token_scan(const TokenScan& a, int dtype, hipStream_t s);
+hipError_t launch_token_scan_bwd(const TokenScan& a, int dtype, hipStream_t s);
+hipError_t launch_token_scan_step(const TokenScan& a, int dtype, hipStream_t s);
+
+// ---- root-mean-square norm of rows and 8-bit values (row_norm.hip)
+struct RmsNorm {
+  const void* x;           // (M, C); adjoint: the rounded sum the forward normalised
+  const void* res;         // (M, C) or null
+  long long M;
+  int C;
+  const float* w;
+  float eps;
+  void* s;                 // (M, C): the rounded x + res, or null with res null
+  void* y;                 // (M, C) of the inputs' type, or e4m3 with scales
+  uint8_t* scales;         // (M, ceil(C / 128)) exponents, or null
+  // adjoint
+  const void* dy;
+  const void* ds;          // or null
+  void* dx;
+  float* dw;
+  float* parts;            // workspace: (workgroups, C), then the rows' rstd
+  float* rstds;
+};
+size_t rms_norm_bwd_workspace(long long M, int C);
+hipError_t launch_rms_norm(const RmsNorm& a, int dtype, hipStream_t s);
+hipError_t launch_rms_norm_bwd(const RmsNorm& a, int dtype, hipStream_t s);
+hipError_t launch_quantize_rows(const void* x, int dtype, long long M, int K, uint8_t* q, uint8_t* scales,
+                                hipStream_t s);
+hipError_t launch_quantize_weight(const float* w, int K, int N, uint8_t* q, uint8_t* scales, hipStream_t s);
+
+// ---- product of 8-bit matrices (product8.hip)
+struct Product8 {
+  const uint8_t* a;        // (M, K) e4m3, exponents sa (M, ceil(K / 128))
+  const uint8_t* sa;
+  const uint8_t* w;        // (N, K) e4m3, exponents sw (ceil(N / 128), ceil(K / 128))
+  const uint8_t* sw;
+  int M, N, K;
+  const float* bias;       // (N) or null
+  int act;                 // 0 none, 1 gelu (tanh form), 2 silu
+  void* out;               // (M, N)
+};
+hipError_t launch_product8(const Product8& p, int out_dtype, hipStream_t s);
+
 }  // namespace cssm

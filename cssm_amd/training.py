@@ -15,7 +15,9 @@ GOOM floor terms folded in).
 
 ``gated_train_apply(cell, params, x)`` returns the layer output with the
 autograd graph attached; ``params`` is the cell's parameter tree of leaf
-tensors (``requires_grad`` where gradients are wanted).
+tensors (``requires_grad`` where gradients are wanted).  ``token_scan_train`` and
+``rms_norm_train`` are the differentiable forms of the operators over token sequences
+(:mod:`cssm_amd.sequence`).
 """
 from __future__ import annotations
 
@@ -24,6 +26,7 @@ from typing import Any, Dict
 import torch
 import torch.nn.functional as Fn
 
+from . import sequence as Q
 from . import spectral as S
 
 
@@ -825,3 +828,88 @@ def gdn_train_apply(cell, params: Dict[str, Any], x: torch.Tensor) -> torch.Tens
              + p["output_layernorm"]["bias"][None, :, None])
     out = _ProjOutFn.apply((o * gv).contiguous(), p["output_proj"]["kernel"], p["output_proj"]["bias"])
     return out.view(B, T, H, W, C)
+
+
+# ------------------------------------------------------------------ token sequences
+
+def _side_by_side(t: torch.Tensor) -> torch.Tensor:
+    """t with its last axis contiguous, as the row kernels read it (any other strides)."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+class _TokenScanFn(torch.autograd.Function):
+    """(y, final state) of the gated recurrence, its adjoint on cssm_token_scan_bwd.  Kept between the two passes: the
+    inputs themselves, or with ``e4m3`` their 8-bit checkpoint, and the float32 state before every 128th row."""
+
+    @staticmethod
+    def forward(ctx, x, delta, z, kappa, bias, state, offsets, e4m3):
+        y, final, states, kept, scales = Q.scan_forward(x, delta, kappa, bias, z, state, offsets, keep_states=True,
+                                                        keep_e4m3=e4m3)
+        ctx.gated = z is not None
+        if e4m3:
+            x = delta = z = None
+        ctx.save_for_backward(x, delta, z, kappa, bias, state, offsets, states, kept, scales)
+        ctx.like = (y.shape, y.dtype, y.device)
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dfinal):
+        x, delta, z, kappa, bias, state, offsets, states, kept, scales = ctx.saved_tensors
+        if dy is None:
+            shape, dtype, device = ctx.like
+            dy = torch.zeros(shape, dtype=dtype, device=device)
+        if dfinal is not None:
+            dfinal = dfinal.contiguous()
+        dx, dd, dz, dk, db, dh0 = Q.scan_backward(x, delta, kappa, bias, z, state, offsets, states, kept, scales,
+                                                  _side_by_side(dy), dfinal, ctx.gated)
+        return dx, dd, dz, dk, db, dh0 if state is not None else None, None, None
+
+
+def token_scan_train(x: torch.Tensor, delta: torch.Tensor, kappa: torch.Tensor, bias: torch.Tensor, z=None, state=None,
+                     offsets=None, checkpoint: str = "none"):
+    """:func:`cssm_amd.sequence.token_scan`, differentiable in x, delta, z, kappa, bias and state: (y, final state).
+
+    ``checkpoint='e4m3'`` keeps x, delta and z in 8 bits for the backward pass (a power of two for each 8 rows x 16
+    channels), one byte a value in place of two or four.  The outputs are those without it; the gradients are the
+    recurrence's at the kept values, the states of each 128 rows computed again from the float32 state before them."""
+    if checkpoint not in ("none", "e4m3"):
+        raise ValueError(f"checkpoint={checkpoint!r}: 'none' or 'e4m3'")
+    return _TokenScanFn.apply(_side_by_side(x), _side_by_side(delta), None if z is None else _side_by_side(z),
+                              kappa.contiguous(), bias.contiguous(), None if state is None else state.contiguous(),
+                              offsets, checkpoint == "e4m3")
+
+
+class _RmsNormFn(torch.autograd.Function):
+    """(y, s) of the norm behind the residual's addition, its adjoint on cssm_rms_norm_bwd."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        y, s = Q.rms_norm(x, weight, residual, eps)
+        if residual is None:
+            ctx.save_for_backward(x, weight)
+            out = (y,)
+        else:
+            ctx.save_for_backward(s, weight)
+            out = (y, s)
+        ctx.eps, ctx.added = eps, residual is not None
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, weight = ctx.saved_tensors
+        dy = torch.zeros_like(s) if dy is None else dy.contiguous()
+        dx, dw = Q.rms_norm_backward(dy, None if ds is None else ds.contiguous(), s, weight, ctx.eps)
+        return dx, dx if ctx.added else None, dw, None
+
+
+def rms_norm_train(x: torch.Tensor, weight: torch.Tensor, residual=None, eps: float = 1e-6):
+    """:func:`cssm_amd.sequence.rms_norm`, differentiable in x, residual and weight: (y, s), s being x without a
+    residual."""
+    x = x.contiguous()
+    if residual is None:
+        return _RmsNormFn.apply(x, None, weight.contiguous(), eps)[0], x
+    return _RmsNormFn.apply(x, residual.contiguous(), weight.contiguous(), eps)

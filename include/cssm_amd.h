@@ -50,6 +50,10 @@ typedef enum cssm_status {
 
 typedef enum cssm_dtype { CSSM_F32 = 0, CSSM_BF16 = 1 } cssm_dtype;
 
+/* 8-bit values are e4m3 (3 mantissa bits, largest 448, no infinities) and stand for q * 2^(byte - 127) with one exponent
+ * byte for each block of values; the byte is the least with the block's largest finite magnitude <= 448 * 2^(byte - 127)
+ * (1..247; 127 for a block of zeros).  A NaN or an infinite value is stored as NaN. */
+
 /* gate_type of GatedCSSM (cssm.py:430, :538-545) */
 typedef enum cssm_gate_type { CSSM_GATE_DENSE = 0, CSSM_GATE_FACTORED = 1 } cssm_gate_type;
 
@@ -883,6 +887,109 @@ int cssm_stem_conv(const float* x, int N, int H, int W, int Ci, int Co, const fl
  */
 int cssm_block_residual(const void* res, int T_res, const void* y, int T_y, int dtype, int B, int T_out, int H,
                         int W, int C, int act, void* out, void* stream);
+
+/* ---- token sequences: operators over (B, T, C) activations with long T.  No counterpart in the reference's default
+ * path: the gated cell's recurrence (cssm.py:559-581) in real arithmetic per channel, without the transforms. */
+
+/* A (B, T, C) tensor whose channels lie side by side: element strides of a batch and of a row. */
+typedef struct cssm_token_rows {
+  const void* data;
+  long long batch_stride, row_stride;
+} cssm_token_rows;
+
+/* Rows between the states that cssm_token_scan keeps. */
+#define CSSM_TOKEN_SEGMENT 128
+
+/*
+ * Gated recurrence over token sequences, for each channel c:
+ *   u_t = delta_t + bias, D_t = softplus(u_t), h_t = kappa exp(-D_t) h_{t-1} + D_t x_t, y_t = h_t SiLU(z_t)
+ *   x, delta, z  (B, T, C) of dtype; z NULL: y_t = h_t.  delta = -inf with a finite x scales the state by kappa alone
+ *   kappa, bias  (C) float32
+ *   h0           (n, C) float32 state before each sequence's first row, or NULL (zeros)
+ *   offsets      NULL: n = B sequences of T rows.  Else B = 1 and the rows are n = nseq sequences one behind the
+ *                other: (nseq + 1) int32 on the device, ascending from 0, offsets[nseq] <= T; sequence i is rows
+ *                offsets[i] .. offsets[i + 1] - 1 and may be empty.  Offsets outside that never leave the
+ *                tensors, but which rows then belong together is not defined.
+ *   y            (B, T, C) of dtype, contiguous; rows behind the last sequence are left as they are, or with
+ *                zero_tail != 0 set to zero
+ *   h_out        (n, C) float32 state behind each sequence's last row (h0 for an empty one), or NULL
+ *   states       (B, chunks, C) float32 out, chunks = cssm_token_scan_chunks(T): the state before every 128th row;
+ *                may be NULL where chunks = 1
+ *   kept, kept_scales  NULL, or x, delta and z (if given) in 8 bits for the adjoint: (2 or 3, B, T, C) e4m3 and
+ *                (2 or 3, B, ceil(T / 8), ceil(C / 16)) exponents, a block being 8 rows x 16 channels
+ *   workspace    cssm_token_scan_workspace_size(B, T, C, 0) bytes, 8-byte aligned
+ * The outputs do not overlap the inputs.  The results do not depend on how the work is spread: the same call gives
+ * the same bits.
+ */
+int cssm_token_scan_chunks(int T);
+size_t cssm_token_scan_workspace_size(int B, int T, int C, int backward);
+int cssm_token_scan(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int dtype, int B,
+                    int T, int C, const float* kappa, const float* bias, const float* h0, const int* offsets, int nseq,
+                    void* y, int zero_tail, float* h_out, float* states, void* kept, void* kept_scales, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/*
+ * Adjoint of cssm_token_scan: arguments as its forward call's, with
+ *   x, delta, z  the forward's inputs; with kept != NULL they are not read (may be NULL) and every formula is taken at
+ *                the values kept stands for, each 128 rows from the state the forward kept before them
+ *   gated        whether the forward had a z
+ *   dy           (B, T, C) of dtype; dh (n, C) float32 gradient of h_out, or NULL (zeros)
+ *   dx, ddelta, dz  (B, T, C) of dtype out, contiguous (dz NULL without z); zero behind the last sequence
+ *   dkappa, dbias   (C) float32 out; dh0 (n, C) float32 out, or NULL
+ *   states       as the forward wrote them (required)
+ *   workspace    cssm_token_scan_workspace_size(B, T, C, 1) bytes
+ */
+int cssm_token_scan_bwd(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int gated,
+                        const cssm_token_rows* dy, int dtype, int B, int T, int C, const float* kappa, const float* bias,
+                        const float* h0, const int* offsets, int nseq, const float* states, const void* kept,
+                        const void* kept_scales, const float* dh, void* dx, void* ddelta, void* dz, float* dkappa,
+                        float* dbias, float* dh0, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One token for each of B sequences: cssm_token_scan with T = 1 (the rows' row_stride is not used), state (B, C)
+ * float32 read and state_out (B, C) written, which may be the same buffer.
+ */
+int cssm_token_scan_step(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int dtype, int B,
+                         int C, const float* kappa, const float* bias, const float* state, void* y, float* state_out,
+                         void* stream);
+
+/*
+ * Root-mean-square norm of rows behind the residual's addition:
+ *   s = x + residual rounded to dtype, y = s / sqrt(mean(s^2) + eps) * weight
+ *   x, residual  (M, C) of dtype; residual NULL: s = x
+ *   s_out        (M, C) of dtype out (NULL without a residual)
+ *   y            (M, C) of dtype, or with scales != NULL in 8 bits: e4m3 and (M, ceil(C / 128)) exponents, a block
+ *                being 128 values of a row
+ * Outputs do not overlap inputs.
+ * Adjoint, for an output in dtype: dx = the gradient of x and of the residual, with dy and ds (NULL: zero) those of y and
+ * s_out; s as the forward normalised it; dweight (C) float32; workspace of cssm_rms_norm_bwd_workspace_size(M, C).
+ */
+int cssm_rms_norm(const void* x, const void* residual, int dtype, long long M, int C, const float* weight, float eps,
+                  void* s_out, void* y, void* scales, void* stream);
+size_t cssm_rms_norm_bwd_workspace_size(long long M, int C);
+int cssm_rms_norm_bwd(const void* dy, const void* ds, const void* s, int dtype, long long M, int C, const float* weight,
+                      float eps, void* dx, float* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * 8-bit operands of cssm_scaled_matmul.
+ *   cssm_quantize_rows    x (M, K) of dtype -> q (M, K) e4m3, scales (M, ceil(K / 128)): a block is 128 of a row
+ *   cssm_quantize_weight  Dense kernel (K, N) float32 -> q (N, K) e4m3, scales (ceil(N / 128), ceil(K / 128)): a block
+ *                         is 128 x 128
+ */
+int cssm_quantize_rows(const void* x, int dtype, long long M, int K, void* q, void* scales, void* stream);
+int cssm_quantize_weight(const float* kernel, int K, int N, void* q, void* scales, void* stream);
+
+/*
+ * out = act(A W^T + bias) of 8-bit operands, summed in float32 (with a bfloat16 output by the 8-bit matrix
+ * instruction, which drops what lies about 13 bits below the largest of the products that it adds at once):
+ *   a, a_scales  (M, K) e4m3 and (M, ceil(K / 128)) exponents
+ *   w, w_scales  (N, K) e4m3 and (ceil(N / 128), ceil(K / 128)) exponents
+ *   bias         (N) float32 or NULL; act 0 none, 1 gelu (tanh form), 2 silu
+ *   out          (M, N) of out_dtype
+ * K a multiple of 16 (CSSM_ERR_UNSUPPORTED otherwise), a and w 16-byte aligned.
+ */
+int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const void* w_scales, int M, int N, int K,
+                       const float* bias, int act, void* out, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }
