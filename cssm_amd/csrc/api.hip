@@ -1228,9 +1228,9 @@ int cssm_token_scan_chunks(int T) { return cssm::token_scan_chunks(T); }
 
 size_t cssm_token_scan_workspace_size(int B, int T, int C, int backward) {
   if (B <= 0 || C <= 0 || T < 0) return 0;
-  const size_t n = size_t(cssm::token_scan_chunks(T)), values = size_t(B) * n * size_t(C) * sizeof(float);
-  if (!backward) return n > 1 ? 2 * values : 0;
-  return (n > 1 ? 3 : 0) * values + 2 * values;   // maps and entering gradients, the tiles' sums
+  size_t words = cssm::token_scan_words(B, T, C);
+  if (backward) words += size_t(B) * size_t(cssm::token_scan_chunks(T)) * size_t(C);   // the tiles' two sums
+  return 8 * words;
 }
 
 int cssm_token_scan(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int dtype, int B,
@@ -1243,8 +1243,7 @@ int cssm_token_scan(const cssm_token_rows* x, const cssm_token_rows* delta, cons
   if (T > 0 && (!has(x) || !has(delta) || !y)) return fail(CSSM_ERR_NULL, "%s: x, delta and y must be non-null", who);
   if (z && !z->data && T > 0) return fail(CSSM_ERR_NULL, "%s: z rows without data", who);
   if (!kept != !kept_scales) return fail(CSSM_ERR_NULL, "%s: kept and kept_scales go together", who);
-  const int n = cssm::token_scan_chunks(T);
-  if ((n > 1 || kept) && !states) return fail(CSSM_ERR_NULL, "%s: states must be non-null for T=%d", who, T);
+  if (kept && !states) return fail(CSSM_ERR_NULL, "%s: kept needs states", who);
   const size_t need = cssm_token_scan_workspace_size(B, T, C, 0);
   if (need && (!workspace || workspace_bytes < need))
     return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
@@ -1254,9 +1253,9 @@ int cssm_token_scan(const cssm_token_rows* x, const cssm_token_rows* delta, cons
   a.gated = z != nullptr;
   a.kappa = kappa, a.bias = bias, a.h0 = h0, a.offsets = offsets, a.nseq = nseq, a.B = B, a.T = T, a.C = C;
   a.y = y, a.zero_tail = zero_tail, a.h_out = h_out, a.states = states;
-  a.maps = static_cast<float*>(workspace);
   a.kept = static_cast<uint8_t*>(kept), a.kept_scales = static_cast<uint8_t*>(kept_scales);
-  return hip_status(cssm::launch_token_scan(a, dtype, static_cast<hipStream_t>(stream)), who);
+  return hip_status(cssm::launch_token_scan(a, dtype, static_cast<uint64_t*>(workspace), static_cast<hipStream_t>(stream)),
+                    who);
 }
 
 int cssm_token_scan_bwd(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int gated,
@@ -1290,11 +1289,9 @@ int cssm_token_scan_bwd(const cssm_token_rows* x, const cssm_token_rows* delta, 
   a.kept_scales = static_cast<uint8_t*>(const_cast<void*>(kept_scales));
   a.dh = dh, a.dx = dx, a.ddelta = ddelta, a.dz = gated ? dz : nullptr;
   a.dkappa = dkappa, a.dbias = dbias, a.dh0 = dh0;
-  const size_t values = size_t(B) * size_t(cssm::token_scan_chunks(T)) * size_t(C);
   a.parts = static_cast<float*>(workspace);
-  a.maps = a.parts + 2 * values;
-  a.enter = a.maps + 2 * values;
-  return hip_status(cssm::launch_token_scan_bwd(a, dtype, static_cast<hipStream_t>(stream)), who);
+  uint64_t* words = static_cast<uint64_t*>(workspace) + size_t(B) * size_t(cssm::token_scan_chunks(T)) * size_t(C);
+  return hip_status(cssm::launch_token_scan_bwd(a, dtype, words, static_cast<hipStream_t>(stream)), who);
 }
 
 int cssm_token_scan_step(const cssm_token_rows* x, const cssm_token_rows* delta, const cssm_token_rows* z, int dtype, int B,

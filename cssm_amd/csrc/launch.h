@@ -316,13 +316,14 @@ struct TokenScan {
   void* y;                 // (B, T, C)
   int zero_tail;           // packed: write zeros to the rows of y behind the last sequence
   float* h_out;            // (n, C) or null
-  float* states;           // (B, chunks, C): the state before every 128th row
-  float* maps;             // (B, chunks, C, 2)
+  float* states;           // (B, chunks, C): the state before every 128th row, or null
+  unsigned* ticket;        // set by the launchers, in their `words`: the tiles' counter,
+  uint64_t* maps;          // (B, chunks, C) and
+  uint64_t* heads;         // (B, spans of chunks, C)
   uint8_t* kept;           // (3 or 2, B, T, C) e4m3 of x, delta, z; null: not kept (forward) / not read (adjoint)
   uint8_t* kept_scales;    // (3 or 2, B, ceil(T / 8), ceil(C / 16)) exponents
   // adjoint
   const float* dh;         // (n, C) or null: zeros
-  float* enter;            // (B, chunks, C)
   float* parts;            // (B, chunks, C, 2)
   void* dx;
   void* ddelta;
@@ -332,8 +333,9 @@ struct TokenScan {
   float* dh0;              // (n, C) or null
 };
 int token_scan_chunks(int T);
-hipError_t launch_token_scan(const TokenScan& a, int dtype, hipStream_t s);
-hipError_t launch_token_scan_bwd(const TokenScan& a, int dtype, hipStream_t s);
+size_t token_scan_words(int B, int T, int C);   // 64-bit words of scratch that either call clears and uses
+hipError_t launch_token_scan(const TokenScan& a, int dtype, uint64_t* words, hipStream_t s);
+hipError_t launch_token_scan_bwd(const TokenScan& a, int dtype, uint64_t* words, hipStream_t s);
 hipError_t launch_token_scan_step(const TokenScan& a, int dtype, hipStream_t s);
 
 // ---- root-mean-square norm of rows and 8-bit values (row_norm.hip)

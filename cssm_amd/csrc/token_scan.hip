@@ -5,8 +5,9 @@
 //   g_t = p_t + G_{t+1},  dx = D g,  ddelta = sigmoid(u) g (x - a h_{t-1}),  dz = dy h SiLU'(z)
 //   dkappa = sum g sigmoid(-u) h_{t-1},  dbias = sum ddelta
 // Every step is h -> A h + S, and such maps compose: (A1, S1) then (A2, S2) is (A2 A1, A2 S1 + S2).  So time is cut
-// into tiles of 128 rows.  One pass takes each tile's (A, S), a second joins them into the state before every
-// tile, a third recomputes the tile from that state and writes the outputs; the adjoint does the same backwards.
+// into tiles of 128 rows, and one pass over the data does all: a workgroup loads its tile, publishes the tile's map,
+// gathers the state before the tile from the maps of the tiles before it, and only then walks its rows from
+// registers and writes the outputs.  The adjoint does the same from the end, with the states the forward kept.
 // One tile is 128 rows x 16 V channels on 256 threads: 16 lanes side by side over channels, 16 groups of 8
 // consecutive rows, so a thread's rows stay in registers from load to store.
 // All sums and states are float32; y and the gradients are rounded once, to their type.
@@ -69,20 +70,77 @@ __device__ __forceinline__ int packed_limit(const int* off, int nseq, int T) {
 
 struct Where {
   int ct, chunk, b, sub, c, r;   // channel tile, row tile, batch; row group, first channel, first row
+  int place;                     // of the row tile on the way: chunk, or from the end
 };
-template <int V>
+// Tiles are handed out by a counter in the order of their place on the way, so that every tile waits only for tiles
+// whose workgroups run already; with one tile a sequence nothing waits and the block index does.
+template <int V, bool REV>
 __device__ __forceinline__ Where where(const TokenScan& a, int nchunks) {
-  const int nct = (a.C + kLanes * V - 1) / (kLanes * V);
-  const unsigned blk = blockIdx.x;
+  __shared__ unsigned ticket;
+  unsigned blk = blockIdx.x;
+  if (nchunks > 1) {
+    if (threadIdx.x == 0) ticket = atomicAdd(a.ticket, 1u) + 1u;   // starts at all ones
+    __syncthreads();
+    blk = ticket;
+  }
+  const unsigned nct = unsigned(a.C + kLanes * V - 1) / (kLanes * V);
   Where w;
-  w.ct = int(blk % unsigned(nct));
-  const unsigned rest = blk / unsigned(nct);
-  w.chunk = int(rest % unsigned(nchunks));
-  w.b = int(rest / unsigned(nchunks));
+  w.ct = int(blk % nct);
+  w.b = int(blk / nct % unsigned(a.B));
+  w.place = int(blk / nct / unsigned(a.B));
+  w.chunk = REV ? nchunks - 1 - w.place : w.place;
   w.sub = threadIdx.x / kLanes;
   w.c = (w.ct * kLanes + int(threadIdx.x % kLanes)) * V;
   w.r = w.chunk * kTile + w.sub * kRows;
   return w;
+}
+
+// A map (or with A = 0 a state) as one 64-bit word, which other workgroups see whole or not at all: all ones until it is
+// published, so it is its own flag and needs no fence.
+constexpr uint64_t kNotYet = ~uint64_t(0);
+__device__ __forceinline__ void publish(uint64_t* at, Map m) {
+  uint32_t a = __float_as_uint(m.A);
+  if (a == 0xffffffffu) a = 0x7fc00000u;   // a NaN is a NaN
+  __hip_atomic_store(at, uint64_t(a) << 32 | __float_as_uint(m.S), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t peek(const uint64_t* at) {
+  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The word's publisher has a lower ticket, so it runs and waits only for lower ones: the wait ends.  (The count only
+// keeps a defect from hanging the device; it would end in NaN.)
+__device__ __forceinline__ Map await(const uint64_t* at, uint64_t v) {
+  for (int i = 0; v == kNotYet && i < (1 << 22); ++i) {
+    __builtin_amdgcn_s_sleep(1);
+    v = peek(at);
+  }
+  return {__uint_as_float(uint32_t(v >> 32)), __uint_as_float(uint32_t(v))};
+}
+
+// The value entering the tile at this place for one channel, by its own map `own` and those before it.  Places
+// come in spans of kSpan: a tile joins the maps of its span's earlier places (at most kSpan - 1, published without
+// waiting) and applies them to the value entering the span, which the last tile of the span before published.  So
+// the chain of waits has a link for each kSpan tiles, and the sums come in the same order every time.
+constexpr int kSpan = 16;
+__device__ __forceinline__ float entering(const TokenScan& a, const Where& w, int nchunks, int c, Map own, float first) {
+  if (nchunks == 1) return first;
+  const int spans = (nchunks + kSpan - 1) / kSpan, span = w.place / kSpan, p0 = span * kSpan;
+  uint64_t* maps = a.maps + size_t(w.b) * nchunks * a.C + c;
+  uint64_t* heads = a.heads + size_t(w.b) * spans * a.C + c;
+  if (w.place + 1 < nchunks) publish(maps + size_t(w.place) * a.C, own);
+  Map m = {1.0f, 0.0f};
+  uint64_t v[kSpan];   // the last: the span's head
+  const uint64_t* head = heads + size_t(span) * a.C;
+  if (span > 0) v[kSpan - 1] = peek(head);
+#pragma unroll
+  for (int i = 0; i < kSpan - 1; ++i)
+    if (p0 + i < w.place) v[i] = peek(maps + size_t(p0 + i) * a.C);
+#pragma unroll
+  for (int i = 0; i < kSpan - 1; ++i)
+    if (p0 + i < w.place) m = then(m, await(maps + size_t(p0 + i) * a.C, v[i]));
+  if (span > 0) first = await(head, v[kSpan - 1]).S;
+  const float in = apply(m, first);
+  if (w.place % kSpan == kSpan - 1 && w.place + 1 < nchunks) publish(heads + size_t(span + 1) * a.C, {0.0f, apply(own, in)});
+  return in;
 }
 
 template <typename T, int V>
@@ -195,103 +253,13 @@ __device__ __forceinline__ Map fold(Carry<V>& k, int ch, float in) {
   return all;
 }
 
-// ---- first pass: the map of each tile but the last (REV: but the first)
-
-template <typename T, int V, bool PACKED, bool KEPT, bool REV>
-__global__ void __launch_bounds__(256) token_scan_maps(TokenScan a, int nchunks) {
-  __shared__ Carry<V> k;
-  __shared__ Marks marks;
-  Where w = where<V>(a, nchunks - 1);
-  if (REV) w.chunk += 1, w.r += kTile;
-  const int limit = PACKED ? packed_limit(a.offsets, a.nseq, a.T) : a.T;
-  const bool on = w.c < a.C;
-  Source<T, V, KEPT> d, x, z;   // x only forward, z only backward
-  Raw<T, V> dy[kRows];
-  const int lim = on ? limit : 0;
-  d.load(a, a.delta, 1, w, lim);
-  if (!REV) x.load(a, a.x, 0, w, lim);
-  if (REV) {
-    load_rows<T, V>(dy, a.dy, w, lim);
-    if (a.gated) z.load(a, a.z, 2, w, lim);
-  }
-  float kap[V], bia[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) kap[v] = on ? a.kappa[w.c + v] : 0.0f, bia[v] = on ? a.bias[w.c + v] : 0.0f;
-  if (PACKED) find_marks(marks, a.offsets, a.nseq, w.chunk * kTile, limit);
-  Map m[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) m[v] = {1.0f, 0.0f};
-#pragma unroll
-  for (int j = 0; j < kRows; ++j) {
-    const int i = REV ? kRows - 1 - j : j;
-    if (w.r + i >= lim) continue;
-    const int mark = PACKED ? (REV ? marks.end : marks.start)[w.sub * kRows + i] : -1;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Gains g = gains(d.get(i, v) + bia[v]);
-      const float A = kap[v] * g.keep;
-      if (REV) {
-        float p = dy[i].get(v);
-        if (a.gated) {
-          const float zz = z.get(i, v);
-          p *= zz * sigmoidf(zz);
-        }
-        if (mark >= 0) m[v] = {cut(), a.dh ? a.dh[size_t(mark) * a.C + w.c + v] : 0.0f};
-        m[v] = {is_cut(m[v].A) ? cut() : m[v].A * A, A * (p + m[v].S)};
-      } else {
-        if (mark >= 0) m[v] = {cut(), a.h0 ? a.h0[size_t(mark) * a.C + w.c + v] : 0.0f};
-        m[v] = {is_cut(m[v].A) ? cut() : m[v].A * A, fmaf(A, m[v].S, g.D * x.get(i, v))};
-      }
-    }
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) k.m[w.sub][int(threadIdx.x % kLanes) * V + v] = m[v];
-  __syncthreads();
-  const int ch = threadIdx.x, c = w.ct * kLanes * V + ch;
-  if (ch < kLanes * V && c < a.C)
-    reinterpret_cast<Map*>(a.maps)[(size_t(w.b) * nchunks + w.chunk) * a.C + c] = fold<V, REV, false>(k, ch, 0.0f);
-}
-
-// ---- second pass: the value entering every tile.  16 channels x 64 spans of tiles a workgroup.
-
-template <bool REV>
-__global__ void __launch_bounds__(1024) token_scan_join(TokenScan a, int nchunks, float* __restrict__ enter) {
-  __shared__ Map part[64][16];
-  const int nct = (a.C + 15) / 16, ct = int(blockIdx.x) % nct, b = int(blockIdx.x) / nct;
-  const int c = ct * 16 + int(threadIdx.x % 16), span = threadIdx.x / 16;
-  const bool on = c < a.C;
-  const Map* maps = reinterpret_cast<const Map*>(a.maps) + size_t(b) * nchunks * a.C + (on ? c : 0);
-  enter += size_t(b) * nchunks * a.C + (on ? c : 0);
-  const int n = nchunks - 1, per = (n + 63) / 64, i0 = span * per, i1 = min(n, i0 + per);
-  auto at = [&](int i) { return size_t(REV ? n - i : i) * a.C; };   // the i-th tile on the way
-  Map m = {1.0f, 0.0f};
-#pragma unroll 8
-  for (int i = i0; i < i1; ++i) m = then(m, maps[at(i)]);
-  part[span][threadIdx.x % 16] = m;
-  __syncthreads();
-  // packed rows: the ends carry their own values
-  float h = 0.0f;
-  if (on && !a.offsets) {
-    const float* h0 = REV ? a.dh : a.h0;
-    if (h0) h = h0[size_t(b) * a.C + c];
-  }
-  for (int s = 0; s < span; ++s) h = apply(part[s][threadIdx.x % 16], h);
-  if (!on) return;
-#pragma unroll 8
-  for (int i = i0; i < i1; ++i) {
-    enter[at(i)] = h;
-    h = apply(maps[at(i)], h);
-  }
-  if (i1 == n && i0 < n) enter[at(n)] = h;
-}
-
-// ---- third pass, forward
+// ---- forward
 
 template <typename T, int V, bool PACKED, bool KEEP>
 __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) {
   __shared__ Carry<V> k;
   __shared__ Marks marks;
-  const Where w = where<V>(a, nchunks);
+  const Where w = where<V, false>(a, nchunks);
   const int limit = PACKED ? packed_limit(a.offsets, a.nseq, a.T) : a.T;
   const bool on = w.c < a.C;
   const int lim = on ? limit : 0;
@@ -329,10 +297,9 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
   __syncthreads();
   const int ch = threadIdx.x, c = w.ct * kLanes * V + ch;
   if (ch < kLanes * V && c < a.C) {
-    float in = 0.0f;
-    if (nchunks > 1) in = a.states[(size_t(w.b) * nchunks + w.chunk) * a.C + c];
-    else if (!PACKED && a.h0) in = a.h0[size_t(w.b) * a.C + c];
-    if (nchunks == 1 && a.states) a.states[size_t(w.b) * a.C + c] = in;
+    const float h0 = !PACKED && a.h0 ? a.h0[size_t(w.b) * a.C + c] : 0.0f;   // packed: the starts carry theirs
+    const float in = entering(a, w, nchunks, c, fold<V, false, false>(k, ch, 0.0f), h0);
+    if (a.states) a.states[(size_t(w.b) * nchunks + w.chunk) * a.C + c] = in;
     fold<V, false, true>(k, ch, in);
     if (w.chunk == 0 && a.h_out) {   // sequences without a row end where they start
       if (PACKED) {
@@ -343,6 +310,17 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
       }
     }
   }
+  float sz[kRows][V];   // SiLU(z), by the waves that wait for the states
+#pragma unroll
+  for (int i = 0; i < kRows; ++i)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      sz[i][v] = 1.0f;
+      if (a.gated && w.r + i < lim) {
+        const float zz = z[i].get(v);
+        sz[i][v] = zz * sigmoidf(zz);
+      }
+    }
   if (KEEP) {
     keep_rows<T, V>(a, 0, x, w, limit);
     keep_rows<T, V>(a, 1, d, w, limit);
@@ -368,11 +346,7 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       h[v] = PACKED ? apply({A[i][v], S[i][v]}, h[v]) : fmaf(A[i][v], h[v], S[i][v]);
-      out[v] = h[v];
-      if (a.gated) {
-        const float zz = z[i].get(v);
-        out[v] *= zz * sigmoidf(zz);
-      }
+      out[v] = a.gated ? h[v] * sz[i][v] : h[v];
     }
     store_row<V>(y + size_t(i) * a.C, out);
     const int end = PACKED ? marks.end[w.sub * kRows + i] : w.r + i == a.T - 1 ? w.b : -1;
@@ -382,13 +356,13 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
   }
 }
 
-// ---- third pass, adjoint: the tile's states again from the one before it, then the gradients backwards
+// ---- adjoint: the tile's states again from the one before it, the gradients backwards
 
 template <typename T, int V, bool PACKED, bool KEPT>
 __global__ void __launch_bounds__(256) token_scan_bwd(TokenScan a, int nchunks) {
   __shared__ Carry<V> k, kr;
   __shared__ Marks marks;
-  const Where w = where<V>(a, nchunks);
+  const Where w = where<V, true>(a, nchunks);
   const int limit = PACKED ? packed_limit(a.offsets, a.nseq, a.T) : a.T;
   const bool on = w.c < a.C;
   const int lim = on ? limit : 0;
@@ -447,10 +421,8 @@ __global__ void __launch_bounds__(256) token_scan_bwd(TokenScan a, int nchunks) 
       if (half == 0) {
         fold<V, false, true>(k, ch, a.states[at]);
       } else {
-        float in = 0.0f;
-        if (nchunks > 1) in = a.enter[at];
-        else if (!PACKED && a.dh) in = a.dh[size_t(w.b) * a.C + c];
-        fold<V, true, true>(kr, ch, in);
+        const float dh = !PACKED && a.dh ? a.dh[size_t(w.b) * a.C + c] : 0.0f;
+        fold<V, true, true>(kr, ch, entering(a, w, nchunks, c, fold<V, true, false>(kr, ch, 0.0f), dh));
       }
       if (half == 0 && w.chunk == 0 && a.dh0) {
         if (PACKED) {
@@ -534,6 +506,11 @@ __global__ void __launch_bounds__(256) token_scan_bwd(TokenScan a, int nchunks) 
 }
 
 // dkappa and dbias: the tiles' sums in a fixed order, in float64
+// all ones: nothing published, the counter before 0
+__global__ void __launch_bounds__(256) token_scan_clear(uint64_t* __restrict__ p, size_t n) {
+  for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) p[i] = kNotYet;
+}
+
 __global__ void __launch_bounds__(1024) token_scan_sums(const float2* __restrict__ parts, int n, int C,
                                                         float* __restrict__ dkappa, float* __restrict__ dbias) {
   __shared__ double sk[64][16], sb[64][16];
@@ -608,17 +585,31 @@ hipError_t by_type(const TokenScan& a, int dtype, F&& f) {
 
 int token_scan_chunks(int T) { return T <= kTile ? 1 : (T + kTile - 1) / kTile; }
 
-hipError_t launch_token_scan(const TokenScan& a, int dtype, hipStream_t s) {
+// words of the maps, the spans' heads and the counter
+size_t token_scan_words(int B, int T, int C) {
+  const size_t n = size_t(token_scan_chunks(T));
+  return n == 1 ? 0 : 1 + size_t(B) * size_t(C) * (n + (n + kSpan - 1) / kSpan);
+}
+
+static void clear(TokenScan& a, uint64_t* words, hipStream_t s) {
+  const size_t n = token_scan_words(a.B, a.T, a.C);
+  if (!n) return;
+  const size_t maps = size_t(a.B) * size_t(a.C) * size_t(token_scan_chunks(a.T));
+  a.ticket = reinterpret_cast<unsigned*>(words);
+  a.maps = words + 1;
+  a.heads = a.maps + maps;
+  const size_t g = (n + 1023) / 1024;
+  token_scan_clear<<<unsigned(g < 2048 ? g : 2048), 256, 0, s>>>(words, n);
+}
+
+hipError_t launch_token_scan(const TokenScan& args, int dtype, uint64_t* words, hipStream_t s) {
+  TokenScan a = args;
+  clear(a, words, s);
   const int n = token_scan_chunks(a.T);
   return by_type(a, dtype, [&](auto t, auto vw) {
     using T = decltype(t);
     constexpr int V = decltype(vw)::value;
     const unsigned nct = unsigned((a.C + kLanes * V - 1) / (kLanes * V)) * unsigned(a.B);
-    if (n > 1) {
-      if (a.offsets) token_scan_maps<T, V, true, false, false><<<nct * unsigned(n - 1), 256, 0, s>>>(a, n);
-      else token_scan_maps<T, V, false, false, false><<<nct * unsigned(n - 1), 256, 0, s>>>(a, n);
-      token_scan_join<false><<<unsigned((a.C + 15) / 16) * unsigned(a.B), 1024, 0, s>>>(a, n, a.states);
-    }
     if (a.offsets) {
       if (a.kept) token_scan_fwd<T, V, true, true><<<nct * unsigned(n), 256, 0, s>>>(a, n);
       else token_scan_fwd<T, V, true, false><<<nct * unsigned(n), 256, 0, s>>>(a, n);
@@ -630,7 +621,9 @@ hipError_t launch_token_scan(const TokenScan& a, int dtype, hipStream_t s) {
   });
 }
 
-hipError_t launch_token_scan_bwd(const TokenScan& a, int dtype, hipStream_t s) {
+hipError_t launch_token_scan_bwd(const TokenScan& args, int dtype, uint64_t* words, hipStream_t s) {
+  TokenScan a = args;
+  clear(a, words, s);
   const int n = token_scan_chunks(a.T);
   return by_type(a, dtype, [&](auto t, auto vw) {
     using T = decltype(t);
@@ -638,10 +631,6 @@ hipError_t launch_token_scan_bwd(const TokenScan& a, int dtype, hipStream_t s) {
     const unsigned nct = unsigned((a.C + kLanes * V - 1) / (kLanes * V)) * unsigned(a.B);
     auto run = [&](auto packed, auto kept) {
       constexpr bool P = decltype(packed)::value, K = decltype(kept)::value;
-      if (n > 1) {
-        token_scan_maps<T, V, P, K, true><<<nct * unsigned(n - 1), 256, 0, s>>>(a, n);
-        token_scan_join<true><<<unsigned((a.C + 15) / 16) * unsigned(a.B), 1024, 0, s>>>(a, n, a.enter);
-      }
       token_scan_bwd<T, V, P, K><<<nct * unsigned(n), 256, 0, s>>>(a, n);
     };
     const std::true_type yes;

@@ -116,7 +116,7 @@ def _kept_buffers(planes: int, B: int, T: int, C: int, device):
 
 def scan_forward(x, delta, kappa, bias, z=None, state=None, offsets=None, out=None, keep_states=False, keep_e4m3=False):
     """:func:`token_scan` with what its adjoint needs: (y, final state, states, kept, kept scales); ``states`` (B,
-    segments, C) where ``keep_states``, the last two the 8-bit checkpoint where ``keep_e4m3``, else None."""
+    segments, C) where asked for, the last two the 8-bit checkpoint where ``keep_e4m3``, else None."""
     B, T, C, n, nseq = _sequences(x, kappa, bias, state, offsets)
     packed = offsets is not None
     rx, rd = _rows(x, "x", None, packed), _rows(delta, "delta", x, packed)
@@ -127,20 +127,19 @@ def scan_forward(x, delta, kappa, bias, z=None, state=None, offsets=None, out=No
         y = _check(out, "out", x.shape, x.dtype, x.device)
     final = torch.empty((n, C), dtype=torch.float32, device=x.device)
     lib = _lib.load()
-    chunks = lib.cssm_token_scan_chunks(T)
     states = kept = scales = work = None
-    if chunks > 1 or keep_states or keep_e4m3:
-        states = torch.empty((B, chunks, C), dtype=torch.float32, device=x.device)
+    if keep_states or keep_e4m3:
+        states = torch.empty((B, lib.cssm_token_scan_chunks(T), C), dtype=torch.float32, device=x.device)
     if keep_e4m3:
         kept, scales = _kept_buffers(2 if z is None else 3, B, T, C, x.device)
     need = lib.cssm_token_scan_workspace_size(B, T, C, 0)
     if need:
-        work = torch.empty(need // 4, dtype=torch.float32, device=x.device)
+        work = torch.empty(need // 8, dtype=torch.int64, device=x.device)
     if B and C:
         _call(x.device, "cssm_token_scan", _ref(rx), _ref(rd), _ref(rz), _DTYPES[x.dtype], B, T, C, kappa.data_ptr(),
               bias.data_ptr(), _ptr(state), _ptr(offsets), nseq, y.data_ptr(), int(packed and out is None),
               final.data_ptr(), _ptr(states), _ptr(kept), _ptr(scales), _ptr(work), need)
-    return y, final, states if keep_states else None, kept, scales
+    return y, final, states, kept, scales
 
 
 def scan_backward(x, delta, kappa, bias, z, state, offsets, states, kept, scales, dy, dfinal, gated: bool):
@@ -167,7 +166,7 @@ def scan_backward(x, delta, kappa, bias, z, state, offsets, states, kept, scales
     dk, db = torch.empty_like(kappa), torch.empty_like(bias)
     dh0 = torch.empty((n, C), dtype=torch.float32, device=dy.device)
     need = _lib.load().cssm_token_scan_workspace_size(B, T, C, 1)
-    work = torch.empty(max(1, need // 4), dtype=torch.float32, device=dy.device)
+    work = torch.empty(max(1, need // 8), dtype=torch.int64, device=dy.device)
     if B and C:
         _call(dy.device, "cssm_token_scan_bwd", _ref(rows[0]), _ref(rows[1]), _ref(rows[2]), int(gated), _ref(rdy),
               _DTYPES[dy.dtype], B, T, C, kappa.data_ptr(), bias.data_ptr(), _ptr(state), _ptr(offsets), nseq,

@@ -913,8 +913,8 @@ typedef struct cssm_token_rows {
  *   y            (B, T, C) of dtype, contiguous; rows behind the last sequence are left as they are, or with
  *                zero_tail != 0 set to zero
  *   h_out        (n, C) float32 state behind each sequence's last row (h0 for an empty one), or NULL
- *   states       (B, chunks, C) float32 out, chunks = cssm_token_scan_chunks(T): the state before every 128th row;
- *                may be NULL where chunks = 1
+ *   states       NULL, or (B, chunks, C) float32 out, chunks = cssm_token_scan_chunks(T): the state before every
+ *                128th row, which the adjoint reads
  *   kept, kept_scales  NULL, or x, delta and z (if given) in 8 bits for the adjoint: (2 or 3, B, T, C) e4m3 and
  *                (2 or 3, B, ceil(T / 8), ceil(C / 16)) exponents, a block being 8 rows x 16 channels
  *   workspace    cssm_token_scan_workspace_size(B, T, C, 0) bytes, 8-byte aligned

@@ -29,8 +29,9 @@ def test_scan(lib):
     args = dict(x=R, delta=R, z=R, dtype=0, B=2, T=200, C=8, kappa=P, bias=P, h0=None, offsets=None, nseq=0, y=P,
                 zero_tail=0, h_out=P, states=P, kept=None, kept_scales=None, work=P, bytes=BIG, stream=None)
     fn = lib.cssm_token_scan
-    for name in ("x", "delta", "kappa", "bias", "y", "states"):
+    for name in ("x", "delta", "kappa", "bias", "y"):
         fails(fn, args, -1, **{name: None})
+    fails(fn, args, -1, kept=P, kept_scales=P, states=None)
     fails(fn, args, -1, x=ctypes.addressof(EMPTY))
     fails(fn, args, -1, z=ctypes.addressof(EMPTY))
     fails(fn, args, -1, kept=P)
