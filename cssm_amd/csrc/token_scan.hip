@@ -14,6 +14,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "launch.h"
 #include "token_util.h"
 
@@ -37,14 +39,35 @@ __device__ __forceinline__ Map then(Map first, Map next) {
 }
 __device__ __forceinline__ float apply(Map m, float h) { return is_cut(m.A) ? m.S : fmaf(m.A, h, m.S); }
 
-// D = softplus(u), keep = sigmoid(-u) = exp(-D), gate = sigmoid(u), each to a few ulp: with e = exp(-|u|) and
-// w = 1 + e rounded, ln(1 + e) = ln(w) + (e - (w - 1)) / w holds its relative accuracy down to e alone
+// D = softplus(u), keep = exp(-D) = sigmoid(-u) and gate = sigmoid(u), from v = u log2(e), each to a few ulp: with
+// e = exp(-|u|) and w = 1 + e rounded, ln(w) + (e - (w - 1)) is ln(1 + e) with its relative accuracy down to e alone (what
+// w lost is at most 2^-25, next to ln(1 + e) where that is large).
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 struct Gains { float D, keep, gate; };
-__device__ __forceinline__ Gains gains(float u) {
-  const float e = fast_exp(-fabsf(u)), w = 1.0f + e, r = __builtin_amdgcn_rcpf(w);
-  const float l = fmaf(e - (w - 1.0f), r, 0.69314718055994531f * __builtin_amdgcn_logf(w));
-  const float s = e * r;
-  return {fmaxf(u, 0.0f) + l, u > 0.0f ? s : r, u > 0.0f ? r : s};
+__device__ __forceinline__ Gains gains(float v) {
+  const float e = __builtin_amdgcn_exp2f(-fabsf(v)), w = 1.0f + e, r = __builtin_amdgcn_rcpf(w), s = e * r;
+  const float D = fmaf(kLn2, fmaxf(v, 0.0f) + __builtin_amdgcn_logf(w), e - (w - 1.0f));
+  const bool up = v > 0.0f;
+  return {D, up ? s : r, up ? r : s};
+}
+
+// Hides from the compiler that a register holds what it held before, and fixes the point by which it is computed.  A tile's
+// phases unpack and combine the same packed rows; seen as the same values, the unpacked ones would stay in registers
+// from phase to phase, and a row's results be put off until the last row's: twice the registers, which costs more than
+// unpacking again.
+__device__ __forceinline__ void renew(uint32_t& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void renew(float& v) { asm volatile("" : "+v"(v)); }
+__device__ __forceinline__ void renew(uint2& v) { renew(v.x), renew(v.y); }
+__device__ __forceinline__ void renew(float2& v) { renew(v.x), renew(v.y); }
+__device__ __forceinline__ void renew(uint16_t& v) {
+  uint32_t w = v;
+  renew(w);
+  v = uint16_t(w);
+}
+template <typename T, int V>
+__device__ __forceinline__ void renew(Raw<T, V> (&q)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) renew(q[i].q);
 }
 
 // Which sequence starts / ends at each row of a tile, -1 where none does (packed sequences).
@@ -72,27 +95,28 @@ struct Where {
   int ct, chunk, b, sub, c, r;   // channel tile, row tile, batch; row group, first channel, first row
   int place;                     // of the row tile on the way: chunk, or from the end
 };
-// Tiles are handed out by a counter in the order of their place on the way, so that every tile waits only for tiles
-// whose workgroups run already; with one tile a sequence nothing waits and the block index does.
 template <int V, bool REV>
-__device__ __forceinline__ Where where(const TokenScan& a, int nchunks) {
-  __shared__ unsigned ticket;
-  unsigned blk = blockIdx.x;
-  if (nchunks > 1) {
-    if (threadIdx.x == 0) ticket = atomicAdd(a.ticket, 1u) + 1u;   // starts at all ones
-    __syncthreads();
-    blk = ticket;
-  }
+__device__ __forceinline__ Where where(const TokenScan& a, int nchunks, unsigned tile) {
+  tile = __builtin_amdgcn_readfirstlane(tile);   // it came by shared memory: the same for all
   const unsigned nct = unsigned(a.C + kLanes * V - 1) / (kLanes * V);
   Where w;
-  w.ct = int(blk % nct);
-  w.b = int(blk / nct % unsigned(a.B));
-  w.place = int(blk / nct / unsigned(a.B));
+  w.ct = int(tile % nct);
+  w.b = int(tile / nct % unsigned(a.B));
+  w.place = int(tile / nct / unsigned(a.B));
   w.chunk = REV ? nchunks - 1 - w.place : w.place;
   w.sub = threadIdx.x / kLanes;
   w.c = (w.ct * kLanes + int(threadIdx.x % kLanes)) * V;
   w.r = w.chunk * kTile + w.sub * kRows;
   return w;
+}
+// Tiles are handed out by a counter in the order of their place on the way, so that every tile waits only for tiles
+// that workgroups already have; with one tile a sequence nothing waits.
+__device__ __forceinline__ unsigned my_tile(const TokenScan& a, int nchunks) {
+  __shared__ unsigned tile;
+  if (nchunks == 1) return blockIdx.x;
+  if (threadIdx.x == 0) tile = atomicAdd(a.ticket, 1u) + 1u;   // from all ones
+  __syncthreads();
+  return tile;
 }
 
 // A map (or with A = 0 a state) as one 64-bit word, which other workgroups see whole or not at all: all ones until it is
@@ -106,49 +130,74 @@ __device__ __forceinline__ void publish(uint64_t* at, Map m) {
 __device__ __forceinline__ uint64_t peek(const uint64_t* at) {
   return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// The word's publisher has a lower ticket, so it runs and waits only for lower ones: the wait ends.  (The count only
-// keeps a defect from hanging the device; it would end in NaN.)
-__device__ __forceinline__ Map await(const uint64_t* at, uint64_t v) {
-  for (int i = 0; v == kNotYet && i < (1 << 22); ++i) {
-    __builtin_amdgcn_s_sleep(1);
-    v = peek(at);
-  }
+// The word's publisher has a lower number than the tile that waits, so its workgroup runs already, and waits only for
+// lower ones itself: the wait ends.  (The count only keeps a defect from hanging the device; it would end in NaN.)
+__device__ __forceinline__ Map unpack(uint64_t v) {
   return {__uint_as_float(uint32_t(v >> 32)), __uint_as_float(uint32_t(v))};
+}
+// n <= N words `step` apart, each once it is published; `at` and `step` the same for the wave, `c` its lanes'
+template <int N>
+__device__ __forceinline__ void await(uint64_t (&v)[N], const uint64_t* at, unsigned c, size_t step, int n) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = i < n ? peek(at + step * i + c) : 0;
+  for (int tries = 0; tries < (1 << 22); ++tries) {
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) all = all && v[i] != kNotYet;
+    if (all) break;
+    __builtin_amdgcn_s_sleep(1);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (v[i] == kNotYet) v[i] = peek(at + step * i + c);   // only what is missing: each peek goes to memory
+  }
 }
 
 // The value entering the tile at this place for one channel, by its own map `own` and those before it.  Places
 // come in spans of kSpan: a tile joins the maps of its span's earlier places (at most kSpan - 1, published without
 // waiting) and applies them to the value entering the span, which the last tile of the span before published.  So
 // the chain of waits has a link for each kSpan tiles, and the sums come in the same order every time.
-constexpr int kSpan = 16;
+constexpr int kSpan = 8;
 __device__ __forceinline__ float entering(const TokenScan& a, const Where& w, int nchunks, int c, Map own, float first) {
   if (nchunks == 1) return first;
   const int spans = (nchunks + kSpan - 1) / kSpan, span = w.place / kSpan, p0 = span * kSpan;
-  uint64_t* maps = a.maps + size_t(w.b) * nchunks * a.C + c;
-  uint64_t* heads = a.heads + size_t(w.b) * spans * a.C + c;
-  if (w.place + 1 < nchunks) publish(maps + size_t(w.place) * a.C, own);
+  uint64_t* maps = a.maps + size_t(w.b) * nchunks * a.C;
+  uint64_t* heads = a.heads + size_t(w.b) * spans * a.C;
+  if (w.place + 1 < nchunks) publish(maps + size_t(w.place) * a.C + c, own);
   Map m = {1.0f, 0.0f};
-  uint64_t v[kSpan];   // the last: the span's head
-  const uint64_t* head = heads + size_t(span) * a.C;
-  if (span > 0) v[kSpan - 1] = peek(head);
+  const int before = w.place - p0;
+  if (before > 0) {
+    uint64_t v[kSpan - 1];
+    await(v, maps + size_t(p0) * a.C, unsigned(c), size_t(a.C), before);
 #pragma unroll
-  for (int i = 0; i < kSpan - 1; ++i)
-    if (p0 + i < w.place) v[i] = peek(maps + size_t(p0 + i) * a.C);
-#pragma unroll
-  for (int i = 0; i < kSpan - 1; ++i)
-    if (p0 + i < w.place) m = then(m, await(maps + size_t(p0 + i) * a.C, v[i]));
-  if (span > 0) first = await(head, v[kSpan - 1]).S;
+    for (int i = 0; i < kSpan - 1; ++i)
+      if (i < before) m = then(m, unpack(v[i]));
+  }
+  if (span > 0) {
+    uint64_t v[1];
+    await(v, heads + size_t(span) * a.C, unsigned(c), 0, 1);
+    first = unpack(v[0]).S;
+  }
   const float in = apply(m, first);
-  if (w.place % kSpan == kSpan - 1 && w.place + 1 < nchunks) publish(heads + size_t(span + 1) * a.C, {0.0f, apply(own, in)});
+  if (w.place % kSpan == kSpan - 1 && w.place + 1 < nchunks) publish(heads + size_t(span + 1) * a.C + c, {0.0f, apply(own, in)});
   return in;
 }
 
+// Element offset of a thread's first row and channel from its tile's, and of the rows below: where a thread takes several
+// channels (V > 1) the strides are small enough for 32 bits in bytes (width()), so that a load is a scalar base and
+// one register.
+template <int V>
+using Off = typename std::conditional<V == 1, size_t, uint32_t>::type;
+
+// The thread's 8 rows, every one of them: rows behind the limit (> 0) give the last one again and channels behind C
+// the last ones, which nothing uses.
 template <typename T, int V>
-__device__ __forceinline__ void load_rows(Raw<T, V> (&q)[kRows], const TokenRows& t, const Where& w, int limit) {
-  const T* p = static_cast<const T*>(t.p) + (long long)w.b * t.batch + (long long)w.r * t.row + w.c;
+__device__ __forceinline__ void load_rows(Raw<T, V> (&q)[kRows], const TokenRows& t, const Where& w, int C, int limit) {
+  const int r0 = min(w.chunk * kTile, limit - 1);
+  const char* p = static_cast<const char*>(t.p) + ((long long)w.b * t.batch + (long long)r0 * t.row) * (long long)sizeof(T);
+  const Off<V> row = Off<V>(t.row) * Off<V>(sizeof(T)), c = Off<V>(min(w.c, C - V)) * Off<V>(sizeof(T));
+  const Off<V> at = Off<V>(w.sub * kRows) * row + c, last = Off<V>(limit - 1 - r0) * row + c;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i)
-    if (w.r + i < limit) q[i] = load_raw<T, V>(p + (long long)i * t.row);
+  for (int i = 0; i < kRows; ++i) q[i] = load_raw<T, V>(reinterpret_cast<const T*>(p + min(at + Off<V>(i) * row, last)));
 }
 
 // Rows kept in 8 bits: plane k of (planes, B, T, C) e4m3 and (planes, B, ceil(T / 8), ceil(C / 16)) exponents.  A
@@ -157,16 +206,21 @@ template <int V>
 struct Kept {
   uint32_t q[kRows];
   float s;
+  __device__ __forceinline__ void again() {
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) renew(q[i]);
+  }
   __device__ __forceinline__ void load(const TokenScan& a, int plane, const Where& w, int limit) {
     const size_t pb = size_t(plane) * a.B + w.b;
-    const uint8_t* p = a.kept + (pb * a.T + w.r) * a.C + w.c;
-    if (w.r < limit) s = pow2_of(a.kept_scales[(pb * ((a.T + 7) / 8) + w.r / 8) * ((a.C + 15) / 16) + w.c / 16]);
+    const int c = min(w.c, a.C - V), r0 = min(w.chunk * kTile, limit - 1);
+    const uint8_t* p = a.kept + (pb * a.T + r0) * a.C;
+    s = pow2_of(a.kept_scales[(pb * ((a.T + 7) / 8) + min(w.r, limit - 1) / 8) * ((a.C + 15) / 16) + c / 16]);
+    const Off<V> row = Off<V>(a.C), at = Off<V>(w.sub * kRows) * row + Off<V>(c), last = Off<V>(limit - 1 - r0) * row + Off<V>(c);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
-      if (w.r + i < limit) {
-        const uint8_t* at = p + size_t(i) * a.C;
-        q[i] = V == 4 ? *reinterpret_cast<const uint32_t*>(at) : V == 2 ? *reinterpret_cast<const uint16_t*>(at) : *at;
-      }
+    for (int i = 0; i < kRows; ++i) {
+      const uint8_t* x = p + min(at + Off<V>(i) * row, last);
+      q[i] = V == 4 ? *reinterpret_cast<const uint32_t*>(x) : V == 2 ? *reinterpret_cast<const uint16_t*>(x) : *x;
+    }
   }
   __device__ __forceinline__ float get(int i, int v) const {
     return s * (v == 0   ? __builtin_amdgcn_cvt_f32_fp8(int(q[i]), 0)
@@ -178,12 +232,13 @@ struct Kept {
 template <typename T, int V>
 struct Plain {
   Raw<T, V> q[kRows];
+  __device__ __forceinline__ void again() { renew(q); }
   __device__ __forceinline__ float get(int i, int v) const { return q[i].get(v); }
 };
 template <typename T, int V, bool KEPT>
 struct Source : Plain<T, V> {
   __device__ __forceinline__ void load(const TokenScan& a, const TokenRows& t, int, const Where& w, int limit) {
-    load_rows<T, V>(this->q, t, w, limit);
+    load_rows<T, V>(this->q, t, w, a.C, limit);
   }
 };
 template <typename T, int V>
@@ -198,15 +253,14 @@ struct Source<T, V, true> : Kept<V> {
 template <typename T, int V>
 __device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const Raw<T, V> (&q)[kRows], const Where& w,
                                           int limit) {
-  float top = 0.0f;
+  float top = 0.0f;   // a row or channels twice (load_rows) are of the same block
 #pragma unroll
   for (int i = 0; i < kRows; ++i)
-    if (w.c < a.C && w.r + i < limit)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float m = fabsf(q[i].get(v));
-        top = fmaxf(top, m < INFINITY ? m : 0.0f);
-      }
+    for (int v = 0; v < V; ++v) {
+      const float m = fabsf(q[i].get(v));
+      top = fmaxf(top, m < INFINITY ? m : 0.0f);
+    }
 #pragma unroll
   for (int l = 1; l < 16 / V; l *= 2) top = fmaxf(top, __shfl_xor(top, l));
   if (w.c >= a.C || w.r >= limit) return;
@@ -215,11 +269,12 @@ __device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const R
   const size_t pb = size_t(plane) * a.B + w.b;
   if (w.c % 16 == 0)
     a.kept_scales[(pb * ((a.T + 7) / 8) + w.r / 8) * ((a.C + 15) / 16) + w.c / 16] = uint8_t(byte);
-  uint8_t* p = a.kept + (pb * a.T + w.r) * a.C + w.c;
+  uint8_t* p = a.kept + (pb * a.T + w.chunk * kTile) * a.C;
+  const Off<V> off = Off<V>(w.sub * kRows) * Off<V>(a.C) + Off<V>(w.c);
 #pragma unroll
   for (int i = 0; i < kRows; ++i)
     if (w.r + i < limit) {
-      uint8_t* at = p + size_t(i) * a.C;
+      uint8_t* at = p + size_t(i) * a.C + off;
       if constexpr (V == 4)
         *reinterpret_cast<uint32_t*>(at) = pack_e4m3x4(q[i].get(0) * inv, q[i].get(1) * inv, q[i].get(2) * inv, q[i].get(3) * inv);
       else if constexpr (V == 2) *reinterpret_cast<uint16_t*>(at) = uint16_t(pack_e4m3x2(q[i].get(0) * inv, q[i].get(1) * inv));
@@ -238,16 +293,20 @@ struct Carry {
 template <int V, bool REV, bool WRITE>
 __device__ __forceinline__ Map fold(Carry<V>& k, int ch, float in) {
   Map all = {1.0f, 0.0f};
-  Map m[kSubs];
 #pragma unroll
-  for (int i = 0; i < kSubs; ++i) m[i] = k.m[REV ? kSubs - 1 - i : i][ch];
+  for (int j = 0; j < kSubs; j += 8) {
+    asm volatile("" ::: "memory");   // a second call reads again: 32 registers less than holding all maps between the two
+    Map m[8];
 #pragma unroll
-  for (int i = 0; i < kSubs; ++i) {
-    if (WRITE) {
-      k.in[REV ? kSubs - 1 - i : i][ch] = in;
-      in = apply(m[i], in);
-    } else {
-      all = then(all, m[i]);
+    for (int i = 0; i < 8; ++i) m[i] = k.m[REV ? kSubs - 1 - i - j : i + j][ch];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (WRITE) {
+        k.in[REV ? kSubs - 1 - i - j : i + j][ch] = in;
+        in = apply(m[i], in);
+      } else {
+        all = then(all, m[i]);
+      }
     }
   }
   return all;
@@ -256,20 +315,21 @@ __device__ __forceinline__ Map fold(Carry<V>& k, int ch, float in) {
 // ---- forward
 
 template <typename T, int V, bool PACKED, bool KEEP>
-__global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) {
+__global__ void __launch_bounds__(256, KEEP ? 3 : 4) token_scan_fwd(TokenScan a, int nchunks) {
   __shared__ Carry<V> k;
   __shared__ Marks marks;
-  const Where w = where<V, false>(a, nchunks);
+  const Where w = where<V, false>(a, nchunks, my_tile(a, nchunks));
   const int limit = PACKED ? packed_limit(a.offsets, a.nseq, a.T) : a.T;
   const bool on = w.c < a.C;
-  const int lim = on ? limit : 0;
   Raw<T, V> d[kRows], x[kRows], z[kRows];
-  load_rows<T, V>(d, a.delta, w, lim);
-  load_rows<T, V>(x, a.x, w, lim);
-  if (a.gated) load_rows<T, V>(z, a.z, w, lim);
+  if (limit > 0) {
+    load_rows<T, V>(d, a.delta, w, a.C, limit);
+    load_rows<T, V>(x, a.x, w, a.C, limit);
+    if (a.gated) load_rows<T, V>(z, a.z, w, a.C, limit);
+  }
   float kap[V], bia[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) kap[v] = on ? a.kappa[w.c + v] : 0.0f, bia[v] = on ? a.bias[w.c + v] : 0.0f;
+  for (int v = 0; v < V; ++v) kap[v] = a.kappa[min(w.c, a.C - V) + v], bia[v] = a.bias[min(w.c, a.C - V) + v];
   if (PACKED) find_marks(marks, a.offsets, a.nseq, w.chunk * kTile, limit);
   float A[kRows][V], S[kRows][V];
   Map m[V];
@@ -277,19 +337,18 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
   for (int v = 0; v < V; ++v) m[v] = {1.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const bool row = w.r + i < lim;
-    const int mark = PACKED ? marks.start[w.sub * kRows + i] : -1;
+    // (rows behind the limit come behind all that counts)
+    const int mark = PACKED && on ? marks.start[w.sub * kRows + i] : -1;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      A[i][v] = 1.0f, S[i][v] = 0.0f;
-      if (!row) continue;
-      const Gains g = gains(d[i].get(v) + bia[v]);
+      const Gains g = gains((d[i].get(v) + bia[v]) * kLog2e);
       A[i][v] = kap[v] * g.keep, S[i][v] = g.D * x[i].get(v);
       if (PACKED && mark >= 0) {
         S[i][v] = fmaf(A[i][v], a.h0 ? a.h0[size_t(mark) * a.C + w.c + v] : 0.0f, S[i][v]);
         A[i][v] = cut();
       }
       m[v] = PACKED ? then(m[v], {A[i][v], S[i][v]}) : Map{m[v].A * A[i][v], fmaf(A[i][v], m[v].S, S[i][v])};
+      renew(m[v].S), renew(A[i][v]);
     }
   }
 #pragma unroll
@@ -312,34 +371,38 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
   }
   float sz[kRows][V];   // SiLU(z), by the waves that wait for the states
 #pragma unroll
-  for (int i = 0; i < kRows; ++i)
+  for (int i = 0; i < kRows; ++i) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       sz[i][v] = 1.0f;
-      if (a.gated && w.r + i < lim) {
+      if (a.gated) {
         const float zz = z[i].get(v);
         sz[i][v] = zz * sigmoidf(zz);
+        renew(sz[i][v]);
       }
     }
+  }
   if (KEEP) {
+    renew(x), renew(d), renew(z);
     keep_rows<T, V>(a, 0, x, w, limit);
     keep_rows<T, V>(a, 1, d, w, limit);
     if (a.gated) keep_rows<T, V>(a, 2, z, w, limit);
   }
   __syncthreads();
-  if (!on) return;
   float h[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = k.in[w.sub][int(threadIdx.x % kLanes) * V + v];
-  T* y = static_cast<T*>(a.y) + (size_t(w.b) * a.T + w.r) * a.C + w.c;
+  T* y = static_cast<T*>(a.y) + (size_t(w.b) * a.T + w.chunk * kTile) * a.C;
+  const Off<V> off = Off<V>(w.sub * kRows) * Off<V>(a.C) + Off<V>(w.c);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     float out[V];
+    if (!on) continue;
     if (w.r + i >= limit) {
       if (PACKED && a.zero_tail && w.r + i < a.T) {
 #pragma unroll
         for (int v = 0; v < V; ++v) out[v] = 0.0f;
-        store_row<V>(y + size_t(i) * a.C, out);
+        store_row<V>(y + size_t(i) * a.C + off, out);
       }
       continue;
     }
@@ -348,7 +411,7 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
       h[v] = PACKED ? apply({A[i][v], S[i][v]}, h[v]) : fmaf(A[i][v], h[v], S[i][v]);
       out[v] = a.gated ? h[v] * sz[i][v] : h[v];
     }
-    store_row<V>(y + size_t(i) * a.C, out);
+    store_row<V>(y + size_t(i) * a.C + off, out);
     const int end = PACKED ? marks.end[w.sub * kRows + i] : w.r + i == a.T - 1 ? w.b : -1;
     if (end >= 0 && a.h_out)
 #pragma unroll
@@ -359,57 +422,81 @@ __global__ void __launch_bounds__(256) token_scan_fwd(TokenScan a, int nchunks) 
 // ---- adjoint: the tile's states again from the one before it, the gradients backwards
 
 template <typename T, int V, bool PACKED, bool KEPT>
-__global__ void __launch_bounds__(256) token_scan_bwd(TokenScan a, int nchunks) {
+__global__ void __launch_bounds__(256, 2) token_scan_bwd(TokenScan a, int nchunks) {
   __shared__ Carry<V> k, kr;
   __shared__ Marks marks;
-  const Where w = where<V, true>(a, nchunks);
+  const Where w = where<V, true>(a, nchunks, my_tile(a, nchunks));
   const int limit = PACKED ? packed_limit(a.offsets, a.nseq, a.T) : a.T;
   const bool on = w.c < a.C;
-  const int lim = on ? limit : 0;
   Source<T, V, KEPT> d, x, z;
   Raw<T, V> dy[kRows];
-  d.load(a, a.delta, 1, w, lim);
-  x.load(a, a.x, 0, w, lim);
-  load_rows<T, V>(dy, a.dy, w, lim);
-  if (a.gated) z.load(a, a.z, 2, w, lim);
+  if (limit > 0) {
+    d.load(a, a.delta, 1, w, limit);
+    x.load(a, a.x, 0, w, limit);
+    load_rows<T, V>(dy, a.dy, w, a.C, limit);
+    if (a.gated) z.load(a, a.z, 2, w, limit);
+  }
   float kap[V], bia[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) kap[v] = on ? a.kappa[w.c + v] : 0.0f, bia[v] = on ? a.bias[w.c + v] : 0.0f;
+  for (int v = 0; v < V; ++v) kap[v] = a.kappa[min(w.c, a.C - V) + v], bia[v] = a.bias[min(w.c, a.C - V) + v];
   if (PACKED) find_marks(marks, a.offsets, a.nseq, w.chunk * kTile, limit);
-  // maps of the group's 8 rows, both ways
-  float D[kRows][V], keep[kRows][V], P[kRows][V];
+  auto again = [&] {
+    x.again(), renew(dy);
+    if (a.gated) z.again();
+  };
+  // Rows behind the limit come first on the way back: the end of the last sequence starts afresh.
+  auto ends_at = [&](int i) { return !on ? -1 : PACKED ? marks.end[w.sub * kRows + i] : w.r + i == a.T - 1 ? w.b : -1; };
+  // Maps of the group's 8 rows both ways, from the last row up, where a row enters the forward map by the product of the
+  // A behind it: that product is the A of both.
+  float D[kRows][V], kp[kRows][V], gt[kRows][V], sz[kRows][V];   // softplus, sigmoid(-u), sigmoid(u), sigmoid(z)
   Map m[V], mr[V];
+  bool cut_fwd = false, cut_rev = false;   // packed: a sequence starts / ends in the group
 #pragma unroll
   for (int v = 0; v < V; ++v) m[v] = mr[v] = {1.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    if (w.r + i >= lim) continue;
-    const int mark = PACKED ? marks.start[w.sub * kRows + i] : -1;
+  for (int i = kRows - 1; i >= 0; --i) {
+    const int end = ends_at(i), start = PACKED && on ? marks.start[w.sub * kRows + i] : -1;
+    if (end >= 0) {
+      cut_rev = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) mr[v] = {0.0f, a.dh ? a.dh[size_t(end) * a.C + w.c + v] : 0.0f};
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const Gains g = gains(d.get(i, v) + bia[v]);
-      D[i][v] = g.D, keep[i][v] = g.keep;
+      const Gains g = gains((d.get(i, v) + bia[v]) * kLog2e);
+      D[i][v] = g.D, kp[i][v] = g.keep, gt[i][v] = g.gate;
       const float A = kap[v] * g.keep;
-      if (mark >= 0) m[v] = {cut(), a.h0 ? a.h0[size_t(mark) * a.C + w.c + v] : 0.0f};
-      m[v] = {PACKED && is_cut(m[v].A) ? cut() : m[v].A * A, fmaf(A, m[v].S, g.D * x.get(i, v))};
-      P[i][v] = dy[i].get(v);
+      if (!PACKED || !cut_fwd) {
+        m[v].S = fmaf(m[v].A, g.D * x.get(i, v), m[v].S);
+        m[v].A *= A;
+      }
+      if (PACKED) mr[v].A *= A;
+      float p = dy[i].get(v);
       if (a.gated) {
         const float zz = z.get(i, v);
-        P[i][v] *= zz * sigmoidf(zz);
+        sz[i][v] = sigmoidf(zz);
+        p *= zz * sz[i][v];
+        renew(sz[i][v]);
       }
+      mr[v].S = A * (p + mr[v].S);
+      renew(m[v].A), renew(m[v].S), renew(mr[v].S), renew(D[i][v]), renew(kp[i][v]), renew(gt[i][v]);
+    }
+    if (PACKED && start >= 0 && !cut_fwd) {
+      cut_fwd = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) m[v].S = fmaf(m[v].A, a.h0 ? a.h0[size_t(start) * a.C + w.c + v] : 0.0f, m[v].S);
     }
   }
 #pragma unroll
-  for (int i = kRows - 1; i >= 0; --i) {
-    if (w.r + i >= lim) continue;
-    const int mark = PACKED ? marks.end[w.sub * kRows + i] : -1;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float A = kap[v] * keep[i][v];
-      if (mark >= 0) mr[v] = {cut(), a.dh ? a.dh[size_t(mark) * a.C + w.c + v] : 0.0f};
-      mr[v] = {PACKED && is_cut(mr[v].A) ? cut() : mr[v].A * A, A * (P[i][v] + mr[v].S)};
-    }
+  for (int v = 0; v < V; ++v) {
+    if (!PACKED) mr[v].A = cut_rev ? 0.0f : m[v].A;
+    if (PACKED && cut_rev) mr[v].A = cut();
+    if (PACKED && cut_fwd) m[v].A = cut();
   }
+  again();
+  if (w.r >= limit)
+#pragma unroll
+    for (int v = 0; v < V; ++v) mr[v] = {1.0f, 0.0f};
   const int lc = int(threadIdx.x % kLanes) * V;
 #pragma unroll
   for (int v = 0; v < V; ++v) k.m[w.sub][lc + v] = m[v], kr.m[w.sub][lc + v] = mr[v];
@@ -421,8 +508,7 @@ __global__ void __launch_bounds__(256) token_scan_bwd(TokenScan a, int nchunks) 
       if (half == 0) {
         fold<V, false, true>(k, ch, a.states[at]);
       } else {
-        const float dh = !PACKED && a.dh ? a.dh[size_t(w.b) * a.C + c] : 0.0f;
-        fold<V, true, true>(kr, ch, entering(a, w, nchunks, c, fold<V, true, false>(kr, ch, 0.0f), dh));
+        fold<V, true, true>(kr, ch, entering(a, w, nchunks, c, fold<V, true, false>(kr, ch, 0.0f), 0.0f));
       }
       if (half == 0 && w.chunk == 0 && a.dh0) {
         if (PACKED) {
@@ -443,54 +529,57 @@ __global__ void __launch_bounds__(256) token_scan_bwd(TokenScan a, int nchunks) 
   }
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    if (w.r + i >= lim) continue;
-    const int mark = PACKED ? marks.start[w.sub * kRows + i] : -1;
+    const int mark = PACKED && on ? marks.start[w.sub * kRows + i] : -1;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (mark >= 0) h[v] = a.h0 ? a.h0[size_t(mark) * a.C + w.c + v] : 0.0f;
+      if (PACKED && mark >= 0) h[v] = a.h0 ? a.h0[size_t(mark) * a.C + w.c + v] : 0.0f;
       before[i][v] = h[v];
-      h[v] = fmaf(kap[v] * keep[i][v], h[v], D[i][v] * x.get(i, v));
+      h[v] = fmaf(kap[v] * kp[i][v], h[v], D[i][v] * x.get(i, v));
+      renew(h[v]), renew(kp[i][v]), renew(D[i][v]);
     }
   }
-  const size_t row0 = (size_t(w.b) * a.T + w.r) * a.C + w.c;
+  again();
+  const size_t row0 = (size_t(w.b) * a.T + w.chunk * kTile) * a.C;
+  const Off<V> off = Off<V>(w.sub * kRows) * Off<V>(a.C) + Off<V>(w.c);
 #pragma unroll
   for (int i = kRows - 1; i >= 0; --i) {
     if (!on) continue;
-    const size_t at = row0 + size_t(i) * a.C;
+    const size_t at = row0 + size_t(i) * a.C;   // + off
     float ox[V], od[V], oz[V];
     if (w.r + i >= limit) {
       if (PACKED && w.r + i < a.T) {   // rows behind the last sequence have no gradient
 #pragma unroll
         for (int v = 0; v < V; ++v) ox[v] = 0.0f;
-        store_row<V>(static_cast<T*>(a.dx) + at, ox);
-        store_row<V>(static_cast<T*>(a.ddelta) + at, ox);
-        if (a.gated) store_row<V>(static_cast<T*>(a.dz) + at, ox);
+        store_row<V>(static_cast<T*>(a.dx) + at + off, ox);
+        store_row<V>(static_cast<T*>(a.ddelta) + at + off, ox);
+        if (a.gated) store_row<V>(static_cast<T*>(a.dz) + at + off, ox);
       }
       continue;
     }
-    const int end = PACKED ? marks.end[w.sub * kRows + i] : -1;
+    const int end = ends_at(i);
     const int start = PACKED ? marks.start[w.sub * kRows + i] : w.r + i == 0 ? w.b : -1;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       if (end >= 0) G[v] = a.dh ? a.dh[size_t(end) * a.C + w.c + v] : 0.0f;
-      const float A = kap[v] * keep[i][v], g = P[i][v] + G[v], xx = x.get(i, v);
+      const float A = kap[v] * kp[i][v], xx = x.get(i, v), dyv = dy[i].get(v), zz = a.gated ? z.get(i, v) : 0.0f;
+      const float s = a.gated ? sz[i][v] : 0.0f, w1 = zz * s;
+      const float g = (a.gated ? dyv * w1 : dyv) + G[v];
       ox[v] = D[i][v] * g;
-      const float u = d.get(i, v) + bia[v];
-      const float gate = sigmoidf(u);
-      od[v] = gate * (g * (xx - A * before[i][v]));
-      dk[v] = fmaf(g * keep[i][v], before[i][v], dk[v]);
+      od[v] = gt[i][v] * (g * fmaf(-A, before[i][v], xx));
+      dk[v] = fmaf(g * kp[i][v], before[i][v], dk[v]);
       db[v] += od[v];
-      if (a.gated) {
-        const float zz = z.get(i, v), s = sigmoidf(zz);
-        const float hh = fmaf(A, before[i][v], D[i][v] * xx);
-        oz[v] = dy[i].get(v) * hh * (s * fmaf(zz, 1.0f - s, 1.0f));
+      if (a.gated) {   // SiLU'(z) = s (1 + z (1 - s)) = s + w1 (1 - s)
+        const float hh = !PACKED ? (i + 1 < kRows ? before[i + 1 < kRows ? i + 1 : i][v] : h[v])
+                                 : fmaf(A, before[i][v], D[i][v] * xx);
+        oz[v] = dyv * hh * fmaf(w1, 1.0f - s, s);
       }
       G[v] = A * g;
+      renew(G[v]), renew(dk[v]), renew(db[v]);
       if (start >= 0 && a.dh0) a.dh0[size_t(start) * a.C + w.c + v] = G[v];
     }
-    store_row<V>(static_cast<T*>(a.dx) + at, ox);
-    store_row<V>(static_cast<T*>(a.ddelta) + at, od);
-    if (a.gated) store_row<V>(static_cast<T*>(a.dz) + at, oz);
+    store_row<V>(static_cast<T*>(a.dx) + at + off, ox);
+    store_row<V>(static_cast<T*>(a.ddelta) + at + off, od);
+    if (a.gated) store_row<V>(static_cast<T*>(a.dz) + at + off, oz);
   }
   __syncthreads();
 #pragma unroll
@@ -547,7 +636,7 @@ __global__ void __launch_bounds__(256) token_scan_one(TokenScan a) {
   float h[V], y[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const Gains g = gains(d.get(v) + bia.get(v));
+    const Gains g = gains((d.get(v) + bia.get(v)) * kLog2e);
     h[v] = fmaf(kap.get(v) * g.keep, h0.get(v), g.D * x.get(v));
     y[v] = h[v];
     if (a.gated) {
@@ -560,15 +649,16 @@ __global__ void __launch_bounds__(256) token_scan_one(TokenScan a) {
 }
 
 bool fits(const void* p, long long batch, long long row, int V, size_t size) {
-  return reinterpret_cast<uintptr_t>(p) % (V * size) == 0 && batch % V == 0 && row % V == 0;
+  return reinterpret_cast<uintptr_t>(p) % (V * size) == 0 && batch % V == 0 && row % V == 0 && row >= 0 && row <= 1 << 22;
 }
 bool fits(const TokenRows& t, int V, size_t size) { return !t.p || fits(t.p, t.batch, t.row, V, size); }
 
-// channels a thread takes: 4 (bf16) or 2 (float32) where every row is aligned for it, else 1
+// channels a thread takes: 4 (bf16) or 2 (float32) where every row is aligned for it and a tile's 128 rows lie within
+// 2^31 bytes, else 1
 int width(const TokenScan& a, int dtype) {
   const int V = dtype == 0 ? 2 : 4;
   const size_t size = dtype == 0 ? 4 : 2;
-  const bool ok = a.C % V == 0 && fits(a.x, V, size) && fits(a.delta, V, size) && fits(a.z, V, size) &&
+  const bool ok = a.C % V == 0 && a.C <= 1 << 22 && fits(a.x, V, size) && fits(a.delta, V, size) && fits(a.z, V, size) &&
                   fits(a.dy, V, size) && fits(a.y, 0, 0, V, size) && fits(a.dx, 0, 0, V, size) &&
                   fits(a.ddelta, 0, 0, V, size) && fits(a.dz, 0, 0, V, size) && fits(a.kept, 0, 0, V, 1);
   return ok ? V : 1;
@@ -609,13 +699,13 @@ hipError_t launch_token_scan(const TokenScan& args, int dtype, uint64_t* words, 
   return by_type(a, dtype, [&](auto t, auto vw) {
     using T = decltype(t);
     constexpr int V = decltype(vw)::value;
-    const unsigned nct = unsigned((a.C + kLanes * V - 1) / (kLanes * V)) * unsigned(a.B);
+    const unsigned grid = unsigned((a.C + kLanes * V - 1) / (kLanes * V)) * unsigned(a.B) * unsigned(n);
     if (a.offsets) {
-      if (a.kept) token_scan_fwd<T, V, true, true><<<nct * unsigned(n), 256, 0, s>>>(a, n);
-      else token_scan_fwd<T, V, true, false><<<nct * unsigned(n), 256, 0, s>>>(a, n);
+      if (a.kept) token_scan_fwd<T, V, true, true><<<grid, 256, 0, s>>>(a, n);
+      else token_scan_fwd<T, V, true, false><<<grid, 256, 0, s>>>(a, n);
     } else {
-      if (a.kept) token_scan_fwd<T, V, false, true><<<nct * unsigned(n), 256, 0, s>>>(a, n);
-      else token_scan_fwd<T, V, false, false><<<nct * unsigned(n), 256, 0, s>>>(a, n);
+      if (a.kept) token_scan_fwd<T, V, false, true><<<grid, 256, 0, s>>>(a, n);
+      else token_scan_fwd<T, V, false, false><<<grid, 256, 0, s>>>(a, n);
     }
     return hipGetLastError();
   });
