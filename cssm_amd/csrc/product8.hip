@@ -78,6 +78,11 @@ __device__ __forceinline__ void tile_of(int id, int nmt, int nnt, int& mt, int& 
   nt = in / rows;
 }
 
+template <typename O>
+struct Whole {
+  O v[16 / sizeof(O)];
+};
+
 template <int BM, int BN, int WM, int WN, typename O, bool WIDE>
 __global__ void __launch_bounds__(WM* WN * 64) product_tiles(Product8 p) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, PIECES = (BM + BN) / 8 / WAVES;
@@ -195,25 +200,49 @@ __global__ void __launch_bounds__(WM* WN * 64) product_tiles(Product8 p) {
     if (b + 1 < nkb) fetch(b + 1);
     step(b);
   }
-  const bool wide = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(O)) == 0;
+  // To memory by way of LDS, 32 rows of each wave at a time, so that whole lines are written: a lane holds 4 columns of a
+  // row, 32 lanes 32 rows.  The 16-byte pieces of a row lie at piece ^ row, which spreads both ways over the banks.
+  constexpr int LINE = BN * int(sizeof(O)) / 16, ROWS = WM * 32, HALF = LINE * ROWS;   // pieces of a row, rows and pieces of a turn
+  constexpr bool TWICE = 2 * HALF <= 2 * (BM + BN) * 8;   // room for two turns: one barrier each
+  uint4* buf = &lds[0][0];
+  const bool whole16 = p.N % (16 / int(sizeof(O))) == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  auto write_out = [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < TN; ++i)
+    for (int j = 0; j < TM; ++j) {
+      uint4* to = buf + (TWICE ? (j & 1) * HALF : 0);
+      if (j == 0 || !TWICE) __syncthreads();   // the products, or the turn before, are done with LDS
+      const int row = wave % WM * 32 + l % 32;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int n = nw + i * 32 + e * 8 + l / 32 * 4;
-      float bias[4];
+      for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) bias[v] = p.bias && n + v < p.N ? p.bias[n + v] : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+          const int col = nw - n0 + i * 32 + e * 8 + l / 32 * 4, n = n0 + col;
+          float o[4];
 #pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        const int m = mw + j * 32 + l % 32;
+          for (int v = 0; v < 4; ++v) o[v] = activate(acc[i][j][e * 4 + v] + (p.bias ? p.bias[min(n + v, p.N - 1)] : 0.0f), decltype(act)::value);
+          const int at = col * int(sizeof(O));
+          store_row<4>(reinterpret_cast<O*>(reinterpret_cast<uint8_t*>(to + row * LINE + (at / 16 ^ row % LINE)) + at % 16), o);
+        }
+      __syncthreads();   // (the turn before last has been read by then)
+      for (int k = threadIdx.x; k < HALF; k += WAVES * 64) {
+        const int r = k / LINE, c = k % LINE, m = m0 + r / 32 * (TM * 32) + j * 32 + r % 32;
+        const int n = n0 + c * (16 / int(sizeof(O)));
         if (m >= p.M || n >= p.N) continue;
-        float o[4];
+        const uint4 q = to[r * LINE + (c ^ r % LINE)];
+        O* out = static_cast<O*>(p.out) + size_t(m) * p.N + n;
+        if (whole16) {
+          *reinterpret_cast<uint4*>(out) = q;
+        } else {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = activate(acc[i][j][e * 4 + v] + bias[v], p.act);
-        store4(static_cast<O*>(p.out), size_t(m) * p.N + n, n, p.N, wide, o);
+          for (int v = 0; v < 16 / int(sizeof(O)); ++v)
+            if (n + v < p.N) out[v] = __builtin_bit_cast(Whole<O>, q).v[v];
+        }
       }
     }
+  };
+  if (p.act == 1) write_out(std::integral_constant<int, 1>());
+  else if (p.act == 2) write_out(std::integral_constant<int, 2>());
+  else write_out(std::integral_constant<int, 0>());
 }
 
 // ---- few rows: the weight streams past
