@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(WM* WN * 64) product_tiles(Product8 p) {
   int mt, nt;
   tile_of(int(blockIdx.x), (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, mt, nt);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64;
-  const int m0 = mt * BM, n0 = nt * BN, mw = m0 + wave % WM * (TM * 32), nw = n0 + wave / WM * (TN * 32);
+  const int m0 = mt * BM, n0 = nt * BN, nw = n0 + wave / WM * (TN * 32);
   const int nkb = (p.K + 127) / 128, whole = p.K / 128;
   const uint8_t* ab = p.a + size_t(m0) * p.K;
   const uint8_t* wb = p.w + size_t(n0) * p.K;
@@ -185,7 +185,6 @@ __global__ void __launch_bounds__(WM* WN * 64) product_tiles(Product8 p) {
           for (int i = 0; i < TN; ++i)
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[i], fa, acc[i][j], 0, 0, 0, ew, 0, ea[j]);
         }
-        asm volatile("" ::: "memory");   // the second half's pieces are read after: registers
       }
     }
   };
@@ -246,76 +245,85 @@ __global__ void __launch_bounds__(WM* WN * 64) product_tiles(Product8 p) {
 }
 
 // ---- few rows: the weight streams past
-// 16 columns a workgroup, the blocks of k dealt to its 4 waves, whose sums meet in LDS in order.  A wave reads 16 whole
-// lines of the weight a block, AHEAD blocks at a time.  Bound by the weight's bytes.
+// 16 TN columns a workgroup, the blocks of k dealt to its waves, whose sums meet in LDS in order.  A wave reads whole
+// lines of the weight, AHEAD blocks at a time, and the rows (few: L2 holds them) beside.  Bound by the weight's bytes; from
+// 17 rows on 32 columns a workgroup halve what the rows cost.
 
-// 32 bytes of a row at k, zeros behind K (a multiple of 16)
-__device__ __forceinline__ i32x8_t load32(const uint8_t* row, int k, int K) {
+// 32 bytes at base + offset, zeros behind the `left` that there are of the row (a multiple of 16)
+__device__ __forceinline__ i32x8_t load32(const uint8_t* base, uint32_t offset, int left) {
   uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  if (k < K) lo = *reinterpret_cast<const uint4*>(row + k);
-  if (k + 16 < K) hi = *reinterpret_cast<const uint4*>(row + k + 16);
+  if (left > 0) lo = *reinterpret_cast<const uint4*>(base + offset);
+  if (left > 16) hi = *reinterpret_cast<const uint4*>(base + offset + 16);
   return i32x8_t{int(lo.x), int(lo.y), int(lo.z), int(lo.w), int(hi.x), int(hi.y), int(hi.z), int(hi.w)};
 }
 
-template <int TM, typename O, bool WIDE>
-__global__ void __launch_bounds__(256) product_rows(Product8 p) {
-  constexpr int AHEAD = TM == 1 ? 4 : 2;
-  __shared__ float sums[4][TM][4][64];
-  const int wave = threadIdx.x / 64, l = threadIdx.x % 64, r = l % 16, kq = l / 16;
-  const int n0 = int(blockIdx.x) * 16, nkb = (p.K + 127) / 128;
-  const uint8_t* wr = p.w + size_t(min(n0 + r, p.N - 1)) * p.K;
+template <int TM, int TN, int WAVES, int AHEAD, typename O, bool WIDE>
+__global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
+  __shared__ float sums[WAVES][TN][TM][4][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64, r = l % 16, kq = l / 16;
+  const int n0 = int(blockIdx.x) * (16 * TN), nkb = (p.K + 127) / 128;
+  const uint8_t* wb = p.w + size_t(n0) * p.K;
   const uint8_t* ws = p.sw + size_t(n0 / 128) * nkb;
-  const uint8_t *ar[TM], *as[TM];
+  uint32_t wr[TN], ar[TM], as[TM];   // (at most 64 rows of at most 2^24 bytes)
+#pragma unroll
+  for (int i = 0; i < TN; ++i) wr[i] = uint32_t(min(i * 16 + r, p.N - 1 - n0)) * uint32_t(p.K) + uint32_t(kq * 32);
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
-    const int m = min(j * 16 + r, p.M - 1);
-    ar[j] = p.a + size_t(m) * p.K;
-    as[j] = p.sa + size_t(m) * nkb;
+    const uint32_t m = uint32_t(min(j * 16 + r, p.M - 1));
+    ar[j] = m * uint32_t(p.K) + uint32_t(kq * 32);
+    as[j] = m * uint32_t(nkb);
   }
-  f32x4_t acc[TM] = {};
-  for (int b0 = wave; b0 < nkb; b0 += 4 * AHEAD) {
-    i32x8_t fw[AHEAD], fa[AHEAD][TM];
+  f32x4_t acc[TN][TM] = {};
+  for (int b0 = wave; b0 < nkb; b0 += WAVES * AHEAD) {
+    i32x8_t fw[AHEAD][TN], fa[AHEAD][TM];
     int sw[AHEAD], sa[AHEAD][TM];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int b = min(b0 + 4 * u, nkb - 1);
-      fw[u] = load32(wr, b * 128 + kq * 32, p.K);
+      const int b = min(b0 + WAVES * u, nkb - 1), k = b * 128 + kq * 32;
+#pragma unroll
+      for (int i = 0; i < TN; ++i) fw[u][i] = load32(wb + size_t(b) * 128, wr[i], p.K - k);
       sw[u] = ws[b];
 #pragma unroll
-      for (int j = 0; j < TM; ++j) fa[u][j] = load32(ar[j], b * 128 + kq * 32, p.K), sa[u][j] = as[j][b];
+      for (int j = 0; j < TM; ++j) fa[u][j] = load32(p.a + size_t(b) * 128, ar[j], p.K - k), sa[u][j] = (p.sa + b)[as[j]];
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      if (b0 + 4 * u >= nkb) continue;
+      if (b0 + WAVES * u >= nkb) continue;
 #pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        if constexpr (WIDE) {
-          f32x4_t part = {};
+      for (int j = 0; j < TM; ++j)
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-            part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(fw[u][2 * s], fw[u][2 * s + 1]),
-                                                           widen(fa[u][j][2 * s], fa[u][j][2 * s + 1]), part, 0, 0, 0);
+        for (int i = 0; i < TN; ++i) {
+          if constexpr (WIDE) {
+            f32x4_t part = {};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] += __builtin_amdgcn_ldexpf(part[e], sw[u] + sa[u][j] - 254);
-        } else {
-          acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u], fa[u][j], acc[j], 0, 0, 0, sw[u], 0, sa[u][j]);
+            for (int s = 0; s < 4; ++s)
+              part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(fw[u][i][2 * s], fw[u][i][2 * s + 1]),
+                                                             widen(fa[u][j][2 * s], fa[u][j][2 * s + 1]), part, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] += __builtin_amdgcn_ldexpf(part[e], sw[u] + sa[u][j] - 254);
+          } else {
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[u][i], fa[u][j], acc[i][j], 0, 0, 0, sw[u], 0, sa[u][j]);
+          }
         }
-      }
     }
   }
 #pragma unroll
-  for (int j = 0; j < TM; ++j)
+  for (int i = 0; i < TN; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sums[wave][j][e][l] = acc[j][e];
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[wave][i][j][e][l] = acc[i][j][e];
   __syncthreads();
   const bool wide = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(O)) == 0;
-  for (int j = wave; j < TM; j += 4) {
-    const int m = j * 16 + r, n = n0 + kq * 4;
+  for (int t = wave; t < TN * TM; t += WAVES) {
+    const int i = t / TM, j = t % TM, m = j * 16 + r, n = n0 + i * 16 + kq * 4;
     if (m >= p.M || n >= p.N) continue;
     float o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float s = (sums[0][j][e][l] + sums[1][j][e][l]) + (sums[2][j][e][l] + sums[3][j][e][l]);
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) s += sums[w][i][j][e][l];
       o[e] = activate(s + (p.bias && n + e < p.N ? p.bias[n + e] : 0.0f), p.act);
     }
     store4(static_cast<O*>(p.out), size_t(m) * p.N + n, n, p.N, wide, o);
@@ -325,11 +333,10 @@ __global__ void __launch_bounds__(256) product_rows(Product8 p) {
 template <typename O, bool WIDE>
 void launch(const Product8& p, hipStream_t s) {
   const auto over = [](int n, int d) { return unsigned((n + d - 1) / d); };
-  if (p.M <= 64) {
-    const unsigned g = over(p.N, 16);
-    if (p.M <= 16) product_rows<1, O, WIDE><<<g, 256, 0, s>>>(p);
-    else if (p.M <= 32) product_rows<2, O, WIDE><<<g, 256, 0, s>>>(p);
-    else product_rows<4, O, WIDE><<<g, 256, 0, s>>>(p);
+  if (p.M <= 64 && p.K <= 1 << 24) {
+    if (p.M <= 16) product_rows<1, 1, 4, 8, O, WIDE><<<over(p.N, 16), 256, 0, s>>>(p);
+    else if (p.M <= 32) product_rows<2, 2, 8, 2, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);
+    else product_rows<4, 2, 8, 2, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);
   } else if (over(p.M, 256) * over(p.N, 256) >= 192) {
     if constexpr (WIDE) product_tiles<256, 128, 4, 2, O, WIDE><<<over(p.M, 256) * over(p.N, 128), 512, 0, s>>>(p);
     else product_tiles<256, 256, 2, 4, O, WIDE><<<over(p.M, 256) * over(p.N, 256), 512, 0, s>>>(p);
