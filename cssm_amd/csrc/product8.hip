@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(WM* WN * 64) product_tiles(Product8 p) {
 // ---- few rows: the weight streams past
 // 16 TN columns a workgroup, the blocks of k dealt to its waves, whose sums meet in LDS in order.  A wave reads whole
 // lines of the weight, AHEAD blocks at a time, and the rows (few: L2 holds them) beside.  Bound by the weight's bytes; from
-// 17 rows on 32 columns a workgroup halve what the rows cost.
+// 17 rows on, and where N gives every CU a workgroup, 32 columns halve what the rows cost (16 x 8192 x 4096 11.9 -> 9.6
+// us; 16 x 1024 x 1024 the other way, 4.0 -> 7.0).
 
 // 32 bytes at base + offset, zeros behind the `left` that there are of the row (a multiple of 16)
 __device__ __forceinline__ i32x8_t load32(const uint8_t* base, uint32_t offset, int left) {
@@ -261,7 +262,9 @@ template <int TM, int TN, int WAVES, int AHEAD, typename O, bool WIDE>
 __global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
   __shared__ float sums[WAVES][TN][TM][4][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), l = threadIdx.x % 64, r = l % 16, kq = l / 16;
-  const int n0 = int(blockIdx.x) * (16 * TN), nkb = (p.K + 127) / 128;
+  const int n0 = int(blockIdx.x) * (16 * TN), m0 = int(blockIdx.y) * (16 * TM), nkb = (p.K + 127) / 128;
+  const uint8_t* ab = p.a + size_t(m0) * p.K;
+  const uint8_t* sb = p.sa + size_t(m0) * nkb;
   const uint8_t* wb = p.w + size_t(n0) * p.K;
   const uint8_t* ws = p.sw + size_t(n0 / 128) * nkb;
   uint32_t wr[TN], ar[TM], as[TM];   // (at most 64 rows of at most 2^24 bytes)
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
   for (int i = 0; i < TN; ++i) wr[i] = uint32_t(min(i * 16 + r, p.N - 1 - n0)) * uint32_t(p.K) + uint32_t(kq * 32);
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
-    const uint32_t m = uint32_t(min(j * 16 + r, p.M - 1));
+    const uint32_t m = uint32_t(min(j * 16 + r, p.M - 1 - m0));
     ar[j] = m * uint32_t(p.K) + uint32_t(kq * 32);
     as[j] = m * uint32_t(nkb);
   }
@@ -279,12 +282,13 @@ __global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
     int sw[AHEAD], sa[AHEAD][TM];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int b = min(b0 + WAVES * u, nkb - 1), k = b * 128 + kq * 32;
+      const int b = b0 + WAVES * u, k = b * 128 + kq * 32;
+      if (b >= nkb) continue;
 #pragma unroll
       for (int i = 0; i < TN; ++i) fw[u][i] = load32(wb + size_t(b) * 128, wr[i], p.K - k);
       sw[u] = ws[b];
 #pragma unroll
-      for (int j = 0; j < TM; ++j) fa[u][j] = load32(p.a + size_t(b) * 128, ar[j], p.K - k), sa[u][j] = (p.sa + b)[as[j]];
+      for (int j = 0; j < TM; ++j) fa[u][j] = load32(ab + size_t(b) * 128, ar[j], p.K - k), sa[u][j] = (sb + b)[as[j]];
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
   __syncthreads();
   const bool wide = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.out) % (4 * sizeof(O)) == 0;
   for (int t = wave; t < TN * TM; t += WAVES) {
-    const int i = t / TM, j = t % TM, m = j * 16 + r, n = n0 + i * 16 + kq * 4;
+    const int i = t / TM, j = t % TM, m = m0 + j * 16 + r, n = n0 + i * 16 + kq * 4;
     if (m >= p.M || n >= p.N) continue;
     float o[4];
 #pragma unroll
@@ -333,10 +337,12 @@ __global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
 template <typename O, bool WIDE>
 void launch(const Product8& p, hipStream_t s) {
   const auto over = [](int n, int d) { return unsigned((n + d - 1) / d); };
-  if (p.M <= 64 && p.K <= 1 << 24) {
-    if (p.M <= 16) product_rows<1, 1, 4, 8, O, WIDE><<<over(p.N, 16), 256, 0, s>>>(p);
+  // up to 128 rows this way where the tiles would leave most CUs without one (128 x 4096 x 4096, 32 tiles: 25 us)
+  if (p.K <= 1 << 24 && (p.M <= 64 || (p.M <= 128 && over(p.N, 128) < 64))) {
+    if (p.M <= 16 && p.N < 8192) product_rows<1, 1, 4, 4, O, WIDE><<<over(p.N, 16), 256, 0, s>>>(p);
+    else if (p.M <= 16) product_rows<1, 2, 8, 4, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);
     else if (p.M <= 32) product_rows<2, 2, 8, 2, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);
-    else product_rows<4, 2, 8, 2, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);
+    else product_rows<4, 2, 8, 2, O, WIDE><<<dim3(over(p.N, 32), over(p.M, 64)), 512, 0, s>>>(p);
   } else if (over(p.M, 256) * over(p.N, 256) >= 192) {
     if constexpr (WIDE) product_tiles<256, 128, 4, 2, O, WIDE><<<over(p.M, 256) * over(p.N, 128), 512, 0, s>>>(p);
     else product_tiles<256, 256, 2, 4, O, WIDE><<<over(p.M, 256) * over(p.N, 256), 512, 0, s>>>(p);
