@@ -223,10 +223,8 @@ struct Kept {
     }
   }
   __device__ __forceinline__ float get(int i, int v) const {
-    return s * (v == 0   ? __builtin_amdgcn_cvt_f32_fp8(int(q[i]), 0)
-                : v == 1 ? __builtin_amdgcn_cvt_f32_fp8(int(q[i]), 1)
-                : v == 2 ? __builtin_amdgcn_cvt_f32_fp8(int(q[i]), 2)
-                         : __builtin_amdgcn_cvt_f32_fp8(int(q[i]), 3));
+    const f32x2_t two = v < 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[i], s, false) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[i], s, true);
+    return two[v & 1];
   }
 };
 template <typename T, int V>
@@ -250,22 +248,69 @@ struct Source<T, V, true> : Kept<V> {
 
 // Keeps 8 rows x V channels in e4m3: the block's largest finite magnitude sets the power of two (16 / V lanes share a
 // block of 16 channels); a NaN or an infinite value is kept as NaN.
-template <typename T, int V>
-__device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const Raw<T, V> (&q)[kRows], const Where& w,
-                                          int limit) {
-  float top = 0.0f;   // a row or channels twice (load_rows) are of the same block
+template <int V>
+__device__ __forceinline__ float largest(const Raw<float, V> (&q)[kRows]) {
+  float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < kRows; ++i)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float m = fabsf(q[i].get(v));
-      top = fmaxf(top, m < INFINITY ? m : 0.0f);
-    }
+    for (int v = 0; v < V; ++v) top = fmaxf(top, fabsf(q[i].get(v)));   // a NaN gives way
+  return top;
+}
+template <int V>
+__device__ __forceinline__ float largest(const Raw<Bf16, V> (&q)[kRows]) {   // magnitudes order as their bits
+  if constexpr (V == 4) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t w = (k ? q[i].q.y : q[i].q.x) & 0x7fff7fffu;
+        m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, m), __builtin_bit_cast(u16x2_t, w)));
+      }
+    return __uint_as_float(max(m << 16, m & 0xffff0000u));
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) m = max(m, uint32_t(q[i].q) & 0x7fffu);
+    return __uint_as_float(m << 16);
+  }
+}
+// V values over the block's power of two, to nearest even
+template <int V>
+__device__ __forceinline__ uint32_t keep_row(const Raw<float, V>& q, float scale) {
+  s16x2_t r = {};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, q.get(0), V > 1 ? q.get(V > 1) : 0.0f, scale, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
+template <int V>
+__device__ __forceinline__ uint32_t keep_row(const Raw<Bf16, V>& q, float scale) {
+  s16x2_t r = {};
+  if constexpr (V == 4) {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, q.q.x), scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, q.q.y), scale, true);
+  } else {
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, uint32_t(q.q)), scale, false);
+  }
+  return __builtin_bit_cast(uint32_t, r);
+}
+template <typename T, int V>
+__device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const Raw<T, V> (&q)[kRows], const Where& w,
+                                          int limit) {
+  float top = largest<V>(q);   // a row or channels twice (load_rows) are of the same block
+  if (!(top < INFINITY)) {     // something is not finite: the largest of what is
+    top = 0.0f;
+    for (int i = 0; i < kRows; ++i)
+      for (int v = 0; v < V; ++v) {
+        const float m = fabsf(q[i].get(v));
+        top = fmaxf(top, m < INFINITY ? m : 0.0f);
+      }
+  }
 #pragma unroll
   for (int l = 1; l < 16 / V; l *= 2) top = fmaxf(top, __shfl_xor(top, l));
   if (w.c >= a.C || w.r >= limit) return;
   const int byte = e4m3_scale_byte(top);
-  const float inv = pow2_inv(byte);
+  const float scale = pow2_of(byte);
   const size_t pb = size_t(plane) * a.B + w.b;
   if (w.c % 16 == 0)
     a.kept_scales[(pb * ((a.T + 7) / 8) + w.r / 8) * ((a.C + 15) / 16) + w.c / 16] = uint8_t(byte);
@@ -275,10 +320,10 @@ __device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const R
   for (int i = 0; i < kRows; ++i)
     if (w.r + i < limit) {
       uint8_t* at = p + size_t(i) * a.C + off;
-      if constexpr (V == 4)
-        *reinterpret_cast<uint32_t*>(at) = pack_e4m3x4(q[i].get(0) * inv, q[i].get(1) * inv, q[i].get(2) * inv, q[i].get(3) * inv);
-      else if constexpr (V == 2) *reinterpret_cast<uint16_t*>(at) = uint16_t(pack_e4m3x2(q[i].get(0) * inv, q[i].get(1) * inv));
-      else *at = uint8_t(pack_e4m3x2(q[i].get(0) * inv, 0.0f));
+      const uint32_t k = keep_row<V>(q[i], scale);
+      if constexpr (V == 4) *reinterpret_cast<uint32_t*>(at) = k;
+      else if constexpr (V == 2) *reinterpret_cast<uint16_t*>(at) = uint16_t(k);
+      else *at = uint8_t(k);
     }
 }
 

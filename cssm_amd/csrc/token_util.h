@@ -8,6 +8,8 @@ namespace cssm {
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 
 struct Bf16 { uint16_t u; };   // storage type of a bfloat16 tensor
 struct E4m3 { uint8_t u; };    // storage type of 8-bit values, each to be multiplied by its block's power of two

@@ -33,48 +33,54 @@ class Blocks8(NamedTuple):
     scales: torch.Tensor
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    """The entry point on the current stream of ``device``, whatever the current device is."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _stream(device.index))
+def _call(dev: int, name: str, *args) -> None:
+    """The entry point on the current stream of GPU ``dev``, whatever the current device is."""
+    if dev == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(dev))
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, _stream(device.index))
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream(dev))
 
 
-def _stream(index: int) -> int:
-    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+def _stream(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
-def _check(t, name: str, shape, dtype, device) -> torch.Tensor:
-    """t, contiguous, of this shape, type and device."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+def _gpu(t, name: str) -> int:
+    """The GPU's number of a tensor on one."""
+    dev = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if dev < 0:
         raise ValueError(f"{name} must be a GPU tensor")
+    return dev
+
+
+def _check(t, name: str, shape, dtype, dev: int) -> torch.Tensor:
+    """t, contiguous, of this shape and type on this GPU."""
+    if _gpu(t, name) != dev:
+        raise ValueError(f"{name} is on {t.device}, expected GPU {dev}")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t
 
 
-def _rows(t, name: str, like: Optional[torch.Tensor], packed: bool) -> _lib.TokenRows:
+def _rows(t, name: str, like: torch.Tensor, dev: int, packed: bool) -> _lib.TokenRows:
     """cssm_token_rows of (B, T, C), or (T, C) packed rows / (B, C) tokens: any strides but the channels'."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a GPU tensor")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(like.shape)} "
-                         f"{like.dtype} on {like.device}")
-    if t.dtype not in _DTYPES:
+    if t is not like:
+        if _gpu(t, name) != dev or t.dtype is not like.dtype or t.shape != like.shape:
+            raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(like.shape)} "
+                             f"{like.dtype} on {like.device}")
+    elif t.dtype not in _DTYPES:
         raise ValueError(f"{name}: unsupported dtype {t.dtype}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} must have its channels side by side (strides {t.stride()})")
-    if t.dim() == 3:
-        return _lib.TokenRows(t.data_ptr(), t.stride(0), t.stride(1))
-    return _lib.TokenRows(t.data_ptr(), 0, t.stride(0)) if packed else _lib.TokenRows(t.data_ptr(), t.stride(0), 0)
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have its channels side by side (strides {st})")
+    if len(st) == 3:
+        return _lib.TokenRows(t.data_ptr(), st[0], st[1])
+    return _lib.TokenRows(t.data_ptr(), 0, st[0]) if packed else _lib.TokenRows(t.data_ptr(), st[0], 0)
 
 
 def _ref(rows):
@@ -86,27 +92,27 @@ def _ptr(t):
 
 
 def _sequences(x, kappa, bias, state, offsets):
-    """(B, T, C, sequences, number of offsets) of checked arguments."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise ValueError("x must be a GPU tensor")
+    """(GPU, B, T, C, sequences, number of offsets) of checked arguments."""
+    dev = _gpu(x, "x")
     if x.dim() != (3 if offsets is None else 2):
         raise ValueError(f"x has shape {tuple(x.shape)}, expected " +
                          ("(B, T, C)" if offsets is None else "(T, C) rows with offsets"))
     C = x.shape[-1]
-    _check(kappa, "kappa", (C,), torch.float32, x.device)
-    _check(bias, "bias", (C,), torch.float32, x.device)
+    _check(kappa, "kappa", (C,), torch.float32, dev)
+    _check(bias, "bias", (C,), torch.float32, dev)
     if offsets is None:
         B, T, n, nseq = x.shape[0], x.shape[1], x.shape[0], 0
     else:
-        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 1:
+        _gpu(offsets, "offsets")
+        if offsets.dim() != 1 or offsets.numel() < 1:
             raise ValueError("offsets must be a tensor of n + 1 row numbers")
-        _check(offsets, "offsets", offsets.shape, torch.int32, x.device)
+        _check(offsets, "offsets", offsets.shape, torch.int32, dev)
         B, T, n, nseq = 1, x.shape[0], offsets.numel() - 1, offsets.numel() - 1
     if max(B, T, C) > 0x7fffffff:
         raise ValueError(f"x has shape {tuple(x.shape)}: a size is over 2^31 - 1")
     if state is not None:
-        _check(state, "state", (n, C), torch.float32, x.device)
-    return B, T, C, n, nseq
+        _check(state, "state", (n, C), torch.float32, dev)
+    return dev, B, T, C, n, nseq
 
 
 def _kept_buffers(planes: int, B: int, T: int, C: int, device):
@@ -117,14 +123,14 @@ def _kept_buffers(planes: int, B: int, T: int, C: int, device):
 def scan_forward(x, delta, kappa, bias, z=None, state=None, offsets=None, out=None, keep_states=False, keep_e4m3=False):
     """:func:`token_scan` with what its adjoint needs: (y, final state, states, kept, kept scales); ``states`` (B,
     segments, C) where asked for, the last two the 8-bit checkpoint where ``keep_e4m3``, else None."""
-    B, T, C, n, nseq = _sequences(x, kappa, bias, state, offsets)
+    dev, B, T, C, n, nseq = _sequences(x, kappa, bias, state, offsets)
     packed = offsets is not None
-    rx, rd = _rows(x, "x", None, packed), _rows(delta, "delta", x, packed)
-    rz = None if z is None else _rows(z, "z", x, packed)
+    rx, rd = _rows(x, "x", x, dev, packed), _rows(delta, "delta", x, dev, packed)
+    rz = None if z is None else _rows(z, "z", x, dev, packed)
     if out is None:
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     else:
-        y = _check(out, "out", x.shape, x.dtype, x.device)
+        y = _check(out, "out", x.shape, x.dtype, dev)
     final = torch.empty((n, C), dtype=torch.float32, device=x.device)
     lib = _lib.load()
     states = kept = scales = work = None
@@ -136,7 +142,7 @@ def scan_forward(x, delta, kappa, bias, z=None, state=None, offsets=None, out=No
     if need:
         work = torch.empty(need // 8, dtype=torch.int64, device=x.device)
     if B and C:
-        _call(x.device, "cssm_token_scan", _ref(rx), _ref(rd), _ref(rz), _DTYPES[x.dtype], B, T, C, kappa.data_ptr(),
+        _call(dev, "cssm_token_scan", _ref(rx), _ref(rd), _ref(rz), _DTYPES[x.dtype], B, T, C, kappa.data_ptr(),
               bias.data_ptr(), _ptr(state), _ptr(offsets), nseq, y.data_ptr(), int(packed and out is None),
               final.data_ptr(), _ptr(states), _ptr(kept), _ptr(scales), _ptr(work), need)
     return y, final, states, kept, scales
@@ -146,17 +152,17 @@ def scan_backward(x, delta, kappa, bias, z, state, offsets, states, kept, scales
     """Adjoint of :func:`token_scan` (cssm_token_scan_bwd): (dx, ddelta, dz, dkappa, dbias, dstate); from the 8-bit
     checkpoint where ``kept`` is given (x, delta and z are then None), dz None without a gate."""
     packed = offsets is not None
-    B, T, C, n, nseq = _sequences(dy, kappa, bias, state, offsets)
-    rows = [None if t is None else _rows(t, name, dy, packed) for t, name in ((x, "x"), (delta, "delta"), (z, "z"))]
-    rdy = _rows(dy, "dy", None, packed)
+    dev, B, T, C, n, nseq = _sequences(dy, kappa, bias, state, offsets)
+    rdy = _rows(dy, "dy", dy, dev, packed)
+    rows = [None if t is None else _rows(t, name, dy, dev, packed) for t, name in ((x, "x"), (delta, "delta"), (z, "z"))]
     if dfinal is not None:
-        _check(dfinal, "dfinal", (n, C), torch.float32, dy.device)
+        _check(dfinal, "dfinal", (n, C), torch.float32, dev)
     chunks = _lib.load().cssm_token_scan_chunks(T)
-    _check(states, "states", (B, chunks, C), torch.float32, dy.device)
+    _check(states, "states", (B, chunks, C), torch.float32, dev)
     if kept is not None:
         planes = 3 if gated else 2
-        _check(kept, "kept", (planes, B, T, C), torch.uint8, dy.device)
-        _check(scales, "scales", (planes, B, -(-T // KEPT_ROWS), -(-C // KEPT_CHANNELS)), torch.uint8, dy.device)
+        _check(kept, "kept", (planes, B, T, C), torch.uint8, dev)
+        _check(scales, "scales", (planes, B, -(-T // KEPT_ROWS), -(-C // KEPT_CHANNELS)), torch.uint8, dev)
     elif x is None or delta is None or gated != (z is not None):
         raise ValueError("the adjoint needs x, delta and, with a gate, z, or the kept checkpoint")
 
@@ -168,7 +174,7 @@ def scan_backward(x, delta, kappa, bias, z, state, offsets, states, kept, scales
     need = _lib.load().cssm_token_scan_workspace_size(B, T, C, 1)
     work = torch.empty(max(1, need // 8), dtype=torch.int64, device=dy.device)
     if B and C:
-        _call(dy.device, "cssm_token_scan_bwd", _ref(rows[0]), _ref(rows[1]), _ref(rows[2]), int(gated), _ref(rdy),
+        _call(dev, "cssm_token_scan_bwd", _ref(rows[0]), _ref(rows[1]), _ref(rows[2]), int(gated), _ref(rdy),
               _DTYPES[dy.dtype], B, T, C, kappa.data_ptr(), bias.data_ptr(), _ptr(state), _ptr(offsets), nseq,
               states.data_ptr(), _ptr(kept), _ptr(scales), _ptr(dfinal), dx.data_ptr(), dd.data_ptr(), _ptr(dz),
               dk.data_ptr(), db.data_ptr(), dh0.data_ptr(), work.data_ptr(), need)
@@ -199,36 +205,36 @@ def token_scan_step(x: torch.Tensor, delta: torch.Tensor, kappa: torch.Tensor, b
                     ) -> Tuple[torch.Tensor, torch.Tensor]:
     """One token for each sequence: (y, state) from ``x``, ``delta``, ``z`` (B, C) and ``state`` (B, C) float32, which
     ``out_state=state`` updates in place; the same values as :func:`token_scan` of one row."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
-        raise ValueError("x must be a (B, C) GPU tensor")
+    dev = _gpu(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x has shape {tuple(x.shape)}, expected (B, C)")
     B, C = x.shape
-    _check(kappa, "kappa", (C,), torch.float32, x.device)
-    _check(bias, "bias", (C,), torch.float32, x.device)
-    _check(state, "state", (B, C), torch.float32, x.device)
-    rx, rd = _rows(x, "x", None, False), _rows(delta, "delta", x, False)
-    rz = None if z is None else _rows(z, "z", x, False)
+    _check(kappa, "kappa", (C,), torch.float32, dev)
+    _check(bias, "bias", (C,), torch.float32, dev)
+    _check(state, "state", (B, C), torch.float32, dev)
+    rx, rd = _rows(x, "x", x, dev, False), _rows(delta, "delta", x, dev, False)
+    rz = None if z is None else _rows(z, "z", x, dev, False)
     if out_state is None:
         out_state = torch.empty_like(state)
-    else:
-        _check(out_state, "out_state", (B, C), torch.float32, x.device)
+    elif out_state is not state:
+        _check(out_state, "out_state", (B, C), torch.float32, dev)
     y = torch.empty((B, C), dtype=x.dtype, device=x.device)
     if B and C:
-        _call(x.device, "cssm_token_scan_step", _ref(rx), _ref(rd), _ref(rz), _DTYPES[x.dtype], B, C, kappa.data_ptr(),
+        _call(dev, "cssm_token_scan_step", _ref(rx), _ref(rd), _ref(rz), _DTYPES[x.dtype], B, C, kappa.data_ptr(),
               bias.data_ptr(), state.data_ptr(), y.data_ptr(), out_state.data_ptr())
     return y, out_state
 
 
 def _norm_args(x, weight, residual):
-    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 1:
-        raise ValueError("x must be a GPU tensor")
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"unsupported dtype {x.dtype}")
-    _check(x, "x", x.shape, x.dtype, None)
+    dev = _gpu(x, "x")
+    if x.dtype not in _DTYPES or x.dim() < 1:
+        raise ValueError(f"x is {tuple(x.shape)} {x.dtype}, expected rows in float32 or bfloat16")
+    _check(x, "x", x.shape, x.dtype, dev)
     C = x.shape[-1]
-    _check(weight, "weight", (C,), torch.float32, x.device)
+    _check(weight, "weight", (C,), torch.float32, dev)
     if residual is not None:
-        _check(residual, "residual", x.shape, x.dtype, x.device)
-    return (x.numel() // C if C else 0), C
+        _check(residual, "residual", x.shape, x.dtype, dev)
+    return dev, (x.numel() // C if C else 0), C
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -236,7 +242,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     """(y, s): s = x + residual rounded to x's type (x itself without a residual), y = s / rms(s) * weight over the last
     axis, rms(s) = sqrt(mean(s^2) + eps).  ``out`` 'same': y of x's shape and type; 'e4m3': y a :class:`Blocks8` of x's
     shape, an exponent for each 128 of a row.  Not differentiable: see :func:`cssm_amd.training.rms_norm_train`."""
-    M, C = _norm_args(x, weight, residual)
+    dev, M, C = _norm_args(x, weight, residual)
     if out not in ("same", "e4m3"):
         raise ValueError(f"out={out!r}: 'same' or 'e4m3'")
     s = x if residual is None else torch.empty_like(x)
@@ -247,7 +253,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     else:
         y = torch.empty_like(x)
     if M:
-        _call(x.device, "cssm_rms_norm", x.data_ptr(), _ptr(residual), _DTYPES[x.dtype], M, C, weight.data_ptr(),
+        _call(dev, "cssm_rms_norm", x.data_ptr(), _ptr(residual), _DTYPES[x.dtype], M, C, weight.data_ptr(),
               float(eps), None if residual is None else s.data_ptr(), y.data_ptr(), _ptr(scales))
     return (y if scales is None else Blocks8(y, scales)), s
 
@@ -255,30 +261,31 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
 def rms_norm_backward(dy, ds, s, weight, eps: float):
     """(dx, dweight) of :func:`rms_norm` (cssm_rms_norm_bwd): dx is x's and the residual's gradient, ``s`` what the
     forward returned, ``ds`` its gradient or None."""
-    M, C = _norm_args(s, weight, None)
-    _check(dy, "dy", s.shape, s.dtype, s.device)
+    dev, M, C = _norm_args(s, weight, None)
+    _check(dy, "dy", s.shape, s.dtype, dev)
     if ds is not None:
-        _check(ds, "ds", s.shape, s.dtype, s.device)
+        _check(ds, "ds", s.shape, s.dtype, dev)
     dx, dw = torch.empty_like(s), torch.empty_like(weight)
     if not M:
         return dx, dw.zero_()
     need = _lib.load().cssm_rms_norm_bwd_workspace_size(M, C)
     work = torch.empty(need // 4, dtype=torch.float32, device=s.device)
-    _call(s.device, "cssm_rms_norm_bwd", dy.data_ptr(), _ptr(ds), s.data_ptr(), _DTYPES[s.dtype], M, C,
+    _call(dev, "cssm_rms_norm_bwd", dy.data_ptr(), _ptr(ds), s.data_ptr(), _DTYPES[s.dtype], M, C,
           weight.data_ptr(), float(eps), dx.data_ptr(), dw.data_ptr(), work.data_ptr(), need)
     return dx, dw
 
 
 def quantize_rows(x: torch.Tensor) -> Blocks8:
     """x (..., K) float32 or bfloat16 in 8 bits, an exponent for each 128 of a row (cssm_quantize_rows)."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() < 1 or x.dtype not in _DTYPES:
-        raise ValueError("x must be a float32 or bfloat16 GPU tensor")
-    _check(x, "x", x.shape, x.dtype, None)
+    dev = _gpu(x, "x")
+    if x.dim() < 1 or x.dtype not in _DTYPES:
+        raise ValueError(f"x is {tuple(x.shape)} {x.dtype}, expected rows in float32 or bfloat16")
+    _check(x, "x", x.shape, x.dtype, dev)
     K = x.shape[-1]
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     s = torch.empty((*x.shape[:-1], -(-K // 128)), dtype=torch.float8_e8m0fnu, device=x.device)
     if x.numel():
-        _call(x.device, "cssm_quantize_rows", x.data_ptr(), _DTYPES[x.dtype], x.numel() // K, K, q.data_ptr(),
+        _call(dev, "cssm_quantize_rows", x.data_ptr(), _DTYPES[x.dtype], x.numel() // K, K, q.data_ptr(),
               s.data_ptr())
     return Blocks8(q, s)
 
@@ -286,13 +293,14 @@ def quantize_rows(x: torch.Tensor) -> Blocks8:
 def quantize_weight(kernel: torch.Tensor) -> Blocks8:
     """A Dense kernel (K, N) float32 as :func:`scaled_matmul` reads it: (N, K) in 8 bits, an exponent for each 128 x 128
     (cssm_quantize_weight).  Laid out once for a weight that stays."""
-    if not isinstance(kernel, torch.Tensor) or kernel.dim() != 2:
-        raise ValueError("kernel must be a (K, N) tensor")
+    dev = _gpu(kernel, "kernel")
+    if kernel.dim() != 2:
+        raise ValueError(f"kernel has shape {tuple(kernel.shape)}, expected (K, N)")
     K, N = kernel.shape
-    _check(kernel, "kernel", (K, N), torch.float32, None)
+    _check(kernel, "kernel", (K, N), torch.float32, dev)
     q = torch.empty((N, K), dtype=torch.float8_e4m3fn, device=kernel.device)
     s = torch.empty((-(-N // 128), -(-K // 128)), dtype=torch.float8_e8m0fnu, device=kernel.device)
-    _call(kernel.device, "cssm_quantize_weight", kernel.data_ptr(), K, N, q.data_ptr(), s.data_ptr())
+    _call(dev, "cssm_quantize_weight", kernel.data_ptr(), K, N, q.data_ptr(), s.data_ptr())
     return Blocks8(q, s)
 
 
@@ -303,21 +311,23 @@ def scaled_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None, a
     av, sa = a
     wv, sw = w
     f8, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
-    if not isinstance(av, torch.Tensor) or not isinstance(wv, torch.Tensor) or av.dim() < 1 or wv.dim() != 2:
+    dev = _gpu(av, "a.values")
+    _gpu(wv, "w.values")
+    if av.dim() < 1 or wv.dim() != 2:
         raise ValueError("a must be (..., K) rows and w a (N, K) weight in 8 bits")
     K, N = av.shape[-1], wv.shape[0]
-    _check(av, "a.values", av.shape, f8, None)
-    _check(sa, "a.scales", (*av.shape[:-1], -(-K // 128)), e8, av.device)
-    _check(wv, "w.values", (N, K), f8, av.device)
-    _check(sw, "w.scales", (-(-N // 128), -(-K // 128)), e8, av.device)
+    _check(av, "a.values", av.shape, f8, dev)
+    _check(sa, "a.scales", (*av.shape[:-1], -(-K // 128)), e8, dev)
+    _check(wv, "w.values", (N, K), f8, dev)
+    _check(sw, "w.scales", (-(-N // 128), -(-K // 128)), e8, dev)
     if bias is not None:
-        _check(bias, "bias", (N,), torch.float32, av.device)
+        _check(bias, "bias", (N,), torch.float32, dev)
     if act not in OUTPUT_ACTS:
         raise ValueError(f"act={act!r}: one of {sorted(OUTPUT_ACTS)}")
     if out_dtype not in _DTYPES:
         raise ValueError(f"unsupported out_dtype {out_dtype}")
     out = torch.empty((*av.shape[:-1], N), dtype=out_dtype, device=av.device)
     if out.numel():
-        _call(av.device, "cssm_scaled_matmul", av.data_ptr(), sa.data_ptr(), wv.data_ptr(), sw.data_ptr(),
+        _call(dev, "cssm_scaled_matmul", av.data_ptr(), sa.data_ptr(), wv.data_ptr(), sw.data_ptr(),
               av.numel() // K, N, K, _ptr(bias), OUTPUT_ACTS[act], out.data_ptr(), _DTYPES[out_dtype])
     return out
