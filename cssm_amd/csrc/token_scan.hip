@@ -8,7 +8,7 @@
 // into tiles of 128 rows, and one pass over the data does all: a workgroup loads its tile, publishes the tile's map,
 // gathers the state before the tile from the maps of the tiles before it, and only then walks its rows from
 // registers and writes the outputs.  The adjoint does the same from the end, with the states the forward kept.
-// One tile is 128 rows x 16 V channels on 256 threads: 16 lanes side by side over channels, 16 groups of 8
+// One tile is 128 rows of 16 V or 32 V channels: LX = 16 or 32 threads side by side over channels, 16 groups of 8
 // consecutive rows, so a thread's rows stay in registers from load to store.
 // All sums and states are float32; y and the gradients are rounded once, to their type.
 #include <hip/hip_runtime.h>
@@ -23,7 +23,7 @@ namespace cssm {
 
 namespace {
 
-constexpr int kTile = kTokenTile, kRows = 8, kSubs = kTile / kRows, kLanes = 16;
+constexpr int kTile = kTokenTile, kRows = 8, kSubs = kTile / kRows;
 
 // the A of a tile's map in which a sequence starts: nothing from before comes through (not 0 times it, which
 // would let an infinite state of the sequence before leak).  A NaN that no arithmetic makes.
@@ -76,9 +76,9 @@ struct Marks {
 };
 // Offsets are compared, never used as an index, so a bad one cannot leave the tensors.  Ends in a barrier.
 __device__ __forceinline__ void find_marks(Marks& m, const int* __restrict__ off, int nseq, int r0, int limit) {
-  for (int i = threadIdx.x; i < kTile; i += 256) m.start[i] = m.end[i] = -1;
+  for (int i = threadIdx.x; i < kTile; i += blockDim.x) m.start[i] = m.end[i] = -1;
   __syncthreads();
-  for (int s = threadIdx.x; s < nseq; s += 256) {
+  for (int s = threadIdx.x; s < nseq; s += blockDim.x) {
     const int b = off[s], e = off[s + 1];
     if (e <= b || e > limit || b < 0) continue;
     if (b >= r0 && b - r0 < kTile) m.start[b - r0] = s;
@@ -95,17 +95,17 @@ struct Where {
   int ct, chunk, b, sub, c, r;   // channel tile, row tile, batch; row group, first channel, first row
   int place;                     // of the row tile on the way: chunk, or from the end
 };
-template <int V, bool REV>
+template <int LX, int V, bool REV>
 __device__ __forceinline__ Where where(const TokenScan& a, int nchunks, unsigned tile) {
   tile = __builtin_amdgcn_readfirstlane(tile);   // it came by shared memory: the same for all
-  const unsigned nct = unsigned(a.C + kLanes * V - 1) / (kLanes * V);
+  const unsigned nct = unsigned(a.C + LX * V - 1) / (LX * V);
   Where w;
   w.ct = int(tile % nct);
   w.b = int(tile / nct % unsigned(a.B));
   w.place = int(tile / nct / unsigned(a.B));
   w.chunk = REV ? nchunks - 1 - w.place : w.place;
-  w.sub = threadIdx.x / kLanes;
-  w.c = (w.ct * kLanes + int(threadIdx.x % kLanes)) * V;
+  w.sub = threadIdx.x / LX;
+  w.c = (w.ct * LX + int(threadIdx.x % LX)) * V;
   w.r = w.chunk * kTile + w.sub * kRows;
   return w;
 }
@@ -327,16 +327,16 @@ __device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const R
     }
 }
 
-template <int V>
+template <int CW>
 struct Carry {
-  Map m[kSubs][kLanes * V];
-  float in[kSubs][kLanes * V];
+  Map m[kSubs][CW];
+  float in[kSubs][CW];
 };
 
 // The 16 row groups' maps of each channel, joined in order (REV: from the last): the whole tile's map, and with WRITE
-// the value entering each group.  The threads tid < 16 V take a channel each.
-template <int V, bool REV, bool WRITE>
-__device__ __forceinline__ Map fold(Carry<V>& k, int ch, float in) {
+// the value entering each group.  A thread takes a channel.
+template <int CW, bool REV, bool WRITE>
+__device__ __forceinline__ Map fold(Carry<CW>& k, int ch, float in) {
   Map all = {1.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < kSubs; j += 8) {
@@ -359,11 +359,11 @@ __device__ __forceinline__ Map fold(Carry<V>& k, int ch, float in) {
 
 // ---- forward
 
-template <typename T, int V, bool PACKED, bool KEEP>
-__global__ void __launch_bounds__(256, KEEP ? 3 : 4) token_scan_fwd(TokenScan a, int nchunks) {
-  __shared__ Carry<V> k;
+template <typename T, int V, int LX, bool PACKED, bool KEEP>
+__global__ void __launch_bounds__(LX * kSubs, KEEP ? 3 : 4) token_scan_fwd(TokenScan a, int nchunks) {
+  __shared__ Carry<LX * V> k;
   __shared__ Marks marks;
-  const Where w = where<V, false>(a, nchunks, my_tile(a, nchunks));
+  const Where w = where<LX, V, false>(a, nchunks, my_tile(a, nchunks));
   const int limit = PACKED ? packed_limit(a.offsets, a.nseq, a.T) : a.T;
   const bool on = w.c < a.C;
   Raw<T, V> d[kRows], x[kRows], z[kRows];
@@ -397,14 +397,14 @@ __global__ void __launch_bounds__(256, KEEP ? 3 : 4) token_scan_fwd(TokenScan a,
     }
   }
 #pragma unroll
-  for (int v = 0; v < V; ++v) k.m[w.sub][int(threadIdx.x % kLanes) * V + v] = m[v];
+  for (int v = 0; v < V; ++v) k.m[w.sub][int(threadIdx.x % LX) * V + v] = m[v];
   __syncthreads();
-  const int ch = threadIdx.x, c = w.ct * kLanes * V + ch;
-  if (ch < kLanes * V && c < a.C) {
+  const int ch = threadIdx.x, c = w.ct * LX * V + ch;
+  if (ch < LX * V && c < a.C) {
     const float h0 = !PACKED && a.h0 ? a.h0[size_t(w.b) * a.C + c] : 0.0f;   // packed: the starts carry theirs
-    const float in = entering(a, w, nchunks, c, fold<V, false, false>(k, ch, 0.0f), h0);
+    const float in = entering(a, w, nchunks, c, fold<LX * V, false, false>(k, ch, 0.0f), h0);
     if (a.states) a.states[(size_t(w.b) * nchunks + w.chunk) * a.C + c] = in;
-    fold<V, false, true>(k, ch, in);
+    fold<LX * V, false, true>(k, ch, in);
     if (w.chunk == 0 && a.h_out) {   // sequences without a row end where they start
       if (PACKED) {
         for (int s = 0; s < a.nseq; ++s)
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(256, KEEP ? 3 : 4) token_scan_fwd(TokenScan a,
   __syncthreads();
   float h[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) h[v] = k.in[w.sub][int(threadIdx.x % kLanes) * V + v];
+  for (int v = 0; v < V; ++v) h[v] = k.in[w.sub][int(threadIdx.x % LX) * V + v];
   T* y = static_cast<T*>(a.y) + (size_t(w.b) * a.T + w.chunk * kTile) * a.C;
   const Off<V> off = Off<V>(w.sub * kRows) * Off<V>(a.C) + Off<V>(w.c);
 #pragma unroll
@@ -466,11 +466,11 @@ __global__ void __launch_bounds__(256, KEEP ? 3 : 4) token_scan_fwd(TokenScan a,
 
 // ---- adjoint: the tile's states again from the one before it, the gradients backwards
 
-template <typename T, int V, bool PACKED, bool KEPT>
-__global__ void __launch_bounds__(256, 2) token_scan_bwd(TokenScan a, int nchunks) {
-  __shared__ Carry<V> k, kr;
+template <typename T, int V, int LX, bool PACKED, bool KEPT>
+__global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int nchunks) {
+  __shared__ Carry<LX * V> k, kr;
   __shared__ Marks marks;
-  const Where w = where<V, true>(a, nchunks, my_tile(a, nchunks));
+  const Where w = where<LX, V, true>(a, nchunks, my_tile(a, nchunks));
   const int limit = PACKED ? packed_limit(a.offsets, a.nseq, a.T) : a.T;
   const bool on = w.c < a.C;
   Source<T, V, KEPT> d, x, z;
@@ -542,18 +542,18 @@ __global__ void __launch_bounds__(256, 2) token_scan_bwd(TokenScan a, int nchunk
   if (w.r >= limit)
 #pragma unroll
     for (int v = 0; v < V; ++v) mr[v] = {1.0f, 0.0f};
-  const int lc = int(threadIdx.x % kLanes) * V;
+  const int lc = int(threadIdx.x % LX) * V;
 #pragma unroll
   for (int v = 0; v < V; ++v) k.m[w.sub][lc + v] = m[v], kr.m[w.sub][lc + v] = mr[v];
   __syncthreads();
   {
-    const int half = threadIdx.x / 128, ch = threadIdx.x % 128, c = w.ct * kLanes * V + ch;
-    if (ch < kLanes * V && c < a.C) {
+    const int half = threadIdx.x / (LX * 8), ch = threadIdx.x % (LX * 8), c = w.ct * LX * V + ch;
+    if (ch < LX * V && c < a.C) {
       const size_t at = (size_t(w.b) * nchunks + w.chunk) * a.C + c;
       if (half == 0) {
-        fold<V, false, true>(k, ch, a.states[at]);
+        fold<LX * V, false, true>(k, ch, a.states[at]);
       } else {
-        fold<V, true, true>(kr, ch, entering(a, w, nchunks, c, fold<V, true, false>(kr, ch, 0.0f), 0.0f));
+        fold<LX * V, true, true>(kr, ch, entering(a, w, nchunks, c, fold<LX * V, true, false>(kr, ch, 0.0f), 0.0f));
       }
       if (half == 0 && w.chunk == 0 && a.dh0) {
         if (PACKED) {
@@ -630,8 +630,8 @@ __global__ void __launch_bounds__(256, 2) token_scan_bwd(TokenScan a, int nchunk
 #pragma unroll
   for (int v = 0; v < V; ++v) k.m[w.sub][lc + v] = {dk[v], db[v]};
   __syncthreads();
-  const int ch = threadIdx.x, c = w.ct * kLanes * V + ch;
-  if (ch < kLanes * V && c < a.C) {
+  const int ch = threadIdx.x, c = w.ct * LX * V + ch;
+  if (ch < LX * V && c < a.C) {
     Map sum = k.m[0][ch];
 #pragma unroll
     for (int s = 1; s < kSubs; ++s) sum.A += k.m[s][ch].A, sum.S += k.m[s][ch].S;
@@ -726,6 +726,17 @@ size_t token_scan_words(int B, int T, int C) {
   return n == 1 ? 0 : 1 + size_t(B) * size_t(C) * (n + (n + kSpan - 1) / kSpan);
 }
 
+// Threads side by side in a tile.  32 of them read 256 bytes of a row in one piece instead of 128, which the memory serves
+// faster once there is a tile for every CU: bf16, 1 x 4096 x 1024 (256 wide tiles) 22.5 -> 18.7 us, 8 x 4096 x 1024
+// (2048) 79 -> 72, 1 x 65536 x 1024 141 -> 133; with 8 x 256 x 1024 (128) it costs, 18.4 -> 19.3.  The forward that keeps
+// checkpoints (161 registers, so one workgroup of 512 threads a CU; 105 -> 111 us, 188 -> 214) and the adjoint (143 ->
+// 152, 272 -> 290) are slower with it.
+constexpr int kNarrow = 16, kWide = 32;
+constexpr unsigned kWideFrom = 256;
+static unsigned tiles(const TokenScan& a, int channels) {
+  return unsigned((a.C + channels - 1) / channels) * unsigned(a.B) * unsigned(token_scan_chunks(a.T));
+}
+
 static void clear(TokenScan& a, uint64_t* words, hipStream_t s) {
   const size_t n = token_scan_words(a.B, a.T, a.C);
   if (!n) return;
@@ -744,14 +755,22 @@ hipError_t launch_token_scan(const TokenScan& args, int dtype, uint64_t* words, 
   return by_type(a, dtype, [&](auto t, auto vw) {
     using T = decltype(t);
     constexpr int V = decltype(vw)::value;
-    const unsigned grid = unsigned((a.C + kLanes * V - 1) / (kLanes * V)) * unsigned(a.B) * unsigned(n);
-    if (a.offsets) {
-      if (a.kept) token_scan_fwd<T, V, true, true><<<grid, 256, 0, s>>>(a, n);
-      else token_scan_fwd<T, V, true, false><<<grid, 256, 0, s>>>(a, n);
-    } else {
-      if (a.kept) token_scan_fwd<T, V, false, true><<<grid, 256, 0, s>>>(a, n);
-      else token_scan_fwd<T, V, false, false><<<grid, 256, 0, s>>>(a, n);
+    const unsigned grid = tiles(a, kNarrow * V);
+    if (a.kept) {
+      if (a.offsets) token_scan_fwd<T, V, kNarrow, true, true><<<grid, kNarrow * kSubs, 0, s>>>(a, n);
+      else token_scan_fwd<T, V, kNarrow, false, true><<<grid, kNarrow * kSubs, 0, s>>>(a, n);
+      return hipGetLastError();
     }
+    if constexpr (V > 1) {
+      const unsigned wide = tiles(a, kWide * V);
+      if (wide >= kWideFrom) {
+        if (a.offsets) token_scan_fwd<T, V, kWide, true, false><<<wide, kWide * kSubs, 0, s>>>(a, n);
+        else token_scan_fwd<T, V, kWide, false, false><<<wide, kWide * kSubs, 0, s>>>(a, n);
+        return hipGetLastError();
+      }
+    }
+    if (a.offsets) token_scan_fwd<T, V, kNarrow, true, false><<<grid, kNarrow * kSubs, 0, s>>>(a, n);
+    else token_scan_fwd<T, V, kNarrow, false, false><<<grid, kNarrow * kSubs, 0, s>>>(a, n);
     return hipGetLastError();
   });
 }
@@ -762,16 +781,15 @@ hipError_t launch_token_scan_bwd(const TokenScan& args, int dtype, uint64_t* wor
   const int n = token_scan_chunks(a.T);
   return by_type(a, dtype, [&](auto t, auto vw) {
     using T = decltype(t);
-    constexpr int V = decltype(vw)::value;
-    const unsigned nct = unsigned((a.C + kLanes * V - 1) / (kLanes * V)) * unsigned(a.B);
-    auto run = [&](auto packed, auto kept) {
-      constexpr bool P = decltype(packed)::value, K = decltype(kept)::value;
-      token_scan_bwd<T, V, P, K><<<nct * unsigned(n), 256, 0, s>>>(a, n);
-    };
-    const std::true_type yes;
-    const std::false_type no;
-    if (a.offsets) a.kept ? run(yes, yes) : run(yes, no);
-    else a.kept ? run(no, yes) : run(no, no);
+    constexpr int V = decltype(vw)::value, LX = kNarrow;
+    const unsigned grid = tiles(a, LX * V);
+    if (a.offsets) {
+      if (a.kept) token_scan_bwd<T, V, LX, true, true><<<grid, LX * kSubs, 0, s>>>(a, n);
+      else token_scan_bwd<T, V, LX, true, false><<<grid, LX * kSubs, 0, s>>>(a, n);
+    } else {
+      if (a.kept) token_scan_bwd<T, V, LX, false, true><<<grid, LX * kSubs, 0, s>>>(a, n);
+      else token_scan_bwd<T, V, LX, false, false><<<grid, LX * kSubs, 0, s>>>(a, n);
+    }
     token_scan_sums<<<unsigned((a.C + 15) / 16), 1024, 0, s>>>(reinterpret_cast<const float2*>(a.parts), n * a.B, a.C,
                                                                a.dkappa, a.dbias);
     return hipGetLastError();
