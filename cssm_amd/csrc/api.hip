@@ -1207,6 +1207,9 @@ bool has(const cssm_token_rows* r) { return r && r->data; }
 
 size_t elem_size(int dtype) { return dtype == CSSM_F32 ? 4 : 2; }
 
+constexpr long long kMostGroups = (1 << 24) - 1;   // workgroups of 256 threads in a launch: fewer than 2^32 threads
+long long blocks128(long long n) { return (n + 127) / 128; }
+
 // what the forward and the adjoint check alike; 0 or the failing status
 int token_scan_check(const char* who, int dtype, int B, int T, int C, const float* kappa, const float* bias,
                      const int* offsets, int nseq) {
@@ -1214,8 +1217,8 @@ int token_scan_check(const char* who, int dtype, int B, int T, int C, const floa
   if (B < 0 || T < 0 || C < 0) return fail(CSSM_ERR_SHAPE, "%s: B=%d T=%d C=%d", who, B, T, C);
   if (offsets && (B != 1 || nseq < 0)) return fail(CSSM_ERR_SHAPE, "%s: packed rows need B = 1 (B=%d nseq=%d)", who, B, nseq);
   if (!kappa || !bias) return fail(CSSM_ERR_NULL, "%s: kappa and bias must be non-null", who);
-  // workgroups of a launch (at least 16 channels x 128 rows each)
-  if ((long long)B * cssm_token_scan_chunks(T) * ((C + 15) / 16) > 0x7fffffffLL)
+  // workgroups of a launch (at least 16 channels x 128 rows each, 256 threads: fewer than 2^32 threads)
+  if ((long long)B * cssm_token_scan_chunks(T) * ((C + 15) / 16) >= 1 << 24 || C > 1 << 25)
     return fail(CSSM_ERR_UNSUPPORTED, "%s: B=%d T=%d C=%d is too large for one launch", who, B, T, C);
   return CSSM_OK;
 }
@@ -1317,10 +1320,12 @@ int cssm_rms_norm(const void* x, const void* residual, int dtype, long long M, i
   if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
   if (M < 0 || C < 0 || M > 0x7fffffffLL) return fail(CSSM_ERR_SHAPE, "%s: M=%lld C=%d", who, M, C);
   if (M == 0 || C == 0) return ok();
+  if (M > kMostGroups) return fail(CSSM_ERR_UNSUPPORTED, "%s: M=%lld is too large for one launch", who, M);
   if (!x || !weight || !y) return fail(CSSM_ERR_NULL, "%s: x, weight and y must be non-null", who);
   if (!residual != !s_out) return fail(CSSM_ERR_NULL, "%s: residual and s_out go together", who);
   if (!(eps >= 0.0f)) return fail(CSSM_ERR_ARG, "%s: eps=%g", who, double(eps));
-  if (!aligned(x, elem_size(dtype)) || !aligned(residual, elem_size(dtype)) || !aligned(weight, 4))
+  if (!aligned(x, elem_size(dtype)) || !aligned(residual, elem_size(dtype)) || !aligned(weight, 4) ||
+      !aligned(s_out, elem_size(dtype)) || !(scales || aligned(y, elem_size(dtype))))
     return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
   cssm::RmsNorm a = {};
   a.x = x, a.res = residual, a.M = M, a.C = C, a.w = weight, a.eps = eps, a.s = s_out, a.y = y;
@@ -1336,7 +1341,9 @@ int cssm_rms_norm_bwd(const void* dy, const void* ds, const void* s, int dtype, 
                       float eps, void* dx, float* dweight, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "cssm_rms_norm_bwd";
   if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
-  if (M <= 0 || C <= 0 || M > 0x7fffffffLL) return fail(CSSM_ERR_SHAPE, "%s: M=%lld C=%d must be positive", who, M, C);
+  if (M <= 0 || C <= 0) return fail(CSSM_ERR_SHAPE, "%s: M=%lld C=%d must be positive", who, M, C);
+  if (M > kMostGroups || C > 1 << 23)
+    return fail(CSSM_ERR_UNSUPPORTED, "%s: M=%lld C=%d is too large for one launch", who, M, C);
   if (!dy || !s || !weight || !dx || !dweight)
     return fail(CSSM_ERR_NULL, "%s: dy, s, weight, dx and dweight must be non-null", who);
   if (!(eps >= 0.0f)) return fail(CSSM_ERR_ARG, "%s: eps=%g", who, double(eps));
@@ -1344,6 +1351,10 @@ int cssm_rms_norm_bwd(const void* dy, const void* ds, const void* s, int dtype, 
   if (!workspace || workspace_bytes < need)
     return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
   if (!aligned(workspace, 4)) return fail(CSSM_ERR_ALIGN, "%s: workspace must be 4-byte aligned", who);
+  for (const void* p : {dy, ds, s, (const void*)dx})
+    if (!aligned(p, elem_size(dtype))) return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
+  if (!aligned(weight, 4) || !aligned(dweight, 4))
+    return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
   cssm::RmsNorm a = {};
   a.dy = dy, a.ds = ds, a.x = s, a.M = M, a.C = C, a.w = weight, a.eps = eps, a.dx = dx, a.dw = dweight;
   a.rstds = static_cast<float*>(workspace);
@@ -1354,9 +1365,12 @@ int cssm_rms_norm_bwd(const void* dy, const void* ds, const void* s, int dtype, 
 int cssm_quantize_rows(const void* x, int dtype, long long M, int K, void* q, void* scales, void* stream) {
   const char* who = "cssm_quantize_rows";
   if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
-  if (M < 0 || K < 0 || M * ((K + 127) / 128) > 0x1ffffffffLL) return fail(CSSM_ERR_SHAPE, "%s: M=%lld K=%d", who, M, K);
+  if (M < 0 || K < 0) return fail(CSSM_ERR_SHAPE, "%s: M=%lld K=%d", who, M, K);
   if (M == 0 || K == 0) return ok();
+  if (M > 4 * kMostGroups / blocks128(K))   // a workgroup takes 4 blocks of 128
+    return fail(CSSM_ERR_UNSUPPORTED, "%s: M=%lld K=%d is too large for one launch", who, M, K);
   if (!x || !q || !scales) return fail(CSSM_ERR_NULL, "%s: x, q and scales must be non-null", who);
+  if (!aligned(x, elem_size(dtype))) return fail(CSSM_ERR_ALIGN, "%s: x must be aligned to its elements", who);
   return hip_status(cssm::launch_quantize_rows(x, dtype, M, K, static_cast<uint8_t*>(q), static_cast<uint8_t*>(scales),
                                                static_cast<hipStream_t>(stream)),
                     who);
@@ -1365,7 +1379,10 @@ int cssm_quantize_rows(const void* x, int dtype, long long M, int K, void* q, vo
 int cssm_quantize_weight(const float* kernel, int K, int N, void* q, void* scales, void* stream) {
   const char* who = "cssm_quantize_weight";
   if (K <= 0 || N <= 0) return fail(CSSM_ERR_SHAPE, "%s: K=%d N=%d must be positive", who, K, N);
+  if (blocks128(K) * blocks128(N) > kMostGroups)
+    return fail(CSSM_ERR_UNSUPPORTED, "%s: K=%d N=%d is too large for one launch", who, K, N);
   if (!kernel || !q || !scales) return fail(CSSM_ERR_NULL, "%s: kernel, q and scales must be non-null", who);
+  if (!aligned(kernel, 4)) return fail(CSSM_ERR_ALIGN, "%s: kernel must be aligned to its elements", who);
   return hip_status(cssm::launch_quantize_weight(kernel, K, N, static_cast<uint8_t*>(q), static_cast<uint8_t*>(scales),
                                                  static_cast<hipStream_t>(stream)),
                     who);
@@ -1379,6 +1396,9 @@ int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const
   if (M < 0 || N <= 0 || K <= 0) return fail(CSSM_ERR_SHAPE, "%s: M=%d N=%d K=%d", who, M, N, K);
   if (K % 16) return fail(CSSM_ERR_UNSUPPORTED, "%s: K=%d is not a multiple of 16", who, K);
   if (M == 0) return ok();
+  // the kernels count bytes of 256 rows and threads of a launch in 32 bits
+  if (K >= 1 << 24 || M > 1 << 30 || N > 1 << 27 || blocks128(M) * blocks128(N) > kMostGroups)
+    return fail(CSSM_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d is too large for one launch", who, M, N, K);
   if (!a || !a_scales || !w || !w_scales || !out)
     return fail(CSSM_ERR_NULL, "%s: a, w, their scales and out must be non-null", who);
   if (!aligned(a, 16) || !aligned(w, 16)) return fail(CSSM_ERR_ALIGN, "%s: a and w must be 16-byte aligned", who);

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
   const uint8_t* sb = p.sa + size_t(m0) * nkb;
   const uint8_t* wb = p.w + size_t(n0) * p.K;
   const uint8_t* ws = p.sw + size_t(n0 / 128) * nkb;
-  uint32_t wr[TN], ar[TM], as[TM];   // (at most 64 rows of at most 2^24 bytes)
+  uint32_t wr[TN], ar[TM], as[TM];   // (at most 64 rows of fewer than 2^24 bytes)
 #pragma unroll
   for (int i = 0; i < TN; ++i) wr[i] = uint32_t(min(i * 16 + r, p.N - 1 - n0)) * uint32_t(p.K) + uint32_t(kq * 32);
 #pragma unroll
@@ -338,7 +338,7 @@ template <typename O, bool WIDE>
 void launch(const Product8& p, hipStream_t s) {
   const auto over = [](int n, int d) { return unsigned((n + d - 1) / d); };
   // up to 128 rows this way where the tiles would leave most CUs without one (128 x 4096 x 4096, 32 tiles: 25 us)
-  if (p.K <= 1 << 24 && (p.M <= 64 || (p.M <= 128 && over(p.N, 128) < 64))) {
+  if (p.M <= 64 || (p.M <= 128 && over(p.N, 128) < 64)) {
     if (p.M <= 16 && p.N < 8192) product_rows<1, 1, 4, 4, O, WIDE><<<over(p.N, 16), 256, 0, s>>>(p);
     else if (p.M <= 16) product_rows<1, 2, 8, 4, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);
     else if (p.M <= 32) product_rows<2, 2, 8, 2, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);

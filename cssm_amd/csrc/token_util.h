@@ -12,7 +12,6 @@ typedef short s16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 
 struct Bf16 { uint16_t u; };   // storage type of a bfloat16 tensor
-struct E4m3 { uint8_t u; };    // storage type of 8-bit values, each to be multiplied by its block's power of two
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const f32x2_t v = {lo, hi};
@@ -55,11 +54,6 @@ struct Raw<Bf16, 4> {
   }
 };
 template <>
-struct Raw<Bf16, 2> {
-  uint32_t q;
-  __device__ __forceinline__ float get(int i) const { return __uint_as_float(i ? (q & 0xffff0000u) : (q << 16)); }
-};
-template <>
 struct Raw<Bf16, 1> {
   uint16_t q;
   __device__ __forceinline__ float get(int) const { return __uint_as_float(uint32_t(q) << 16); }
@@ -83,7 +77,6 @@ __device__ __forceinline__ void store_row(Bf16* p, const float* v) {
     *reinterpret_cast<uint4*>(p) =
         make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
   else if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-  else if constexpr (V == 2) *reinterpret_cast<uint32_t*>(p) = pack_bf16(v[0], v[1]);
   else p->u = uint16_t(pack_bf16(v[0], 0.0f) & 0xffffu);
 }
 

@@ -986,7 +986,8 @@ int cssm_quantize_weight(const float* kernel, int K, int N, void* q, void* scale
  *   w, w_scales  (N, K) e4m3 and (ceil(N / 128), ceil(K / 128)) exponents
  *   bias         (N) float32 or NULL; act 0 none, 1 gelu (tanh form), 2 silu
  *   out          (M, N) of out_dtype
- * K a multiple of 16 (CSSM_ERR_UNSUPPORTED otherwise), a and w 16-byte aligned.
+ * K a multiple of 16 below 2^24, M to 2^30 and N to 2^27 (CSSM_ERR_UNSUPPORTED otherwise), a and w 16-byte aligned.
+ * An exponent byte b stands for 2^(b - 127), b in 1..254; the quantizers write 1..247.
  */
 int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const void* w_scales, int M, int N, int K,
                        const float* bias, int act, void* out, int out_dtype, void* stream);

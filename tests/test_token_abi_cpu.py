@@ -127,3 +127,33 @@ def test_quantize_and_product(lib):
     fails(fn, args, -5, w=P + 8)
     fails(fn, args, -5, out=P + 1)
     assert fn(*dict(args, M=0).values()) == 0
+
+
+def test_too_large_for_one_launch(lib):
+    """sizes whose launch would pass 2^32 threads, or 32-bit byte offsets"""
+    scan = dict(x=R, delta=R, z=R, dtype=0, B=1 << 24, T=1, C=1, kappa=P, bias=P, h0=None, offsets=None, nseq=0, y=P,
+                zero_tail=0, h_out=P, states=None, kept=None, kept_scales=None, work=None, bytes=0, stream=None)
+    fails(lib.cssm_token_scan, scan, -3)
+    fails(lib.cssm_token_scan, scan, -3, B=1, C=1 << 26)
+    step = dict(x=R, delta=R, z=None, dtype=1, B=1 << 24, C=8, kappa=P, bias=P, state=P, y=P, out=P, stream=None)
+    fails(lib.cssm_token_scan_step, step, -3)
+    M = 1 << 24
+    fails(lib.cssm_rms_norm, dict(x=P, r=None, dtype=0, M=M, C=8, w=P, eps=1e-6, s=None, y=P, sc=None, st=None), -3)
+    bwd = dict(dy=P, ds=None, s=P, dtype=0, M=M, C=8, w=P, eps=1e-6, dx=P, dw=P, work=P, bytes=1 << 50, st=None)
+    fails(lib.cssm_rms_norm_bwd, bwd, -3)
+    fails(lib.cssm_rms_norm_bwd, bwd, -3, M=4, C=1 << 24)
+    fails(lib.cssm_quantize_rows, dict(x=P, dtype=0, M=1 << 26, K=8, q=P, s=P, st=None), -3)
+    fails(lib.cssm_quantize_weight, dict(w=P, K=1 << 20, N=1 << 20, q=P, s=P, st=None), -3)
+    prod = dict(a=P, sa=P, w=P, sw=P, M=4, N=8, K=1 << 24, bias=None, act=0, out=P, dtype=1, st=None)
+    fails(lib.cssm_scaled_matmul, prod, -3)
+    fails(lib.cssm_scaled_matmul, prod, -3, M=1 << 30, N=1 << 20, K=16)
+    fails(lib.cssm_scaled_matmul, prod, -3, M=4, N=1 << 28, K=16)
+
+
+def test_misaligned(lib):
+    bwd = dict(dy=P, ds=None, s=P, dtype=0, M=4, C=8, w=P, eps=1e-6, dx=P, dw=P, work=P, bytes=1 << 20, st=None)
+    for name in ("dy", "s", "dx", "w", "dw"):
+        fails(lib.cssm_rms_norm_bwd, bwd, -5, **{name: P + 2})
+    norm = dict(x=P, r=P, dtype=0, M=4, C=8, w=P, eps=1e-6, s=P, y=P, sc=None, st=None)
+    for name in ("x", "r", "s", "y", "w"):
+        fails(lib.cssm_rms_norm, norm, -5, **{name: P + 2})
