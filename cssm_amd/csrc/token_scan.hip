@@ -48,7 +48,8 @@ __device__ __forceinline__ Gains gains(float v) {
   const float e = __builtin_amdgcn_exp2f(-fabsf(v)), w = 1.0f + e, r = __builtin_amdgcn_rcpf(w), s = e * r;
   const float D = fmaf(kLn2, fmaxf(v, 0.0f) + __builtin_amdgcn_logf(w), e - (w - 1.0f));
   const bool up = v > 0.0f;
-  return {D, up ? s : r, up ? r : s};
+  const float t = 1.0f - s;   // nearer to 1 / w than r where that is near 1: half a step, not w's and r's roundings
+  return {D, up ? s : t, up ? t : s};
 }
 
 // Hides from the compiler that a register holds what it held before, and fixes the point by which it is computed.  A tile's
@@ -639,12 +640,12 @@ __global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int
   }
 }
 
-// dkappa and dbias: the tiles' sums in a fixed order, in float64
 // all ones: nothing published, the counter before 0
 __global__ void __launch_bounds__(256) token_scan_clear(uint64_t* __restrict__ p, size_t n) {
   for (size_t i = size_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += size_t(gridDim.x) * 256) p[i] = kNotYet;
 }
 
+// dkappa and dbias: the tiles' sums in a fixed order, in float64
 __global__ void __launch_bounds__(1024) token_scan_sums(const float2* __restrict__ parts, int n, int C,
                                                         float* __restrict__ dkappa, float* __restrict__ dbias) {
   __shared__ double sk[64][16], sb[64][16];
