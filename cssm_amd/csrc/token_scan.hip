@@ -359,6 +359,9 @@ __device__ __forceinline__ Map fold(Carry<CW>& k, int ch, float in) {
 }
 
 // ---- forward
+// Bound by HBM and by the wait for the tiles before: bf16 with a gate 8 x 4096 x 1024 72 us (3.7 TB/s; its loads and stores
+// alone 54, without the wait 64), 1 x 65536 x 1024 134 us.  8 rows a thread keep the tile in registers between the map
+// and the walk; 16 rows would leave two workgroups a CU, too few loads in flight.
 
 template <typename T, int V, int LX, bool PACKED, bool KEEP>
 __global__ void __launch_bounds__(LX * kSubs, KEEP ? 3 : 4) token_scan_fwd(TokenScan a, int nchunks) {
@@ -466,6 +469,8 @@ __global__ void __launch_bounds__(LX * kSubs, KEEP ? 3 : 4) token_scan_fwd(Token
 }
 
 // ---- adjoint: the tile's states again from the one before it, the gradients backwards
+// 8 x 4096 x 1024 bf16 143 us (3.3 TB/s), from the 8-bit checkpoint 141; the loads and stores alone take 95 to 104.  Its
+// 245 registers leave two workgroups a CU, whose loads, arithmetic and stores overlap only with each other's.
 
 template <typename T, int V, int LX, bool PACKED, bool KEPT>
 __global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int nchunks) {
@@ -665,7 +670,8 @@ __global__ void __launch_bounds__(1024) token_scan_sums(const float2* __restrict
   if (grp == 0 && c < C) dkappa[c] = float(sk[0][l]), dbias[c] = float(sb[0][l]);
 }
 
-// ---- one token for each sequence: h = a state + D x, elementwise over (B, C)
+// ---- one token for each sequence: h = a state + D x, elementwise over (B, C).  16 x 1024 3 us, a launch's least;
+// 8192 x 4096 bf16 89 us, 6.0 TB/s
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) token_scan_one(TokenScan a) {

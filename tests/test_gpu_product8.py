@@ -133,3 +133,23 @@ def test_refusals(Q):
     a, w, b = make(Q, 4, 8, 24)
     with pytest.raises(CssmError):
         Q.scaled_matmul(a, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,K,shift", [(1, 8, 0), (3, 120, 0), (5, 136, 0), (33, 1000, 0), (7, 256, 1), (4, 300, 0)])
+def test_quantize_rows_forms(M, K, shift, dtype):
+    """8 values a thread where rows are aligned for it, 2 where they are not: the same bytes as the definition"""
+    from cssm_amd import sequence as Q
+    from tests import token_reference as R
+    gen = torch.Generator(device="cuda").manual_seed(M + K)
+    flat = torch.randn(M * K + shift, generator=gen, device="cuda") * torch.exp2(
+        torch.randint(-40, 40, (M * K + shift,), generator=gen, device="cuda").float())
+    x = flat.to(dtype)[shift:].view(M, K)
+    if K > 100:
+        x[0, 3], x[-1, K - 1] = float("inf"), float("nan")
+    q = Q.quantize_rows(x)
+    want, e = R.e4m3_blocks(x.double().cpu(), 1, 128)
+    got_e = q.scales.view(torch.uint8).cpu().double() - 127
+    assert torch.equal(got_e, e.reshape(got_e.shape).double())
+    got = q.values.float().double().cpu() * torch.exp2(got_e).repeat_interleave(128, -1)[:, :K]
+    assert torch.equal(torch.nan_to_num(got, nan=1e300), torch.nan_to_num(want, nan=1e300))
