@@ -361,7 +361,7 @@ __device__ __forceinline__ Map fold(Carry<CW>& k, int ch, float in) {
 // ---- forward
 // Bound by HBM and by the wait for the tiles before: bf16 with a gate 8 x 4096 x 1024 72 us (3.7 TB/s; its loads and stores
 // alone 54, without the wait 64), 1 x 65536 x 1024 134 us.  8 rows a thread keep the tile in registers between the map
-// and the walk; 16 rows would leave two workgroups a CU, too few loads in flight.
+// and the walk, so every value is read once.
 
 template <typename T, int V, int LX, bool PACKED, bool KEEP>
 __global__ void __launch_bounds__(LX * kSubs, KEEP ? 3 : 4) token_scan_fwd(TokenScan a, int nchunks) {

@@ -168,3 +168,52 @@ def test_training_pass(Q, B, T, K, C, checkpoint):
     ((n6 @ k6) * p.grad.double().cpu()).sum().add((s6 * gs.double().cpu()).sum()).backward()
     for got, ref in ((x, x6), (res, r6), (w, w6), (kernel, k6)):
         assert float((got.grad.double().cpu() - ref.grad).norm() / ref.grad.norm()) <= 2.0 ** -13
+
+
+def test_two_streams_at_once(Q):
+    """Two recurrences of many tiles, and their adjoints, side by side on two streams: each as it is alone."""
+    _, r = layer(16, 16, 9)
+    sets = [(r(1, 20000, 128).bfloat16(), r(1, 20000, 128).bfloat16(), 0.9 + 0.01 * r(128), r(128) - 2,
+             r(1, 20000, 128).bfloat16()) for _ in range(2)]
+
+    def run(a):
+        x, d, k, b, z = a
+        y, h, st, _, _ = Q.scan_forward(x, d, k, b, z, None, None, keep_states=True)
+        return (y, h, *Q.scan_backward(x, d, k, b, z, None, None, st, None, None, y, None, True))
+    want = [run(a) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for a, b in zip(g, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_same_tensor_twice(Q):
+    """one tensor as x, delta and z, and as x and its own residual, with gradients that add up"""
+    from cssm_amd import training
+    L, r = layer(64, 64, 11)
+    v = r(2, 50, 64).requires_grad_()
+    g = r(2, 50, 64)
+    y, _ = training.token_scan_train(v, v, L["kappa"], L["bias"], z=v)
+    y.backward(g)
+    D = [t.detach().double().cpu() for t in (v, v, L["kappa"], L["bias"], v)]
+    w = R.scan(*D, dy=g.double().cpu())
+    err = sum(w[n + "_err"] + 4 * R.U * w[n].abs() for n in ("dx", "ddelta", "dz"))
+    assert R.off(v.grad, w["dx"] + w["ddelta"] + w["dz"], err) <= 1
+    u = r(5, 64).requires_grad_()
+    n, s = training.rms_norm_train(u, L["w"], residual=u)
+    gn, gs = r(5, 64), r(5, 64)
+    torch.autograd.backward([n, s], [gn, gs])
+    u6 = u.detach().double().cpu().requires_grad_()
+    s6 = u6 + u6
+    n6 = s6 * torch.rsqrt(s6.square().mean(-1, keepdim=True) + 1e-6) * L["w"].double().cpu()
+    torch.autograd.backward([n6, s6], [gn.double().cpu(), gs.double().cpu()])
+    # 64 terms and a handful of operations, each 2^-24: under 2^-17 of the gradient's length
+    assert float((u.grad.double().cpu() - u6.grad).norm() / u6.grad.norm()) <= 2.0 ** -17
