@@ -304,7 +304,6 @@ struct TokenRows {         // rows of a (B, T, C) tensor: element strides of a b
   const void* p;
   long long batch, row;
 };
-constexpr int kTokenTile = 128;
 struct TokenScan {
   TokenRows x, delta, z, dy;
   int gated;               // z is there

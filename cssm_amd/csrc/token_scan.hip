@@ -17,13 +17,14 @@
 #include <type_traits>
 
 #include "launch.h"
+#include "token_rows.h"
 #include "token_util.h"
 
 namespace cssm {
 
 namespace {
 
-constexpr int kTile = kTokenTile, kRows = 8, kSubs = kTile / kRows;
+constexpr int kTile = kTokenTile, kRows = kTokenRows, kSubs = kTile / kRows;
 
 // the A of a tile's map in which a sequence starts: nothing from before comes through (not 0 times it, which
 // would let an infinite state of the sequence before leak).  A NaN that no arithmetic makes.
@@ -183,11 +184,8 @@ __device__ __forceinline__ float entering(const TokenScan& a, const Where& w, in
   return in;
 }
 
-// Element offset of a thread's first row and channel from its tile's, and of the rows below: where a thread takes several
-// channels (V > 1) the strides are small enough for 32 bits in bytes (width()), so that a load is a scalar base and
-// one register.
 template <int V>
-using Off = typename std::conditional<V == 1, size_t, uint32_t>::type;
+using Off = TileOff<V>;
 
 // The thread's 8 rows, every one of them: rows behind the limit (> 0) give the last one again and channels behind C
 // the last ones, which nothing uses.
@@ -195,10 +193,9 @@ template <typename T, int V>
 __device__ __forceinline__ void load_rows(Raw<T, V> (&q)[kRows], const TokenRows& t, const Where& w, int C, int limit) {
   const int r0 = min(w.chunk * kTile, limit - 1);
   const char* p = static_cast<const char*>(t.p) + ((long long)w.b * t.batch + (long long)r0 * t.row) * (long long)sizeof(T);
-  const Off<V> row = Off<V>(t.row) * Off<V>(sizeof(T)), c = Off<V>(min(w.c, C - V)) * Off<V>(sizeof(T));
-  const Off<V> at = Off<V>(w.sub * kRows) * row + c, last = Off<V>(limit - 1 - r0) * row + c;
+  const TileRows<Off<V>> at(Off<V>(t.row) * Off<V>(sizeof(T)), w.sub, Off<V>(min(w.c, C - V)) * Off<V>(sizeof(T)), limit - 1 - r0);
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) q[i] = load_raw<T, V>(reinterpret_cast<const T*>(p + min(at + Off<V>(i) * row, last)));
+  for (int i = 0; i < kRows; ++i) q[i] = load_raw<T, V>(reinterpret_cast<const T*>(p + at(i)));
 }
 
 // Rows kept in 8 bits: plane k of (planes, B, T, C) e4m3 and (planes, B, ceil(T / 8), ceil(C / 16)) exponents.  A
@@ -216,10 +213,10 @@ struct Kept {
     const int c = min(w.c, a.C - V), r0 = min(w.chunk * kTile, limit - 1);
     const uint8_t* p = a.kept + (pb * a.T + r0) * a.C;
     s = pow2_of(a.kept_scales[(pb * ((a.T + 7) / 8) + min(w.r, limit - 1) / 8) * ((a.C + 15) / 16) + c / 16]);
-    const Off<V> row = Off<V>(a.C), at = Off<V>(w.sub * kRows) * row + Off<V>(c), last = Off<V>(limit - 1 - r0) * row + Off<V>(c);
+    const TileRows<Off<V>> at(Off<V>(a.C), w.sub, Off<V>(c), limit - 1 - r0);
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const uint8_t* x = p + min(at + Off<V>(i) * row, last);
+      const uint8_t* x = p + at(i);
       q[i] = V == 4 ? *reinterpret_cast<const uint32_t*>(x) : V == 2 ? *reinterpret_cast<const uint16_t*>(x) : *x;
     }
   }
