@@ -722,7 +722,7 @@ hipError_t by_type(const TokenScan& a, int dtype, F&& f) {
 
 }  // namespace
 
-int token_scan_chunks(int T) { return T <= kTile ? 1 : (T + kTile - 1) / kTile; }
+int token_scan_chunks(int T) { return T <= kTile ? 1 : (T - 1) / kTile + 1; }
 
 // words of the maps, the spans' heads and the counter
 size_t token_scan_words(int B, int T, int C) {

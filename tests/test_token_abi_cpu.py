@@ -157,3 +157,15 @@ def test_misaligned(lib):
     norm = dict(x=P, r=P, dtype=0, M=4, C=8, w=P, eps=1e-6, s=P, y=P, sc=None, st=None)
     for name in ("x", "r", "s", "y", "w"):
         fails(lib.cssm_rms_norm, norm, -5, **{name: P + 2})
+
+
+def test_longest_sequences(lib):
+    """rows up to 2^31 - 1: the tiles are counted without overflow, and what has 2^24 of them or more is refused"""
+    most = (1 << 31) - 1
+    assert [lib.cssm_token_scan_chunks(most - k) for k in (0, 126, 127, 128)] == [1 << 24, 1 << 24, (1 << 24) - 1, (1 << 24) - 1]
+    n = 1 << 24
+    assert lib.cssm_token_scan_workspace_size(1, most, 1, 0) == 8 * (1 + n + n // 8)
+    scan = dict(x=R, delta=R, z=None, dtype=1, B=1, T=most, C=1, kappa=P, bias=P, h0=None, offsets=None, nseq=0, y=P,
+                zero_tail=0, h_out=P, states=None, kept=None, kept_scales=None, work=P, bytes=1 << 62, stream=None)
+    fails(lib.cssm_token_scan, scan, -3)
+    fails(lib.cssm_token_scan, scan, -3, T=most - 126)
