@@ -199,7 +199,13 @@ __device__ __forceinline__ void load_rows(Raw<T, V> (&q)[kRows], const TokenRows
 }
 
 // Rows kept in 8 bits: plane k of (planes, B, T, C) e4m3 and (planes, B, ceil(T / 8), ceil(C / 16)) exponents.  A
-// thread's 8 rows x V channels lie in one block, so it has one scale.
+// thread's 8 rows x V channels lie in one block, so it has one scale.  Where u = delta + bias <= -104, exp(u) is under
+// half of the least float32: D and sigmoid(u) are 0, as for delta = -inf, whatever x is.  That is how such a value is
+// kept, as -inf with x = 0, and neither counts for its block's exponent: masked rows, with the type's lowest value in
+// delta or anything finite in x, leave the rows beside them their bits.
+constexpr float kNoGain = -104.0f;
+constexpr int kPlaneX = 0, kPlaneDelta = 1, kPlaneZ = 2;
+constexpr uint32_t kNaN8 = 0x7f, kMasked8 = 0xff;   // e4m3 has two NaN; in delta's plane the negative one is -inf
 template <int V>
 struct Kept {
   uint32_t q[kRows];
@@ -224,6 +230,20 @@ struct Kept {
     const f32x2_t two = v < 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[i], s, false) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(q[i], s, true);
     return two[v & 1];
   }
+  // whether a value of the wave's is masked (uniform); a row's masked values as -inf
+  __device__ __forceinline__ bool any_masked() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) m |= (~q[i] - 0x01010101u) & q[i];
+    return __any((m & 0x80808080u) != 0);
+  }
+  __device__ __forceinline__ void mask(int i, float (&f)[V]) const {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if ((q[i] >> (8 * v) & 0xffu) == kMasked8) f[v] = -INFINITY;
+      asm volatile("" : "+v"(f[v]));   // kept behind the branch: selects in every row would cost 2 % of the adjoint
+    }
+  }
 };
 template <typename T, int V>
 struct Plain {
@@ -245,18 +265,18 @@ struct Source<T, V, true> : Kept<V> {
 };
 
 // Keeps 8 rows x V channels in e4m3: the block's largest finite magnitude sets the power of two (16 / V lanes share a
-// block of 16 channels); a NaN or an infinite value is kept as NaN.
+// block of 16 channels); a NaN or an infinite value is kept as NaN, but delta's -inf as itself.
 template <int V>
-__device__ __forceinline__ float largest(const Raw<float, V> (&q)[kRows]) {
-  float top = 0.0f;
+__device__ __forceinline__ float largest(const Raw<float, V> (&q)[kRows]) {   // magnitudes order as their bits
+  uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < kRows; ++i)
 #pragma unroll
-    for (int v = 0; v < V; ++v) top = fmaxf(top, fabsf(q[i].get(v)));   // a NaN gives way
-  return top;
+    for (int v = 0; v < V; ++v) m = max(m, __float_as_uint(q[i].get(v)) & 0x7fffffffu);
+  return __uint_as_float(m);
 }
 template <int V>
-__device__ __forceinline__ float largest(const Raw<Bf16, V> (&q)[kRows]) {   // magnitudes order as their bits
+__device__ __forceinline__ float largest(const Raw<Bf16, V> (&q)[kRows]) {
   if constexpr (V == 4) {
     uint32_t m = 0;
 #pragma unroll
@@ -292,11 +312,46 @@ __device__ __forceinline__ uint32_t keep_row(const Raw<Bf16, V>& q, float scale)
   }
   return __builtin_bit_cast(uint32_t, r);
 }
+// value v of a row as T's nearest to f
+template <int V>
+__device__ __forceinline__ void put(Raw<float, V>& r, int v, float f) {
+  if constexpr (V == 2) (v ? r.q.y : r.q.x) = f;
+  else r.q = f;
+}
+template <int V>
+__device__ __forceinline__ void put(Raw<Bf16, V>& r, int v, float f) {
+  const uint32_t b = __float_as_uint(f) >> 16;
+  if constexpr (V == 4) {
+    uint32_t& w = v < 2 ? r.q.x : r.q.y;
+    w = v & 1 ? (w & 0xffffu) | b << 16 : (w & 0xffff0000u) | b;
+  } else {
+    r.q = uint16_t(b);
+  }
+}
+// masked values (kNoGain) become delta = -inf and x = 0; an x that is not finite stays, as it made the state not a number
+// The largest magnitude of d afterwards.
 template <typename T, int V>
-__device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const Raw<T, V> (&q)[kRows], const Where& w,
-                                          int limit) {
-  float top = largest<V>(q);   // a row or channels twice (load_rows) are of the same block
-  if (!(top < INFINITY)) {     // something is not finite: the largest of what is
+__device__ __forceinline__ float hide_masked(Raw<T, V> (&d)[kRows], Raw<T, V> (&x)[kRows], const float* bias) {
+  float b[V], most = 0.0f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) b[v] = bias[v], most = fmaxf(most, fabsf(b[v]));
+  const float top = largest<V>(d);
+  if (top + most < -kNoGain) return top;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (d[i].get(v) + b[v] <= kNoGain) {
+        put(d[i], v, -INFINITY);
+        if (fabsf(x[i].get(v)) < INFINITY) put(x[i], v, 0.0f);
+      }
+  return largest<V>(d);
+}
+template <typename T, int V>
+__device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const Raw<T, V> (&q)[kRows], float top,
+                                          const Where& w, int limit) {   // top: the largest of q
+  const bool odd = !(top < INFINITY);
+  if (odd) {                   // something is not finite: the largest of what is
     top = 0.0f;
     for (int i = 0; i < kRows; ++i)
       for (int v = 0; v < V; ++v) {
@@ -318,7 +373,12 @@ __device__ __forceinline__ void keep_rows(const TokenScan& a, int plane, const R
   for (int i = 0; i < kRows; ++i)
     if (w.r + i < limit) {
       uint8_t* at = p + size_t(i) * a.C + off;
-      const uint32_t k = keep_row<V>(q[i], scale);
+      uint32_t k = keep_row<V>(q[i], scale);
+      if (plane == kPlaneDelta && odd)
+        for (int v = 0; v < V; ++v) {
+          const float f = q[i].get(v);
+          if (!(fabsf(f) < INFINITY)) k = (k & ~(0xffu << (8 * v))) | (f == -INFINITY ? kMasked8 : kNaN8) << (8 * v);
+        }
       if constexpr (V == 4) *reinterpret_cast<uint32_t*>(at) = k;
       else if constexpr (V == 2) *reinterpret_cast<uint16_t*>(at) = uint16_t(k);
       else *at = uint8_t(k);
@@ -430,9 +490,11 @@ __global__ void __launch_bounds__(LX * kSubs, KEEP ? 3 : 4) token_scan_fwd(Token
   }
   if (KEEP) {
     renew(x), renew(d), renew(z);
-    keep_rows<T, V>(a, 0, x, w, limit);
-    keep_rows<T, V>(a, 1, d, w, limit);
-    if (a.gated) keep_rows<T, V>(a, 2, z, w, limit);
+    // (a row or channels twice, see load_rows, are of the same block)
+    const float top = hide_masked<T, V>(d, x, a.bias + min(w.c, a.C - V));
+    keep_rows<T, V>(a, kPlaneX, x, largest<V>(x), w, limit);
+    keep_rows<T, V>(a, kPlaneDelta, d, top, w, limit);
+    if (a.gated) keep_rows<T, V>(a, kPlaneZ, z, largest<V>(z), w, limit);
   }
   __syncthreads();
   float h[V];
@@ -479,10 +541,10 @@ __global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int
   Source<T, V, KEPT> d, x, z;
   Raw<T, V> dy[kRows];
   if (limit > 0) {
-    d.load(a, a.delta, 1, w, limit);
-    x.load(a, a.x, 0, w, limit);
+    d.load(a, a.delta, kPlaneDelta, w, limit);
+    x.load(a, a.x, kPlaneX, w, limit);
     load_rows<T, V>(dy, a.dy, w, a.C, limit);
-    if (a.gated) z.load(a, a.z, 2, w, limit);
+    if (a.gated) z.load(a, a.z, kPlaneZ, w, limit);
   }
   float kap[V], bia[V];
 #pragma unroll
@@ -499,6 +561,8 @@ __global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int
   float D[kRows][V], kp[kRows][V], gt[kRows][V], sz[kRows][V];   // softplus, sigmoid(-u), sigmoid(u), sigmoid(z)
   Map m[V], mr[V];
   bool cut_fwd = false, cut_rev = false;   // packed: a sequence starts / ends in the group
+  bool masks = false;
+  if constexpr (KEPT) masks = limit > 0 && d.any_masked();
 #pragma unroll
   for (int v = 0; v < V; ++v) m[v] = mr[v] = {1.0f, 0.0f};
 #pragma unroll
@@ -509,9 +573,14 @@ __global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int
 #pragma unroll
       for (int v = 0; v < V; ++v) mr[v] = {0.0f, a.dh ? a.dh[size_t(end) * a.C + w.c + v] : 0.0f};
     }
+    float dl[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) dl[v] = d.get(i, v);
+    if constexpr (KEPT)
+      if (masks) d.mask(i, dl);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const Gains g = gains((d.get(i, v) + bia[v]) * kLog2e);
+      const Gains g = gains((dl[v] + bia[v]) * kLog2e);
       D[i][v] = g.D, kp[i][v] = g.keep, gt[i][v] = g.gate;
       const float A = kap[v] * g.keep;
       if (!PACKED || !cut_fwd) {

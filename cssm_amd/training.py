@@ -873,7 +873,9 @@ def token_scan_train(x: torch.Tensor, delta: torch.Tensor, kappa: torch.Tensor, 
 
     ``checkpoint='e4m3'`` keeps x, delta and z in 8 bits for the backward pass (a power of two for each 8 rows x 16
     channels), one byte a value in place of two or four.  The outputs are those without it; the gradients are the
-    recurrence's at the kept values, the states of each 128 rows computed again from the float32 state before them."""
+    recurrence's at the kept values, the states of each 128 rows computed again from the float32 state before them.
+    Masked rows (delta = -inf, or so low that softplus is 0 in float32) are kept as such and do not touch the values
+    beside them."""
     if checkpoint not in ("none", "e4m3"):
         raise ValueError(f"checkpoint={checkpoint!r}: 'none' or 'e4m3'")
     return _TokenScanFn.apply(_side_by_side(x), _side_by_side(delta), None if z is None else _side_by_side(z),

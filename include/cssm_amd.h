@@ -916,7 +916,9 @@ typedef struct cssm_token_rows {
  *   states       NULL, or (B, chunks, C) float32 out, chunks = cssm_token_scan_chunks(T): the state before every
  *                128th row, which the adjoint reads
  *   kept, kept_scales  NULL, or x, delta and z (if given) in 8 bits for the adjoint: (2 or 3, B, T, C) e4m3 and
- *                (2 or 3, B, ceil(T / 8), ceil(C / 16)) exponents, a block being 8 rows x 16 channels
+ *                (2 or 3, B, ceil(T / 8), ceil(C / 16)) exponents, a block being 8 rows x 16 channels.  Where delta + bias
+ *                <= -104 (softplus is 0 in float32: masked rows) delta is kept as -inf, which 0xff stands for in its
+ *                plane, and a finite x as 0, and neither counts for its block's exponent
  *   workspace    cssm_token_scan_workspace_size(B, T, C, 0) bytes, 8-byte aligned
  * The outputs do not overlap the inputs.  The results do not depend on how the work is spread: the same call gives
  * the same bits.
