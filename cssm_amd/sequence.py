@@ -329,5 +329,5 @@ def scaled_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None, a
     out = torch.empty((*av.shape[:-1], N), dtype=out_dtype, device=av.device)
     if out.numel():
         _call(dev, "cssm_scaled_matmul", av.data_ptr(), sa.data_ptr(), wv.data_ptr(), sw.data_ptr(),
-              av.numel() // K, N, K, _ptr(bias), OUTPUT_ACTS[act], out.data_ptr(), _DTYPES[out_dtype])
+              av.shape[:-1].numel(), N, K, _ptr(bias), OUTPUT_ACTS[act], out.data_ptr(), _DTYPES[out_dtype])
     return out
