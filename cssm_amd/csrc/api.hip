@@ -1208,6 +1208,7 @@ bool has(const cssm_token_rows* r) { return r && r->data; }
 size_t elem_size(int dtype) { return dtype == CSSM_F32 ? 4 : 2; }
 
 constexpr long long kMostGroups = (1 << 24) - 1;   // workgroups of 256 threads in a launch: fewer than 2^32 threads
+constexpr int kMostColumns = 0x7fffffff - 1023;    // values of a row: its end and a workgroup's step past it fit 31 bits
 long long blocks128(long long n) { return (n + 127) / 128; }
 
 // what the forward and the adjoint check alike; 0 or the failing status
@@ -1320,7 +1321,8 @@ int cssm_rms_norm(const void* x, const void* residual, int dtype, long long M, i
   if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
   if (M < 0 || C < 0 || M > 0x7fffffffLL) return fail(CSSM_ERR_SHAPE, "%s: M=%lld C=%d", who, M, C);
   if (M == 0 || C == 0) return ok();
-  if (M > kMostGroups) return fail(CSSM_ERR_UNSUPPORTED, "%s: M=%lld is too large for one launch", who, M);
+  if (M > kMostGroups || C > kMostColumns)
+    return fail(CSSM_ERR_UNSUPPORTED, "%s: M=%lld C=%d is too large for one launch", who, M, C);
   if (!x || !weight || !y) return fail(CSSM_ERR_NULL, "%s: x, weight and y must be non-null", who);
   if (!residual != !s_out) return fail(CSSM_ERR_NULL, "%s: residual and s_out go together", who);
   if (!(eps >= 0.0f)) return fail(CSSM_ERR_ARG, "%s: eps=%g", who, double(eps));
@@ -1367,7 +1369,7 @@ int cssm_quantize_rows(const void* x, int dtype, long long M, int K, void* q, vo
   if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
   if (M < 0 || K < 0) return fail(CSSM_ERR_SHAPE, "%s: M=%lld K=%d", who, M, K);
   if (M == 0 || K == 0) return ok();
-  if (M > 4 * kMostGroups / blocks128(K))   // a workgroup takes 4 blocks of 128
+  if (K > kMostColumns || M > 4 * kMostGroups / blocks128(K))   // a workgroup takes 4 blocks of 128
     return fail(CSSM_ERR_UNSUPPORTED, "%s: M=%lld K=%d is too large for one launch", who, M, K);
   if (!x || !q || !scales) return fail(CSSM_ERR_NULL, "%s: x, q and scales must be non-null", who);
   if (!aligned(x, elem_size(dtype))) return fail(CSSM_ERR_ALIGN, "%s: x must be aligned to its elements", who);

@@ -67,6 +67,12 @@ def _check(t, name: str, shape, dtype, dev: int) -> torch.Tensor:
     return t
 
 
+def _sizes(name: str, shape, *sizes: int) -> None:
+    """Refuses sizes that the C entry points' 32-bit arguments would cut."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f"{name} has shape {tuple(shape)}: a size is over 2^31 - 1")
+
+
 def _rows(t, name: str, like: torch.Tensor, dev: int, packed: bool) -> _lib.TokenRows:
     """cssm_token_rows of (B, T, C), or (T, C) packed rows / (B, C) tokens: any strides but the channels'."""
     if t is not like:
@@ -108,8 +114,7 @@ def _sequences(x, kappa, bias, state, offsets):
             raise ValueError("offsets must be a tensor of n + 1 row numbers")
         _check(offsets, "offsets", offsets.shape, torch.int32, dev)
         B, T, n, nseq = 1, x.shape[0], offsets.numel() - 1, offsets.numel() - 1
-    if max(B, T, C) > 0x7fffffff:
-        raise ValueError(f"x has shape {tuple(x.shape)}: a size is over 2^31 - 1")
+    _sizes("x", x.shape, B, T, C, n)
     if state is not None:
         _check(state, "state", (n, C), torch.float32, dev)
     return dev, B, T, C, n, nseq
@@ -209,6 +214,7 @@ def token_scan_step(x: torch.Tensor, delta: torch.Tensor, kappa: torch.Tensor, b
     if x.dim() != 2:
         raise ValueError(f"x has shape {tuple(x.shape)}, expected (B, C)")
     B, C = x.shape
+    _sizes("x", x.shape, B, C)
     _check(kappa, "kappa", (C,), torch.float32, dev)
     _check(bias, "bias", (C,), torch.float32, dev)
     _check(state, "state", (B, C), torch.float32, dev)
@@ -231,6 +237,7 @@ def _norm_args(x, weight, residual):
         raise ValueError(f"x is {tuple(x.shape)} {x.dtype}, expected rows in float32 or bfloat16")
     _check(x, "x", x.shape, x.dtype, dev)
     C = x.shape[-1]
+    _sizes("x", x.shape, C)
     _check(weight, "weight", (C,), torch.float32, dev)
     if residual is not None:
         _check(residual, "residual", x.shape, x.dtype, dev)
@@ -282,6 +289,7 @@ def quantize_rows(x: torch.Tensor) -> Blocks8:
         raise ValueError(f"x is {tuple(x.shape)} {x.dtype}, expected rows in float32 or bfloat16")
     _check(x, "x", x.shape, x.dtype, dev)
     K = x.shape[-1]
+    _sizes("x", x.shape, K)
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     s = torch.empty((*x.shape[:-1], -(-K // 128)), dtype=torch.float8_e8m0fnu, device=x.device)
     if x.numel():
@@ -297,6 +305,7 @@ def quantize_weight(kernel: torch.Tensor) -> Blocks8:
     if kernel.dim() != 2:
         raise ValueError(f"kernel has shape {tuple(kernel.shape)}, expected (K, N)")
     K, N = kernel.shape
+    _sizes("kernel", kernel.shape, K, N)
     _check(kernel, "kernel", (K, N), torch.float32, dev)
     q = torch.empty((N, K), dtype=torch.float8_e4m3fn, device=kernel.device)
     s = torch.empty((-(-N // 128), -(-K // 128)), dtype=torch.float8_e8m0fnu, device=kernel.device)
@@ -316,6 +325,9 @@ def scaled_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None, a
     if av.dim() < 1 or wv.dim() != 2:
         raise ValueError("a must be (..., K) rows and w a (N, K) weight in 8 bits")
     K, N = av.shape[-1], wv.shape[0]
+    M = av.shape[:-1].numel()
+    _sizes("a", av.shape, M, K)
+    _sizes("w", wv.shape, N)
     _check(av, "a.values", av.shape, f8, dev)
     _check(sa, "a.scales", (*av.shape[:-1], -(-K // 128)), e8, dev)
     _check(wv, "w.values", (N, K), f8, dev)
@@ -329,5 +341,5 @@ def scaled_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None, a
     out = torch.empty((*av.shape[:-1], N), dtype=out_dtype, device=av.device)
     if out.numel():
         _call(dev, "cssm_scaled_matmul", av.data_ptr(), sa.data_ptr(), wv.data_ptr(), sw.data_ptr(),
-              av.shape[:-1].numel(), N, K, _ptr(bias), OUTPUT_ACTS[act], out.data_ptr(), _DTYPES[out_dtype])
+              M, N, K, _ptr(bias), OUTPUT_ACTS[act], out.data_ptr(), _DTYPES[out_dtype])
     return out

@@ -169,3 +169,10 @@ def test_longest_sequences(lib):
                 zero_tail=0, h_out=P, states=None, kept=None, kept_scales=None, work=P, bytes=1 << 62, stream=None)
     fails(lib.cssm_token_scan, scan, -3)
     fails(lib.cssm_token_scan, scan, -3, T=most - 126)
+
+
+def test_longest_rows(lib):
+    """row lengths whose end, rounded up to a block or a workgroup's step, passes 2^31"""
+    for n in ((1 << 31) - 1, (1 << 31) - 512):
+        fails(lib.cssm_rms_norm, dict(x=P, r=None, dtype=1, M=1, C=n, w=P, eps=1e-6, s=None, y=P, sc=None, st=None), -3)
+        fails(lib.cssm_quantize_rows, dict(x=P, dtype=1, M=1, K=n, q=P, s=P, st=None), -3)
