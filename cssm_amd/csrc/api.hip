@@ -6,6 +6,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/cssm_amd.h"
@@ -1211,6 +1212,15 @@ constexpr long long kMostGroups = (1 << 24) - 1;   // workgroups of 256 threads 
 constexpr int kMostColumns = 0x7fffffff - 1023;    // values of a row: its end and a workgroup's step past it fit 31 bits
 long long blocks128(long long n) { return (n + 127) / 128; }
 
+// pointers to rows and outputs of dtype, and to float32 or int32 values, each aligned to its elements; 0 or the status
+int token_align_check(const char* who, int dtype, std::initializer_list<const void*> typed, std::initializer_list<const void*> words) {
+  for (const void* p : typed)
+    if (!aligned(p, elem_size(dtype))) return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
+  for (const void* p : words)
+    if (!aligned(p, 4)) return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
+  return CSSM_OK;
+}
+
 // what the forward and the adjoint check alike; 0 or the failing status
 int token_scan_check(const char* who, int dtype, int B, int T, int C, const float* kappa, const float* bias,
                      const int* offsets, int nseq) {
@@ -1254,6 +1264,7 @@ int cssm_token_scan(const cssm_token_rows* x, const cssm_token_rows* delta, cons
   if (!aligned(workspace, 8)) return fail(CSSM_ERR_ALIGN, "%s: workspace must be 8-byte aligned", who);
   TokenScan a = {};
   a.x = rows_of(x), a.delta = rows_of(delta), a.z = rows_of(z);
+  if (const int st = token_align_check(who, dtype, {a.x.p, a.delta.p, a.z.p, y}, {kappa, bias, h0, offsets, h_out, states})) return st;
   a.gated = z != nullptr;
   a.kappa = kappa, a.bias = bias, a.h0 = h0, a.offsets = offsets, a.nseq = nseq, a.B = B, a.T = T, a.C = C;
   a.y = y, a.zero_tail = zero_tail, a.h_out = h_out, a.states = states;
@@ -1286,6 +1297,9 @@ int cssm_token_scan_bwd(const cssm_token_rows* x, const cssm_token_rows* delta, 
   TokenScan a = {};
   if (!kept) a.x = rows_of(x), a.delta = rows_of(delta), a.z = gated ? rows_of(z) : rows_of(nullptr);
   a.dy = rows_of(dy);
+  if (const int st = token_align_check(who, dtype, {a.x.p, a.delta.p, a.z.p, a.dy.p, dx, ddelta, gated ? dz : nullptr},
+                                       {kappa, bias, h0, offsets, states, dh, dkappa, dbias, dh0}))
+    return st;
   a.gated = gated != 0;
   a.kappa = kappa, a.bias = bias, a.h0 = h0, a.offsets = offsets, a.nseq = nseq, a.B = B, a.T = T, a.C = C;
   a.states = const_cast<float*>(states);
@@ -1308,6 +1322,7 @@ int cssm_token_scan_step(const cssm_token_rows* x, const cssm_token_rows* delta,
     return fail(CSSM_ERR_NULL, "%s: x, delta, state, y and state_out must be non-null", who);
   TokenScan a = {};
   a.x = rows_of(x), a.delta = rows_of(delta), a.z = rows_of(z);
+  if (const int st = token_align_check(who, dtype, {a.x.p, a.delta.p, a.z.p, y}, {kappa, bias, state, state_out})) return st;
   a.gated = z != nullptr;
   a.kappa = kappa, a.bias = bias, a.h0 = state, a.B = B, a.T = 1, a.C = C, a.y = y, a.h_out = state_out;
   return hip_status(cssm::launch_token_scan_step(a, dtype, static_cast<hipStream_t>(stream)), who);

@@ -176,3 +176,31 @@ def test_longest_rows(lib):
     for n in ((1 << 31) - 1, (1 << 31) - 512):
         fails(lib.cssm_rms_norm, dict(x=P, r=None, dtype=1, M=1, C=n, w=P, eps=1e-6, s=None, y=P, sc=None, st=None), -3)
         fails(lib.cssm_quantize_rows, dict(x=P, dtype=1, M=1, K=n, q=P, s=P, st=None), -3)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_scan_misaligned(lib, dtype):
+    """rows and outputs to their type's size, the float32 and offset arguments to 4 bytes"""
+    off = _lib.TokenRows(P + (2 if dtype == 0 else 1), 64, 8)
+    bad, plain = ctypes.addressof(off), P + (2 if dtype == 0 else 1)
+    scan = dict(x=R, delta=R, z=R, dtype=dtype, B=1, T=200, C=8, kappa=P, bias=P, h0=P, offsets=P, nseq=3, y=P, zero_tail=0,
+                h_out=P, states=P, kept=None, kept_scales=None, work=P, bytes=BIG, stream=None)
+    for name in ("x", "delta", "z"):
+        fails(lib.cssm_token_scan, scan, -5, **{name: bad})
+    fails(lib.cssm_token_scan, scan, -5, y=plain)
+    for name in ("kappa", "bias", "h0", "offsets", "h_out", "states"):
+        fails(lib.cssm_token_scan, scan, -5, **{name: P + 2})
+    back = dict(x=R, delta=R, z=R, gated=1, dy=R, dtype=dtype, B=1, T=200, C=8, kappa=P, bias=P, h0=P, offsets=P, nseq=3,
+                states=P, kept=None, kept_scales=None, dh=P, dx=P, dd=P, dz=P, dk=P, db=P, dh0=P, work=P, bytes=BIG, stream=None)
+    for name in ("x", "delta", "z", "dy"):
+        fails(lib.cssm_token_scan_bwd, back, -5, **{name: bad})
+    for name in ("dx", "dd", "dz"):
+        fails(lib.cssm_token_scan_bwd, back, -5, **{name: plain})
+    for name in ("kappa", "bias", "h0", "offsets", "states", "dh", "dk", "db", "dh0"):
+        fails(lib.cssm_token_scan_bwd, back, -5, **{name: P + 2})
+    step = dict(x=R, delta=R, z=R, dtype=dtype, B=2, C=8, kappa=P, bias=P, state=P, y=P, out=P, stream=None)
+    for name in ("x", "delta", "z"):
+        fails(lib.cssm_token_scan_step, step, -5, **{name: bad})
+    fails(lib.cssm_token_scan_step, step, -5, y=plain)
+    for name in ("kappa", "bias", "state", "out"):
+        fails(lib.cssm_token_scan_step, step, -5, **{name: P + 2})
