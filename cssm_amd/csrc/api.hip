@@ -1221,6 +1221,13 @@ int token_align_check(const char* who, int dtype, std::initializer_list<const vo
   return CSSM_OK;
 }
 
+// a tile's rows are counted upwards from its first (csrc/token_rows.h)
+int token_stride_check(const char* who, std::initializer_list<const cssm_token_rows*> rows) {
+  for (const cssm_token_rows* r : rows)
+    if (r && r->row_stride < 0) return fail(CSSM_ERR_ARG, "%s: row_stride=%lld", who, r->row_stride);
+  return CSSM_OK;
+}
+
 // what the forward and the adjoint check alike; 0 or the failing status
 int token_scan_check(const char* who, int dtype, int B, int T, int C, const float* kappa, const float* bias,
                      const int* offsets, int nseq) {
@@ -1258,6 +1265,7 @@ int cssm_token_scan(const cssm_token_rows* x, const cssm_token_rows* delta, cons
   if (z && !z->data && T > 0) return fail(CSSM_ERR_NULL, "%s: z rows without data", who);
   if (!kept != !kept_scales) return fail(CSSM_ERR_NULL, "%s: kept and kept_scales go together", who);
   if (kept && !states) return fail(CSSM_ERR_NULL, "%s: kept needs states", who);
+  if (const int st = token_stride_check(who, {x, delta, z})) return st;
   const size_t need = cssm_token_scan_workspace_size(B, T, C, 0);
   if (need && (!workspace || workspace_bytes < need))
     return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
@@ -1290,6 +1298,7 @@ int cssm_token_scan_bwd(const cssm_token_rows* x, const cssm_token_rows* delta, 
     if (!kept && (!has(x) || !has(delta) || (gated && !has(z))))
       return fail(CSSM_ERR_NULL, "%s: x, delta and, with a gate, z must be non-null unless kept", who);
   }
+  if (const int st = token_stride_check(who, {kept ? nullptr : x, kept ? nullptr : delta, kept || !gated ? nullptr : z, dy})) return st;
   const size_t need = cssm_token_scan_workspace_size(B, T, C, 1);
   if (!workspace || workspace_bytes < need)
     return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);

@@ -891,7 +891,7 @@ int cssm_block_residual(const void* res, int T_res, const void* y, int T_y, int 
 /* ---- token sequences: operators over (B, T, C) activations with long T.  No counterpart in the reference's default
  * path: the gated cell's recurrence (cssm.py:559-581) in real arithmetic per channel, without the transforms. */
 
-/* A (B, T, C) tensor whose channels lie side by side: element strides of a batch and of a row. */
+/* A (B, T, C) tensor whose channels lie side by side: element strides of a batch and of a row, the row's not negative. */
 typedef struct cssm_token_rows {
   const void* data;
   long long batch_stride, row_stride;

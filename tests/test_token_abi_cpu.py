@@ -204,3 +204,17 @@ def test_scan_misaligned(lib, dtype):
     fails(lib.cssm_token_scan_step, step, -5, y=plain)
     for name in ("kappa", "bias", "state", "out"):
         fails(lib.cssm_token_scan_step, step, -5, **{name: P + 2})
+
+
+def test_rows_upwards(lib):
+    """a negative row stride is refused (that of the step is not used, and rows that are not read are not looked at)"""
+    down = _lib.TokenRows(P, 64, -8)
+    bad = ctypes.addressof(down)
+    scan = dict(x=R, delta=R, z=R, dtype=0, B=1, T=200, C=8, kappa=P, bias=P, h0=P, offsets=None, nseq=0, y=P, zero_tail=0,
+                h_out=P, states=P, kept=None, kept_scales=None, work=P, bytes=BIG, stream=None)
+    for name in ("x", "delta", "z"):
+        fails(lib.cssm_token_scan, scan, -4, **{name: bad})
+    back = dict(x=R, delta=R, z=R, gated=1, dy=R, dtype=0, B=1, T=200, C=8, kappa=P, bias=P, h0=P, offsets=None, nseq=0,
+                states=P, kept=None, kept_scales=None, dh=P, dx=P, dd=P, dz=P, dk=P, db=P, dh0=P, work=P, bytes=BIG, stream=None)
+    for name in ("x", "delta", "z", "dy"):
+        fails(lib.cssm_token_scan_bwd, back, -4, **{name: bad})
