@@ -63,10 +63,12 @@ __device__ __forceinline__ void store4(O* out, size_t at, int n, int N, bool wid
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-// 16 bytes a lane from base + offset to LDS at `to` + 16 lane (to: the same for the wave).  No register is written; the
-// wait is wait_copies().
+// 16 bytes a lane from base + offset to LDS at `to` + 16 lane (to: the same for the wave).  No vector register is written;
+// the wait is wait_copies().  The place goes by way of m0, which a clobber list cannot name: it is handed back as it was.
 __device__ __forceinline__ void copy_to_lds(const uint8_t* base, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+  uint32_t was;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+               : "=&s"(was) : "s"(to), "v"(offset), "s"(base) : "memory");
 }
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
