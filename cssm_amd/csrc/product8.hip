@@ -57,9 +57,11 @@ __device__ __forceinline__ void store4(O* out, size_t at, int n, int N, bool wid
 // stored at piece ^ (row % 8), so that the 8 lanes that LDS serves at once, 8 rows at the same piece, meet 8 different
 // bank groups.  256 x 256 on 8 waves (128 x 64 each): 192 KB of LDS reads a step against 2061 cycles of products, 75 % of
 // what LDS gives; a smaller tile's waves would wait for LDS instead.
-// Bound by the matrix cores where the tiles fill the chip: 8192 x 8192 x 4096 to bf16 264 us, 2.08 PFLOP/s; to float32
-// 600 us, 0.92 (the bf16 instruction has half the 8-bit one's rate, and the widening).  128 x 128 tiles where the large ones
-// would leave a quarter of the CUs without one.
+// Bound by the matrix cores where the tiles fill the chip: 8192 x 8192 x 4096 to bf16 277 us, 1.98 PFLOP/s (the median of 100
+// in a row; 270 to 310 with other pauses between them, as the clock goes); to float32 630 us, 0.87 (the bf16 instruction
+// has half the 8-bit one's rate, and every row fragment is widened for each of the wave's two column tiles).  128 x 128 tiles
+// where the large ones would leave a quarter of the CUs without one; they do not split K, so that few of them cannot fill the
+// chip: 256 x 4096 x 4096 28 us, 1024 x 4096 x 4096 33.
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -252,7 +254,8 @@ __global__ void __launch_bounds__(WM* WN * 64) product_tiles(Product8 p) {
 // 16 TN columns a workgroup, the blocks of k dealt to its waves, whose sums meet in LDS in order.  A wave reads whole
 // lines of the weight, AHEAD blocks at a time, and the rows (few: L2 holds them) beside.  Bound by the weight's bytes; from
 // 17 rows on, and where N gives every CU a workgroup, 32 columns halve what the rows cost (16 x 8192 x 4096 11.9 -> 9.6
-// us; 16 x 1024 x 1024 the other way, 4.0 -> 7.0).
+// us on the same operands each time, 11 on others in turn; 16 x 1024 x 1024 the other way, 4.0 -> 7.0).  Each workgroup reads
+// all rows again, which counts from 32 rows on: 32 x 8192 x 4096 13.6 us, 64 x 8192 x 4096 20.
 
 // 32 bytes at base + offset, zeros behind the `left` that there are of the row (a multiple of 16)
 __device__ __forceinline__ i32x8_t load32(const uint8_t* base, uint32_t offset, int left) {
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(WAVES * 64) product_rows(Product8 p) {
 template <typename O, bool WIDE>
 void launch(const Product8& p, hipStream_t s) {
   const auto over = [](int n, int d) { return unsigned((n + d - 1) / d); };
-  // up to 128 rows this way where the tiles would leave most CUs without one (128 x 4096 x 4096, 32 tiles: 25 us)
+  // up to 128 rows this way where the tiles would leave most CUs without one (128 x 4096 x 4096, 32 tiles: 25 us, this way 19)
   if (p.M <= 64 || (p.M <= 128 && over(p.N, 128) < 64)) {
     if (p.M <= 16 && p.N < 8192) product_rows<1, 1, 4, 4, O, WIDE><<<over(p.N, 16), 256, 0, s>>>(p);
     else if (p.M <= 16) product_rows<1, 2, 8, 4, O, WIDE><<<over(p.N, 32), 512, 0, s>>>(p);

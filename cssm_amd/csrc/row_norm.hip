@@ -52,8 +52,8 @@ __device__ __forceinline__ float top_of(float top) {
   return top;
 }
 
-// C % V == 0, 16-byte aligned rows, C <= V NV TPR.  Bound by HBM: 16384 x 4096 bf16 with a residual, to 8 bits, 84 us,
-// 5.6 TB/s; to bf16 77 us (s and y are both 128 MB, part of which the caches hold)
+// C % V == 0, 16-byte aligned rows, C <= V NV TPR.  Bound by HBM: 16384 x 4096 bf16 with a residual, to 8 bits, 85 us,
+// 5.5 TB/s; to bf16 98 us, 5.5 TB/s
 template <typename T, int V, int NV, int TPR, bool E4M3>
 __global__ void __launch_bounds__(256) rms_norm_fwd(const T* __restrict__ x, const T* __restrict__ res, long long M,
                                                     int C, const float* __restrict__ w, float eps, T* __restrict__ s,
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) rms_norm_fwd(const T* __restrict__ x, con
 }
 
 // any C and alignment: a workgroup a row, a wave for each 128 columns, the rounded sum read again for the output.
-// Element loads: 16384 x 4095 bf16 takes 241 us where 4096 takes 77
+// Element loads: 16384 x 4095 bf16 takes 301 us where 4096 takes 98; 8192 x 8192 float32, past the registers' widths, 317
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(256) rms_norm_any(const T* __restrict__ x, const T* __restrict__ res, int C,
                                                     const float* __restrict__ w, float eps, T* __restrict__ s,
@@ -165,7 +165,8 @@ __global__ void __launch_bounds__(256) rms_norm_any(const T* __restrict__ x, con
 }
 
 // the adjoint; each workgroup walks rows row0, row0 + grid, .. and keeps its columns' sums of dw in registers.  Bound by
-// HBM: 32768 x 1024 bf16 with the stream's gradient 46 us, 5.8 TB/s, and 4 for the sums behind it
+// HBM: 32768 x 1024 bf16 with the stream's gradient, right behind the forward, 47 us, 5.7 TB/s, and 4 for the sums behind
+// it; both 62 us on tensors that no cache holds
 template <typename T, int V, int NV, int TPR>
 __global__ void __launch_bounds__(256) rms_norm_bwd(const T* __restrict__ dy, const T* __restrict__ ds,
                                                     const T* __restrict__ s, long long M, int C,
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(256) rms_norm_bwd(const T* __restrict__ dy, co
   }
 }
 
-// any C and alignment: ds and the rows' rstd, then dw's partial sums from both (16384 x 4095 bf16 174 us, 4096: 90)
+// any C and alignment: ds and the rows' rstd, then dw's partial sums from both (16384 x 4095 bf16 310 us, 4096: 129)
 template <typename T>
 __global__ void __launch_bounds__(256) rms_norm_bwd_any(const T* __restrict__ dy, const T* __restrict__ ds,
                                                         const T* __restrict__ s, int C, const float* __restrict__ w,
@@ -361,7 +362,7 @@ hipError_t norm_bwd(const RmsNorm& a, hipStream_t st) {
 // ---- 8-bit values of whole tensors: rows for the left side of a product, a weight for the right
 
 // (M, K) -> e4m3 and the exponent of each 128 of a row.  Bound by HBM: 16 threads a block of 128, 8 values a thread in 16-
-// or 32-byte loads, where the rows are aligned for it (K % 8 == 0): 16384 x 4096 bf16 34 us, 5.9 TB/s
+// or 32-byte loads, where the rows are aligned for it (K % 8 == 0): 16384 x 4096 bf16 41 us, 4.9 TB/s
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows8(const T* __restrict__ x, long long M, int K,
                                                       uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(256) quantize_rows8(const T* __restrict__ x, l
                                                    pack_e4m3x4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
   if (l == 0) scales[i] = uint8_t(byte);
 }
-// any K and alignment: a wave a block, 2 values a lane (16384 x 4096 bf16 this way: 113 us)
+// any K and alignment: a wave a block, 2 values a lane (16384 x 4090 bf16: 142 us)
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows(const T* __restrict__ x, long long M, int K,
                                                      uint8_t* __restrict__ q, uint8_t* __restrict__ scales) {
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(256) quantize_rows(const T* __restrict__ x, lo
 }
 
 // Dense kernel (K, N) float32 -> (N, K) e4m3 and the exponent of each 128 x 128: a workgroup a tile, in registers, turned
-// in LDS.  Done once a weight: 4096 x 8192 39 us, 4.3 TB/s
+// in LDS.  Done once a weight: 4096 x 8192 49 us, 3.4 TB/s
 __global__ void __launch_bounds__(256) quantize_weight(const float* __restrict__ w, int K, int N, uint8_t* __restrict__ q,
                                                        uint8_t* __restrict__ scales) {
   __shared__ float tops[4];

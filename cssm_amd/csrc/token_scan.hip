@@ -40,7 +40,8 @@ __device__ __forceinline__ Map then(Map first, Map next) {
 }
 __device__ __forceinline__ float apply(Map m, float h) { return is_cut(m.A) ? m.S : fmaf(m.A, h, m.S); }
 
-// D = softplus(u), keep = exp(-D) = sigmoid(-u) and gate = sigmoid(u), from v = u log2(e), each to a few ulp: with
+// D = softplus(u), keep = exp(-D) = sigmoid(-u) and gate = sigmoid(u), from v = u log2(e), each to a few ulp and |u| half
+// steps of float32 (v's rounding moves the logarithm of exp(-|u|) by that much): with
 // e = exp(-|u|) and w = 1 + e rounded, ln(w) + (e - (w - 1)) is ln(1 + e) with its relative accuracy down to e alone (what
 // w lost is at most 2^-25, next to ln(1 + e) where that is large).
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
@@ -416,9 +417,11 @@ __device__ __forceinline__ Map fold(Carry<CW>& k, int ch, float in) {
 }
 
 // ---- forward
-// Bound by HBM and by the wait for the tiles before: bf16 with a gate 8 x 4096 x 1024 72 us (3.7 TB/s; its loads and stores
-// alone 54, without the wait 64), 1 x 65536 x 1024 134 us.  8 rows a thread keep the tile in registers between the map
-// and the walk, so every value is read once.
+// Bound by HBM, then by the arithmetic between a tile's loads and its stores (about 10 of 72 us: the loads and stores alone
+// took 54) and the wait for the tiles before (8).  bf16 with a gate 8 x 4096 x 1024 76 us, 3.5 TB/s (float32 122, 4.4), 1 x
+// 65536 x 1024 137 us; with the 8-bit checkpoint 106 us.  8 rows a thread keep the tile in registers between the map and the
+// walk, so every value is read once.  Packed rows pay in every tile for its marks, each a look at all offsets, and the first
+// tile for empty sequences one by one: 16001 x 2048 in 23 sequences 83 us, in 4096 of them 710.
 
 template <typename T, int V, int LX, bool PACKED, bool KEEP>
 __global__ void __launch_bounds__(LX * kSubs, KEEP ? 3 : 4) token_scan_fwd(TokenScan a, int nchunks) {
@@ -528,8 +531,9 @@ __global__ void __launch_bounds__(LX * kSubs, KEEP ? 3 : 4) token_scan_fwd(Token
 }
 
 // ---- adjoint: the tile's states again from the one before it, the gradients backwards
-// 8 x 4096 x 1024 bf16 143 us (3.3 TB/s), from the 8-bit checkpoint 141; the loads and stores alone take 95 to 104.  Its
-// 245 registers leave two workgroups a CU, whose loads, arithmetic and stores overlap only with each other's.
+// 8 x 4096 x 1024 bf16 141 us (3.3 TB/s); from the 8-bit checkpoint, which is 3 bytes a value less to read, 140 all the same.
+// The loads and stores alone take 95 to 104.  Its 253 registers (243 from the checkpoint) leave two workgroups a CU, whose
+// loads, arithmetic and stores overlap only with each other's.
 
 template <typename T, int V, int LX, bool PACKED, bool KEPT>
 __global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int nchunks) {
@@ -737,7 +741,7 @@ __global__ void __launch_bounds__(1024) token_scan_sums(const float2* __restrict
 }
 
 // ---- one token for each sequence: h = a state + D x, elementwise over (B, C).  16 x 1024 3 us, a launch's least;
-// 8192 x 4096 bf16 89 us, 6.0 TB/s
+// 8192 x 4096 bf16 97 us, 5.5 TB/s
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) token_scan_one(TokenScan a) {
@@ -802,7 +806,7 @@ size_t token_scan_words(int B, int T, int C) {
 // Threads side by side in a tile.  32 of them read 256 bytes of a row in one piece instead of 128, which the memory serves
 // faster once there is a tile for every CU: bf16, 1 x 4096 x 1024 (256 wide tiles) 22.5 -> 18.7 us, 8 x 4096 x 1024
 // (2048) 79 -> 72, 1 x 65536 x 1024 141 -> 133; with 8 x 256 x 1024 (128) it costs, 18.4 -> 19.3.  The forward that keeps
-// checkpoints (161 registers, so one workgroup of 512 threads a CU; 105 -> 111 us, 188 -> 214) and the adjoint (143 ->
+// checkpoints (162 registers, so one workgroup of 512 threads a CU; 105 -> 111 us, 188 -> 214) and the adjoint (143 ->
 // 152, 272 -> 290) are slower with it.
 constexpr int kNarrow = 16, kWide = 32;
 constexpr unsigned kWideFrom = 256;

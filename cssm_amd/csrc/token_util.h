@@ -80,7 +80,7 @@ __device__ __forceinline__ void store_row(Bf16* p, const float* v) {
   else p->u = uint16_t(pack_bf16(v[0], 0.0f) & 0xffffu);
 }
 
-// exp(x) and ln(x) for x > 0 on the hardware's exp2 / log2 (each within an ulp or two)
+// exp(x) on the hardware's exp2: within an ulp or two, and |x| half steps for the rounding of x log2(e)
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 __device__ __forceinline__ float sigmoidf(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
 

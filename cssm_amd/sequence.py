@@ -316,7 +316,9 @@ def quantize_weight(kernel: torch.Tensor) -> Blocks8:
 def scaled_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None, act: str = "none",
                   out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """act(a W^T + bias) (..., N) of 8-bit rows ``a`` (..., K) and an 8-bit weight ``w`` (N, K), summed in float32;
-    ``act`` 'none', 'gelu' (tanh form) or 'silu', ``out_dtype`` float32 or bfloat16.  K a multiple of 16."""
+    ``act`` 'none', 'gelu' (tanh form) or 'silu', ``out_dtype`` float32 or bfloat16.  K a multiple of 16.  With a bfloat16
+    output the 8-bit matrix instruction drops what lies about 13 bits below the largest of the few products that it adds
+    at once, before they join the float32 sum; with float32 every product counts in full."""
     av, sa = a
     wv, sw = w
     f8, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
