@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(LX * kSubs, 2) token_scan_bwd(TokenScan a, int
       const float s = a.gated ? sz[i][v] : 0.0f, w1 = zz * s;
       const float g = (a.gated ? dyv * w1 : dyv) + G[v];
       ox[v] = D[i][v] * g;
-      od[v] = gt[i][v] * (g * fmaf(-A, before[i][v], xx));
+      od[v] = gt[i][v] * g * fmaf(-A, before[i][v], xx);   // (in this order a masked x, gt = 0, cannot overflow with g)
       dk[v] = fmaf(g * kp[i][v], before[i][v], dk[v]);
       db[v] += od[v];
       if (a.gated) {   // SiLU'(z) = s (1 + z (1 - s)) = s + w1 (1 - s)

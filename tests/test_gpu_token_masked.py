@@ -142,3 +142,23 @@ def test_not_a_number_is_no_mask(T, C, dtype):
     d[3, 10], x[3, 10] = -INF, INF
     _, _, g = grads(T, x, d, z, kap, bias, h0, dy, df)
     assert bool(torch.isnan(g["ddelta"][:, 10]).all()) and bool(torch.isnan(g["dstate"][:2]).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("checkpoint", ["none", "e4m3"])
+@pytest.mark.parametrize("C", [7, 32])
+def test_largest_x_under_the_mask(T, C, checkpoint, dtype):
+    """x at the type's largest value where delta masks it, with gradients above 1: as with 0 there, in every output"""
+    x, d, z, dy, kap, bias, h0, df, gen = make(2, 150, C, dtype, seed=2)
+    dy, df = 100 * dy, 100 * df
+    gone = places("rows", 2, 150, C, gen)
+    gone[:, 3:9] = True
+    d = torch.where(gone, torch.full_like(d, -INF), d)
+    got = []
+    for fill in (torch.finfo(dtype).max, 0.0):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (torch.where(gone, torch.full_like(x, fill), x), d, z, kap, bias, h0)]
+        y, final = T.token_scan_train(leaves[0], leaves[1], leaves[3], leaves[4], z=leaves[2], state=leaves[5], checkpoint=checkpoint)
+        got.append((y, final, *torch.autograd.grad((y, final), leaves, (dy, df))))
+    assert not got[0][3][gone].any()
+    for a, b in zip(*got):
+        assert bool(torch.isfinite(a).all()) and bool((a == b).all())
