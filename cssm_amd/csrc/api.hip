@@ -1438,3 +1438,81 @@ int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- gated delta rule
+
+namespace {
+
+using cssm::DeltaRule;
+
+// the arguments that every form takes; 0 or the failing status.  T = 1 without offsets for the step
+int delta_rule_args(const char* who, DeltaRule& a, const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v,
+                    int dtype, const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int T, int Hk, int Hv, int dk,
+                    int dv, float scale, const int* offsets, int nseq) {
+  if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
+  if (B < 0 || T < 0 || Hk <= 0 || Hv <= 0 || dk <= 0 || dv <= 0)
+    return fail(CSSM_ERR_SHAPE, "%s: B=%d T=%d Hk=%d Hv=%d dk=%d dv=%d", who, B, T, Hk, Hv, dk, dv);
+  if (Hv % Hk) return fail(CSSM_ERR_SHAPE, "%s: Hv=%d is not a multiple of Hk=%d", who, Hv, Hk);
+  if (offsets && (B != 1 || nseq < 1)) return fail(CSSM_ERR_SHAPE, "%s: packed rows need B = 1 and a sequence (B=%d nseq=%d)", who, B, nseq);
+  if (dk > 128 || dv > 128) return fail(CSSM_ERR_UNSUPPORTED, "%s: dk=%d and dv=%d are taken up to 128", who, dk, dv);
+  // workgroups of a launch of at most 512 threads, and slots counted in 31 bits
+  const long long n = offsets ? nseq : B, slots = offsets ? T / 32 + (long long)nseq : B * ((T + 31LL) / 32);
+  if (Hv > 65535 || n * Hv * 8 >= 1 << 23 || slots * Hv >= 1 << 23)
+    return fail(CSSM_ERR_UNSUPPORTED, "%s: B=%d T=%d nseq=%d Hv=%d is too large for one launch", who, B, T, nseq, Hv);
+  if (T > 0 && n > 0 && (!has(q) || !has(k) || !has(v) || !has(beta) || (decay && !decay->data)))
+    return fail(CSSM_ERR_NULL, "%s: q, k, v and beta must be non-null", who);
+  if (const int st = token_stride_check(who, {q, k, v, beta, decay})) return st;
+  a.q = rows_of(q), a.k = rows_of(k), a.v = rows_of(v), a.beta = rows_of(beta), a.decay = rows_of(decay);
+  a.B = B, a.T = T, a.Hk = Hk, a.Hv = Hv, a.dk = dk, a.dv = dv, a.scale = scale, a.offsets = offsets, a.nseq = nseq;
+  return token_align_check(who, dtype, {a.q.p, a.k.p, a.v.p}, {a.beta.p, a.decay.p, offsets});
+}
+
+int delta_workspace_check(const char* who, size_t need, const void* workspace, size_t bytes) {
+  if (need && (!workspace || bytes < need))
+    return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? bytes : (size_t)0);
+  return aligned(workspace, 16) ? CSSM_OK : fail(CSSM_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+}
+
+}  // namespace
+
+extern "C" {
+
+int cssm_delta_rule_segments(int B, int T, int nseq, int packed) {
+  return B <= 0 || T < 0 || nseq < 0 ? 0 : cssm::delta_rule_segments(B, T, nseq, packed != 0);
+}
+
+size_t cssm_delta_rule_workspace_size(int B, int T, int Hv, int nseq, int packed) {
+  return B <= 0 || T < 0 || Hv <= 0 || nseq < 0 ? 0 : cssm::delta_rule_workspace(B, T, Hv, nseq, packed != 0);
+}
+
+int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v, int dtype,
+                    const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int T, int Hk, int Hv, int dk, int dv,
+                    float scale, const float* h0, const int* offsets, int nseq, void* y, int zero_tail, float* h_out,
+                    float* errors, float* states, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "cssm_delta_rule";
+  DeltaRule a = {};
+  if (const int st = delta_rule_args(who, a, q, k, v, dtype, beta, decay, B, T, Hk, Hv, dk, dv, scale, offsets, nseq)) return st;
+  if (B == 0) return ok();
+  if (T > 0 && !y) return fail(CSSM_ERR_NULL, "%s: y must be non-null", who);
+  if (const int st = delta_workspace_check(who, cssm_delta_rule_workspace_size(B, T, Hv, offsets ? nseq : 0, offsets != nullptr),
+                                           workspace, workspace_bytes))
+    return st;
+  if (const int st = token_align_check(who, dtype, {y}, {h0, h_out, errors, states})) return st;
+  a.h0 = h0, a.y = y, a.zero_tail = zero_tail, a.h_out = h_out, a.errors = errors, a.states = states;
+  return hip_status(cssm::launch_delta_rule(a, dtype, workspace, static_cast<hipStream_t>(stream)), who);
+}
+
+int cssm_delta_rule_step(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v, int dtype,
+                         const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int Hk, int Hv, int dk, int dv,
+                         float scale, const float* state, void* y, float* state_out, void* stream) {
+  const char* who = "cssm_delta_rule_step";
+  DeltaRule a = {};
+  if (const int st = delta_rule_args(who, a, q, k, v, dtype, beta, decay, B, 1, Hk, Hv, dk, dv, scale, nullptr, 0)) return st;
+  if (B == 0) return ok();
+  if (!state || !y || !state_out) return fail(CSSM_ERR_NULL, "%s: state, y and state_out must be non-null", who);
+  if (const int st = token_align_check(who, dtype, {y}, {state, state_out})) return st;
+  a.h0 = state, a.y = y, a.h_out = state_out;
+  return hip_status(cssm::launch_delta_rule_step(a, dtype, static_cast<hipStream_t>(stream)), who);
+}
+
+}  // extern "C"

@@ -1,0 +1,535 @@
+// The gated delta rule over token sequences (gfx950).  For each value head, S (dk, dv) the state, a = exp(decay):
+//   e_t = v_t - a_t S_{t-1}^T k_t,  S_t = a_t S_{t-1} + k_t (beta_t e_t)^T,  y_t = scale S_t^T q_t
+// G value heads next to each other share one query and key head.
+//
+// In chunks of 32 rows, with D_ij = a_{j+1} .. a_i (i >= j), gamma_i = a_0 .. a_i and d_j = D_31,j, all as products, so
+// that no difference of large sums enters and a = 0 is just that:
+//   A_ij = D_ij k_i.k_j (i > j),  P_ij = scale D_ij q_i.k_j (i >= j),  L = (1 + A beta)^-1 A   (from the rows above, in order)
+//   R = V - gamma K S,  E = R - L beta R,  Y = scale gamma Q S + P beta E,  S <- gamma_31 S + K^T (d beta E)
+// delta_prepare computes L and P of all chunks at once; delta_walk then carries S from chunk to chunk, a wave 16 of
+// the state's columns, which lie in its registers as the result of one product and the operand of the next.
+// The state is float32 and enters its products in three bfloat16 parts (csrc/delta_rule.h); y's own products take two
+// where y is bfloat16.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "delta_rule.h"
+#include "launch.h"
+#include "token_util.h"
+
+namespace cssm {
+
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr int kPad = kChunk + 4;
+
+// the 8 values of a row from `at` on, in their parts
+template <typename T>
+__device__ __forceinline__ void load_unit(const T* row, bool live, int at, int n, bool vec, Unit (&u)[PartsOf<T>::n]) {
+  if constexpr (sizeof(T) == 2) {
+    if (vec) {
+      u[0] = __builtin_bit_cast(Unit, live && at < n ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = at + 2 * i;
+        u[0].w[i] = (live && c < n ? uint32_t(row[c].u) : 0u) | (live && c + 1 < n ? uint32_t(row[c + 1].u) << 16 : 0u);
+      }
+    }
+  } else {
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (vec) {
+        const float4 q = live && at < n ? reinterpret_cast<const float4*>(row + at)[h] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[4 * h] = q.x, v[4 * h + 1] = q.y, v[4 * h + 2] = q.z, v[4 * h + 3] = q.w;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * h + i] = live && at + 4 * h + i < n ? row[at + 4 * h + i] : 0.0f;
+      }
+    }
+    split<3>(v, u);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ f32x16_t product32(const Unit (&a)[N], const Unit (&b)[N], f32x16_t c) {
+#pragma unroll
+  for (int s = N - 1; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i <= s; ++i)
+      c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[i]), __builtin_bit_cast(bf16x8_t, b[s - i]), c, 0, 0, 0);
+  return c;
+}
+
+// parts of P: those that y's type shows
+template <typename T>
+constexpr int kPParts = sizeof(T) == 2 ? 2 : 3;
+template <typename T>
+constexpr int kUnits = (3 + kPParts<T>) * 128;   // units of L and P of one chunk and head
+
+// One wave for a chunk of one key head: K K^T and Q K^T, then for two value heads at a time, one in each half of the
+// wave with a column of the chunk's 32 x 32 a lane, their decays, L row by row, and both written as first operands
+// (TURNED: their transposes, which the adjoint takes).
+template <typename T, bool TURNED>
+__global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
+  __shared__ float s_kk[kChunk * 33], s_qk[kChunk * 33];
+  __shared__ __attribute__((aligned(16))) float s_m[2][kChunk * kPad];
+  __shared__ float s_alpha[2][kChunk], s_beta[2][kChunk];
+  const int lane = threadIdx.x, j = lane % 32, half = lane / 32, hk = blockIdx.y, G = a.Hv / a.Hk;
+  int b = 0, row, rows, slot;
+  if (!a.offsets) {
+    const int n = chunks_of(a.T);
+    slot = blockIdx.x, b = slot / n;
+    row = (slot - b * n) * kChunk, rows = a.T - row;
+  } else {
+    slot = blockIdx.x;
+    int lo = 0, hi = a.nseq;   // the last sequence whose chunks begin at or before this slot
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (span_of(a, mid).slot <= slot) lo = mid;
+      else hi = mid;
+    }
+    const Span sp = span_of(a, lo);
+    const int c = slot - sp.slot;
+    if (c < 0 || c >= chunks_of(sp.rows)) return;
+    row = sp.row + c * kChunk, rows = sp.rows - c * kChunk;
+  }
+  if (rows > kChunk) rows = kChunk;
+  const bool live = j < rows;
+  const long long t = row + (live ? j : 0);
+  {
+    const T* k = row_at<T>(a.k, b, t) + hk * a.dk;
+    const T* q = row_at<T>(a.q, b, t) + hk * a.dk;
+    f32x16_t kk = {}, qk = {};
+    for (int at = 0; at < a.dk; at += 16) {
+      Unit uk[PartsOf<T>::n], uq[PartsOf<T>::n];
+      load_unit(k, live, at + 8 * half, a.dk, a.vec_qk, uk);
+      load_unit(q, live, at + 8 * half, a.dk, a.vec_qk, uq);
+      kk = product32(uk, uk, kk);
+      qk = product32(uq, uk, qk);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = 8 * (i / 4) + 4 * half + i % 4;
+      s_kk[r * 33 + j] = kk[i], s_qk[r * 33 + j] = qk[i];
+    }
+  }
+  for (int p = 0; p < G; p += 2) {
+    const int h = hk * G + p + half;
+    const bool on = p + half < G;
+    float beta = 0.0f, alpha = 1.0f;
+    if (on && live) {
+      beta = row_at<float>(a.beta, b, t)[h];
+      if (a.decay.p) alpha = expf(row_at<float>(a.decay, b, t)[h]);
+    }
+    s_alpha[half][j] = alpha, s_beta[half][j] = beta;
+    __syncthreads();
+    float A[kChunk], P[kChunk], d = 0.0f, gamma = 1.0f;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      const float al = s_alpha[half][i];
+      d = i == j ? 1.0f : i > j ? d * al : 0.0f;
+      gamma = i <= j ? gamma * al : gamma;
+      A[i] = i > j ? d * s_kk[i * 33 + j] : 0.0f;
+      P[i] = i >= j ? a.scale * d * s_qk[i * 33 + j] : 0.0f;
+      s_m[half][i * kPad + j] = A[i] * beta;
+    }
+    const size_t head = size_t(slot) * a.Hv + h;
+    if (on) {
+      float* g = a.gains + head * 96;
+      g[j] = gamma, g[32 + j] = d, g[64 + j] = beta;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 1; i < kChunk; ++i) {
+      float sum = A[i];
+#pragma unroll
+      for (int l = 0; l < i; l += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(&s_m[half][i * kPad + l]);
+        sum -= m.x * A[l];
+        if (l + 1 < i) sum -= m.y * A[l + 1];
+        if (l + 2 < i) sum -= m.z * A[l + 2];
+        if (l + 3 < i) sum -= m.w * A[l + 3];
+      }
+      A[i] = sum;
+    }
+#pragma unroll
+    for (int what = 0; what < 2; ++what) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) s_m[half][i * kPad + j] = what ? P[i] : A[i];
+      __syncthreads();
+      for (int o = 0; o < 2 && p + o < G; ++o) {
+        uint4* u = a.units + (size_t(slot) * a.Hv + hk * G + p + o) * kUnits<T> + (what ? 3 * 128 : 0);
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+          const int r = 16 * tile + lane % 16, c = lane / 16 * 4;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int cc = c + (i < 4 ? i : 12 + i);
+            v[i] = TURNED ? s_m[o][cc * kPad + r] : s_m[o][r * kPad + cc];
+          }
+          if (what) {
+            Unit w[kPParts<T>];
+            split<kPParts<T>>(v, w);
+#pragma unroll
+            for (int n = 0; n < kPParts<T>; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
+          } else {
+            Unit w[3];
+            split<3>(v, w);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int kWalkColumns = 64;   // of a workgroup: 16 for each of its four waves
+
+template <int DKP, typename T>
+struct WalkLds {
+  static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
+  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[kUnits<T>];
+  float gains[96];
+};
+
+// One workgroup carries 64 columns of one sequence's and head's state through the chunks.  While a chunk is computed
+// from LDS, the next one's rows are on their way into registers.
+template <int DKP, typename T>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void delta_walk(DeltaRule a) {
+  using Lds = WalkLds<DKP, T>;
+  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, PP = kPParts<T>;
+  constexpr int LP = (kUnits<T> + 255) / 256;
+  __shared__ Lds lds[Lds::kBufs];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
+  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int b = a.offsets ? 0 : seq;
+  const Span sp = span_of(a, seq);
+  const int chunks = chunks_of(sp.rows);
+  const int col = blockIdx.y * kWalkColumns + wave * 16 + lane % 16;
+  const bool mine = col < a.dv;
+  const size_t state = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
+  T* const y = static_cast<T*>(a.y) + (size_t(b) * a.T * a.Hv + h) * a.dv + col;
+  const size_t y_row = size_t(a.Hv) * a.dv;
+
+  f32x4_t S[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * m + 4 * g + i;
+      S[m][i] = a.h0 && mine && r < a.dk ? a.h0[state + size_t(r) * a.dv] : 0.0f;
+    }
+
+  // a thread's share of a chunk's rows
+  const int p_tok = tid % 8 + tid / (8 * 2 * KS) * 8, p_at = tid / 8 % (2 * KS);   // row, 32 (p_at / 2) + 8 (p_at % 2)
+  const bool p_on = tid < 64 * KS;
+  const int p_col = p_at / 2 * 32 + p_at % 2 * 8;
+  const int p_unit = ((p_at / 2 * 2 + p_tok / 16) * 4 + p_at % 2 * 2) * 16 + p_tok % 16;
+  const int c_g = tid / (DKP / 2), c_col = tid % (DKP / 2) * 2;
+  const bool c_on = tid < 2 * DKP;
+  const int c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
+  Piece<T> pk, pq;
+  Columns<T> ck;
+  uint4 lp[LP];
+  float gain = 0.0f;
+  T v[8];
+  const auto fetch = [&](int c) {
+    const long long t = sp.row + (long long)c * kChunk;
+    const int rows = sp.rows - c * kChunk;
+    const T* k = row_at<T>(a.k, b, t) + hk * a.dk;
+    const T* q = row_at<T>(a.q, b, t) + hk * a.dk;
+    if (p_on) {
+      load_piece(k + p_tok * a.k.row, p_tok < rows, p_col, a.dk, a.vec_qk, pk);
+      load_piece(q + p_tok * a.q.row, p_tok < rows, p_col, a.dk, a.vec_qk, pq);
+    }
+    if (c_on) load_columns(k, a.k.row, 4 * c_g, rows, c_col, a.dk, a.vec_qk, ck);
+    const size_t head = size_t(sp.slot + c) * a.Hv + h;
+#pragma unroll
+    for (int i = 0; i < LP; ++i)
+      if (tid + 256 * i < kUnits<T>) lp[i] = a.units[head * kUnits<T> + tid + 256 * i];
+    if (tid < 96) gain = a.gains[head * 96 + tid];
+    const T* vv = row_at<T>(a.v, b, t) + h * a.dv + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * g + (i < 4 ? i : 12 + i);
+      v[i] = mine && r < rows ? vv[r * a.v.row] : T{};
+    }
+  };
+  const auto stash = [&](Lds& to) {
+    if (p_on) {
+      store_piece(pk, to.k + p_unit, PLANE);
+      store_piece(pq, to.q + p_unit, PLANE);
+    }
+    if (c_on) store_columns(ck, to.kt + c_unit, PLANE);
+#pragma unroll
+    for (int i = 0; i < LP; ++i)
+      if (tid + 256 * i < kUnits<T>) to.lp[tid + 256 * i] = lp[i];
+    if (tid < 96) to.gains[tid] = gain;
+  };
+
+  if (chunks) {
+    fetch(0);
+    stash(lds[0]);
+  }
+  for (int c = 0; c < chunks; ++c) {
+    __syncthreads();
+    const Lds& in = lds[c % Lds::kBufs];
+    float V[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) V[i] = to_f32(v[i]);
+    if (c + 1 < chunks) fetch(c + 1);
+
+    if (a.states && c % (kSegment / kChunk) == 0 && mine) {
+      float* st = a.states + (size_t(sp.segment + c / (kSegment / kChunk)) * a.Hv + h) * a.dk * a.dv + col;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * m + 4 * g + i < a.dk) st[size_t(16 * m + 4 * g + i) * a.dv] = S[m][i];
+    }
+    f32x4_t ks[2] = {}, qs[2] = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
+                          S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
+      Unit u[3];
+      split<3>(x, u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[N];
+        take(in.k + (s * 2 + t) * 64 + lane, PLANE, w);
+        ks[t] = product(w, u, ks[t]);
+        take(in.q + (s * 2 + t) * 64 + lane, PLANE, w);
+        if constexpr (PP == 3) {
+          qs[t] = product(w, u, qs[t]);
+        } else {
+          const Unit u2[2] = {u[0], u[1]};
+          qs[t] = product(w, u2, qs[t]);
+        }
+      }
+    }
+    float R[8], E[8], x[8], gm[8], dd[8], bt[8];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float4 g4 = *reinterpret_cast<const float4*>(&in.gains[16 * t + 4 * g]);
+      const float4 d4 = *reinterpret_cast<const float4*>(&in.gains[32 + 16 * t + 4 * g]);
+      const float4 b4 = *reinterpret_cast<const float4*>(&in.gains[64 + 16 * t + 4 * g]);
+      gm[4 * t] = g4.x, gm[4 * t + 1] = g4.y, gm[4 * t + 2] = g4.z, gm[4 * t + 3] = g4.w;
+      dd[4 * t] = d4.x, dd[4 * t + 1] = d4.y, dd[4 * t + 2] = d4.z, dd[4 * t + 3] = d4.w;
+      bt[4 * t] = b4.x, bt[4 * t + 1] = b4.y, bt[4 * t + 2] = b4.z, bt[4 * t + 3] = b4.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      R[i] = V[i] - gm[i] * ks[i / 4][i % 4];
+      x[i] = bt[i] * R[i];
+      qs[i / 4][i % 4] *= a.scale * gm[i];
+    }
+    {
+      Unit u[3];
+      split<3>(x, u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[3];
+        take(in.lp + t * 64 + lane, 128, w);
+        const f32x4_t le = product(w, u, f32x4_t{});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) E[4 * t + i] = R[4 * t + i] - le[i];
+      }
+    }
+    {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = bt[i] * E[i];
+      Unit u[PP];
+      split<PP>(x, u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[PP];
+        take(in.lp + 3 * 128 + t * 64 + lane, 128, w);
+        qs[t] = product(w, u, qs[t]);
+      }
+    }
+    {
+      const long long t0 = sp.row + (long long)c * kChunk;
+      const int rows = sp.rows - c * kChunk;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * g + (i < 4 ? i : 12 + i);
+        if (mine && r < rows) {
+          put(y + size_t(t0 + r) * y_row, qs[i / 4][i % 4]);
+          if (a.errors) a.errors[((size_t(b) * a.T + t0 + r) * a.Hv + h) * a.dv + col] = E[i];
+        }
+      }
+    }
+    {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= dd[i];
+      Unit u[3];
+      split<3>(x, u);
+      const float all = in.gains[31];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        Unit w[N];
+        take(in.kt + m * 64 + lane, PLANE, w);
+        S[m] = product(w, u, S[m] * all);
+      }
+    }
+    if (c + 1 < chunks) {
+      if (Lds::kBufs == 1) __syncthreads();
+      stash(lds[(c + 1) % Lds::kBufs]);
+    }
+  }
+  if (a.h_out && mine)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * m + 4 * g + i;
+        if (r < a.dk) a.h_out[state + size_t(r) * a.dv] = S[m][i];
+      }
+  // rows behind the last sequence
+  if (a.offsets && a.zero_tail && seq == a.nseq - 1 && mine)
+    for (int t = sp.row + sp.rows + g; t < a.T; t += 4) put(y + size_t(t) * y_row, 0.0f);
+}
+
+// One token: 32 columns of a head's state to a workgroup, 8 threads of 4 columns side by side and 32 rows, or with
+// element loads 32 threads of one column and 8 rows, at a time.  The state is read once, kept in registers between
+// the two sums over its rows, and written once.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void delta_step(DeltaRule a) {
+  constexpr int X = 32 / V, RG = 256 / X, R = 128 / RG, W = RG * X / 64;   // rows side by side, rows a thread, waves
+  __shared__ float s_k[128], s_q[128], s_sum[W][32];
+  const int tid = threadIdx.x, tx = tid % X, ty = tid / X, seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv;
+  const int hk = h / (a.Hv / a.Hk), col = blockIdx.y * 32 + tx * V;
+  if (tid < 128) {
+    const bool in = tid < a.dk;
+    s_k[tid] = in ? to_f32(row_at<T>(a.k, seq, 0)[hk * a.dk + tid]) : 0.0f;
+    s_q[tid] = in ? to_f32(row_at<T>(a.q, seq, 0)[hk * a.dk + tid]) : 0.0f;
+  }
+  const bool mine = col < a.dv;
+  const float beta = row_at<float>(a.beta, seq, 0)[h];
+  const float alpha = a.decay.p ? expf(row_at<float>(a.decay, seq, 0)[h]) : 1.0f;
+  const size_t at = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
+  float S[R][V], e[V];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = ty + i * RG;
+    if (mine && r < a.dk) {
+      const auto raw = load_raw<float, V>(a.h0 + at + size_t(r) * a.dv);
+#pragma unroll
+      for (int x = 0; x < V; ++x) S[i][x] = raw.get(x);
+    } else {
+#pragma unroll
+      for (int x = 0; x < V; ++x) S[i][x] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < V; ++x) e[x] = mine ? to_f32(row_at<T>(a.v, seq, 0)[h * a.dv + col + x]) : 0.0f;
+  __syncthreads();
+  // the workgroup's sum over rows of w_r S_r, for the thread's columns
+  const auto over_rows = [&](const float* w, float (&sum)[V]) {
+#pragma unroll
+    for (int x = 0; x < V; ++x) sum[x] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float f = w[ty + i * RG];
+#pragma unroll
+      for (int x = 0; x < V; ++x) sum[x] = fmaf(f, S[i][x], sum[x]);
+    }
+#pragma unroll
+    for (int o = X; o < 64; o *= 2)
+#pragma unroll
+      for (int x = 0; x < V; ++x) sum[x] += __shfl_xor(sum[x], o);
+    if (tid % 64 < X)
+#pragma unroll
+      for (int x = 0; x < V; ++x) s_sum[tid / 64][tx * V + x] = sum[x];
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      sum[x] = 0.0f;
+#pragma unroll
+      for (int w2 = 0; w2 < W; ++w2) sum[x] += s_sum[w2][tx * V + x];
+    }
+    __syncthreads();
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int x = 0; x < V; ++x) S[i][x] *= alpha;
+  float sum[V];
+  over_rows(s_k, sum);
+#pragma unroll
+  for (int x = 0; x < V; ++x) e[x] = beta * (e[x] - sum[x]);
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = ty + i * RG;
+    const float f = s_k[r];
+#pragma unroll
+    for (int x = 0; x < V; ++x) S[i][x] = fmaf(f, e[x], S[i][x]);
+    if (mine && r < a.dk) store_row<V>(a.h_out + at + size_t(r) * a.dv, S[i]);
+  }
+  over_rows(s_q, sum);
+  if (mine && ty == 0) {
+    T* y = static_cast<T*>(a.y) + (size_t(seq) * a.Hv + h) * a.dv + col;
+#pragma unroll
+    for (int x = 0; x < V; ++x) put(y + x, a.scale * sum[x]);
+  }
+}
+
+template <typename T>
+bool wide_rows(const TokenRows& r, int n) {
+  return n % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.batch * (long long)sizeof(T) % 16 == 0 &&
+         r.row * (long long)sizeof(T) % 16 == 0;
+}
+
+template <typename T>
+void run(DeltaRule& a, hipStream_t s) {
+  a.vec_qk = wide_rows<T>(a.q, a.dk) && wide_rows<T>(a.k, a.dk);
+  const int n = a.offsets ? a.nseq : a.B, slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
+  if (slots) delta_prepare<T, false><<<dim3(slots, a.Hk), 64, 0, s>>>(a);
+  const dim3 grid(n * a.Hv, (a.dv + kWalkColumns - 1) / kWalkColumns);
+  if (a.dk <= 64) delta_walk<64, T><<<grid, 256, 0, s>>>(a);
+  else delta_walk<128, T><<<grid, 256, 0, s>>>(a);
+}
+
+template <typename T>
+void step(DeltaRule& a, hipStream_t s) {
+  const dim3 grid(a.B * a.Hv, (a.dv + 31) / 32);
+  const bool vec = a.dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.h0) % 16 == 0 && reinterpret_cast<uintptr_t>(a.h_out) % 16 == 0;
+  if (vec) delta_step<T, 4><<<grid, 256, 0, s>>>(a);
+  else delta_step<T, 1><<<grid, 256, 0, s>>>(a);
+}
+
+}  // namespace
+
+int delta_rule_slots(int B, int T, int nseq, bool packed) { return packed ? T / kChunk + nseq : B * chunks_of(T); }
+
+int delta_rule_segments(int B, int T, int nseq, bool packed) { return packed ? T / kSegment + nseq : B * segments_of(T); }
+
+size_t delta_rule_workspace(int B, int T, int Hv, int nseq, bool packed) {
+  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float> * sizeof(uint4) + 96 * sizeof(float));
+}
+
+hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s) {
+  const size_t heads = size_t(delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr)) * a.Hv;
+  a.units = static_cast<uint4*>(workspace);
+  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float> : kUnits<Bf16>));
+  if (dtype == 0) run<float>(a, s);
+  else run<Bf16>(a, s);
+  return hipGetLastError();
+}
+
+hipError_t launch_delta_rule_step(DeltaRule a, int dtype, hipStream_t s) {
+  if (dtype == 0) step<float>(a, s);
+  else step<Bf16>(a, s);
+  return hipGetLastError();
+}
+
+}  // namespace cssm

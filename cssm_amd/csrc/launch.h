@@ -376,4 +376,28 @@ struct Product8 {
 };
 hipError_t launch_product8(const Product8& p, int out_dtype, hipStream_t s);
 
+// ---- gated delta rule over token sequences (delta_rule.hip, delta_rule_bwd.hip)
+struct DeltaRule {
+  TokenRows q, k, v;       // (B, T, heads x width) of the inputs' type
+  TokenRows beta, decay;   // (B, T, Hv) float32; decay.p null: none
+  int B, T, Hk, Hv, dk, dv;
+  float scale;
+  const int* offsets;      // packed rows (B = 1): nseq + 1 starts; null: n = B sequences of T rows
+  int nseq;
+  const float* h0;         // (n, Hv, dk, dv) or null: zeros
+  void* y;                 // (B, T, Hv, dv)
+  int zero_tail;           // packed: write zeros to the rows of y behind the last sequence
+  float* h_out;            // (n, Hv, dk, dv) or null
+  float* errors;           // (B, T, Hv, dv) out, for the adjoint: e; or null
+  float* states;           // (segments, Hv, dk, dv) out, for the adjoint: S before every 128th row of a sequence; or null
+  int vec_qk;              // set by the launchers: rows of q and k take 16-byte loads
+  uint4* units;            // workspace: each chunk's and head's L and P (csrc/delta_rule.h)
+  float* gains;            // workspace: (slots, Hv, 96) gamma, d and beta of a chunk's rows
+};
+int delta_rule_slots(int B, int T, int nseq, bool packed);     // chunks that the workspace has room for
+int delta_rule_segments(int B, int T, int nseq, bool packed);
+size_t delta_rule_workspace(int B, int T, int Hv, int nseq, bool packed);
+hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s);
+hipError_t launch_delta_rule_step(DeltaRule a, int dtype, hipStream_t s);
+
 }  // namespace cssm

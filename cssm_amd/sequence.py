@@ -345,3 +345,154 @@ def scaled_matmul(a: Blocks8, w: Blocks8, bias: Optional[torch.Tensor] = None, a
         _call(dev, "cssm_scaled_matmul", av.data_ptr(), sa.data_ptr(), wv.data_ptr(), sw.data_ptr(),
               M, N, K, _ptr(bias), OUTPUT_ACTS[act], out.data_ptr(), _DTYPES[out_dtype])
     return out
+
+
+def _heads(t, name: str, lead, width: int, dtype, dev: int, like: str) -> Tuple[_lib.TokenRows, int]:
+    """cssm_token_rows and the number of heads of (..., H, width) whose heads lie side by side; ``lead`` its leading sizes.
+    (B, T, H, width), or (T, H, width) packed rows / (B, H, width) tokens as ``like`` says."""
+    if _gpu(t, name) != dev:
+        raise ValueError(f"{name} is on {t.device}, expected GPU {dev}")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != len(lead) + 2 or t.shape[:-2] != lead or (width and t.shape[-1] != width) or not t.shape[-2]:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(lead)} rows of heads" +
+                         (f" of {width}" if width else ""))
+    H, D = t.shape[-2:]
+    st = t.stride()
+    if (D > 1 and st[-1] != 1) or (H > 1 and st[-2] != D):
+        raise ValueError(f"{name} must have its heads side by side (strides {st})")
+    return _lead_rows(t, st, like), H
+
+
+def _lead_rows(t, st, like: str) -> _lib.TokenRows:
+    if like == "batch":
+        return _lib.TokenRows(t.data_ptr(), st[0], st[1])
+    return _lib.TokenRows(t.data_ptr(), 0, st[0]) if like == "packed" else _lib.TokenRows(t.data_ptr(), st[0], 0)
+
+
+def _gate_rows(t, name: str, lead, H: int, dev: int, like: str) -> _lib.TokenRows:
+    """cssm_token_rows of (..., H) float32, any strides but the heads'."""
+    if _gpu(t, name) != dev:
+        raise ValueError(f"{name} is on {t.device}, expected GPU {dev}")
+    if t.dtype is not torch.float32:
+        raise ValueError(f"{name} must be torch.float32, got {t.dtype}")
+    if t.shape != (*lead, H):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(*lead, H)}")
+    st = t.stride()
+    if H > 1 and st[-1] != 1:
+        raise ValueError(f"{name} must have its heads side by side (strides {st})")
+    return _lead_rows(t, st, like)
+
+
+class _Delta(NamedTuple):
+    """Checked arguments of the delta rule: GPU, rows, sizes."""
+    dev: int
+    q: _lib.TokenRows
+    k: _lib.TokenRows
+    v: _lib.TokenRows
+    beta: _lib.TokenRows
+    decay: Optional[_lib.TokenRows]
+    dtype: int
+    B: int
+    T: int
+    Hk: int
+    Hv: int
+    dk: int
+    dv: int
+    n: int          # sequences
+    nseq: int       # with offsets, else 0
+
+
+def _delta(q, k, v, beta, decay, state, offsets, step: bool = False, need_state: bool = False) -> _Delta:
+    dev = _gpu(v, "v")
+    if v.dtype not in _DTYPES:
+        raise ValueError(f"v: unsupported dtype {v.dtype}")
+    like = "step" if step else "batch" if offsets is None else "packed"
+    if v.dim() != (4 if like == "batch" else 3):
+        raise ValueError(f"v has shape {tuple(v.shape)}, expected " +
+                         {"step": "(B, Hv, dv)", "batch": "(B, T, Hv, dv)", "packed": "(T, Hv, dv) rows with offsets"}[like])
+    lead = v.shape[:-2]
+    B, T = (lead[0], 1) if step else lead if offsets is None else (1, lead[0])
+    _sizes("v", v.shape, *v.shape)
+    rv, Hv = _heads(v, "v", lead, 0, v.dtype, dev, like)
+    rk, Hk = _heads(k, "k", lead, 0, v.dtype, dev, like)
+    dk, dv = k.shape[-1], v.shape[-1]
+    rq, Hq = _heads(q, "q", lead, dk, v.dtype, dev, like)
+    if Hq != Hk or Hv % Hk:
+        raise ValueError(f"{Hq} query, {Hk} key and {Hv} value heads: as many queries as keys, and values a multiple of them")
+    if not 0 < dk <= 128 or not 0 < dv <= 128:
+        raise ValueError(f"heads of {dk} and {dv}: widths of 1 to 128 are taken")
+    rb = _gate_rows(beta, "beta", lead, Hv, dev, like)
+    rd = None if decay is None else _gate_rows(decay, "decay", lead, Hv, dev, like)
+    n, nseq = B, 0
+    if offsets is not None:
+        _gpu(offsets, "offsets")
+        if offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets must be a tensor of n + 1 row numbers")
+        _check(offsets, "offsets", offsets.shape, torch.int32, dev)
+        n = nseq = offsets.numel() - 1
+    if state is not None or need_state:
+        _check(state, "state", (n, Hv, dk, dv), torch.float32, dev)
+    return _Delta(dev, rq, rk, rv, rb, rd, _DTYPES[v.dtype], B, T, Hk, Hv, dk, dv, n, nseq)
+
+
+def delta_forward(q, k, v, beta, decay=None, state=None, offsets=None, out=None, scale=None, keep=False):
+    """:func:`delta_rule` with what its adjoint needs: (y, final state, errors, states), the last two None unless ``keep``."""
+    d = _delta(q, k, v, beta, decay, state, offsets)
+    packed = offsets is not None
+    if out is None:
+        y = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    else:
+        y = _check(out, "out", v.shape, v.dtype, d.dev)
+    final = torch.empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32, device=v.device)
+    lib = _lib.load()
+    errors = states = None
+    if keep:
+        errors = torch.empty(v.shape, dtype=torch.float32, device=v.device)
+        states = torch.empty((lib.cssm_delta_rule_segments(d.B, d.T, d.nseq, int(packed)), d.Hv, d.dk, d.dv),
+                             dtype=torch.float32, device=v.device)
+    if d.n:
+        need = lib.cssm_delta_rule_workspace_size(d.B, d.T, d.Hv, d.nseq, int(packed))
+        work = torch.empty(need, dtype=torch.uint8, device=v.device)
+        _call(d.dev, "cssm_delta_rule", _ref(d.q), _ref(d.k), _ref(d.v), d.dtype, _ref(d.beta), _ref(d.decay), d.B, d.T,
+              d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), _ptr(state), _ptr(offsets), d.nseq,
+              y.data_ptr(), int(packed and out is None), final.data_ptr(), _ptr(errors), _ptr(states), work.data_ptr(), need)
+    elif packed and out is None:
+        y.zero_()
+    return y, final, errors, states
+
+
+def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, decay: Optional[torch.Tensor] = None,
+               state: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The gated delta rule over whole sequences: (y, final state).  For each value head, S (dk, dv) its state:
+
+        e_t = v_t - a_t S_{t-1}^T k_t,  S_t = a_t S_{t-1} + k_t (beta_t e_t)^T,  y_t = scale S_t^T q_t,  a = exp(decay)
+
+    ``q``, ``k`` (B, T, Hk, dk) and ``v`` (B, T, Hv, dv), float32 or bfloat16 and alike, widths to 128, the heads side by
+    side (slices of one projection's output will do); Hv / Hk value heads next to each other share a query and key head.
+    ``beta``, ``decay`` (B, T, Hv) float32, decay <= 0 (None: 0, no decay; -inf clears the state).  The rule is stable for
+    keys of at most unit length and 0 <= beta <= 2; nothing checks that.  ``state`` (B, Hv, dk, dv) float32 before the first
+    row (None: zeros); ``scale`` dk^-0.5 unless given.  ``offsets`` and ``out`` as in :func:`token_scan`: packed rows
+    (T, H, width), states (n, Hv, dk, dv).  Rows are taken 32 at a time, and a value that is not finite spoils its sequence
+    from the 32 rows on in which it stands.  Not differentiable: see :func:`cssm_amd.training.delta_rule_train`.
+    """
+    return delta_forward(q, k, v, beta, decay, state, offsets, out, scale)[:2]
+
+
+def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, state: torch.Tensor,
+                    decay: Optional[torch.Tensor] = None, out_state: Optional[torch.Tensor] = None,
+                    scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One token for each sequence: (y, state) from ``q``, ``k`` (B, Hk, dk), ``v`` (B, Hv, dv), ``beta``, ``decay`` (B, Hv)
+    and ``state`` (B, Hv, dk, dv) float32, which ``out_state=state`` updates in place."""
+    d = _delta(q, k, v, beta, decay, state, None, step=True, need_state=True)
+    if out_state is None:
+        out_state = torch.empty_like(state)
+    elif out_state is not state:
+        _check(out_state, "out_state", state.shape, torch.float32, d.dev)
+    y = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if d.B:
+        _call(d.dev, "cssm_delta_rule_step", _ref(d.q), _ref(d.k), _ref(d.v), d.dtype, _ref(d.beta), _ref(d.decay), d.B,
+              d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), state.data_ptr(), y.data_ptr(),
+              out_state.data_ptr())
+    return y, out_state

@@ -994,6 +994,41 @@ int cssm_quantize_weight(const float* kernel, int K, int N, void* q, void* scale
 int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const void* w_scales, int M, int N, int K,
                        const float* bias, int act, void* out, int out_dtype, void* stream);
 
+/*
+ * Gated delta rule over token sequences, for each of Hv value heads, of which Hv / Hk next to each other share a query and
+ * key head, with S (dk, dv) the state and a = exp(decay):
+ *   e_t = v_t - a_t S_{t-1}^T k_t,  S_t = a_t S_{t-1} + k_t (beta_t e_t)^T,  y_t = scale S_t^T q_t
+ *   q, k         (B, T, Hk x dk) of dtype, the heads side by side; v (B, T, Hv x dv) of dtype
+ *   beta, decay  (B, T, Hv) float32; decay NULL: a = 1.  A row with beta = 0 and decay = 0 leaves the state; decay = -inf
+ *                clears it
+ *   h0, h_out    (n, Hv, dk, dv) float32 state before each sequence's first row (NULL: zeros) and behind its last (or NULL)
+ *   offsets      as in cssm_token_scan, nseq >= 1
+ *   y            (B, T, Hv, dv) of dtype, contiguous; rows behind the last sequence are left as they are, or with
+ *                zero_tail != 0 set to zero
+ *   errors       NULL, or (B, T, Hv, dv) float32 out: e, which the adjoint reads; rows behind the last sequence are left
+ *   states       NULL, or (cssm_delta_rule_segments, Hv, dk, dv) float32 out: the state before every 128th row of each
+ *                sequence, which the adjoint reads
+ *   workspace    cssm_delta_rule_workspace_size bytes, 16-byte aligned
+ * dk and dv to 128 (CSSM_ERR_UNSUPPORTED otherwise).  The outputs do not overlap the inputs.  Sums and states are float32.
+ * Rows are taken 32 at a time: a value that is not finite spoils its sequence from the 32 rows on in which it stands.
+ * The same call gives the same bits.
+ */
+#define CSSM_DELTA_SEGMENT 128
+int cssm_delta_rule_segments(int B, int T, int nseq, int packed);
+size_t cssm_delta_rule_workspace_size(int B, int T, int Hv, int nseq, int packed);
+int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v, int dtype,
+                    const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int T, int Hk, int Hv, int dk, int dv,
+                    float scale, const float* h0, const int* offsets, int nseq, void* y, int zero_tail, float* h_out,
+                    float* errors, float* states, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One token for each of B sequences: cssm_delta_rule with T = 1 (the rows' row_stride is not used), state (B, Hv, dk, dv)
+ * float32 read and state_out written, which may be the same buffer.
+ */
+int cssm_delta_rule_step(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v, int dtype,
+                         const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int Hk, int Hv, int dk, int dv,
+                         float scale, const float* state, void* y, float* state_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
