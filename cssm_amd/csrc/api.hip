@@ -1462,6 +1462,10 @@ int delta_rule_args(const char* who, DeltaRule& a, const cssm_token_rows* q, con
   if (T > 0 && n > 0 && (!has(q) || !has(k) || !has(v) || !has(beta) || (decay && !decay->data)))
     return fail(CSSM_ERR_NULL, "%s: q, k, v and beta must be non-null", who);
   if (const int st = token_stride_check(who, {q, k, v, beta, decay})) return st;
+  if (T > 1)   // a chunk's rows lie within 2^31 bytes
+    for (const cssm_token_rows* r : {q, k, v})
+      if (has(r) && r->row_stride > 1 << 24) return fail(CSSM_ERR_UNSUPPORTED, "%s: row_stride=%lld", who, r->row_stride);
+  if ((long long)Hv * dv > 1 << 24) return fail(CSSM_ERR_UNSUPPORTED, "%s: Hv=%d dv=%d", who, Hv, dv);
   a.q = rows_of(q), a.k = rows_of(k), a.v = rows_of(v), a.beta = rows_of(beta), a.decay = rows_of(decay);
   a.B = B, a.T = T, a.Hk = Hk, a.Hv = Hv, a.dk = dk, a.dv = dv, a.scale = scale, a.offsets = offsets, a.nseq = nseq;
   return token_align_check(who, dtype, {a.q.p, a.k.p, a.v.p}, {a.beta.p, a.decay.p, offsets});

@@ -78,148 +78,169 @@ __device__ __forceinline__ float to_f32(Bf16 v) { return __uint_as_float(uint32_
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(Bf16* p, float v) { p->u = uint16_t(pack_bf16(v, 0.0f) & 0xffffu); }
 
+// ---- a chunk's rows in memory.  They are read through buffer descriptors, which give 0 beyond their end: loads need no
+// branches, so that all of a chunk's are on their way at once.  WIDE: aligned 16-byte vectors, and rows that do not
+// overlap, so that a row behind the last lies beyond the descriptor's end; else single elements with every row's number
+// looked at.
+
+constexpr uint32_t kNowhere = 0x80000000u;   // beyond the end of every descriptor
+constexpr int kMostStride = 1 << 24;         // elements from row to row: 31 rows within 2^31 bytes
+
+struct Rows {
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t stride;   // elements
+  int rows;
+  // `rows` rows of `width` elements (more than 32: the first 32)
+  template <typename T>
+  __device__ __forceinline__ Rows(const T* base, long long stride_, int rows_, int width)
+      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0,
+                                            rows_ <= 0 ? 0 : int((uint32_t((rows_ < kChunk ? rows_ : kChunk) - 1) * uint32_t(stride_) + uint32_t(width)) * sizeof(T)),
+                                            0x00020000)),
+        stride(uint32_t(stride_)), rows(rows_) {}
+  // byte offset of an element
+  template <typename T, bool WIDE>
+  __device__ __forceinline__ uint32_t at(int row, int col, int width) const {
+    const bool in = col < width && (WIDE || row < rows);
+    return in ? (uint32_t(row) * stride + uint32_t(col)) * uint32_t(sizeof(T)) : kNowhere;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t load_element(const Rows& m, uint32_t off) {
+  if constexpr (sizeof(T) == 2) return uint16_t(__builtin_amdgcn_raw_buffer_load_b16(m.r, int(off), 0, 0));
+  else return __builtin_amdgcn_raw_buffer_load_b32(m.r, int(off), 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ float element(uint32_t raw) { return __uint_as_float(sizeof(T) == 2 ? raw << 16 : raw); }
+template <typename T>
+__device__ __forceinline__ void store_element(const Rows& m, uint32_t off, float v) {
+  if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(short(pack_bf16(v, 0.0f) & 0xffffu), m.r, int(off), 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b32(int(__float_as_uint(v)), m.r, int(off), 0, 0);
+}
+__device__ __forceinline__ uint4 load16(const Rows& m, uint32_t off) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(m.r, int(off), 0, 0));
+}
+
 // ---- rows as first operands (16 rows a tile, the terms along the row)
 
-// 8 values from each of two places 16 apart
-template <typename T>
-struct Piece;
-template <>
-struct Piece<Bf16> {
-  uint4 q[2];
-  __device__ __forceinline__ float get(int i) const { return Raw<Bf16, 8>{q[i / 8]}.get(i % 8); }
-};
-template <>
-struct Piece<float> {
-  float4 q[4];
-  __device__ __forceinline__ float get(int i) const { return Raw<float, 4>{q[i / 4]}.get(i % 4); }
-};
-
-// values at .. at + 7 and at + 16 .. at + 23 of a row of n; zero behind its end, or without a row
-__device__ __forceinline__ void load_piece(const Bf16* row, bool live, int at, int n, bool vec, Piece<Bf16>& p) {
+// 8 values from each of two places of a row 16 apart
+template <typename T, bool WIDE>
+struct Piece {
+  static constexpr int kWords = WIDE ? 4 * sizeof(T) : 16;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const Rows& m, int row, int col, int n) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int c = at + 16 * h;
-    p.q[h] = make_uint4(0, 0, 0, 0);
-    if (vec) {
-      if (live && c < n) p.q[h] = *reinterpret_cast<const uint4*>(row + c);
-    } else {
-      uint32_t w[8];
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (WIDE) {
+        const uint32_t o = m.at<T, true>(row, col + 16 * h, n);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = live && c + i < n ? row[c + i].u : 0u;
-      p.q[h] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+          const uint4 q = load16(m, o + 16 * i);
+          uint32_t* d = w + 2 * h * sizeof(T) + 4 * i;
+          d[0] = q.x, d[1] = q.y, d[2] = q.z, d[3] = q.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[8 * h + i] = load_element<T>(m, m.at<T, false>(row, col + 16 * h + i, n));
+      }
     }
   }
-}
-__device__ __forceinline__ void load_piece(const float* row, bool live, int at, int n, bool vec, Piece<float>& p) {
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (WIDE && sizeof(T) == 2) return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return element<T>(w[i]);
+  }
+  // values 2 i and 2 i + 1 of bfloat16
+  __device__ __forceinline__ uint32_t pair(int i) const {
+    if constexpr (WIDE) return w[i];
+    else return w[2 * i] | w[2 * i + 1] << 16;
+  }
+  // as two units (g = 2 p and 2 p + 1), each in N parts `plane` apart, times `by`
+  template <int N>
+  __device__ __forceinline__ void store_by(float by, uint4* at, int plane) const {
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const int c = at + 16 * (h / 2) + 4 * (h % 2);
-    p.q[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (vec) {
-      if (live && c < n) p.q[h] = *reinterpret_cast<const float4*>(row + c);
-    } else {
-      if (live && c < n) p.q[h].x = row[c];
-      if (live && c + 1 < n) p.q[h].y = row[c + 1];
-      if (live && c + 2 < n) p.q[h].z = row[c + 2];
-      if (live && c + 3 < n) p.q[h].w = row[c + 3];
+    for (int h = 0; h < 2; ++h) {
+      Unit u[N];
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = get(4 * h + i) * by, v[4 + i] = get(8 + 4 * h + i) * by;
+      split<N>(v, u);
+#pragma unroll
+      for (int n = 0; n < N; ++n) at[n * plane + h * 16] = __builtin_bit_cast(uint4, u[n]);
     }
   }
-}
-
-// the piece as two units (g = 2 p and 2 p + 1), each in N parts `plane` apart, times `by`
-template <int N, typename T>
-__device__ __forceinline__ void store_piece(const Piece<T>& p, float by, uint4* at, int plane) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    Unit u[N];
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = p.get(4 * h + i) * by, v[4 + i] = p.get(8 + 4 * h + i) * by;
-    split<N>(v, u);
-#pragma unroll
-    for (int n = 0; n < N; ++n) at[n * plane + h * 16] = __builtin_bit_cast(uint4, u[n]);
+  // as they are
+  __device__ __forceinline__ void store(uint4* at, int plane) const {
+    if constexpr (sizeof(T) == 2) {
+      at[0] = make_uint4(pair(0), pair(1), pair(4), pair(5));
+      at[16] = make_uint4(pair(2), pair(3), pair(6), pair(7));
+    } else {
+      store_by<3>(1.0f, at, plane);
+    }
   }
-}
-// as it is
-__device__ __forceinline__ void store_piece(const Piece<Bf16>& p, uint4* at, int) {
-  at[0] = make_uint4(p.q[0].x, p.q[0].y, p.q[1].x, p.q[1].y);
-  at[16] = make_uint4(p.q[0].z, p.q[0].w, p.q[1].z, p.q[1].w);
-}
-__device__ __forceinline__ void store_piece(const Piece<float>& p, uint4* at, int plane) { store_piece<3>(p, 1.0f, at, plane); }
+};
 
 // ---- columns as first operands, or rows as second ones (16 columns a tile, the terms down the chunk's rows)
 
-// two columns of the 8 rows first .. first + 3 and first + 16 .. first + 19
-template <typename T>
-struct Columns;
-template <>
-struct Columns<Bf16> {
-  uint32_t w[8];
-  __device__ __forceinline__ float get(int j, int h) const { return __uint_as_float(h ? w[j] & 0xffff0000u : w[j] << 16); }
-};
-template <>
-struct Columns<float> {
-  float2 w[8];
-  __device__ __forceinline__ float get(int j, int h) const { return h ? w[j].y : w[j].x; }
-};
+// row j of a unit of column operands whose first is `first`
+__device__ __forceinline__ int unit_row(int first, int j) { return first + (j < 4 ? j : 12 + j); }
 
-template <typename T>
-__device__ __forceinline__ void load_columns(const T* base, long long stride, int first, int rows, int at, int n, bool vec,
-                                             Columns<T>& c) {
+// two columns of 8 rows
+template <typename T, bool WIDE>
+struct Columns {
+  static constexpr int kWords = WIDE ? sizeof(T) / 2 : 2;
+  uint32_t w[8][kWords];
+  __device__ __forceinline__ void load(const Rows& m, int first, int col, int n) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int r = first + (j < 4 ? j : 12 + j);
-    const T* p = base + (long long)r * stride + at;
-    const bool one = r < rows && at < n, two = r < rows && at + 1 < n;
-    if constexpr (sizeof(T) == 2) {
-      c.w[j] = 0;
-      if (vec) {
-        if (one) c.w[j] = *reinterpret_cast<const uint32_t*>(p);
+    for (int j = 0; j < 8; ++j) {
+      const int r = unit_row(first, j);
+      if constexpr (WIDE && sizeof(T) == 2) {
+        w[j][0] = __builtin_amdgcn_raw_buffer_load_b32(m.r, int(m.at<T, true>(r, col, n)), 0, 0);
+      } else if constexpr (WIDE) {
+        const uint2 q = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(m.r, int(m.at<T, true>(r, col, n)), 0, 0));
+        w[j][0] = q.x, w[j][1] = q.y;
       } else {
-        if (one) c.w[j] = p[0].u;
-        if (two) c.w[j] |= uint32_t(p[1].u) << 16;
-      }
-    } else {
-      c.w[j] = make_float2(0.0f, 0.0f);
-      if (vec) {
-        if (one) c.w[j] = *reinterpret_cast<const float2*>(p);
-      } else {
-        if (one) c.w[j].x = p[0];
-        if (two) c.w[j].y = p[1];
+        w[j][0] = load_element<T>(m, m.at<T, false>(r, col, n));
+        w[j][1] = load_element<T>(m, m.at<T, false>(r, col + 1, n));
       }
     }
   }
-}
-
-// the two units, each in N parts, row j times by[j]
-template <int N, typename T>
-__device__ __forceinline__ void store_columns(const Columns<T>& c, const float (&by)[8], uint4* at, int plane) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    Unit u[N];
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c.get(j, h) * by[j];
-    split<N>(v, u);
-#pragma unroll
-    for (int n = 0; n < N; ++n) at[n * plane + h] = __builtin_bit_cast(uint4, u[n]);
+  __device__ __forceinline__ float get(int j, int h) const {
+    if constexpr (WIDE && sizeof(T) == 2) return __uint_as_float(h ? w[j][0] & 0xffff0000u : w[j][0] << 16);
+    else return element<T>(w[j][h]);
   }
-}
-// as they are
-__device__ __forceinline__ void store_columns(const Columns<Bf16>& c, uint4* at, int) {
+  // the two units, each in N parts, row j times by[j]
+  template <int N>
+  __device__ __forceinline__ void store_by(const float (&by)[8], uint4* at, int plane) const {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    Unit u;
+    for (int h = 0; h < 2; ++h) {
+      Unit u[N];
+      float v[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      u.w[i] = h ? c.w[2 * i] >> 16 | (c.w[2 * i + 1] & 0xffff0000u) : (c.w[2 * i] & 0xffffu) | c.w[2 * i + 1] << 16;
-    at[h] = __builtin_bit_cast(uint4, u);
+      for (int j = 0; j < 8; ++j) v[j] = get(j, h) * by[j];
+      split<N>(v, u);
+#pragma unroll
+      for (int n = 0; n < N; ++n) at[n * plane + h] = __builtin_bit_cast(uint4, u[n]);
+    }
   }
-}
-__device__ __forceinline__ void store_columns(const Columns<float>& c, uint4* at, int plane) {
-  const float one[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-  store_columns<3>(c, one, at, plane);
-}
+  __device__ __forceinline__ void store(uint4* at, int plane) const {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        Unit u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (WIDE)
+            u.w[i] = h ? w[2 * i][0] >> 16 | (w[2 * i + 1][0] & 0xffff0000u) : (w[2 * i][0] & 0xffffu) | w[2 * i + 1][0] << 16;
+          else u.w[i] = w[2 * i][h] | w[2 * i + 1][h] << 16;
+        }
+        at[h] = __builtin_bit_cast(uint4, u);
+      }
+    } else {
+      const float one[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+      store_by<3>(one, at, plane);
+    }
+  }
+};
 
 // ---- sequences and their chunks
 

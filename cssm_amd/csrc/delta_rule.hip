@@ -26,31 +26,24 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 constexpr int kPad = kChunk + 4;
 
 // the 8 values of a row from `at` on, in their parts
-template <typename T>
-__device__ __forceinline__ void load_unit(const T* row, bool live, int at, int n, bool vec, Unit (&u)[PartsOf<T>::n]) {
-  if constexpr (sizeof(T) == 2) {
-    if (vec) {
-      u[0] = __builtin_bit_cast(Unit, live && at < n ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0));
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_unit(const Rows& m, int row, int at, int n, Unit (&u)[PartsOf<T>::n]) {
+  float v[8];
+  if constexpr (WIDE) {
+    const uint32_t o = m.at<T, true>(row, at, n);
+    const uint4 q = load16(m, o);
+    if constexpr (sizeof(T) == 2) {
+      u[0] = __builtin_bit_cast(Unit, q);
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = at + 2 * i;
-        u[0].w[i] = (live && c < n ? uint32_t(row[c].u) : 0u) | (live && c + 1 < n ? uint32_t(row[c + 1].u) << 16 : 0u);
-      }
+      const uint4 r = load16(m, o + 16);
+      v[0] = __uint_as_float(q.x), v[1] = __uint_as_float(q.y), v[2] = __uint_as_float(q.z), v[3] = __uint_as_float(q.w);
+      v[4] = __uint_as_float(r.x), v[5] = __uint_as_float(r.y), v[6] = __uint_as_float(r.z), v[7] = __uint_as_float(r.w);
+      split<3>(v, u);
     }
   } else {
-    float v[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (vec) {
-        const float4 q = live && at < n ? reinterpret_cast<const float4*>(row + at)[h] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        v[4 * h] = q.x, v[4 * h + 1] = q.y, v[4 * h + 2] = q.z, v[4 * h + 3] = q.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * h + i] = live && at + 4 * h + i < n ? row[at + 4 * h + i] : 0.0f;
-      }
-    }
-    split<3>(v, u);
+    for (int i = 0; i < 8; ++i) v[i] = element<T>(load_element<T>(m, m.at<T, false>(row, at + i, n)));
+    split<PartsOf<T>::n>(v, u);
   }
 }
 
@@ -73,7 +66,7 @@ constexpr int kUnits = (3 + kPParts<T>) * 128;   // units of L and P of one chun
 // One wave for a chunk of one key head: K K^T and Q K^T, then for two value heads at a time, one in each half of the
 // wave with a column of the chunk's 32 x 32 a lane, their decays, L row by row, and both written as first operands
 // (TURNED: their transposes, which the adjoint takes).
-template <typename T, bool TURNED>
+template <typename T, bool WIDE, bool TURNED>
 __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
   __shared__ float s_kk[kChunk * 33], s_qk[kChunk * 33];
   __shared__ __attribute__((aligned(16))) float s_m[2][kChunk * kPad];
@@ -101,13 +94,12 @@ __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
   const bool live = j < rows;
   const long long t = row + (live ? j : 0);
   {
-    const T* k = row_at<T>(a.k, b, t) + hk * a.dk;
-    const T* q = row_at<T>(a.q, b, t) + hk * a.dk;
+    const Rows k(row_at<T>(a.k, b, row) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, row) + hk * a.dk, a.q.row, rows, a.dk);
     f32x16_t kk = {}, qk = {};
     for (int at = 0; at < a.dk; at += 16) {
       Unit uk[PartsOf<T>::n], uq[PartsOf<T>::n];
-      load_unit(k, live, at + 8 * half, a.dk, a.vec_qk, uk);
-      load_unit(q, live, at + 8 * half, a.dk, a.vec_qk, uq);
+      load_unit<T, WIDE>(k, j, at + 8 * half, a.dk, uk);
+      load_unit<T, WIDE>(q, j, at + 8 * half, a.dk, uq);
       kk = product32(uk, uk, kk);
       qk = product32(uq, uk, qk);
     }
@@ -196,14 +188,14 @@ constexpr int kWalkColumns = 64;   // of a workgroup: 16 for each of its four wa
 template <int DKP, typename T>
 struct WalkLds {
   static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
-  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[kUnits<T>];
-  float gains[96];
+  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[(kUnits<T> + 255) / 256 * 256];
+  float gains[256];   // gamma, d, beta; the rest takes what threads without a value write
 };
 
 // One workgroup carries 64 columns of one sequence's and head's state through the chunks.  While a chunk is computed
 // from LDS, the next one's rows are on their way into registers.
-template <int DKP, typename T>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void delta_walk(DeltaRule a) {
+template <int DKP, typename T, bool WIDE>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && WIDE ? 2 : 1) void delta_walk(DeltaRule a) {
   using Lds = WalkLds<DKP, T>;
   constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, PP = kPParts<T>;
   constexpr int LP = (kUnits<T> + 255) / 256;
@@ -216,8 +208,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void delta_walk(DeltaR
   const int col = blockIdx.y * kWalkColumns + wave * 16 + lane % 16;
   const bool mine = col < a.dv;
   const size_t state = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
-  T* const y = static_cast<T*>(a.y) + (size_t(b) * a.T * a.Hv + h) * a.dv + col;
-  const size_t y_row = size_t(a.Hv) * a.dv;
+  const int y_row = a.Hv * a.dv;
 
   f32x4_t S[MT];
 #pragma unroll
@@ -230,49 +221,37 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void delta_walk(DeltaR
 
   // a thread's share of a chunk's rows
   const int p_tok = tid % 8 + tid / (8 * 2 * KS) * 8, p_at = tid / 8 % (2 * KS);   // row, 32 (p_at / 2) + 8 (p_at % 2)
-  const bool p_on = tid < 64 * KS;
+  const bool p_on = KS == 4 || tid < 64 * KS;
   const int p_col = p_at / 2 * 32 + p_at % 2 * 8;
   const int p_unit = ((p_at / 2 * 2 + p_tok / 16) * 4 + p_at % 2 * 2) * 16 + p_tok % 16;
   const int c_g = tid / (DKP / 2), c_col = tid % (DKP / 2) * 2;
-  const bool c_on = tid < 2 * DKP;
+  const bool c_on = DKP == 128 || tid < 2 * DKP;
   const int c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
-  Piece<T> pk, pq;
-  Columns<T> ck;
+  Piece<T, WIDE> pk, pq;
+  Columns<T, WIDE> ck;
   uint4 lp[LP];
-  float gain = 0.0f;
-  T v[8];
+  uint32_t gain, v[8];
   const auto fetch = [&](int c) {
     const long long t = sp.row + (long long)c * kChunk;
     const int rows = sp.rows - c * kChunk;
-    const T* k = row_at<T>(a.k, b, t) + hk * a.dk;
-    const T* q = row_at<T>(a.q, b, t) + hk * a.dk;
-    if (p_on) {
-      load_piece(k + p_tok * a.k.row, p_tok < rows, p_col, a.dk, a.vec_qk, pk);
-      load_piece(q + p_tok * a.q.row, p_tok < rows, p_col, a.dk, a.vec_qk, pq);
-    }
-    if (c_on) load_columns(k, a.k.row, 4 * c_g, rows, c_col, a.dk, a.vec_qk, ck);
+    const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
+    const Rows vv(row_at<T>(a.v, b, t) + h * a.dv, a.v.row, rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
+    const Rows units(a.units + head * kUnits<T>, 0, 1, kUnits<T>), gains(a.gains + head * 96, 0, 1, 96);
 #pragma unroll
-    for (int i = 0; i < LP; ++i)
-      if (tid + 256 * i < kUnits<T>) lp[i] = a.units[head * kUnits<T> + tid + 256 * i];
-    if (tid < 96) gain = a.gains[head * 96 + tid];
-    const T* vv = row_at<T>(a.v, b, t) + h * a.dv + col;
+    for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
+    if (p_on) pk.load(k, p_tok, p_col, a.dk), pq.load(q, p_tok, p_col, a.dk);
+    if (c_on) ck.load(k, 4 * c_g, c_col, a.dk);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * g + (i < 4 ? i : 12 + i);
-      v[i] = mine && r < rows ? vv[r * a.v.row] : T{};
-    }
+    for (int i = 0; i < LP; ++i) lp[i] = load16(units, (tid + 256 * i) * 16);
+    gain = load_element<float>(gains, tid * 4);
   };
   const auto stash = [&](Lds& to) {
-    if (p_on) {
-      store_piece(pk, to.k + p_unit, PLANE);
-      store_piece(pq, to.q + p_unit, PLANE);
-    }
-    if (c_on) store_columns(ck, to.kt + c_unit, PLANE);
+    if (p_on) pk.store(to.k + p_unit, PLANE), pq.store(to.q + p_unit, PLANE);
+    if (c_on) ck.store(to.kt + c_unit, PLANE);
 #pragma unroll
-    for (int i = 0; i < LP; ++i)
-      if (tid + 256 * i < kUnits<T>) to.lp[tid + 256 * i] = lp[i];
-    if (tid < 96) to.gains[tid] = gain;
+    for (int i = 0; i < LP; ++i) to.lp[tid + 256 * i] = lp[i];
+    to.gains[tid] = __uint_as_float(gain);
   };
 
   if (chunks) {
@@ -284,7 +263,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void delta_walk(DeltaR
     const Lds& in = lds[c % Lds::kBufs];
     float V[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) V[i] = to_f32(v[i]);
+    for (int i = 0; i < 8; ++i) V[i] = element<T>(v[i]);
     if (c + 1 < chunks) fetch(c + 1);
 
     if (a.states && c % (kSegment / kChunk) == 0 && mine) {
@@ -359,13 +338,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void delta_walk(DeltaR
     {
       const long long t0 = sp.row + (long long)c * kChunk;
       const int rows = sp.rows - c * kChunk;
+      const size_t head = ((size_t(b) * a.T + t0) * a.Hv + h) * a.dv;
+      const Rows yy(static_cast<T*>(a.y) + head, y_row, rows, a.dv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * g + (i < 4 ? i : 12 + i);
-        if (mine && r < rows) {
-          put(y + size_t(t0 + r) * y_row, qs[i / 4][i % 4]);
-          if (a.errors) a.errors[((size_t(b) * a.T + t0 + r) * a.Hv + h) * a.dv + col] = E[i];
-        }
+      for (int i = 0; i < 8; ++i) store_element<T>(yy, yy.at<T, true>(unit_row(4 * g, i), col, a.dv), qs[i / 4][i % 4]);
+      if (a.errors) {
+        const Rows ee(a.errors + head, y_row, rows, a.dv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) store_element<float>(ee, ee.at<float, true>(unit_row(4 * g, i), col, a.dv), E[i]);
       }
     }
     {
@@ -396,7 +376,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void delta_walk(DeltaR
       }
   // rows behind the last sequence
   if (a.offsets && a.zero_tail && seq == a.nseq - 1 && mine)
-    for (int t = sp.row + sp.rows + g; t < a.T; t += 4) put(y + size_t(t) * y_row, 0.0f);
+    for (int t = sp.row + sp.rows + g; t < a.T; t += 4) put(static_cast<T*>(a.y) + (size_t(t) * a.Hv + h) * a.dv + col, 0.0f);
 }
 
 // One token: 32 columns of a head's state to a workgroup, 8 threads of 4 columns side by side and 32 rows, or with
@@ -483,20 +463,27 @@ __global__ __launch_bounds__(256) void delta_step(DeltaRule a) {
   }
 }
 
+// rows that WIDE takes: 16-byte vectors, and none overlapping the next
 template <typename T>
-bool wide_rows(const TokenRows& r, int n) {
+bool wide_rows(const TokenRows& r, int heads, int n) {
   return n % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.batch * (long long)sizeof(T) % 16 == 0 &&
-         r.row * (long long)sizeof(T) % 16 == 0;
+         r.row * (long long)sizeof(T) % 16 == 0 && r.row >= (long long)heads * n;
+}
+
+template <typename T, bool WIDE>
+void run_as(const DeltaRule& a, hipStream_t s) {
+  const int n = a.offsets ? a.nseq : a.B, slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
+  if (slots) delta_prepare<T, WIDE, false><<<dim3(slots, a.Hk), 64, 0, s>>>(a);
+  const dim3 grid(n * a.Hv, (a.dv + kWalkColumns - 1) / kWalkColumns);
+  if (a.dk <= 64) delta_walk<64, T, WIDE><<<grid, 256, 0, s>>>(a);
+  else delta_walk<128, T, WIDE><<<grid, 256, 0, s>>>(a);
 }
 
 template <typename T>
-void run(DeltaRule& a, hipStream_t s) {
-  a.vec_qk = wide_rows<T>(a.q, a.dk) && wide_rows<T>(a.k, a.dk);
-  const int n = a.offsets ? a.nseq : a.B, slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
-  if (slots) delta_prepare<T, false><<<dim3(slots, a.Hk), 64, 0, s>>>(a);
-  const dim3 grid(n * a.Hv, (a.dv + kWalkColumns - 1) / kWalkColumns);
-  if (a.dk <= 64) delta_walk<64, T><<<grid, 256, 0, s>>>(a);
-  else delta_walk<128, T><<<grid, 256, 0, s>>>(a);
+void run(const DeltaRule& a, hipStream_t s) {
+  if (wide_rows<T>(a.q, a.Hk, a.dk) && wide_rows<T>(a.k, a.Hk, a.dk) && a.v.row >= (long long)a.Hv * a.dv)
+    run_as<T, true>(a, s);
+  else run_as<T, false>(a, s);
 }
 
 template <typename T>

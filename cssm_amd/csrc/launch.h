@@ -390,7 +390,6 @@ struct DeltaRule {
   float* h_out;            // (n, Hv, dk, dv) or null
   float* errors;           // (B, T, Hv, dv) out, for the adjoint: e; or null
   float* states;           // (segments, Hv, dk, dv) out, for the adjoint: S before every 128th row of a sequence; or null
-  int vec_qk;              // set by the launchers: rows of q and k take 16-byte loads
   uint4* units;            // workspace: each chunk's and head's L and P (csrc/delta_rule.h)
   float* gains;            // workspace: (slots, Hv, 96) gamma, d and beta of a chunk's rows
 };
