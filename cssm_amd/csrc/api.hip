@@ -1501,6 +1501,7 @@ int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cs
   if (const int st = delta_workspace_check(who, cssm_delta_rule_workspace_size(B, T, Hv, offsets ? nseq : 0, offsets != nullptr),
                                            workspace, workspace_bytes))
     return st;
+  if (!errors != !states) return fail(CSSM_ERR_NULL, "%s: errors and states go together", who);
   if (const int st = token_align_check(who, dtype, {y}, {h0, h_out, errors, states})) return st;
   a.h0 = h0, a.y = y, a.zero_tail = zero_tail, a.h_out = h_out, a.errors = errors, a.states = states;
   return hip_status(cssm::launch_delta_rule(a, dtype, workspace, static_cast<hipStream_t>(stream)), who);

@@ -25,6 +25,7 @@ constexpr int kSegment = 128;  // rows between the states that a training pass k
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
 struct Unit { uint32_t w[4]; };
 

@@ -63,22 +63,14 @@ constexpr int kPParts = sizeof(T) == 2 ? 2 : 3;
 template <typename T>
 constexpr int kUnits = (3 + kPParts<T>) * 128;   // units of L and P of one chunk and head
 
-// One wave for a chunk of one key head: K K^T and Q K^T, then for two value heads at a time, one in each half of the
-// wave with a column of the chunk's 32 x 32 a lane, their decays, L row by row, and both written as first operands
-// (TURNED: their transposes, which the adjoint takes).
-template <typename T, bool WIDE, bool TURNED>
-__global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
-  __shared__ float s_kk[kChunk * 33], s_qk[kChunk * 33];
-  __shared__ __attribute__((aligned(16))) float s_m[2][kChunk * kPad];
-  __shared__ float s_alpha[2][kChunk], s_beta[2][kChunk];
-  const int lane = threadIdx.x, j = lane % 32, half = lane / 32, hk = blockIdx.y, G = a.Hv / a.Hk;
-  int b = 0, row, rows, slot;
+// The chunk that a slot of the workspace stands for; false for a slot that no chunk takes
+__device__ __forceinline__ bool chunk_at(const DeltaRule& a, int slot, int& b, int& row, int& rows) {
+  b = 0;
   if (!a.offsets) {
     const int n = chunks_of(a.T);
-    slot = blockIdx.x, b = slot / n;
+    b = slot / n;
     row = (slot - b * n) * kChunk, rows = a.T - row;
   } else {
-    slot = blockIdx.x;
     int lo = 0, hi = a.nseq;   // the last sequence whose chunks begin at or before this slot
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -87,99 +79,129 @@ __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
     }
     const Span sp = span_of(a, lo);
     const int c = slot - sp.slot;
-    if (c < 0 || c >= chunks_of(sp.rows)) return;
+    if (c < 0 || c >= chunks_of(sp.rows)) return false;
     row = sp.row + c * kChunk, rows = sp.rows - c * kChunk;
   }
   if (rows > kChunk) rows = kChunk;
-  const bool live = j < rows;
-  const long long t = row + (live ? j : 0);
-  {
-    const Rows k(row_at<T>(a.k, b, row) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, row) + hk * a.dk, a.q.row, rows, a.dk);
-    f32x16_t kk = {}, qk = {};
-    for (int at = 0; at < a.dk; at += 16) {
-      Unit uk[PartsOf<T>::n], uq[PartsOf<T>::n];
-      load_unit<T, WIDE>(k, j, at + 8 * half, a.dk, uk);
-      load_unit<T, WIDE>(q, j, at + 8 * half, a.dk, uq);
-      kk = product32(uk, uk, kk);
-      qk = product32(uq, uk, qk);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int r = 8 * (i / 4) + 4 * half + i % 4;
-      s_kk[r * 33 + j] = kk[i], s_qk[r * 33 + j] = qk[i];
-    }
+  return true;
+}
+
+// One wave for a chunk of two value heads: K K^T and Q K^T of their key heads (one, or two), then one value head in each
+// half of the wave, a column of its 32 x 32 a lane: decays, L row by row, and both written as first operands (TURNED: their
+// transposes, which the adjoint takes).  What bounds it is the 500 multiplications in a row behind L and the traffic through
+// LDS between the layouts; four waves a SIMD hide most of their latencies.
+template <typename T, bool WIDE, bool TURNED>
+__global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
+  __shared__ __attribute__((aligned(16))) float s_m[2][kChunk * kPad];
+  __shared__ float s_alpha[2][kChunk];
+  const int lane = threadIdx.x, j = lane % 32, half = lane / 32, G = a.Hv / a.Hk, h0 = 2 * blockIdx.y, h = h0 + half;
+  const int slot = blockIdx.x;
+  int b, row, rows;
+  if (!chunk_at(a, slot, b, row, rows)) return;
+  const bool two = h0 + 1 < a.Hv, on = half == 0 || two;
+  const int hk[2] = {h0 / G, (two ? h0 + 1 : h0) / G};
+  float beta = 0.0f, alpha = 1.0f;
+  if (on && j < rows) {
+    beta = row_at<float>(a.beta, b, row + j)[h];
+    if (a.decay.p) alpha = expf(row_at<float>(a.decay, b, row + j)[h]);
   }
-  for (int p = 0; p < G; p += 2) {
-    const int h = hk * G + p + half;
-    const bool on = p + half < G;
-    float beta = 0.0f, alpha = 1.0f;
-    if (on && live) {
-      beta = row_at<float>(a.beta, b, t)[h];
-      if (a.decay.p) alpha = expf(row_at<float>(a.decay, b, t)[h]);
-    }
-    s_alpha[half][j] = alpha, s_beta[half][j] = beta;
-    __syncthreads();
-    float A[kChunk], P[kChunk], d = 0.0f, gamma = 1.0f;
+  s_alpha[half][j] = alpha;
+  float A[kChunk], P[kChunk];
+  {
+    f32x16_t kk[2] = {}, qk[2] = {};
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      const float al = s_alpha[half][i];
-      d = i == j ? 1.0f : i > j ? d * al : 0.0f;
-      gamma = i <= j ? gamma * al : gamma;
-      A[i] = i > j ? d * s_kk[i * 33 + j] : 0.0f;
-      P[i] = i >= j ? a.scale * d * s_qk[i * 33 + j] : 0.0f;
-      s_m[half][i * kPad + j] = A[i] * beta;
-    }
-    const size_t head = size_t(slot) * a.Hv + h;
-    if (on) {
-      float* g = a.gains + head * 96;
-      g[j] = gamma, g[32 + j] = d, g[64 + j] = beta;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 1; i < kChunk; ++i) {
-      float sum = A[i];
-#pragma unroll
-      for (int l = 0; l < i; l += 4) {
-        const float4 m = *reinterpret_cast<const float4*>(&s_m[half][i * kPad + l]);
-        sum -= m.x * A[l];
-        if (l + 1 < i) sum -= m.y * A[l + 1];
-        if (l + 2 < i) sum -= m.z * A[l + 2];
-        if (l + 3 < i) sum -= m.w * A[l + 3];
+    for (int o = 0; o < 2; ++o) {
+      if (o == 1 && hk[1] == hk[0]) {
+        kk[1] = kk[0], qk[1] = qk[0];
+        break;
       }
-      A[i] = sum;
+      const Rows k(row_at<T>(a.k, b, row) + hk[o] * a.dk, a.k.row, rows, a.dk);
+      const Rows q(row_at<T>(a.q, b, row) + hk[o] * a.dk, a.q.row, rows, a.dk);
+      for (int at = 0; at < a.dk; at += 16) {
+        Unit uk[PartsOf<T>::n], uq[PartsOf<T>::n];
+        load_unit<T, WIDE>(k, j, at + 8 * half, a.dk, uk);
+        load_unit<T, WIDE>(q, j, at + 8 * half, a.dk, uq);
+        kk[o] = product32(uk, uk, kk[o]);
+        qk[o] = product32(uq, uk, qk[o]);
+      }
     }
 #pragma unroll
     for (int what = 0; what < 2; ++what) {
+#pragma unroll
+      for (int o = 0; o < 2; ++o)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s_m[o][(8 * (i / 4) + 4 * half + i % 4) * kPad + j] = what ? qk[o][i] : kk[o][i];
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) s_m[half][i * kPad + j] = what ? P[i] : A[i];
+      for (int i = 0; i < kChunk; ++i) (what ? P : A)[i] = s_m[half][i * kPad + j];
       __syncthreads();
-      for (int o = 0; o < 2 && p + o < G; ++o) {
-        uint4* u = a.units + (size_t(slot) * a.Hv + hk * G + p + o) * kUnits<T> + (what ? 3 * 128 : 0);
+    }
+  }
+  float d = 0.0f;
 #pragma unroll
-        for (int tile = 0; tile < 2; ++tile) {
-          const int r = 16 * tile + lane % 16, c = lane / 16 * 4;
-          float v[8];
+  for (int i = 0; i < kChunk; ++i) {
+    const bool at = i == j;
+    d = at ? 1.0f : d * s_alpha[half][i];   // 0 above the diagonal
+    A[i] = at ? 0.0f : d * A[i];
+    P[i] *= d * a.scale;
+    s_m[half][i * kPad + j] = A[i] * beta;
+  }
+  float gamma = alpha;   // of this row and those before it in the chunk
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int cc = c + (i < 4 ? i : 12 + i);
-            v[i] = TURNED ? s_m[o][cc * kPad + r] : s_m[o][r * kPad + cc];
-          }
-          if (what) {
-            Unit w[kPParts<T>];
-            split<kPParts<T>>(v, w);
+  for (int o = 1; o < kChunk; o *= 2) {
+    const float before = __shfl_up(gamma, o, kChunk);
+    if (j >= o) gamma *= before;
+  }
+  if (on) {
+    float* g = a.gains + (size_t(slot) * a.Hv + h) * 96;
+    g[j] = gamma, g[32 + j] = d, g[64 + j] = beta;
+  }
+  __syncthreads();
 #pragma unroll
-            for (int n = 0; n < kPParts<T>; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
-          } else {
-            Unit w[3];
-            split<3>(v, w);
+  for (int i = 2; i < kChunk; ++i) {
+    float sum = A[i];
 #pragma unroll
-            for (int n = 0; n < 3; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
-          }
+    for (int l = 0; l < i; l += 4) {
+      const float4 m = *reinterpret_cast<const float4*>(&s_m[half][i * kPad + l]);
+      sum -= m.x * A[l];
+      if (l + 1 < i) sum -= m.y * A[l + 1];
+      if (l + 2 < i) sum -= m.z * A[l + 2];
+      if (l + 3 < i) sum -= m.w * A[l + 3];
+    }
+    A[i] = sum;
+  }
+#pragma unroll
+  for (int what = 0; what < 2; ++what) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) s_m[half][i * kPad + j] = what ? P[i] : A[i];
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      if (o == 1 && !two) break;
+      uint4* u = a.units + (size_t(slot) * a.Hv + h0 + o) * kUnits<T> + (what ? 3 * 128 : 0);
+#pragma unroll
+      for (int tile = 0; tile < 2; ++tile) {
+        const int r = 16 * tile + lane % 16, c = lane / 16 * 4;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int cc = unit_row(c, i);
+          v[i] = TURNED ? s_m[o][cc * kPad + r] : s_m[o][r * kPad + cc];
+        }
+        if (what) {
+          Unit w[kPParts<T>];
+          split<kPParts<T>>(v, w);
+#pragma unroll
+          for (int n = 0; n < kPParts<T>; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
+        } else {
+          Unit w[3];
+          split<3>(v, w);
+#pragma unroll
+          for (int n = 0; n < 3; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
         }
       }
     }
-    __syncthreads();
   }
 }
 
@@ -194,8 +216,8 @@ struct WalkLds {
 
 // One workgroup carries 64 columns of one sequence's and head's state through the chunks.  While a chunk is computed
 // from LDS, the next one's rows are on their way into registers.
-template <int DKP, typename T, bool WIDE>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && WIDE ? 2 : 1) void delta_walk(DeltaRule a) {
+template <int DKP, typename T, bool WIDE, bool KEEP>
+__global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
   using Lds = WalkLds<DKP, T>;
   constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, PP = kPParts<T>;
   constexpr int LP = (kUnits<T> + 255) / 256;
@@ -229,29 +251,30 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && WIDE ? 2 : 1) void delta_wal
   const int c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
   Piece<T, WIDE> pk, pq;
   Columns<T, WIDE> ck;
-  uint4 lp[LP];
-  uint32_t gain, v[8];
+  u32x4_t lp[LP];
+  float gain;
+  uint32_t v[8];
   const auto fetch = [&](int c) {
     const long long t = sp.row + (long long)c * kChunk;
     const int rows = sp.rows - c * kChunk;
     const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
     const Rows vv(row_at<T>(a.v, b, t) + h * a.dv, a.v.row, rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
-    const Rows units(a.units + head * kUnits<T>, 0, 1, kUnits<T>), gains(a.gains + head * 96, 0, 1, 96);
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T> + tid;   // the last ones past this chunk's: into the next, or the end's room
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
     if (p_on) pk.load(k, p_tok, p_col, a.dk), pq.load(q, p_tok, p_col, a.dk);
     if (c_on) ck.load(k, 4 * c_g, c_col, a.dk);
 #pragma unroll
-    for (int i = 0; i < LP; ++i) lp[i] = load16(units, (tid + 256 * i) * 16);
-    gain = load_element<float>(gains, tid * 4);
+    for (int i = 0; i < LP; ++i) lp[i] = units[256 * i];
+    gain = a.gains[head * 96 + tid];
   };
   const auto stash = [&](Lds& to) {
     if (p_on) pk.store(to.k + p_unit, PLANE), pq.store(to.q + p_unit, PLANE);
     if (c_on) ck.store(to.kt + c_unit, PLANE);
 #pragma unroll
-    for (int i = 0; i < LP; ++i) to.lp[tid + 256 * i] = lp[i];
-    to.gains[tid] = __uint_as_float(gain);
+    for (int i = 0; i < LP; ++i) to.lp[tid + 256 * i] = __builtin_bit_cast(uint4, lp[i]);
+    to.gains[tid] = gain;
   };
 
   if (chunks) {
@@ -266,7 +289,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && WIDE ? 2 : 1) void delta_wal
     for (int i = 0; i < 8; ++i) V[i] = element<T>(v[i]);
     if (c + 1 < chunks) fetch(c + 1);
 
-    if (a.states && c % (kSegment / kChunk) == 0 && mine) {
+    if (KEEP && c % (kSegment / kChunk) == 0 && mine) {
       float* st = a.states + (size_t(sp.segment + c / (kSegment / kChunk)) * a.Hv + h) * a.dk * a.dv + col;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -342,7 +365,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && WIDE ? 2 : 1) void delta_wal
       const Rows yy(static_cast<T*>(a.y) + head, y_row, rows, a.dv);
 #pragma unroll
       for (int i = 0; i < 8; ++i) store_element<T>(yy, yy.at<T, true>(unit_row(4 * g, i), col, a.dv), qs[i / 4][i % 4]);
-      if (a.errors) {
+      if constexpr (KEEP) {
         const Rows ee(a.errors + head, y_row, rows, a.dv);
 #pragma unroll
         for (int i = 0; i < 8; ++i) store_element<float>(ee, ee.at<float, true>(unit_row(4 * g, i), col, a.dv), E[i]);
@@ -473,10 +496,12 @@ bool wide_rows(const TokenRows& r, int heads, int n) {
 template <typename T, bool WIDE>
 void run_as(const DeltaRule& a, hipStream_t s) {
   const int n = a.offsets ? a.nseq : a.B, slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
-  if (slots) delta_prepare<T, WIDE, false><<<dim3(slots, a.Hk), 64, 0, s>>>(a);
+  if (slots) delta_prepare<T, WIDE, false><<<dim3(slots, (a.Hv + 1) / 2), 64, 0, s>>>(a);
   const dim3 grid(n * a.Hv, (a.dv + kWalkColumns - 1) / kWalkColumns);
-  if (a.dk <= 64) delta_walk<64, T, WIDE><<<grid, 256, 0, s>>>(a);
-  else delta_walk<128, T, WIDE><<<grid, 256, 0, s>>>(a);
+  if (a.errors && a.dk <= 64) delta_walk<64, T, WIDE, true><<<grid, 256, 0, s>>>(a);
+  else if (a.errors) delta_walk<128, T, WIDE, true><<<grid, 256, 0, s>>>(a);
+  else if (a.dk <= 64) delta_walk<64, T, WIDE, false><<<grid, 256, 0, s>>>(a);
+  else delta_walk<128, T, WIDE, false><<<grid, 256, 0, s>>>(a);
 }
 
 template <typename T>
@@ -501,13 +526,13 @@ int delta_rule_slots(int B, int T, int nseq, bool packed) { return packed ? T / 
 int delta_rule_segments(int B, int T, int nseq, bool packed) { return packed ? T / kSegment + nseq : B * segments_of(T); }
 
 size_t delta_rule_workspace(int B, int T, int Hv, int nseq, bool packed) {
-  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float> * sizeof(uint4) + 96 * sizeof(float));
+  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float> * sizeof(uint4) + 96 * sizeof(float)) + 256 * sizeof(uint4);
 }
 
 hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s) {
   const size_t heads = size_t(delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr)) * a.Hv;
   a.units = static_cast<uint4*>(workspace);
-  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float> : kUnits<Bf16>));
+  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float> : kUnits<Bf16>));   // 160 more behind the last
   if (dtype == 0) run<float>(a, s);
   else run<Bf16>(a, s);
   return hipGetLastError();

@@ -1007,7 +1007,7 @@ int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const
  *                zero_tail != 0 set to zero
  *   errors       NULL, or (B, T, Hv, dv) float32 out: e, which the adjoint reads; rows behind the last sequence are left
  *   states       NULL, or (cssm_delta_rule_segments, Hv, dk, dv) float32 out: the state before every 128th row of each
- *                sequence, which the adjoint reads
+ *                sequence, which the adjoint reads; given with errors or not at all
  *   workspace    cssm_delta_rule_workspace_size bytes, 16-byte aligned
  * dk and dv to 128 (CSSM_ERR_UNSUPPORTED otherwise).  The outputs do not overlap the inputs.  Sums and states are float32.
  * Rows are taken 32 at a time: a value that is not finite spoils its sequence from the 32 rows on in which it stands.
