@@ -181,6 +181,9 @@ SIGNATURES = {
     "cssm_delta_rule_workspace_size": (_Z, [_I, _I, _I, _I, _I]),
     "cssm_delta_rule": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I, _P, _I, _P, _P, _P, _P, _Z,
                              _P]),
+    "cssm_delta_rule_bwd_workspace_size": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
+    "cssm_delta_rule_bwd": (_I, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P,
+                                 _P, _P, _Z, _P]),
     "cssm_delta_rule_step": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P]),
     "cssm_block_residual": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                                            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,

@@ -1507,6 +1507,32 @@ int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cs
   return hip_status(cssm::launch_delta_rule(a, dtype, workspace, static_cast<hipStream_t>(stream)), who);
 }
 
+size_t cssm_delta_rule_bwd_workspace_size(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, int packed) {
+  return B <= 0 || T < 0 || Hk <= 0 || Hv <= 0 || dk <= 0 || dv <= 0 || nseq < 0
+             ? 0 : cssm::delta_rule_bwd_workspace(B, T, Hk, Hv, dk, dv, nseq, packed != 0);
+}
+
+int cssm_delta_rule_bwd(const cssm_token_rows* q, const cssm_token_rows* k, int dtype, const cssm_token_rows* beta,
+                        const cssm_token_rows* decay, const cssm_token_rows* dy, int B, int T, int Hk, int Hv, int dk, int dv,
+                        float scale, const int* offsets, int nseq, const float* errors, const float* states, const float* dh,
+                        void* dq, void* dk_out, void* dv_out, float* dbeta, float* ddecay, float* dh0, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  const char* who = "cssm_delta_rule_bwd";
+  DeltaRule a = {};
+  if (const int st = delta_rule_args(who, a, q, k, dy, dtype, beta, decay, B, T, Hk, Hv, dk, dv, scale, offsets, nseq)) return st;
+  if (B == 0) return ok();
+  if (T > 0 && (!errors || !states || !dq || !dk_out || !dv_out || !dbeta || !decay != !ddecay))
+    return fail(CSSM_ERR_NULL, "%s: errors, states and the gradients must be non-null", who);
+  if (const int st = delta_workspace_check(
+          who, cssm_delta_rule_bwd_workspace_size(B, T, Hk, Hv, dk, dv, offsets ? nseq : 0, offsets != nullptr), workspace, workspace_bytes))
+    return st;
+  if (const int st = token_align_check(who, dtype, {dq, dk_out, dv_out}, {errors, states, dh, dbeta, ddecay, dh0})) return st;
+  a.dy = a.v, a.v = rows_of(nullptr);
+  a.errors = const_cast<float*>(errors), a.states = const_cast<float*>(states), a.dh = dh;
+  a.dq = dq, a.dkey = dk_out, a.dv_out = dv_out, a.dbeta = dbeta, a.ddecay = ddecay, a.dh0 = dh0;
+  return hip_status(cssm::launch_delta_rule_bwd(a, dtype, workspace, static_cast<hipStream_t>(stream)), who);
+}
+
 int cssm_delta_rule_step(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v, int dtype,
                          const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int Hk, int Hv, int dk, int dv,
                          float scale, const float* state, void* y, float* state_out, void* stream) {

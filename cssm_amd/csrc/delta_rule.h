@@ -243,6 +243,12 @@ struct Columns {
   }
 };
 
+// parts of P: those that y's type shows; its transpose has all, since the gates' gradients are float32
+template <typename T, bool TURNED>
+constexpr int kPParts = sizeof(T) == 2 && !TURNED ? 2 : 3;
+template <typename T, bool TURNED>
+constexpr int kUnits = (3 + kPParts<T, TURNED>) * 128;   // units of L and P of one chunk and head
+
 // ---- sequences and their chunks
 
 struct Span { int row, rows, slot, segment; };   // first row, number of rows, first chunk's and first segment's slot
@@ -258,6 +264,17 @@ __device__ __forceinline__ Span span_of(const DeltaRule& a, int i) {
   hi = hi < lo ? lo : hi > a.T ? a.T : hi;
   return {lo, hi - lo, lo / kChunk + i, lo / kSegment + i};
 }
+
+// rows that WIDE takes: 16-byte vectors, and none overlapping the next
+template <typename T>
+inline bool wide_rows(const TokenRows& r, int heads, int n) {
+  return n % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.batch * (long long)sizeof(T) % 16 == 0 &&
+         r.row * (long long)sizeof(T) % 16 == 0 && r.row >= (long long)heads * n;
+}
+
+// L and P of all chunks, or their transposes and D, into the workspace
+template <typename T, bool TURNED>
+void launch_delta_prepare(const DeltaRule& a, bool wide, hipStream_t s);
 
 // batch b's row t of a tensor of rows
 template <typename T>

@@ -57,12 +57,6 @@ __device__ __forceinline__ f32x16_t product32(const Unit (&a)[N], const Unit (&b
   return c;
 }
 
-// parts of P: those that y's type shows
-template <typename T>
-constexpr int kPParts = sizeof(T) == 2 ? 2 : 3;
-template <typename T>
-constexpr int kUnits = (3 + kPParts<T>) * 128;   // units of L and P of one chunk and head
-
 // The chunk that a slot of the workspace stands for; false for a slot that no chunk takes
 __device__ __forceinline__ bool chunk_at(const DeltaRule& a, int slot, int& b, int& row, int& rows) {
   b = 0;
@@ -142,6 +136,7 @@ __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
   for (int i = 0; i < kChunk; ++i) {
     const bool at = i == j;
     d = at ? 1.0f : d * s_alpha[half][i];   // 0 above the diagonal
+    if (TURNED && on) a.decays[(size_t(slot) * a.Hv + h) * (kChunk * kChunk) + i * kChunk + j] = d;
     A[i] = at ? 0.0f : d * A[i];
     P[i] *= d * a.scale;
     s_m[half][i * kPad + j] = A[i] * beta;
@@ -179,7 +174,7 @@ __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
       if (o == 1 && !two) break;
-      uint4* u = a.units + (size_t(slot) * a.Hv + h0 + o) * kUnits<T> + (what ? 3 * 128 : 0);
+      uint4* u = a.units + (size_t(slot) * a.Hv + h0 + o) * kUnits<T, TURNED> + (what ? 3 * 128 : 0);
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
         const int r = 16 * tile + lane % 16, c = lane / 16 * 4;
@@ -190,10 +185,10 @@ __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
           v[i] = TURNED ? s_m[o][cc * kPad + r] : s_m[o][r * kPad + cc];
         }
         if (what) {
-          Unit w[kPParts<T>];
-          split<kPParts<T>>(v, w);
+          Unit w[kPParts<T, TURNED>];
+          split<kPParts<T, TURNED>>(v, w);
 #pragma unroll
-          for (int n = 0; n < kPParts<T>; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
+          for (int n = 0; n < kPParts<T, TURNED>; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
         } else {
           Unit w[3];
           split<3>(v, w);
@@ -210,7 +205,7 @@ constexpr int kWalkColumns = 64;   // of a workgroup: 16 for each of its four wa
 template <int DKP, typename T>
 struct WalkLds {
   static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
-  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[(kUnits<T> + 255) / 256 * 256];
+  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[(kUnits<T, false> + 255) / 256 * 256];
   float gains[256];   // gamma, d, beta; the rest takes what threads without a value write
 };
 
@@ -219,8 +214,8 @@ struct WalkLds {
 template <int DKP, typename T, bool WIDE, bool KEEP>
 __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
   using Lds = WalkLds<DKP, T>;
-  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, PP = kPParts<T>;
-  constexpr int LP = (kUnits<T> + 255) / 256;
+  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, PP = kPParts<T, false>;
+  constexpr int LP = (kUnits<T, false> + 255) / 256;
   __shared__ Lds lds[Lds::kBufs];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
   const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
@@ -260,7 +255,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
     const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
     const Rows vv(row_at<T>(a.v, b, t) + h * a.dv, a.v.row, rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
-    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T> + tid;   // the last ones past this chunk's: into the next, or the end's room
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T, false> + tid;   // the last ones past this chunk's: into the next, or the end's room
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
     if (p_on) pk.load(k, p_tok, p_col, a.dk), pq.load(q, p_tok, p_col, a.dk);
@@ -486,17 +481,10 @@ __global__ __launch_bounds__(256) void delta_step(DeltaRule a) {
   }
 }
 
-// rows that WIDE takes: 16-byte vectors, and none overlapping the next
-template <typename T>
-bool wide_rows(const TokenRows& r, int heads, int n) {
-  return n % 8 == 0 && reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.batch * (long long)sizeof(T) % 16 == 0 &&
-         r.row * (long long)sizeof(T) % 16 == 0 && r.row >= (long long)heads * n;
-}
-
 template <typename T, bool WIDE>
 void run_as(const DeltaRule& a, hipStream_t s) {
-  const int n = a.offsets ? a.nseq : a.B, slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
-  if (slots) delta_prepare<T, WIDE, false><<<dim3(slots, (a.Hv + 1) / 2), 64, 0, s>>>(a);
+  const int n = a.offsets ? a.nseq : a.B;
+  launch_delta_prepare<T, false>(a, WIDE, s);
   const dim3 grid(n * a.Hv, (a.dv + kWalkColumns - 1) / kWalkColumns);
   if (a.errors && a.dk <= 64) delta_walk<64, T, WIDE, true><<<grid, 256, 0, s>>>(a);
   else if (a.errors) delta_walk<128, T, WIDE, true><<<grid, 256, 0, s>>>(a);
@@ -521,18 +509,29 @@ void step(DeltaRule& a, hipStream_t s) {
 
 }  // namespace
 
+template <typename T, bool TURNED>
+void launch_delta_prepare(const DeltaRule& a, bool wide, hipStream_t s) {
+  const int slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
+  if (!slots) return;
+  const dim3 grid(slots, (a.Hv + 1) / 2);
+  if (wide) delta_prepare<T, true, TURNED><<<grid, 64, 0, s>>>(a);
+  else delta_prepare<T, false, TURNED><<<grid, 64, 0, s>>>(a);
+}
+template void launch_delta_prepare<float, true>(const DeltaRule&, bool, hipStream_t);
+template void launch_delta_prepare<Bf16, true>(const DeltaRule&, bool, hipStream_t);
+
 int delta_rule_slots(int B, int T, int nseq, bool packed) { return packed ? T / kChunk + nseq : B * chunks_of(T); }
 
 int delta_rule_segments(int B, int T, int nseq, bool packed) { return packed ? T / kSegment + nseq : B * segments_of(T); }
 
 size_t delta_rule_workspace(int B, int T, int Hv, int nseq, bool packed) {
-  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float> * sizeof(uint4) + 96 * sizeof(float)) + 256 * sizeof(uint4);
+  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float, false> * sizeof(uint4) + 96 * sizeof(float)) + 256 * sizeof(uint4);
 }
 
 hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s) {
   const size_t heads = size_t(delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr)) * a.Hv;
   a.units = static_cast<uint4*>(workspace);
-  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float> : kUnits<Bf16>));   // 160 more behind the last
+  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float, false> : kUnits<Bf16, false>));   // 160 more behind the last
   if (dtype == 0) run<float>(a, s);
   else run<Bf16>(a, s);
   return hipGetLastError();

@@ -1,0 +1,649 @@
+// Adjoint of the gated delta rule over token sequences (gfx950).  In a chunk (csrc/delta_rule.hip has the forward's form and
+// its L, P, D, gamma, d), with E the errors and S the states that the forward kept, U = beta E, and dS the state's gradient:
+//   dU = P^T dY + d K dS',  X = dU - L^T beta dU,  dV = beta X,  dbeta = X.E (row by row)
+//   dS <- gamma_31 dS' + scale Q^T gamma dY - K^T gamma beta X
+//   Y_ij = scale D_ij dY_i.U_j (i >= j),  Z_ij = D_ij beta_i X_i.U_j (i > j)
+//   dQ = Y K + scale gamma dY S^T,  read = -Z K - gamma beta X S^T,  write = Y^T Q - Z^T K + d U dS'^T,  dK = read + write
+// A decay enters through products over the rows between a reader and a writer, so its gradient is what the rows from it on
+// read, less what they write, down to the end, where the rest of the sequence enters as one number:
+//   ddecay_l = <S, dS>_end + sum over i >= l of (q_i.dq_i + k_i.read_i - k_i.write_i)
+// delta_walk_back carries dS from chunk to chunk, as the forward does S, and keeps it behind every 128th row; then
+// delta_grads takes each 128 rows by themselves, forwards with S and backwards with dS, a wave 16 of the keys' columns, so
+// that the sums over dv lie within a wave.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "delta_rule.h"
+#include "launch.h"
+#include "token_util.h"
+
+namespace cssm {
+
+namespace {
+
+constexpr int kBackColumns = 64;   // of a workgroup: 16 for each of its four waves
+constexpr int kChunks = kSegment / kChunk;
+
+template <int DKP, typename T>
+struct BackLds {
+  static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
+  uint4 k[kN * kPlane], kt[kN * kPlane], qt[kN * kPlane], lp[kUnits<T, true>];
+  float gains[256];
+};
+
+// 8 values of a result's rows from LDS: those of the rows that a lane holds
+__device__ __forceinline__ void take_rows(const float* s, int g, float (&v)[8]) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const float4 q = *reinterpret_cast<const float4*>(s + 16 * t + 4 * g);
+    v[4 * t] = q.x, v[4 * t + 1] = q.y, v[4 * t + 2] = q.z, v[4 * t + 3] = q.w;
+  }
+}
+
+template <int DKP, typename T, bool WIDE>
+__global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
+  using Lds = BackLds<DKP, T>;
+  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, LP = kUnits<T, true> / 256;
+  __shared__ Lds lds[Lds::kBufs];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
+  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int b = a.offsets ? 0 : seq;
+  const Span sp = span_of(a, seq);
+  const int chunks = chunks_of(sp.rows);
+  const int col = blockIdx.y * kBackColumns + wave * 16 + lane % 16;
+  const bool mine = col < a.dv;
+  const size_t state = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
+  const int v_row = a.Hv * a.dv;
+
+  f32x4_t S[MT];   // the state's gradient
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * m + 4 * g + i;
+      S[m][i] = a.dh && mine && r < a.dk ? a.dh[state + size_t(r) * a.dv] : 0.0f;
+    }
+
+  const int p_tok = tid % 8 + tid / (8 * 2 * KS) * 8, p_at = tid / 8 % (2 * KS);
+  const bool p_on = KS == 4 || tid < 64 * KS;
+  const int p_col = p_at / 2 * 32 + p_at % 2 * 8;
+  const int p_unit = ((p_at / 2 * 2 + p_tok / 16) * 4 + p_at % 2 * 2) * 16 + p_tok % 16;
+  const int c_g = tid / (DKP / 2), c_col = tid % (DKP / 2) * 2;
+  const bool c_on = DKP == 128 || tid < 2 * DKP;
+  const int c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
+  Piece<T, WIDE> pk;
+  Columns<T, WIDE> ck, cq;
+  u32x4_t lp[LP];
+  float gain;
+  uint32_t dy[8];
+  const auto fetch = [&](int c) {
+    const long long t = sp.row + (long long)c * kChunk;
+    const int rows = sp.rows - c * kChunk;
+    const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
+    const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
+    const size_t head = size_t(sp.slot + c) * a.Hv + h;
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T, true> + tid;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dy[i] = load_element<T>(y, y.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
+    if (p_on) pk.load(k, p_tok, p_col, a.dk);
+    if (c_on) ck.load(k, 4 * c_g, c_col, a.dk), cq.load(q, 4 * c_g, c_col, a.dk);
+#pragma unroll
+    for (int i = 0; i < LP; ++i) lp[i] = units[256 * i];
+    gain = a.gains[head * 96 + tid];   // past the 96: the next ones, or the room behind the last
+  };
+  const auto stash = [&](Lds& to) {
+    if (p_on) pk.store(to.k + p_unit, PLANE);
+    if (c_on) ck.store(to.kt + c_unit, PLANE), cq.store(to.qt + c_unit, PLANE);
+#pragma unroll
+    for (int i = 0; i < LP; ++i) to.lp[tid + 256 * i] = __builtin_bit_cast(uint4, lp[i]);
+    to.gains[tid] = gain;
+  };
+
+  if (chunks) {
+    fetch(chunks - 1);
+    stash(lds[(chunks - 1) % Lds::kBufs]);
+  }
+  for (int c = chunks - 1; c >= 0; --c) {
+    __syncthreads();
+    const Lds& in = lds[c % Lds::kBufs];
+    float dY[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dY[i] = element<T>(dy[i]);
+    if (c > 0) fetch(c - 1);
+
+    if ((c % kChunks == kChunks - 1 || c == chunks - 1) && mine) {
+      float* st = a.dstates + (size_t(sp.segment + c / kChunks) * a.Hv + h) * a.dk * a.dv + col;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * m + 4 * g + i < a.dk) st[size_t(16 * m + 4 * g + i) * a.dv] = S[m][i];
+    }
+    f32x4_t ks[2] = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
+                          S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
+      Unit u[3];
+      split<3>(x, u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[N];
+        take(in.k + (s * 2 + t) * 64 + lane, PLANE, w);
+        ks[t] = product(w, u, ks[t]);
+      }
+    }
+    float gm[8], dd[8], bt[8], x[8], dU[8], X[8];
+    take_rows(in.gains, g, gm), take_rows(in.gains + 32, g, dd), take_rows(in.gains + 64, g, bt);
+    {
+      Unit u[N];
+      split<N>(dY, u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[3];
+        take(in.lp + 3 * 128 + t * 64 + lane, 128, w);
+        const f32x4_t py = product(w, u, f32x4_t{});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dU[4 * t + i] = py[i] + dd[4 * t + i] * ks[t][i], x[4 * t + i] = bt[4 * t + i] * dU[4 * t + i];
+      }
+    }
+    {
+      Unit u[3];
+      split<3>(x, u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[3];
+        take(in.lp + t * 64 + lane, 128, w);
+        const f32x4_t le = product(w, u, f32x4_t{});
+#pragma unroll
+        for (int i = 0; i < 4; ++i) X[4 * t + i] = dU[4 * t + i] - le[i];
+      }
+    }
+    {
+      const int rows = sp.rows - c * kChunk;
+      const size_t head = ((size_t(b) * a.T + sp.row + (long long)c * kChunk) * a.Hv + h) * a.dv;
+      const Rows dv(static_cast<T*>(a.dv_out) + head, v_row, rows, a.dv), xx(a.duals + head, v_row, rows, a.dv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        store_element<T>(dv, dv.at<T, true>(unit_row(4 * g, i), col, a.dv), bt[i] * X[i]);
+        store_element<float>(xx, xx.at<float, true>(unit_row(4 * g, i), col, a.dv), X[i]);
+      }
+    }
+    {
+      float z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = a.scale * gm[i] * dY[i], z[i] = -gm[i] * bt[i] * X[i];
+      Unit u[3], v[3];
+      split<3>(x, u), split<3>(z, v);
+      const float all = in.gains[31];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        Unit w[N];
+        S[m] *= all;
+        take(in.qt + m * 64 + lane, PLANE, w);
+        S[m] = product(w, u, S[m]);
+        take(in.kt + m * 64 + lane, PLANE, w);
+        S[m] = product(w, v, S[m]);
+      }
+    }
+    if (c > 0) {
+      if (Lds::kBufs == 1) __syncthreads();
+      stash(lds[(c - 1) % Lds::kBufs]);
+    }
+  }
+  if (a.dh0 && mine)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * m + 4 * g + i;
+        if (r < a.dk) a.dh0[state + size_t(r) * a.dv] = S[m][i];
+      }
+}
+
+// the value of element i of a lane's unit, all parts together
+template <int N>
+__device__ __forceinline__ float value_of(const Unit (&u)[N], int i) {
+  float v = 0.0f;
+#pragma unroll
+  for (int n = N - 1; n >= 0; --n) v += __uint_as_float(i % 2 ? u[n].w[i / 2] & 0xffff0000u : u[n].w[i / 2] << 16);
+  return v;
+}
+
+// P: dk and dv up to it.  One workgroup for 128 rows of one value head, P / 16 waves.
+template <int P, typename T, bool WIDE>
+__global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
+  constexpr int N = PartsOf<T>::n, W = P / 16, KS = P / 32, MT = P / 16, PLANE = P * 4, TASKS = (6 + W - 1) / W;
+  constexpr int UROOM = 3 * PLANE > 12 * 128 ? 3 * PLANE : 12 * 128;
+  __shared__ uint4 s_y[N * PLANE], s_x[3 * PLANE], s_u[UROOM], s_ut[3 * PLANE], s_kt[N * PLANE], s_qt[N * PLANE];
+  __shared__ __attribute__((aligned(16))) float s_gains[kChunks][96];
+  __shared__ float s_read[W][kSegment], s_write[W][kSegment], s_sum[W];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, h = blockIdx.y, hk = h / (a.Hv / a.Hk);
+  const bool shared = a.Hv != a.Hk;
+  int seq, seg, b = 0;
+  if (!a.offsets) {
+    const int n = segments_of(a.T);
+    seq = b = blockIdx.x / n, seg = blockIdx.x - seq * n;
+  } else {
+    int lo = 0, hi = a.nseq;   // the last sequence whose segments begin at or before this slot
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (span_of(a, mid).segment <= int(blockIdx.x)) lo = mid;
+      else hi = mid;
+    }
+    seq = lo, seg = blockIdx.x - span_of(a, lo).segment;
+  }
+  const Span sp = span_of(a, seq);
+  if (seg < 0 || seg >= segments_of(sp.rows)) return;
+  const int row0 = sp.row + seg * kSegment;
+  const int left = sp.rows - seg * kSegment, rows_all = left < kSegment ? left : kSegment, chunks = chunks_of(rows_all);
+  const size_t slot0 = size_t(sp.slot) + size_t(seg) * kChunks;
+  const int col = wave * 16 + lane % 16;   // of the keys
+  const bool mine = col < a.dk;
+  const int v_row = a.Hv * a.dv;
+  for (int i = tid; i < chunks * 96; i += 4 * P) s_gains[i / 96][i % 96] = a.gains[((slot0 + i / 96) * a.Hv + h) * 96 + i % 96];
+
+  // S^T, or its gradient's: rows of dv, a lane one column of dk
+  f32x4_t S[MT];
+  const auto load_state = [&](const float* from) {
+    const float* p = from + (size_t(sp.segment + seg) * a.Hv + h) * a.dk * a.dv + size_t(col) * a.dv;
+    f32x4_t r[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[m][i] = mine && 16 * m + 4 * g + i < a.dv ? p[16 * m + 4 * g + i] : 0.0f;
+    float with = 0.0f;   // <S, r>
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) with = fmaf(S[m][i], r[m][i], with), S[m][i] = r[m][i];
+    return with;
+  };
+#pragma unroll
+  for (int m = 0; m < MT; ++m) S[m] = f32x4_t{};
+  load_state(a.states);
+
+  // the first half of the threads takes E and X, the second dy, k and q
+  const bool first = tid < 2 * P;
+  const int id = first ? tid : tid - 2 * P;
+  const int p_tok = id % 8 + id / (8 * 2 * KS) * 8, p_at = id / 8 % (2 * KS), p_col = p_at / 2 * 32 + p_at % 2 * 8;
+  const int p_unit = ((p_at / 2 * 2 + p_tok / 16) * 4 + p_at % 2 * 2) * 16 + p_tok % 16;
+  const int c_g = id / (P / 2), c_col = id % (P / 2) * 2, c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
+  const auto head_of = [&](int c) { return ((size_t(b) * a.T + row0 + c * kChunk) * a.Hv + h) * a.dv; };
+
+  {
+    Piece<float, WIDE> px, pe;
+    Columns<float, WIDE> ce;
+    Piece<T, WIDE> py;
+    Columns<T, WIDE> ck, cq;
+    const auto fetch = [&](int c) {
+      const int rows = rows_all - c * kChunk;
+      const long long t = row0 + c * kChunk;
+      if (first) {
+        const Rows x(a.duals + head_of(c), v_row, rows, a.dv), e(a.errors + head_of(c), v_row, rows, a.dv);
+        px.load(x, p_tok, p_col, a.dv), pe.load(e, p_tok, p_col, a.dv);
+        ce.load(e, 4 * c_g, c_col, a.dv);
+      } else {
+        const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
+        const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
+        py.load(y, p_tok, p_col, a.dv);
+        ck.load(k, 4 * c_g, c_col, a.dk), cq.load(q, 4 * c_g, c_col, a.dk);
+      }
+    };
+    fetch(0);
+    for (int c = 0; c < chunks; ++c) {
+      const int rows = rows_all - c * kChunk;
+      __syncthreads();
+      const float* gains = s_gains[c];
+      if (first) {
+        const float beta = gains[64 + p_tok];
+        px.template store_by<3>(beta, s_x + p_unit, PLANE);
+        pe.template store_by<3>(beta, s_u + p_unit, PLANE);
+        float by[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) by[j] = gains[64 + unit_row(4 * c_g, j)] * gains[32 + unit_row(4 * c_g, j)];
+        ce.template store_by<3>(by, s_ut + c_unit, PLANE);
+        float dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dot = fmaf(px.get(i), pe.get(i), dot);
+#pragma unroll
+        for (int o = 8; o < 16 * KS; o *= 2) dot += __shfl_xor(dot, o);
+        if (p_at == 0 && p_tok < rows) a.dbeta[(size_t(b) * a.T + row0 + c * kChunk + p_tok) * a.Hv + h] = dot;
+      } else {
+        py.store(s_y + p_unit, PLANE);
+        ck.store(s_kt + c_unit, PLANE), cq.store(s_qt + c_unit, PLANE);
+      }
+      __syncthreads();
+      if (c + 1 < chunks) fetch(c + 1);
+
+      // Y and Z, a 16 x 16 tile a wave: (0, 0), (1, 0) and (1, 1) of both
+      f32x4_t tile[TASKS];
+#pragma unroll
+      for (int n = 0; n < TASKS; ++n) {
+        const int task = wave + n * W, z = task / 3, ti = task % 3 > 0, tj = task % 3 == 2;
+        tile[n] = f32x4_t{};
+        if (task < 6) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            Unit u[3];
+            take(s_u + (s * 2 + tj) * 64 + lane, PLANE, u);
+            if (z) {
+              Unit w[3];
+              take(s_x + (s * 2 + ti) * 64 + lane, PLANE, w);
+              tile[n] = product(w, u, tile[n]);
+            } else {
+              Unit w[N];
+              take(s_y + (s * 2 + ti) * 64 + lane, PLANE, w);
+              tile[n] = product(w, u, tile[n]);
+            }
+          }
+          const float* D = a.decays + ((slot0 + c) * a.Hv + h) * (kChunk * kChunk) + 16 * tj + lane % 16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 16 * ti + 4 * g + i;
+            tile[n][i] *= z ? (r == 16 * tj + lane % 16 ? 0.0f : D[r * kChunk]) : a.scale * D[r * kChunk];
+          }
+        }
+      }
+      f32x4_t ys[2] = {}, xs[2] = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
+                            S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
+        Unit u[3];
+        split<3>(x, u);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Unit w[N], w3[3];
+          take(s_y + (s * 2 + t) * 64 + lane, PLANE, w);
+          ys[t] = product(w, u, ys[t]);
+          take(s_x + (s * 2 + t) * 64 + lane, PLANE, w3);
+          xs[t] = product(w3, u, xs[t]);
+        }
+      }
+      __syncthreads();   // U's rows are read: Y, Z, Y^T and Z^T take their place, 3 parts of 128 units each
+#pragma unroll
+      for (int n = 0; n < TASKS; ++n) {
+        const int task = wave + n * W, z = task / 3, ti = task % 3 > 0, tj = task % 3 == 2;
+        if (task < 6) {
+          const float v[8] = {tile[n][0], tile[n][1], tile[n][2], tile[n][3], 0.0f, 0.0f, 0.0f, 0.0f};
+          Unit u[3];
+          split<3>(v, u);
+          uint16_t* rows16 = reinterpret_cast<uint16_t*>(s_u + z * 3 * 128);
+          uint2* turned = reinterpret_cast<uint2*>(s_u + (2 + z) * 3 * 128);
+          const int j = lane % 16;
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            // row 16 ti + 4 g + i, column 16 tj + j: unit (ti, j / 4, row), place 4 tj + j % 4
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint16_t* at = rows16 + (p * 128 + ti * 64 + j / 4 * 16 + 4 * g + i) * 8 + j % 4;
+              at[4 * tj] = uint16_t(u[p].w[i / 2] >> (i % 2 * 16));
+              if (ti == 0) at[4] = 0;                            // tile (0, 1)
+            }
+            // turned: row 16 tj + j, columns 16 ti + 4 g + 0 .. 3: unit (tj, g, j), places 4 ti ..
+            uint2* at = turned + (p * 128 + tj * 64 + g * 16 + j) * 2;
+            at[ti] = make_uint2(u[p].w[0], u[p].w[1]);
+            if (tj == 1) at[0] = make_uint2(0u, 0u);
+          }
+        }
+      }
+      __syncthreads();
+      Unit kb[N], qb[N];
+      take(s_kt + wave * 64 + lane, PLANE, kb);
+      take(s_qt + wave * 64 + lane, PLANE, qb);
+      float gm[8], dq[8], rd[8], wr[8];
+      take_rows(gains, g, gm);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ys[t][i] *= a.scale * gm[4 * t + i], xs[t][i] *= gm[4 * t + i];
+        f32x4_t yq = {}, zk = {};
+        take(s_u + t * 64 + lane, 128, w);
+        ys[t] = product(w, kb, ys[t]);
+        take(s_u + 384 + t * 64 + lane, 128, w);
+        xs[t] = product(w, kb, xs[t]);
+        take(s_u + 768 + t * 64 + lane, 128, w);
+        yq = product(w, qb, yq);
+        take(s_u + 1152 + t * 64 + lane, 128, w);
+        zk = product(w, kb, zk);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dq[4 * t + i] = ys[t][i], rd[4 * t + i] = -xs[t][i], wr[4 * t + i] = yq[i] - zk[i];
+      }
+      const float all = gains[31];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        Unit w[3];
+        take(s_ut + m * 64 + lane, PLANE, w);
+        S[m] = product(w, kb, S[m] * all);
+      }
+      const size_t at_row = size_t(b) * a.T + row0 + c * kChunk;
+      const Rows dkh(a.dk_heads + (at_row * a.Hv + h) * a.dk, a.Hv * a.dk, rows, a.dk);
+      const Rows dqh(shared ? a.dq_heads + (at_row * a.Hv + h) * a.dk : nullptr, a.Hv * a.dk, shared ? rows : 0, a.dk);
+      const Rows dqo(static_cast<T*>(a.dq) + (at_row * a.Hk + hk) * a.dk, a.Hk * a.dk, shared ? 0 : rows, a.dk);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = unit_row(4 * g, i);
+        store_element<float>(dkh, dkh.at<float, true>(r, col, a.dk), rd[i] + wr[i]);
+        if (shared) store_element<float>(dqh, dqh.at<float, true>(r, col, a.dk), dq[i]);
+        else store_element<T>(dqo, dqo.at<T, true>(r, col, a.dk), dq[i]);
+        const float kv = value_of(kb, i);
+        float x = fmaf(value_of(qb, i), dq[i], kv * rd[i]), y = kv * wr[i];
+#pragma unroll
+        for (int o = 1; o < 16; o *= 2) x += __shfl_xor(x, o), y += __shfl_xor(y, o);
+        if (lane % 16 == 0) s_read[wave][c * kChunk + r] = x, s_write[wave][c * kChunk + r] = y;
+      }
+    }
+  }
+
+  float with = load_state(a.dstates);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) with += __shfl_xor(with, o);
+  if (lane == 0) s_sum[wave] = with;
+  {
+    Piece<float, WIDE> pe;
+    Columns<float, WIDE> cx;
+    Columns<T, WIDE> cy, ck, cq;
+    float part[8];
+    const auto fetch = [&](int c) {
+      const int rows = rows_all - c * kChunk;
+      const long long t = row0 + c * kChunk;
+      const size_t at_row = size_t(b) * a.T + t;
+      const Rows dkh(a.dk_heads + (at_row * a.Hv + h) * a.dk, a.Hv * a.dk, rows, a.dk);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part[i] = element<float>(load_element<float>(dkh, dkh.at<float, true>(unit_row(4 * g, i), col, a.dk)));
+      if (first) {
+        const Rows x(a.duals + head_of(c), v_row, rows, a.dv), e(a.errors + head_of(c), v_row, rows, a.dv);
+        pe.load(e, p_tok, p_col, a.dv);
+        cx.load(x, 4 * c_g, c_col, a.dv);
+      } else {
+        const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
+        const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
+        cy.load(y, 4 * c_g, c_col, a.dv);
+        ck.load(k, 4 * c_g, c_col, a.dk), cq.load(q, 4 * c_g, c_col, a.dk);
+      }
+    };
+    fetch(chunks - 1);
+    for (int c = chunks - 1; c >= 0; --c) {
+      const int rows = rows_all - c * kChunk;
+      __syncthreads();
+      const float* gains = s_gains[c];
+      if (first) {
+        pe.template store_by<3>(gains[64 + p_tok], s_u + p_unit, PLANE);
+        float by[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) by[j] = -gains[64 + unit_row(4 * c_g, j)] * gains[unit_row(4 * c_g, j)];
+        cx.template store_by<3>(by, s_ut + c_unit, PLANE);
+      } else {
+        float by[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) by[j] = a.scale * gains[unit_row(4 * c_g, j)];
+        cy.template store_by<3>(by, s_x + c_unit, PLANE);
+        ck.store(s_kt + c_unit, PLANE), cq.store(s_qt + c_unit, PLANE);
+      }
+      float before[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) before[i] = part[i];
+      __syncthreads();
+      if (c > 0) fetch(c - 1);
+      f32x4_t us[2] = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
+                            S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
+        Unit u[3];
+        split<3>(x, u);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Unit w[3];
+          take(s_u + (s * 2 + t) * 64 + lane, PLANE, w);
+          us[t] = product(w, u, us[t]);
+        }
+      }
+      Unit kb[N], qb[N];
+      take(s_kt + wave * 64 + lane, PLANE, kb);
+      take(s_qt + wave * 64 + lane, PLANE, qb);
+      const float all = gains[31];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        Unit w[3];
+        S[m] *= all;
+        take(s_x + m * 64 + lane, PLANE, w);
+        S[m] = product(w, qb, S[m]);
+        take(s_ut + m * 64 + lane, PLANE, w);
+        S[m] = product(w, kb, S[m]);
+      }
+      float dd[8];
+      take_rows(gains + 32, g, dd);
+      const size_t at_row = size_t(b) * a.T + row0 + c * kChunk;
+      const Rows dkh(a.dk_heads + (at_row * a.Hv + h) * a.dk, a.Hv * a.dk, rows, a.dk);
+      const Rows dko(static_cast<T*>(a.dkey) + (at_row * a.Hk + hk) * a.dk, a.Hk * a.dk, shared ? 0 : rows, a.dk);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = unit_row(4 * g, i);
+        const float w = dd[i] * us[i / 4][i % 4];
+        if (shared) store_element<float>(dkh, dkh.at<float, true>(r, col, a.dk), before[i] + w);
+        else store_element<T>(dko, dko.at<T, true>(r, col, a.dk), before[i] + w);
+        float y = value_of(kb, i) * w;
+#pragma unroll
+        for (int o = 1; o < 16; o *= 2) y += __shfl_xor(y, o);
+        if (lane % 16 == 0) s_write[wave][c * kChunk + r] += y;
+      }
+    }
+  }
+  __syncthreads();
+  if (a.ddecay && wave == 0) {
+    float v[2];   // rows 2 l and 2 l + 1: what they read less what they write, then summed from the end
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 2 * lane + i;
+      v[i] = 0.0f;
+      if (r < rows_all)
+#pragma unroll
+        for (int w = 0; w < W; ++w) v[i] += s_read[w][r] - s_write[w][r];
+    }
+    float all = v[0] + v[1], rest = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) rest += s_sum[w];
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const float after = __shfl_down(all, o);
+      if (lane + o < 64) all += after;
+    }
+    float behind = __shfl_down(all, 1);
+    behind = lane == 63 ? rest : behind + rest;
+    float* out = a.ddecay + (size_t(b) * a.T + row0) * a.Hv + h;
+    if (2 * lane + 1 < rows_all) out[size_t(2 * lane + 1) * a.Hv] = behind + v[1];
+    if (2 * lane < rows_all) out[size_t(2 * lane) * a.Hv] = behind + v[1] + v[0];
+  }
+}
+
+// the value heads' shares of dq and dk added up
+template <typename T>
+__global__ __launch_bounds__(256) void delta_share(const float* q, const float* k, size_t rows, int Hk, int G, int dk, T* dq, T* dkey) {
+  const size_t n = rows * Hk * dk;
+  for (size_t at = size_t(blockIdx.x) * 256 + threadIdx.x; at < n; at += size_t(gridDim.x) * 256) {
+    const size_t head = at / dk, from = head * G * dk + (at - head * dk);
+    float x = 0.0f, y = 0.0f;
+    for (int i = 0; i < G; ++i) x += q[from + size_t(i) * dk], y += k[from + size_t(i) * dk];
+    put(dq + at, x), put(dkey + at, y);
+  }
+}
+
+// zero behind the last sequence
+template <typename T>
+__global__ __launch_bounds__(256) void delta_tail(DeltaRule a) {
+  const Span sp = span_of(a, a.nseq - 1);
+  const int nk = a.Hk * a.dk, nv = a.Hv * a.dv;
+  for (int t = sp.row + sp.rows + blockIdx.x; t < a.T; t += gridDim.x) {
+    for (int i = threadIdx.x; i < nk; i += 256) {
+      put(static_cast<T*>(a.dq) + size_t(t) * nk + i, 0.0f);
+      put(static_cast<T*>(a.dkey) + size_t(t) * nk + i, 0.0f);
+    }
+    for (int i = threadIdx.x; i < nv; i += 256) put(static_cast<T*>(a.dv_out) + size_t(t) * nv + i, 0.0f);
+    for (int i = threadIdx.x; i < a.Hv; i += 256) {
+      a.dbeta[size_t(t) * a.Hv + i] = 0.0f;
+      if (a.ddecay) a.ddecay[size_t(t) * a.Hv + i] = 0.0f;
+    }
+  }
+}
+
+template <typename T, bool WIDE>
+void run_as(const DeltaRule& a, hipStream_t s) {
+  const int n = a.offsets ? a.nseq : a.B, segments = delta_rule_segments(a.B, a.T, a.nseq, a.offsets != nullptr);
+  launch_delta_prepare<T, true>(a, WIDE, s);
+  const dim3 grid(n * a.Hv, (a.dv + kBackColumns - 1) / kBackColumns);
+  if (a.dk <= 64) delta_walk_back<64, T, WIDE><<<grid, 256, 0, s>>>(a);
+  else delta_walk_back<128, T, WIDE><<<grid, 256, 0, s>>>(a);
+  if (!a.T) return;
+  if (a.dk <= 64 && a.dv <= 64) delta_grads<64, T, WIDE><<<dim3(segments, a.Hv), 256, 0, s>>>(a);
+  else delta_grads<128, T, WIDE><<<dim3(segments, a.Hv), 512, 0, s>>>(a);
+  const size_t rows = size_t(a.B) * a.T, groups = (rows * a.Hk * a.dk + 255) / 256;
+  if (a.Hv != a.Hk)
+    delta_share<T><<<unsigned(groups < 1 << 16 ? groups : 1 << 16), 256, 0, s>>>(a.dq_heads, a.dk_heads, rows, a.Hk, a.Hv / a.Hk,
+                                                                              a.dk, static_cast<T*>(a.dq), static_cast<T*>(a.dkey));
+  if (a.offsets) delta_tail<T><<<a.T < 1024 ? a.T : 1024, 256, 0, s>>>(a);
+}
+
+template <typename T>
+void run(const DeltaRule& a, hipStream_t s) {
+  const bool wide = wide_rows<T>(a.q, a.Hk, a.dk) && wide_rows<T>(a.k, a.Hk, a.dk) && wide_rows<T>(a.dy, a.Hv, a.dv) &&
+                    reinterpret_cast<uintptr_t>(a.errors) % 16 == 0;
+  if (wide) run_as<T, true>(a, s);
+  else run_as<T, false>(a, s);
+}
+
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+
+size_t delta_rule_bwd_workspace(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, bool packed) {
+  const size_t heads = size_t(delta_rule_slots(B, T, nseq, packed)) * Hv, rows = size_t(B) * T * Hv;
+  return heads * (kUnits<float, true> * sizeof(uint4) + (96 + kChunk * kChunk) * sizeof(float)) + 256 * sizeof(float) +
+         up16(rows * dv * sizeof(float)) + up16(size_t(delta_rule_segments(B, T, nseq, packed)) * Hv * dk * dv * sizeof(float)) +
+         up16(rows * dk * sizeof(float)) * (Hv != Hk ? 2 : 1);
+}
+
+hipError_t launch_delta_rule_bwd(DeltaRule a, int dtype, void* workspace, hipStream_t s) {
+  const bool packed = a.offsets != nullptr;
+  const size_t heads = size_t(delta_rule_slots(a.B, a.T, a.nseq, packed)) * a.Hv, rows = size_t(a.B) * a.T * a.Hv;
+  char* at = static_cast<char*>(workspace);
+  const auto room = [&](size_t bytes) {
+    char* p = at;
+    at += up16(bytes);
+    return p;
+  };
+  a.units = reinterpret_cast<uint4*>(room(heads * kUnits<float, true> * sizeof(uint4)));
+  a.gains = reinterpret_cast<float*>(room((heads * 96 + 256) * sizeof(float)));   // 160 more behind the last are read
+  a.decays = reinterpret_cast<float*>(room(heads * kChunk * kChunk * sizeof(float)));
+  a.duals = reinterpret_cast<float*>(room(rows * a.dv * sizeof(float)));
+  a.dstates = reinterpret_cast<float*>(room(size_t(delta_rule_segments(a.B, a.T, a.nseq, packed)) * a.Hv * a.dk * a.dv * sizeof(float)));
+  a.dk_heads = reinterpret_cast<float*>(room(rows * a.dk * sizeof(float)));
+  a.dq_heads = a.Hv != a.Hk ? reinterpret_cast<float*>(room(rows * a.dk * sizeof(float))) : nullptr;
+  if (dtype == 0) run<float>(a, s);
+  else run<Bf16>(a, s);
+  return hipGetLastError();
+}
+
+}  // namespace cssm

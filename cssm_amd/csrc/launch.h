@@ -392,11 +392,23 @@ struct DeltaRule {
   float* states;           // (segments, Hv, dk, dv) out, for the adjoint: S before every 128th row of a sequence; or null
   uint4* units;            // workspace: each chunk's and head's L and P (csrc/delta_rule.h)
   float* gains;            // workspace: (slots, Hv, 96) gamma, d and beta of a chunk's rows
+  // adjoint (errors and states as the forward wrote them)
+  TokenRows dy;            // (B, T, Hv x dv)
+  const float* dh;         // (n, Hv, dk, dv) or null: zeros
+  void *dq, *dkey, *dv_out;   // (B, T, heads, width) of the inputs' type
+  float *dbeta, *ddecay;   // (B, T, Hv); ddecay null without decay
+  float* dh0;              // (n, Hv, dk, dv) or null
+  float* decays;           // workspace: (slots, Hv, 32, 32) D
+  float* duals;            // workspace: (B, T, Hv, dv) X
+  float* dstates;          // workspace: (segments, Hv, dk, dv) the state's gradient behind each segment
+  float *dq_heads, *dk_heads;   // workspace: (B, T, Hv, dk) each value head's share (dq_heads only where heads are shared)
 };
 int delta_rule_slots(int B, int T, int nseq, bool packed);     // chunks that the workspace has room for
 int delta_rule_segments(int B, int T, int nseq, bool packed);
 size_t delta_rule_workspace(int B, int T, int Hv, int nseq, bool packed);
 hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s);
+size_t delta_rule_bwd_workspace(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, bool packed);
+hipError_t launch_delta_rule_bwd(DeltaRule a, int dtype, void* workspace, hipStream_t s);
 hipError_t launch_delta_rule_step(DeltaRule a, int dtype, hipStream_t s);
 
 }  // namespace cssm

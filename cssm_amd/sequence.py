@@ -462,6 +462,32 @@ def delta_forward(q, k, v, beta, decay=None, state=None, offsets=None, out=None,
     return y, final, errors, states
 
 
+def delta_backward(q, k, beta, decay, offsets, errors, states, dy, dfinal, scale=None):
+    """Adjoint of :func:`delta_rule` (cssm_delta_rule_bwd): (dq, dk, dv, dbeta, ddecay, dstate), ddecay None without decay."""
+    d = _delta(q, k, dy, beta, decay, dfinal, offsets)
+    packed = offsets is not None
+    lib = _lib.load()
+    _check(errors, "errors", dy.shape, torch.float32, d.dev)
+    _check(states, "states", (lib.cssm_delta_rule_segments(d.B, d.T, d.nseq, int(packed)), d.Hv, d.dk, d.dv), torch.float32, d.dev)
+
+    def like(t, dtype=None):
+        return torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)
+    dq, dk, dv = like(q), like(k), like(dy)
+    db, dg = like(beta), None if decay is None else like(decay)
+    dh0 = torch.empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32, device=dy.device)
+    if d.n:
+        need = lib.cssm_delta_rule_bwd_workspace_size(d.B, d.T, d.Hk, d.Hv, d.dk, d.dv, d.nseq, int(packed))
+        work = torch.empty(need, dtype=torch.uint8, device=dy.device)
+        _call(d.dev, "cssm_delta_rule_bwd", _ref(d.q), _ref(d.k), d.dtype, _ref(d.beta), _ref(d.decay), _ref(d.v), d.B, d.T,
+              d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), _ptr(offsets), d.nseq,
+              errors.data_ptr(), states.data_ptr(), _ptr(dfinal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+              db.data_ptr(), _ptr(dg), dh0.data_ptr(), work.data_ptr(), need)
+    else:
+        for t in (dq, dk, dv, db) if dg is None else (dq, dk, dv, db, dg):
+            t.zero_()
+    return dq, dk, dv, db, dg, dh0
+
+
 def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, decay: Optional[torch.Tensor] = None,
                state: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -17,7 +17,7 @@ GOOM floor terms folded in).
 autograd graph attached; ``params`` is the cell's parameter tree of leaf
 tensors (``requires_grad`` where gradients are wanted).  ``token_scan_train`` and
 ``rms_norm_train`` are the differentiable forms of the operators over token sequences
-(:mod:`cssm_amd.sequence`).
+(:mod:`cssm_amd.sequence`), and ``delta_rule_train`` that of the delta rule over them.
 """
 from __future__ import annotations
 
@@ -915,3 +915,44 @@ def rms_norm_train(x: torch.Tensor, weight: torch.Tensor, residual=None, eps: fl
     if residual is None:
         return _RmsNormFn.apply(x, None, weight.contiguous(), eps)[0], x
     return _RmsNormFn.apply(x, residual.contiguous(), weight.contiguous(), eps)
+
+
+def _heads_side_by_side(t: torch.Tensor) -> torch.Tensor:
+    """(..., H, width) with its heads one behind the other, as the row kernels read it (any other strides)."""
+    H, D = t.shape[-2:]
+    st = t.stride()
+    return t if (D <= 1 or st[-1] == 1) and (H <= 1 or st[-2] == D) else t.contiguous()
+
+
+class _DeltaRuleFn(torch.autograd.Function):
+    """(y, final state) of the gated delta rule, its adjoint on cssm_delta_rule_bwd.  Kept between the two passes: q, k, the
+    gates, the float32 errors and the state before every 128th row."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, beta, decay, state, offsets, scale):
+        y, final, errors, states = Q.delta_forward(q, k, v, beta, decay, state, offsets, None, scale, keep=True)
+        ctx.save_for_backward(q, k, beta, decay, offsets, errors, states)
+        ctx.like = (y.shape, y.dtype, y.device)
+        ctx.scale, ctx.started = scale, state is not None
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dfinal):
+        q, k, beta, decay, offsets, errors, states = ctx.saved_tensors
+        if dy is None:
+            shape, dtype, device = ctx.like
+            dy = torch.zeros(shape, dtype=dtype, device=device)
+        dq, dk, dv, db, dg, dh0 = Q.delta_backward(q, k, beta, decay, offsets, errors, states, _heads_side_by_side(dy),
+                                                   None if dfinal is None else dfinal.contiguous(), ctx.scale)
+        return dq, dk, dv, db, dg, dh0 if ctx.started else None, None, None
+
+
+def delta_rule_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, decay=None, state=None,
+                     offsets=None, scale=None):
+    """:func:`cssm_amd.sequence.delta_rule`, differentiable in q, k, v, beta, decay and state: (y, final state).  The gradients
+    of a query and key head are the sums over the value heads that share it."""
+    return _DeltaRuleFn.apply(_heads_side_by_side(q), _heads_side_by_side(k), _heads_side_by_side(v), _side_by_side(beta),
+                              None if decay is None else _side_by_side(decay), None if state is None else state.contiguous(),
+                              offsets, scale)

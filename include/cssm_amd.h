@@ -1022,6 +1022,23 @@ int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cs
                     float* errors, float* states, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Adjoint of cssm_delta_rule: q, k, beta, decay, h0's sizes, offsets and scale as its forward call's, with
+ *   errors, states  as the forward wrote them (required)
+ *   dy           (B, T, Hv x dv) of dtype; dh (n, Hv, dk, dv) float32 gradient of h_out, or NULL (zeros)
+ *   dq, dk_out   (B, T, Hk, dk) and dv_out (B, T, Hv, dv) of dtype out, contiguous, the value heads' shares added up in order;
+ *   dbeta, ddecay  (B, T, Hv) float32 out, ddecay NULL without decay; all zero behind the last sequence
+ *   dh0          (n, Hv, dk, dv) float32 out, or NULL
+ *   workspace    cssm_delta_rule_bwd_workspace_size bytes, 16-byte aligned
+ * decay's gradient is what a change of it does; where decay is -inf that is none, up to rounding.
+ */
+size_t cssm_delta_rule_bwd_workspace_size(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, int packed);
+int cssm_delta_rule_bwd(const cssm_token_rows* q, const cssm_token_rows* k, int dtype, const cssm_token_rows* beta,
+                        const cssm_token_rows* decay, const cssm_token_rows* dy, int B, int T, int Hk, int Hv, int dk, int dv,
+                        float scale, const int* offsets, int nseq, const float* errors, const float* states, const float* dh,
+                        void* dq, void* dk_out, void* dv_out, float* dbeta, float* ddecay, float* dh0, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
  * One token for each of B sequences: cssm_delta_rule with T = 1 (the rows' row_stride is not used), state (B, Hv, dk, dv)
  * float32 read and state_out written, which may be the same buffer.
  */
