@@ -185,6 +185,10 @@ SIGNATURES = {
     "cssm_delta_rule_bwd": (_I, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P,
                                  _P, _P, _Z, _P]),
     "cssm_delta_rule_step": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P]),
+    "cssm_rotate_heads": (_I, [_P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "cssm_rotate_heads_bwd_workspace_size": (_Z, [_I]),
+    "cssm_rotate_heads_bwd": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _I, _P, _P, _I, _I, _P, _P, _P,
+                                   _P, _P, _Z, _P]),
     "cssm_block_residual": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
                                            ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                            ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),

@@ -19,7 +19,7 @@ BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libcssm_hip.so")
 SOURCES = ["api.hip", "prep.hip", "gated_scan.hip", "gated_bins.hip", "gated_bwd.hip", "proj.hip", "shortconv.hip", "gdn.hip", "gdn_bwd.hip", "gdn_train.hip", "block.hip", "stem.hip",
            "token_scan.hip", "row_norm.hip", "product8.hip", "delta_rule.hip",
-           "delta_rule_bwd.hip"]
+           "delta_rule_bwd.hip", "head_rotary.hip"]
 ARCH = os.environ.get("CSSM_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [

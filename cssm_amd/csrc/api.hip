@@ -1547,3 +1547,81 @@ int cssm_delta_rule_step(const cssm_token_rows* q, const cssm_token_rows* k, con
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- norm and rotation of heads
+
+namespace {
+
+int rotary_args(const char* who, cssm::Rotary& a, const cssm_token_rows* q, const cssm_token_rows* k, int dtype, int B, int T,
+                int Hq, int Hk, int D, const float* q_weight, const float* k_weight, int norm, float eps, const int* positions,
+                int axes, const double* freq, const int* axis, int P, int halves) {
+  if (dtype != CSSM_F32 && dtype != CSSM_BF16) return fail(CSSM_ERR_ARG, "%s: dtype=%d", who, dtype);
+  if (B < 0 || T < 0 || Hq <= 0 || Hk < 0 || D <= 0 || D % 2 || P < 0 || 2 * (long long)P > D)
+    return fail(CSSM_ERR_SHAPE, "%s: B=%d T=%d Hq=%d Hk=%d D=%d P=%d", who, B, T, Hq, Hk, D, P);
+  if (D > 512) return fail(CSSM_ERR_UNSUPPORTED, "%s: D=%d is taken up to 512", who, D);
+  if ((long long)Hq * D > 1 << 24 || (long long)Hk * D > 1 << 24) return fail(CSSM_ERR_UNSUPPORTED, "%s: Hq=%d Hk=%d D=%d", who, Hq, Hk, D);
+  if (norm < 0 || norm > 2) return fail(CSSM_ERR_ARG, "%s: norm=%d", who, norm);
+  if (!(eps >= 0.0f)) return fail(CSSM_ERR_ARG, "%s: eps=%g", who, double(eps));
+  if (P && (axes < 1 || axes > 4)) return fail(CSSM_ERR_UNSUPPORTED, "%s: axes=%d, 1 to 4 are taken", who, axes);
+  if ((long long)B * T > 0) {
+    if (!has(q) || (Hk && !has(k)) || (P && (!positions || !freq || !axis)))
+      return fail(CSSM_ERR_NULL, "%s: q, k, positions, freq and axis must be non-null", who);
+    if (const int st = token_stride_check(who, {q, Hk ? k : nullptr})) return st;
+  }
+  a.of[0].x = rows_of(q), a.of[1].x = rows_of(Hk ? k : nullptr);
+  a.of[0].H = Hq, a.of[1].H = Hk, a.of[0].w = q_weight, a.of[1].w = k_weight;
+  a.M = (long long)B * T, a.T = T, a.D = D, a.P = P, a.axes = axes, a.halves = halves != 0, a.norm = norm, a.eps = eps;
+  a.positions = positions, a.freq = freq, a.axis = axis;
+  if (!aligned(freq, 8)) return fail(CSSM_ERR_ALIGN, "%s: pointers must be aligned to their elements", who);
+  return token_align_check(who, dtype, {a.of[0].x.p, a.of[1].x.p}, {q_weight, k_weight, positions, axis});
+}
+
+}  // namespace
+
+extern "C" {
+
+int cssm_rotate_heads(const cssm_token_rows* q, const cssm_token_rows* k, int dtype, int B, int T, int Hq, int Hk, int D,
+                      const float* q_weight, const float* k_weight, int norm, float eps, const int* positions, int axes,
+                      const double* freq, const int* axis, int P, int halves, void* q_out, void* k_out, void* stream) {
+  const char* who = "cssm_rotate_heads";
+  cssm::Rotary a = {};
+  if (const int st = rotary_args(who, a, q, k, dtype, B, T, Hq, Hk, D, q_weight, k_weight, norm, eps, positions, axes, freq, axis,
+                                 P, halves))
+    return st;
+  if (!a.M) return ok();
+  if (!q_out || (Hk && !k_out)) return fail(CSSM_ERR_NULL, "%s: q_out and k_out must be non-null", who);
+  if (const int st = token_align_check(who, dtype, {q_out, Hk ? k_out : nullptr}, {})) return st;
+  a.of[0].y = q_out, a.of[1].y = k_out;
+  return hip_status(cssm::launch_rotate_heads(a, dtype, false, static_cast<hipStream_t>(stream)), who);
+}
+
+size_t cssm_rotate_heads_bwd_workspace_size(int D) { return D <= 0 ? 0 : cssm::rotate_heads_bwd_workspace(D); }
+
+int cssm_rotate_heads_bwd(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* dq_out,
+                          const cssm_token_rows* dk_out, int dtype, int B, int T, int Hq, int Hk, int D, const float* q_weight,
+                          const float* k_weight, int norm, float eps, const int* positions, int axes, const double* freq,
+                          const int* axis, int P, int halves, void* dq, void* dk, float* dq_weight, float* dk_weight,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "cssm_rotate_heads_bwd";
+  cssm::Rotary a = {};
+  if (const int st = rotary_args(who, a, q, k, dtype, B, T, Hq, Hk, D, q_weight, k_weight, norm, eps, positions, axes, freq, axis,
+                                 P, halves))
+    return st;
+  if (!a.M) return fail(CSSM_ERR_SHAPE, "%s: B=%d and T=%d must be positive", who, B, T);
+  if (!has(dq_out) || !dq || (Hk && (!has(dk_out) || !dk)))
+    return fail(CSSM_ERR_NULL, "%s: the outputs' gradients, dq and dk must be non-null", who);
+  if (const int st = token_stride_check(who, {dq_out, Hk ? dk_out : nullptr})) return st;
+  const bool weights = dq_weight || dk_weight;
+  const size_t need = weights ? cssm_rotate_heads_bwd_workspace_size(D) : 0;
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(CSSM_ERR_ARG, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
+  a.of[0].dy = rows_of(dq_out), a.of[1].dy = rows_of(Hk ? dk_out : nullptr);
+  if (const int st = token_align_check(who, dtype, {a.of[0].dy.p, a.of[1].dy.p, dq, Hk ? dk : nullptr},
+                                       {dq_weight, dk_weight, weights ? workspace : nullptr}))
+    return st;
+  a.of[0].y = dq, a.of[1].y = dk, a.of[0].dw = dq_weight, a.of[1].dw = dk_weight;
+  a.parts = weights ? static_cast<float*>(workspace) : nullptr;
+  return hip_status(cssm::launch_rotate_heads(a, dtype, true, static_cast<hipStream_t>(stream)), who);
+}
+
+}  // extern "C"

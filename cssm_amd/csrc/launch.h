@@ -411,4 +411,26 @@ size_t delta_rule_bwd_workspace(int B, int T, int Hk, int Hv, int dk, int dv, in
 hipError_t launch_delta_rule_bwd(DeltaRule a, int dtype, void* workspace, hipStream_t s);
 hipError_t launch_delta_rule_step(DeltaRule a, int dtype, hipStream_t s);
 
+// ---- norm and rotation of heads (head_rotary.hip)
+struct RotaryHeads {
+  TokenRows x, dy;         // (M rows, H x D); dy for the adjoint
+  int H;                   // 0: not there
+  const float* w;          // (D) or null: ones
+  void* y;                 // (M, H, D): the output, or dx
+  float* dw;               // (D) or null
+};
+struct Rotary {
+  RotaryHeads of[2];       // queries and keys
+  long long M;
+  int T, D, P, axes;       // rows of a batch; values of a head, pairs that turn (0: no rotation), axes of the positions
+  int halves, norm;        // pairs (j, j + P) or (2 j, 2 j + 1); 0 rms, 1 l2, 2 none
+  float eps;
+  const int* positions;    // (M, axes)
+  const double* freq;      // (P) radians a position
+  const int* axis;         // (P)
+  float* parts;            // adjoint with weights: rotate_heads_bwd_workspace bytes, else null
+};
+size_t rotate_heads_bwd_workspace(int D);
+hipError_t launch_rotate_heads(const Rotary& a, int dtype, bool back, hipStream_t s);
+
 }  // namespace cssm

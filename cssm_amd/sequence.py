@@ -5,8 +5,9 @@ The gated cell's recurrence without its transforms, for each channel in real ari
     D_t = softplus(delta_t + bias),  h_t = kappa exp(-D_t) h_{t-1} + D_t x_t,  y_t = h_t SiLU(z_t)
 
 (:func:`token_scan`, one token at a time :func:`token_scan_step`), the root-mean-square norm behind a residual's
-addition (:func:`rms_norm`) and the product of 8-bit operands that its 8-bit output feeds (:func:`scaled_matmul`).
-The differentiable forms are in :mod:`cssm_amd.training`.
+addition (:func:`rms_norm`) and the product of 8-bit operands that its 8-bit output feeds (:func:`scaled_matmul`); the
+gated delta rule, whose state is a matrix for each head (:func:`delta_rule`, :func:`delta_rule_step`), and the norm and
+rotation of the heads that feed it (:func:`rotate_heads`).  The differentiable forms are in :mod:`cssm_amd.training`.
 
 Tensors live on one GPU; the work is enqueued on torch's current stream of that GPU.  Nothing synchronises, and
 nothing falls back: what a kernel does not take raises ValueError or :class:`cssm_amd._lib.CssmError`.
@@ -359,7 +360,7 @@ def _heads(t, name: str, lead, width: int, dtype, dev: int, like: str) -> Tuple[
                          (f" of {width}" if width else ""))
     H, D = t.shape[-2:]
     st = t.stride()
-    if (D > 1 and st[-1] != 1) or (H > 1 and st[-2] != D):
+    if t.numel() and ((D > 1 and st[-1] != 1) or (H > 1 and st[-2] != D)):
         raise ValueError(f"{name} must have its heads side by side (strides {st})")
     return _lead_rows(t, st, like), H
 
@@ -379,7 +380,7 @@ def _gate_rows(t, name: str, lead, H: int, dev: int, like: str) -> _lib.TokenRow
     if t.shape != (*lead, H):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(*lead, H)}")
     st = t.stride()
-    if H > 1 and st[-1] != 1:
+    if t.numel() and H > 1 and st[-1] != 1:
         raise ValueError(f"{name} must have its heads side by side (strides {st})")
     return _lead_rows(t, st, like)
 
@@ -522,3 +523,126 @@ def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: tor
               d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), state.data_ptr(), y.data_ptr(),
               out_state.data_ptr())
     return y, out_state
+
+
+class RotaryTable(NamedTuple):
+    """How the pairs of a head turn: ``frequencies`` (P,) float64 radians a position, ``axes`` (P,) int32, the axis of the
+    positions that each turns with."""
+    frequencies: torch.Tensor
+    axes: torch.Tensor
+
+
+def rotary_table(sections, base: float = 10000.0, device="cuda", shared: bool = False) -> RotaryTable:
+    """The usual table: ``sections[i]`` pairs turn with axis i (time, height, width; one number: plain positions).  Each axis
+    has a geometric row of frequencies base^(-j / n) of its own, j < n its pairs; with ``shared`` one row runs over all
+    pairs.  Laid out once for a model."""
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or not sum(sections):
+        raise ValueError(f"sections={sections}: 1 to 4 numbers of pairs")
+    if not base > 0:
+        raise ValueError(f"base={base} must be positive")
+    total = sum(sections)
+    freq = [base ** (-j / n) for n in sections for j in range(n)] if not shared else [base ** (-j / total) for j in range(total)]
+    return RotaryTable(torch.tensor(freq, dtype=torch.float64, device=device),
+                       torch.tensor([i for i, n in enumerate(sections) for _ in range(n)], dtype=torch.int32, device=device))
+
+
+_HEAD_NORMS = {"rms": 0, "l2": 1, "none": 2}
+_PAIRS = {"neighbours": 0, "halves": 1}
+
+
+class _Rotary(NamedTuple):
+    """Checked arguments of the head rotation."""
+    dev: int
+    q: _lib.TokenRows
+    k: Optional[_lib.TokenRows]
+    head: tuple      # dtype, B, T, Hq, Hk, D
+    rest: tuple      # weights, norm, eps, positions, axes, frequencies, axis, P, halves
+
+
+def _rotary(q, k, positions, table, q_weight, k_weight, norm, eps, pairs) -> _Rotary:
+    dev = _gpu(q, "q")
+    if q.dtype not in _DTYPES:
+        raise ValueError(f"q: unsupported dtype {q.dtype}")
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q has shape {tuple(q.shape)}, expected (B, T, H, D) or (M, H, D)")
+    if norm not in _HEAD_NORMS:
+        raise ValueError(f"norm={norm!r}: one of {sorted(_HEAD_NORMS)}")
+    if pairs not in _PAIRS:
+        raise ValueError(f"pairs={pairs!r}: one of {sorted(_PAIRS)}")
+    lead, D = q.shape[:-2], q.shape[-1]
+    like = "batch" if q.dim() == 4 else "packed"
+    B, T = lead if q.dim() == 4 else (1, lead[0])
+    _sizes("q", q.shape, *q.shape)
+    if D % 2 or not 0 < D <= 512:
+        raise ValueError(f"heads of {D}: even widths to 512 are taken")
+    rq, Hq = _heads(q, "q", lead, D, q.dtype, dev, like)
+    rk, Hk = (None, 0) if k is None else _heads(k, "k", lead, D, q.dtype, dev, like)
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _check(w, name, (D,), torch.float32, dev)
+    if (positions is None) != (table is None):
+        raise ValueError("positions and table go together")
+    axes = P = 0
+    freq = axis = None
+    if table is not None:
+        freq, axis = table
+        _gpu(freq, "table.frequencies")
+        P = freq.numel()
+        _check(freq, "table.frequencies", (P,), torch.float64, dev)
+        _check(axis, "table.axes", (P,), torch.int32, dev)
+        if 2 * P > D:
+            raise ValueError(f"{P} pairs in heads of {D}")
+        axes = positions.shape[-1] if isinstance(positions, torch.Tensor) and positions.dim() else 0
+        _check(positions, "positions", (*lead, axes), torch.int32, dev)
+        if not 1 <= axes <= 4:
+            raise ValueError(f"positions have {axes} axes: 1 to 4 are taken")
+    return _Rotary(dev, rq, rk, (_DTYPES[q.dtype], B, T, Hq, Hk, D),
+                   (_ptr(q_weight), _ptr(k_weight), _HEAD_NORMS[norm], float(eps), _ptr(positions), axes, _ptr(freq),
+                    _ptr(axis), P, _PAIRS[pairs]))
+
+
+def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor] = None, table=None,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, norm: str = "rms",
+                 eps: float = 1e-6, pairs: str = "halves"):
+    """(q', k'): each head's norm and the rotation by its row's positions, in one pass.
+
+    ``q`` (B, T, Hq, D) and ``k`` (B, T, Hk, D) or None, or rows (M, H, D); float32 or bfloat16 and alike, D even and to
+    512, the heads side by side (slices of one projection's output will do).  ``norm`` 'rms' (x / sqrt(mean(x^2) + eps)),
+    'l2' (x / sqrt(sum(x^2) + eps), unit lengths as :func:`delta_rule` takes its keys) or 'none', then times ``q_weight`` /
+    ``k_weight`` (D) float32.  ``positions`` (B, T, A) or (M, A) int32, 1 to 4 axes, negative ones too; ``table`` a
+    :class:`RotaryTable` (:func:`rotary_table`) of P <= D / 2 pairs; both None: no rotation.  ``pairs`` 'halves': (j, j + P);
+    'neighbours': (2 j, 2 j + 1); values from 2 P on are not turned.  Not differentiable: see
+    :func:`cssm_amd.training.rotate_heads_train`.
+    """
+    r = _rotary(q, k, positions, table, q_weight, k_weight, norm, eps, pairs)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.numel():
+        _call(r.dev, "cssm_rotate_heads", _ref(r.q), _ref(r.k), *r.head, *r.rest, q_out.data_ptr(), _ptr(k_out))
+    return q_out, k_out
+
+
+def rotate_heads_backward(q, k, dq_out, dk_out, positions, table, q_weight, k_weight, norm, eps, pairs):
+    """Adjoint of :func:`rotate_heads` (cssm_rotate_heads_bwd): (dq, dk, dq_weight, dk_weight), None where there is none."""
+    r = _rotary(q, k, positions, table, q_weight, k_weight, norm, eps, pairs)
+    like = "batch" if q.dim() == 4 else "packed"
+    gq, _ = _heads(dq_out, "dq_out", q.shape[:-2], q.shape[-1], q.dtype, r.dev, like)
+    gk = None if k is None else _heads(dk_out, "dk_out", q.shape[:-2], q.shape[-1], q.dtype, r.dev, like)[0]
+    if dq_out.shape != q.shape or (k is not None and dk_out.shape != k.shape):
+        raise ValueError("the outputs' gradients have the outputs' shapes")
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dwq, dwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
+    if q.numel():
+        work, need = None, 0
+        if dwq is not None or dwk is not None:
+            need = _lib.load().cssm_rotate_heads_bwd_workspace_size(q.shape[-1])
+            work = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+        _call(r.dev, "cssm_rotate_heads_bwd", _ref(r.q), _ref(r.k), _ref(gq), _ref(gk), *r.head, *r.rest, dq.data_ptr(),
+              _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(work), need)
+    else:
+        for t in (dwq, dwk):
+            if t is not None:
+                t.zero_()
+    return dq, dk, dwq, dwk

@@ -17,7 +17,8 @@ GOOM floor terms folded in).
 autograd graph attached; ``params`` is the cell's parameter tree of leaf
 tensors (``requires_grad`` where gradients are wanted).  ``token_scan_train`` and
 ``rms_norm_train`` are the differentiable forms of the operators over token sequences
-(:mod:`cssm_amd.sequence`), and ``delta_rule_train`` that of the delta rule over them.
+(:mod:`cssm_amd.sequence`), ``delta_rule_train`` and
+``rotate_heads_train`` those of the delta rule over them and of the rotation of its heads.
 """
 from __future__ import annotations
 
@@ -956,3 +957,34 @@ def delta_rule_train(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: to
     return _DeltaRuleFn.apply(_heads_side_by_side(q), _heads_side_by_side(k), _heads_side_by_side(v), _side_by_side(beta),
                               None if decay is None else _side_by_side(decay), None if state is None else state.contiguous(),
                               offsets, scale)
+
+
+class _RotateHeadsFn(torch.autograd.Function):
+    """(q', k') of the heads' norm and rotation, its adjoint on cssm_rotate_heads_bwd.  Kept: the inputs."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, freq, axis, norm, eps, pairs):
+        table = None if freq is None else (freq, axis)
+        out = Q.rotate_heads(q, k, positions, table, q_weight, k_weight, norm, eps, pairs)
+        ctx.save_for_backward(q, k, q_weight, k_weight, positions, freq, axis)
+        ctx.how = (norm, eps, pairs)
+        return out if k is not None else out[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out=None):
+        q, k, q_weight, k_weight, positions, freq, axis = ctx.saved_tensors
+        dq, dk, dwq, dwk = Q.rotate_heads_backward(q, k, _heads_side_by_side(dq_out),
+                                                   None if k is None else _heads_side_by_side(dk_out), positions,
+                                                   None if freq is None else (freq, axis), q_weight, k_weight, *ctx.how)
+        return dq, dk, dwq, dwk, None, None, None, None, None, None
+
+
+def rotate_heads_train(q: torch.Tensor, k, positions=None, table=None, q_weight=None, k_weight=None, norm: str = "rms",
+                       eps: float = 1e-6, pairs: str = "halves"):
+    """:func:`cssm_amd.sequence.rotate_heads`, differentiable in q, k and the weights: (q', k')."""
+    freq, axis = (None, None) if table is None else table
+    q, k = _heads_side_by_side(q), None if k is None else _heads_side_by_side(k)
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    out = _RotateHeadsFn.apply(q, k, q_weight, k_weight, positions, freq, axis, norm, eps, pairs)
+    return out if k is not None else (out, None)

@@ -1046,6 +1046,31 @@ int cssm_delta_rule_step(const cssm_token_rows* q, const cssm_token_rows* k, con
                          const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int Hk, int Hv, int dk, int dv,
                          float scale, const float* state, void* y, float* state_out, void* stream);
 
+/*
+ * Norm of each head of queries and keys, and the rotation of its pairs by the row's positions:
+ *   n = x r weight, r = 1 / sqrt(mean(x^2) + eps) (norm 0), 1 / sqrt(sum(x^2) + eps) (1) or 1 (2);
+ *   pair j of n, j < P, turned by freq[j] positions[axis[j]]: (n_a cos - n_b sin, n_b cos + n_a sin)
+ *   q, k         (B, T, H x D) of dtype, the heads side by side; k NULL (Hk = 0): q alone
+ *   q_weight, k_weight  (D) float32 or NULL (ones)
+ *   positions    (B, T, axes) int32, contiguous, axes 1 to 4; P = 0: no rotation, not read
+ *   freq, axis   (P) float64 radians a position, (P) int32 axis of each pair (outside 0 .. axes - 1: the nearest)
+ *   halves       pairs are (j, j + P); else (2 j, 2 j + 1).  Values from 2 P on are not turned
+ *   q_out, k_out (B, T, H, D) of dtype, contiguous
+ * D even, to 512, P to D / 2.  Outputs do not overlap inputs.  Angles are float64, reduced before they are rounded.
+ * Adjoint: q, k and the rest as the forward had them, dq_out and dk_out the outputs' gradients (rows as q's and k's);
+ * dq, dk (B, T, H, D) of dtype out, dq_weight, dk_weight (D) float32 out or NULL; workspace of
+ * cssm_rotate_heads_bwd_workspace_size(D) bytes where a weight's gradient is wanted.
+ */
+int cssm_rotate_heads(const cssm_token_rows* q, const cssm_token_rows* k, int dtype, int B, int T, int Hq, int Hk, int D,
+                      const float* q_weight, const float* k_weight, int norm, float eps, const int* positions, int axes,
+                      const double* freq, const int* axis, int P, int halves, void* q_out, void* k_out, void* stream);
+size_t cssm_rotate_heads_bwd_workspace_size(int D);
+int cssm_rotate_heads_bwd(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* dq_out,
+                          const cssm_token_rows* dk_out, int dtype, int B, int T, int Hq, int Hk, int D, const float* q_weight,
+                          const float* k_weight, int norm, float eps, const int* positions, int axes, const double* freq,
+                          const int* axis, int P, int halves, void* dq, void* dk, float* dq_weight, float* dk_weight,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -216,5 +216,5 @@ def test_no_rows(T):
     a = [t.requires_grad_() for t in R.inputs(2, 0, 1, 2, 16, 8, BF16, 4)]
     y, f = T.delta_rule_train(*a[:4], decay=a[4], state=a[5])
     g = torch.randn_like(f)
-    grads = torch.autograd.grad(f, a, g)
+    grads = torch.autograd.grad((f, y), a, (g, torch.ones((), device="cuda", dtype=BF16).expand_as(y)))
     assert torch.equal(grads[5], g) and all(not t.numel() for t in grads[:5])
