@@ -1560,6 +1560,7 @@ int rotary_args(const char* who, cssm::Rotary& a, const cssm_token_rows* q, cons
     return fail(CSSM_ERR_SHAPE, "%s: B=%d T=%d Hq=%d Hk=%d D=%d P=%d", who, B, T, Hq, Hk, D, P);
   if (D > 512) return fail(CSSM_ERR_UNSUPPORTED, "%s: D=%d is taken up to 512", who, D);
   if ((long long)Hq * D > 1 << 24 || (long long)Hk * D > 1 << 24) return fail(CSSM_ERR_UNSUPPORTED, "%s: Hq=%d Hk=%d D=%d", who, Hq, Hk, D);
+  if ((long long)B * T > 0x7fffffffLL) return fail(CSSM_ERR_UNSUPPORTED, "%s: B=%d T=%d is too large for one launch", who, B, T);
   if (norm < 0 || norm > 2) return fail(CSSM_ERR_ARG, "%s: norm=%d", who, norm);
   if (!(eps >= 0.0f)) return fail(CSSM_ERR_ARG, "%s: eps=%g", who, double(eps));
   if (P && (axes < 1 || axes > 4)) return fail(CSSM_ERR_UNSUPPORTED, "%s: axes=%d, 1 to 4 are taken", who, axes);
