@@ -243,6 +243,15 @@ struct Columns {
   }
 };
 
+// 8 values of a result's rows from LDS: those of the rows that a lane holds
+__device__ __forceinline__ void take_rows(const float* s, int g, float (&v)[8]) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const float4 q = *reinterpret_cast<const float4*>(s + 16 * t + 4 * g);
+    v[4 * t] = q.x, v[4 * t + 1] = q.y, v[4 * t + 2] = q.z, v[4 * t + 3] = q.w;
+  }
+}
+
 // parts of P: those that y's type shows; its transpose has all, since the gates' gradients are float32
 template <typename T, bool TURNED>
 constexpr int kPParts = sizeof(T) == 2 && !TURNED ? 2 : 3;

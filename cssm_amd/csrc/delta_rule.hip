@@ -397,6 +397,226 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
     for (int t = sp.row + sp.rows + g; t < a.T; t += 4) put(static_cast<T*>(a.y) + (size_t(t) * a.Hv + h) * a.dv + col, 0.0f);
 }
 
+template <int DKP>
+struct PairLds {
+  static constexpr int kPlane = DKP * 4;
+  uint4 k[2][kPlane], kt[2][kPlane], l[2][3 * 128], q[2][kPlane], p[2][2 * 128];
+  uint4 s[2][4][DKP / 32 * 2 * 64], u[2][4][2 * 64];   // two parts of S and U, a wave's columns each
+  float gains[4][96];
+};
+
+// The same for bfloat16 by two kinds of waves, a pair for 16 columns on each SIMD: the first carries the state, the second
+// brings the chunks' rows to LDS and makes y of the chunk before, from S and U that the first leaves in LDS.  A step is
+// then as long as the state's own chain of products, with the second wave's work in its gaps: PLACEHOLDER
+template <int DKP, bool WIDE, bool KEEP>
+__global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
+  using T = Bf16;
+  using Lds = PairLds<DKP>;
+  constexpr int PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16;
+  __shared__ Lds lds;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % 4, g = lane / 16;
+  const bool carries = __builtin_amdgcn_readfirstlane(threadIdx.x / 256) == 0;
+  const int tid = threadIdx.x % 256;
+  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int b = a.offsets ? 0 : seq;
+  const Span sp = span_of(a, seq);
+  const int chunks = chunks_of(sp.rows);
+  const int col = blockIdx.y * kWalkColumns + wave * 16 + lane % 16;
+  const bool mine = col < a.dv;
+  const size_t state = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
+  const int y_row = a.Hv * a.dv;
+
+  if (carries) {
+    f32x4_t S[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * m + 4 * g + i;
+        S[m][i] = a.h0 && mine && r < a.dk ? a.h0[state + size_t(r) * a.dv] : 0.0f;
+      }
+    uint32_t v[8];
+    const auto fetch = [&](int c) {
+      const Rows vv(row_at<T>(a.v, b, sp.row + (long long)c * kChunk) + h * a.dv, a.v.row, sp.rows - c * kChunk, a.dv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
+    };
+    if (chunks) fetch(0);
+    for (int c = 0; c < chunks; ++c) {
+      __syncthreads();
+      const int o = c % 2;
+      const float* gains = lds.gains[c % 4];
+      float V[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) V[i] = element<T>(v[i]);
+      if (c + 1 < chunks) fetch(c + 1);
+      if (KEEP && c % (kSegment / kChunk) == 0 && mine) {
+        float* st = a.states + (size_t(sp.segment + c / (kSegment / kChunk)) * a.Hv + h) * a.dk * a.dv + col;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * m + 4 * g + i < a.dk) st[size_t(16 * m + 4 * g + i) * a.dv] = S[m][i];
+      }
+      f32x4_t ks[2] = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
+                            S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
+        Unit u[3];
+        split<3>(x, u);
+        lds.s[o][wave][(2 * s) * 64 + lane] = __builtin_bit_cast(uint4, u[0]);
+        lds.s[o][wave][(2 * s + 1) * 64 + lane] = __builtin_bit_cast(uint4, u[1]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Unit w[1];
+          take(lds.k[o] + (s * 2 + t) * 64 + lane, PLANE, w);
+          ks[t] = product(w, u, ks[t]);
+        }
+      }
+      float R[8], E[8], x[8], gm[8], dd[8], bt[8];
+      take_rows(gains, g, gm), take_rows(gains + 32, g, dd), take_rows(gains + 64, g, bt);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) R[i] = V[i] - gm[i] * ks[i / 4][i % 4], x[i] = bt[i] * R[i];
+      {
+        Unit u[3];
+        split<3>(x, u);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Unit w[3];
+          take(lds.l[o] + t * 64 + lane, 128, w);
+          const f32x4_t le = product(w, u, f32x4_t{});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) E[4 * t + i] = R[4 * t + i] - le[i];
+        }
+      }
+      {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = bt[i] * E[i];
+        Unit u[2];
+        split<2>(x, u);
+        lds.u[o][wave][lane] = __builtin_bit_cast(uint4, u[0]);
+        lds.u[o][wave][64 + lane] = __builtin_bit_cast(uint4, u[1]);
+      }
+      if constexpr (KEEP) {
+        const Rows ee(a.errors + ((size_t(b) * a.T + sp.row + (long long)c * kChunk) * a.Hv + h) * a.dv, y_row, sp.rows - c * kChunk, a.dv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) store_element<float>(ee, ee.at<float, true>(unit_row(4 * g, i), col, a.dv), E[i]);
+      }
+      {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= dd[i];
+        Unit u[3];
+        split<3>(x, u);
+        const float all = gains[31];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          Unit w[1];
+          take(lds.kt[o] + m * 64 + lane, PLANE, w);
+          S[m] = product(w, u, S[m] * all);
+        }
+      }
+    }
+    __syncthreads();
+    if (a.h_out && mine)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * m + 4 * g + i;
+          if (r < a.dk) a.h_out[state + size_t(r) * a.dv] = S[m][i];
+        }
+    // rows behind the last sequence
+    if (a.offsets && a.zero_tail && seq == a.nseq - 1 && mine)
+      for (int t = sp.row + sp.rows + g; t < a.T; t += 4) put(static_cast<T*>(a.y) + (size_t(t) * a.Hv + h) * a.dv + col, 0.0f);
+    return;
+  }
+
+  // a thread's share of a chunk's rows
+  const int p_tok = tid % 8 + tid / (8 * 2 * KS) * 8, p_at = tid / 8 % (2 * KS);   // row, 32 (p_at / 2) + 8 (p_at % 2)
+  const bool p_on = KS == 4 || tid < 64 * KS;
+  const int p_col = p_at / 2 * 32 + p_at % 2 * 8;
+  const int p_unit = ((p_at / 2 * 2 + p_tok / 16) * 4 + p_at % 2 * 2) * 16 + p_tok % 16;
+  const int c_g = tid / (DKP / 2), c_col = tid % (DKP / 2) * 2;
+  const bool c_on = DKP == 128 || tid < 2 * DKP;
+  const int c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
+  Piece<T, WIDE> pk, pq;
+  Columns<T, WIDE> ck;
+  u32x4_t l[2], p;
+  float gain;
+  const auto units_of = [&](int c) {
+    return reinterpret_cast<const u32x4_t*>(a.units) + (size_t(sp.slot + c) * a.Hv + h) * kUnits<T, false>;
+  };
+  const auto fetch_keys = [&](int c) {   // what the state takes
+    const Rows k(row_at<T>(a.k, b, sp.row + (long long)c * kChunk) + hk * a.dk, a.k.row, sp.rows - c * kChunk, a.dk);
+    if (p_on) pk.load(k, p_tok, p_col, a.dk);
+    if (c_on) ck.load(k, 4 * c_g, c_col, a.dk);
+    l[0] = units_of(c)[tid], l[1] = units_of(c)[256 + tid % 128];
+    gain = a.gains[(size_t(sp.slot + c) * a.Hv + h) * 96 + tid % 96];
+  };
+  const auto stash_keys = [&](int c) {
+    if (p_on) pk.store(lds.k[c % 2] + p_unit, PLANE);
+    if (c_on) ck.store(lds.kt[c % 2] + c_unit, PLANE);
+    lds.l[c % 2][tid] = __builtin_bit_cast(uint4, l[0]);
+    if (tid < 128) lds.l[c % 2][256 + tid] = __builtin_bit_cast(uint4, l[1]);
+    if (tid < 96) lds.gains[c % 4][tid] = gain;
+  };
+  const auto fetch_queries = [&](int c) {   // what y takes
+    const Rows q(row_at<T>(a.q, b, sp.row + (long long)c * kChunk) + hk * a.dk, a.q.row, sp.rows - c * kChunk, a.dk);
+    if (p_on) pq.load(q, p_tok, p_col, a.dk);
+    p = units_of(c)[3 * 128 + tid];
+  };
+  const auto stash_queries = [&](int c) {
+    if (p_on) pq.store(lds.q[c % 2] + p_unit, PLANE);
+    lds.p[c % 2][tid] = __builtin_bit_cast(uint4, p);
+  };
+  // step c: chunk c + 1's keys and chunk c's queries come in, chunk c - 1's y goes out
+  if (chunks) {
+    fetch_keys(0);
+    stash_keys(0);
+    if (chunks > 1) fetch_keys(1);
+    fetch_queries(0);
+  }
+  for (int c = 0; c <= chunks; ++c) {
+    __syncthreads();
+    if (c + 1 < chunks) stash_keys(c + 1);
+    if (c < chunks) stash_queries(c);
+    if (c + 2 < chunks) fetch_keys(c + 2);
+    if (c + 1 < chunks) fetch_queries(c + 1);
+    if (c == 0) continue;
+    const int o = (c - 1) % 2;
+    const float* gains = lds.gains[(c - 1) % 4];
+    f32x4_t qs[2] = {};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Unit u[2];
+      take(lds.s[o][wave] + 2 * s * 64 + lane, 64, u);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        Unit w[1];
+        take(lds.q[o] + (s * 2 + t) * 64 + lane, PLANE, w);
+        qs[t] = product(w, u, qs[t]);
+      }
+    }
+    float gm[8];
+    take_rows(gains, g, gm);
+    Unit u[2];
+    take(lds.u[o][wave] + lane, 64, u);
+    const Rows yy(static_cast<T*>(a.y) + ((size_t(b) * a.T + sp.row + (long long)(c - 1) * kChunk) * a.Hv + h) * a.dv, y_row,
+                  sp.rows - (c - 1) * kChunk, a.dv);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      Unit w[2];
+      take(lds.p[o] + t * 64 + lane, 128, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qs[t][i] *= a.scale * gm[4 * t + i];
+      qs[t] = product(w, u, qs[t]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store_element<T>(yy, yy.at<T, true>(16 * t + 4 * g + i, col, a.dv), qs[t][i]);
+    }
+  }
+}
+
 // One token: 32 columns of a head's state to a workgroup, 8 threads of 4 columns side by side and 32 rows, or with
 // element loads 32 threads of one column and 8 rows, at a time.  The state is read once, kept in registers between
 // the two sums over its rows, and written once.
@@ -486,6 +706,13 @@ void run_as(const DeltaRule& a, hipStream_t s) {
   const int n = a.offsets ? a.nseq : a.B;
   launch_delta_prepare<T, false>(a, WIDE, s);
   const dim3 grid(n * a.Hv, (a.dv + kWalkColumns - 1) / kWalkColumns);
+  if constexpr (sizeof(T) == 2) {
+    if (a.errors && a.dk <= 64) delta_walk_pairs<64, WIDE, true><<<grid, 512, 0, s>>>(a);
+    else if (a.errors) delta_walk_pairs<128, WIDE, true><<<grid, 512, 0, s>>>(a);
+    else if (a.dk <= 64) delta_walk_pairs<64, WIDE, false><<<grid, 512, 0, s>>>(a);
+    else delta_walk_pairs<128, WIDE, false><<<grid, 512, 0, s>>>(a);
+    return;
+  }
   if (a.errors && a.dk <= 64) delta_walk<64, T, WIDE, true><<<grid, 256, 0, s>>>(a);
   else if (a.errors) delta_walk<128, T, WIDE, true><<<grid, 256, 0, s>>>(a);
   else if (a.dk <= 64) delta_walk<64, T, WIDE, false><<<grid, 256, 0, s>>>(a);

@@ -31,15 +31,6 @@ struct BackLds {
   float gains[256];
 };
 
-// 8 values of a result's rows from LDS: those of the rows that a lane holds
-__device__ __forceinline__ void take_rows(const float* s, int g, float (&v)[8]) {
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const float4 q = *reinterpret_cast<const float4*>(s + 16 * t + 4 * g);
-    v[4 * t] = q.x, v[4 * t + 1] = q.y, v[4 * t + 2] = q.z, v[4 * t + 3] = q.w;
-  }
-}
-
 template <int DKP, typename T, bool WIDE>
 __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
   using Lds = BackLds<DKP, T>;
