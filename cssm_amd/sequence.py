@@ -385,6 +385,20 @@ def _gate_rows(t, name: str, lead, H: int, dev: int, like: str) -> _lib.TokenRow
     return _lead_rows(t, st, like)
 
 
+_Rows5, _Rows2 = ctypes.c_longlong * 15, ctypes.c_longlong * 6     # cssm_token_rows one behind the other
+_ROWS = ctypes.sizeof(_lib.TokenRows)
+
+
+def _fine(t, shape, dtype, dev: int) -> bool:
+    """Whether :func:`_check` takes t: what a usual call asks, without naming what is wrong."""
+    return isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous()
+
+
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape, type and GPU."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 class _Delta(NamedTuple):
     """Checked arguments of the delta rule: GPU, rows, sizes."""
     dev: int
@@ -442,7 +456,7 @@ def delta_forward(q, k, v, beta, decay=None, state=None, offsets=None, out=None,
     d = _delta(q, k, v, beta, decay, state, offsets)
     packed = offsets is not None
     if out is None:
-        y = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        y = _new(v)
     else:
         y = _check(out, "out", v.shape, v.dtype, d.dev)
     final = torch.empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32, device=v.device)
@@ -471,10 +485,7 @@ def delta_backward(q, k, beta, decay, offsets, errors, states, dy, dfinal, scale
     _check(errors, "errors", dy.shape, torch.float32, d.dev)
     _check(states, "states", (lib.cssm_delta_rule_segments(d.B, d.T, d.nseq, int(packed)), d.Hv, d.dk, d.dv), torch.float32, d.dev)
 
-    def like(t, dtype=None):
-        return torch.empty(t.shape, dtype=dtype or t.dtype, device=t.device)
-    dq, dk, dv = like(q), like(k), like(dy)
-    db, dg = like(beta), None if decay is None else like(decay)
+    dq, dk, dv, db, dg = _new(q), _new(k), _new(dy), _new(beta), None if decay is None else _new(decay)
     dh0 = torch.empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32, device=dy.device)
     if d.n:
         need = lib.cssm_delta_rule_bwd_workspace_size(d.B, d.T, d.Hk, d.Hv, d.dk, d.dv, d.nseq, int(packed))
@@ -507,21 +518,52 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Te
     return delta_forward(q, k, v, beta, decay, state, offsets, out, scale)[:2]
 
 
+def _plain_tokens(q, k, v, beta, decay, state):
+    """(GPU, B, Hk, Hv, dk, dv) of contiguous tokens that go together: the usual call, without the checks that name what is
+    wrong.  None for any other."""
+    try:
+        dev, dt, f32 = v.get_device(), v.dtype, torch.float32
+        B, Hv, dv = v.shape
+        _, Hk, dk = sk = k.shape
+        gate = beta.shape
+        if (dev >= 0 and dt in _DTYPES and k.dtype is dt and q.dtype is dt and beta.dtype is f32 and state.dtype is f32
+                and q.shape == sk and sk[0] == B and gate == (B, Hv) and state.shape == (B, Hv, dk, dv)
+                and 0 < dk <= 128 and 0 < dv <= 128 and Hk > 0 and Hv > 0 and Hv % Hk == 0
+                and q.get_device() == dev and k.get_device() == dev and beta.get_device() == dev and state.get_device() == dev
+                and v.is_contiguous() and q.is_contiguous() and k.is_contiguous() and beta.is_contiguous()
+                and state.is_contiguous()
+                and (decay is None or (decay.dtype is f32 and decay.shape == gate and decay.get_device() == dev
+                                       and decay.is_contiguous()))):
+            return dev, B, Hk, Hv, dk, dv
+    except (AttributeError, ValueError):
+        pass
+    return None
+
+
 def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, state: torch.Tensor,
                     decay: Optional[torch.Tensor] = None, out_state: Optional[torch.Tensor] = None,
                     scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """One token for each sequence: (y, state) from ``q``, ``k`` (B, Hk, dk), ``v`` (B, Hv, dv), ``beta``, ``decay`` (B, Hv)
     and ``state`` (B, Hv, dk, dv) float32, which ``out_state=state`` updates in place."""
-    d = _delta(q, k, v, beta, decay, state, None, step=True, need_state=True)
+    sizes = _plain_tokens(q, k, v, beta, decay, state)
+    if sizes is not None:
+        dev, B, Hk, Hv, dk, dv = sizes
+        rows = _Rows5(q.data_ptr(), Hk * dk, 0, k.data_ptr(), Hk * dk, 0, v.data_ptr(), Hv * dv, 0, beta.data_ptr(), Hv, 0,
+                      0 if decay is None else decay.data_ptr(), Hv, 0)
+        at = ctypes.addressof(rows)
+        refs = at, at + _ROWS, at + 2 * _ROWS, at + 3 * _ROWS, None if decay is None else at + 4 * _ROWS
+    else:
+        d = _delta(q, k, v, beta, decay, state, None, step=True, need_state=True)
+        dev, B, Hk, Hv, dk, dv = d.dev, d.B, d.Hk, d.Hv, d.dk, d.dv
+        refs = _ref(d.q), _ref(d.k), _ref(d.v), _ref(d.beta), _ref(d.decay)
     if out_state is None:
         out_state = torch.empty_like(state)
     elif out_state is not state:
-        _check(out_state, "out_state", state.shape, torch.float32, d.dev)
-    y = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    if d.B:
-        _call(d.dev, "cssm_delta_rule_step", _ref(d.q), _ref(d.k), _ref(d.v), d.dtype, _ref(d.beta), _ref(d.decay), d.B,
-              d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), state.data_ptr(), y.data_ptr(),
-              out_state.data_ptr())
+        _check(out_state, "out_state", state.shape, torch.float32, dev)
+    y = _new(v)
+    if B:
+        _call(dev, "cssm_delta_rule_step", refs[0], refs[1], refs[2], _DTYPES[v.dtype], refs[3], refs[4], B, Hk, Hv, dk, dv,
+              dk ** -0.5 if scale is None else float(scale), state.data_ptr(), y.data_ptr(), out_state.data_ptr())
     return y, out_state
 
 
@@ -554,8 +596,9 @@ _PAIRS = {"neighbours": 0, "halves": 1}
 class _Rotary(NamedTuple):
     """Checked arguments of the head rotation."""
     dev: int
-    q: _lib.TokenRows
-    k: Optional[_lib.TokenRows]
+    rows: object     # what q and k are the addresses in
+    q: int
+    k: Optional[int]
     head: tuple      # dtype, B, T, Hq, Hk, D
     rest: tuple      # weights, norm, eps, positions, axes, frequencies, axis, P, halves
 
@@ -570,17 +613,26 @@ def _rotary(q, k, positions, table, q_weight, k_weight, norm, eps, pairs) -> _Ro
         raise ValueError(f"norm={norm!r}: one of {sorted(_HEAD_NORMS)}")
     if pairs not in _PAIRS:
         raise ValueError(f"pairs={pairs!r}: one of {sorted(_PAIRS)}")
-    lead, D = q.shape[:-2], q.shape[-1]
-    like = "batch" if q.dim() == 4 else "packed"
-    B, T = lead if q.dim() == 4 else (1, lead[0])
-    _sizes("q", q.shape, *q.shape)
+    lead, (Hq, D) = q.shape[:-2], q.shape[-2:]
+    B, T = lead if len(lead) == 2 else (1, lead[0])
     if D % 2 or not 0 < D <= 512:
         raise ValueError(f"heads of {D}: even widths to 512 are taken")
-    rq, Hq = _heads(q, "q", lead, D, q.dtype, dev, like)
-    rk, Hk = (None, 0) if k is None else _heads(k, "k", lead, D, q.dtype, dev, like)
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            _check(w, name, (D,), torch.float32, dev)
+    sk = None if k is None else k.shape
+    if (Hq and q.is_contiguous() and (k is None or (k.get_device() == dev and k.dtype is q.dtype and len(sk) == len(lead) + 2 and
+                                                    sk[:-2] == lead and sk[-2] and sk[-1] == D and k.is_contiguous()))):
+        Hk = 0 if k is None else sk[-2]     # contiguous, as usual
+        rows = _Rows2(q.data_ptr(), T * Hq * D, Hq * D, 0 if k is None else k.data_ptr(), T * Hk * D, Hk * D)
+        rq, rk = ctypes.addressof(rows), None if k is None else ctypes.addressof(rows) + _ROWS
+    else:
+        like = "batch" if len(lead) == 2 else "packed"
+        tq, Hq = _heads(q, "q", lead, D, q.dtype, dev, like)
+        tk, Hk = (None, 0) if k is None else _heads(k, "k", lead, D, q.dtype, dev, like)
+        rows, rq, rk = (tq, tk), _ref(tq), _ref(tk)
+    _sizes("q", q.shape, B, T, Hq, Hk)
+    if q_weight is not None and not _fine(q_weight, (D,), torch.float32, dev):
+        _check(q_weight, "q_weight", (D,), torch.float32, dev)
+    if k_weight is not None and not _fine(k_weight, (D,), torch.float32, dev):
+        _check(k_weight, "k_weight", (D,), torch.float32, dev)
     if (positions is None) != (table is None):
         raise ValueError("positions and table go together")
     axes = P = 0
@@ -589,17 +641,19 @@ def _rotary(q, k, positions, table, q_weight, k_weight, norm, eps, pairs) -> _Ro
         freq, axis = table
         _gpu(freq, "table.frequencies")
         P = freq.numel()
-        _check(freq, "table.frequencies", (P,), torch.float64, dev)
-        _check(axis, "table.axes", (P,), torch.int32, dev)
+        if not _fine(freq, (P,), torch.float64, dev) or not _fine(axis, (P,), torch.int32, dev):
+            _check(freq, "table.frequencies", (P,), torch.float64, dev)
+            _check(axis, "table.axes", (P,), torch.int32, dev)
         if 2 * P > D:
             raise ValueError(f"{P} pairs in heads of {D}")
         axes = positions.shape[-1] if isinstance(positions, torch.Tensor) and positions.dim() else 0
-        _check(positions, "positions", (*lead, axes), torch.int32, dev)
+        if not _fine(positions, (*lead, axes), torch.int32, dev):
+            _check(positions, "positions", (*lead, axes), torch.int32, dev)
         if not 1 <= axes <= 4:
             raise ValueError(f"positions have {axes} axes: 1 to 4 are taken")
-    return _Rotary(dev, rq, rk, (_DTYPES[q.dtype], B, T, Hq, Hk, D),
-                   (_ptr(q_weight), _ptr(k_weight), _HEAD_NORMS[norm], float(eps), _ptr(positions), axes, _ptr(freq),
-                    _ptr(axis), P, _PAIRS[pairs]))
+    rest = (_ptr(q_weight), _ptr(k_weight), _HEAD_NORMS[norm], float(eps), _ptr(positions), axes, _ptr(freq), _ptr(axis), P,
+            _PAIRS[pairs])
+    return _Rotary(dev, rows, rq, rk, (_DTYPES[q.dtype], B, T, Hq, Hk, D), rest)
 
 
 def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional[torch.Tensor] = None, table=None,
@@ -616,10 +670,9 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
     :func:`cssm_amd.training.rotate_heads_train`.
     """
     r = _rotary(q, k, positions, table, q_weight, k_weight, norm, eps, pairs)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out, k_out = _new(q), None if k is None else _new(k)
     if q.numel():
-        _call(r.dev, "cssm_rotate_heads", _ref(r.q), _ref(r.k), *r.head, *r.rest, q_out.data_ptr(), _ptr(k_out))
+        _call(r.dev, "cssm_rotate_heads", r.q, r.k, *r.head, *r.rest, q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
 
 
@@ -631,15 +684,14 @@ def rotate_heads_backward(q, k, dq_out, dk_out, positions, table, q_weight, k_we
     gk = None if k is None else _heads(dk_out, "dk_out", q.shape[:-2], q.shape[-1], q.dtype, r.dev, like)[0]
     if dq_out.shape != q.shape or (k is not None and dk_out.shape != k.shape):
         raise ValueError("the outputs' gradients have the outputs' shapes")
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dq, dk = _new(q), None if k is None else _new(k)
     dwq, dwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
     if q.numel():
         work, need = None, 0
         if dwq is not None or dwk is not None:
             need = _lib.load().cssm_rotate_heads_bwd_workspace_size(q.shape[-1])
             work = torch.empty(need // 4, dtype=torch.float32, device=q.device)
-        _call(r.dev, "cssm_rotate_heads_bwd", _ref(r.q), _ref(r.k), _ref(gq), _ref(gk), *r.head, *r.rest, dq.data_ptr(),
+        _call(r.dev, "cssm_rotate_heads_bwd", r.q, r.k, _ref(gq), _ref(gk), *r.head, *r.rest, dq.data_ptr(),
               _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(work), need)
     else:
         for t in (dwq, dwk):
