@@ -178,7 +178,7 @@ SIGNATURES = {
     "cssm_quantize_weight": (_I, [_P, _I, _I, _P, _P, _P]),
     "cssm_scaled_matmul": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I, _P, _I, _P]),
     "cssm_delta_rule_segments": (_I, [_I, _I, _I, _I]),
-    "cssm_delta_rule_workspace_size": (_Z, [_I, _I, _I, _I, _I]),
+    "cssm_delta_rule_workspace_size": (_Z, [_I, _I, _I, _I, _I, _I, _I]),
     "cssm_delta_rule": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I, _P, _I, _P, _P, _P, _P, _Z,
                              _P]),
     "cssm_delta_rule_bwd_workspace_size": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),

@@ -1485,8 +1485,9 @@ int cssm_delta_rule_segments(int B, int T, int nseq, int packed) {
   return B <= 0 || T < 0 || nseq < 0 ? 0 : cssm::delta_rule_segments(B, T, nseq, packed != 0);
 }
 
-size_t cssm_delta_rule_workspace_size(int B, int T, int Hv, int nseq, int packed) {
-  return B <= 0 || T < 0 || Hv <= 0 || nseq < 0 ? 0 : cssm::delta_rule_workspace(B, T, Hv, nseq, packed != 0);
+size_t cssm_delta_rule_workspace_size(int B, int T, int Hv, int dk, int dv, int nseq, int packed) {
+  return B <= 0 || T < 0 || Hv <= 0 || dk <= 0 || dv <= 0 || nseq < 0
+             ? 0 : cssm::delta_rule_workspace(B, T, Hv, dk, dv, nseq, packed != 0);
 }
 
 int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v, int dtype,
@@ -1498,7 +1499,7 @@ int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cs
   if (const int st = delta_rule_args(who, a, q, k, v, dtype, beta, decay, B, T, Hk, Hv, dk, dv, scale, offsets, nseq)) return st;
   if (B == 0) return ok();
   if (T > 0 && !y) return fail(CSSM_ERR_NULL, "%s: y must be non-null", who);
-  if (const int st = delta_workspace_check(who, cssm_delta_rule_workspace_size(B, T, Hv, offsets ? nseq : 0, offsets != nullptr),
+  if (const int st = delta_workspace_check(who, cssm_delta_rule_workspace_size(B, T, Hv, dk, dv, offsets ? nseq : 0, offsets != nullptr),
                                            workspace, workspace_bytes))
     return st;
   if (!errors != !states) return fail(CSSM_ERR_NULL, "%s: errors and states go together", who);

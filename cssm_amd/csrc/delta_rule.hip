@@ -200,6 +200,90 @@ __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
   }
 }
 
+// A sequence, or a part of one that is walked by itself
+struct Part {
+  int seq, row, rows, slot, segment;   // as a Span, of the part
+  bool first, last;                    // of its sequence
+};
+
+// part x of the launch; false for a number that no part takes
+__device__ __forceinline__ bool part_of(const DeltaRule& a, int x, Part& p) {
+  if (!a.fold) {
+    const Span sp = span_of(a, x);
+    p = {x, sp.row, sp.rows, sp.slot, sp.segment, true, true};
+    return true;
+  }
+  int seq, i;
+  if (!a.offsets) {
+    const int n = a.T / a.fold + (a.T % a.fold != 0);
+    seq = x / n, i = x - seq * n;
+  } else {   // sequence s begins at its first row's part and s more, so that an empty one has a number too
+    const auto begin = [&](int s) {
+      const int lo = a.offsets[s];
+      return (lo < 0 ? 0 : lo > a.T ? a.T : lo) / a.fold + s;
+    };
+    int lo = 0, hi = a.nseq;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (begin(mid) <= x) lo = mid;
+      else hi = mid;
+    }
+    seq = lo, i = x - begin(lo);
+  }
+  const Span sp = span_of(a, seq);
+  const int parts = sp.rows <= a.fold ? 1 : (sp.rows - 1) / a.fold + 1;
+  if (i < 0 || i >= parts) return false;
+  const int skip = i * a.fold, left = sp.rows - skip;
+  p = {seq, sp.row + skip, left < a.fold ? left : a.fold, sp.slot + skip / kChunk, sp.segment + skip / kSegment, i == 0, i == parts - 1};
+  return true;
+}
+
+// What a walk does with a column: its first state and where its last one goes.  MAP: the part's own effect, for all parts but
+// a sequence's last - on the columns of no state (of the first part, of the state before it), and on those of a unit matrix
+struct Column {
+  int width, col;        // of the states' rows
+  bool mine, unit;       // unit: of the unit matrix, which no value enters
+  const float* from;     // or null: zeros, or the unit matrix
+  float* to;             // or null
+};
+
+template <int DKP, bool MAP>
+__device__ __forceinline__ bool column_of(const DeltaRule& a, const Part& p, int part, int h, int block, int lane_col, int columns, Column& c) {
+  const int values = (a.dv + columns - 1) / columns;
+  c.unit = MAP && block >= values;
+  if (MAP && (p.last || (c.unit && p.first))) return false;
+  c.width = c.unit ? DKP : a.dv;
+  c.col = (c.unit ? block - values : block) * columns + lane_col;
+  c.mine = c.col < c.width;
+  const size_t state = size_t(a.dk) * a.dv, at = size_t(part) * a.Hv + h, seq = size_t(p.seq) * a.Hv + h;
+  c.from = c.unit ? nullptr : p.first ? (a.h0 ? a.h0 + seq * state : nullptr) : MAP ? nullptr : a.ends + (at - a.Hv) * state;
+  c.to = c.unit ? a.maps + at * DKP * DKP : MAP ? a.ends + at * state : p.last && a.h_out ? a.h_out + seq * state : nullptr;
+  return true;
+}
+
+template <int DKP>
+__device__ __forceinline__ void first_state(const DeltaRule& a, const Column& c, int g, f32x4_t (&S)[DKP / 16]) {
+#pragma unroll
+  for (int m = 0; m < DKP / 16; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * m + 4 * g + i;
+      S[m][i] = c.unit ? (r == c.col ? 1.0f : 0.0f) : c.from && c.mine && r < a.dk ? c.from[size_t(r) * c.width + c.col] : 0.0f;
+    }
+}
+
+template <int DKP>
+__device__ __forceinline__ void last_state(const DeltaRule& a, const Column& c, int g, const f32x4_t (&S)[DKP / 16]) {
+  if (!c.to || !c.mine) return;
+#pragma unroll
+  for (int m = 0; m < DKP / 16; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * m + 4 * g + i;
+      if (r < (c.unit ? DKP : a.dk)) c.to[size_t(r) * c.width + c.col] = S[m][i];
+    }
+}
+
 constexpr int kWalkColumns = 64;   // of a workgroup: 16 for each of its four waves
 
 template <int DKP, typename T>
@@ -211,30 +295,23 @@ struct WalkLds {
 
 // One workgroup carries 64 columns of one sequence's and head's state through the chunks.  While a chunk is computed
 // from LDS, the next one's rows are on their way into registers.
-template <int DKP, typename T, bool WIDE, bool KEEP>
+template <int DKP, typename T, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
   using Lds = WalkLds<DKP, T>;
   constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, PP = kPParts<T, false>;
   constexpr int LP = (kUnits<T, false> + 255) / 256;
   __shared__ Lds lds[Lds::kBufs];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
-  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
-  const int b = a.offsets ? 0 : seq;
-  const Span sp = span_of(a, seq);
-  const int chunks = chunks_of(sp.rows);
-  const int col = blockIdx.y * kWalkColumns + wave * 16 + lane % 16;
-  const bool mine = col < a.dv;
-  const size_t state = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
+  const int part = blockIdx.x / a.Hv, h = blockIdx.x - part * a.Hv, hk = h / (a.Hv / a.Hk);
+  Part sp;
+  Column column;
+  if (!part_of(a, part, sp) || !column_of<DKP, MAP>(a, sp, part, h, blockIdx.y, wave * 16 + lane % 16, kWalkColumns, column)) return;
+  const int b = a.offsets ? 0 : sp.seq, chunks = chunks_of(sp.rows), col = column.col;
+  const bool mine = column.mine;
   const int y_row = a.Hv * a.dv;
 
   f32x4_t S[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 16 * m + 4 * g + i;
-      S[m][i] = a.h0 && mine && r < a.dk ? a.h0[state + size_t(r) * a.dv] : 0.0f;
-    }
+  first_state<DKP>(a, column, g, S);
 
   // a thread's share of a chunk's rows
   const int p_tok = tid % 8 + tid / (8 * 2 * KS) * 8, p_at = tid / 8 % (2 * KS);   // row, 32 (p_at / 2) + 8 (p_at % 2)
@@ -253,19 +330,21 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
     const long long t = sp.row + (long long)c * kChunk;
     const int rows = sp.rows - c * kChunk;
     const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
-    const Rows vv(row_at<T>(a.v, b, t) + h * a.dv, a.v.row, rows, a.dv);
+    const Rows vv(row_at<T>(a.v, b, t) + h * a.dv, a.v.row, MAP && column.unit ? 0 : rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
     const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T, false> + tid;   // the last ones past this chunk's: into the next, or the end's room
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
-    if (p_on) pk.load(k, p_tok, p_col, a.dk), pq.load(q, p_tok, p_col, a.dk);
+    if (p_on) pk.load(k, p_tok, p_col, a.dk);
+    if (p_on && !MAP) pq.load(q, p_tok, p_col, a.dk);
     if (c_on) ck.load(k, 4 * c_g, c_col, a.dk);
 #pragma unroll
     for (int i = 0; i < LP; ++i) lp[i] = units[256 * i];
     gain = a.gains[head * 96 + tid];
   };
   const auto stash = [&](Lds& to) {
-    if (p_on) pk.store(to.k + p_unit, PLANE), pq.store(to.q + p_unit, PLANE);
+    if (p_on) pk.store(to.k + p_unit, PLANE);
+    if (p_on && !MAP) pq.store(to.q + p_unit, PLANE);
     if (c_on) ck.store(to.kt + c_unit, PLANE);
 #pragma unroll
     for (int i = 0; i < LP; ++i) to.lp[tid + 256 * i] = __builtin_bit_cast(uint4, lp[i]);
@@ -304,6 +383,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
         Unit w[N];
         take(in.k + (s * 2 + t) * 64 + lane, PLANE, w);
         ks[t] = product(w, u, ks[t]);
+        if constexpr (MAP) continue;
         take(in.q + (s * 2 + t) * 64 + lane, PLANE, w);
         if constexpr (PP == 3) {
           qs[t] = product(w, u, qs[t]);
@@ -344,6 +424,8 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
     {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = bt[i] * E[i];
+    }
+    if constexpr (!MAP) {
       Unit u[PP];
       split<PP>(x, u);
 #pragma unroll
@@ -352,8 +434,6 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
         take(in.lp + 3 * 128 + t * 64 + lane, 128, w);
         qs[t] = product(w, u, qs[t]);
       }
-    }
-    {
       const long long t0 = sp.row + (long long)c * kChunk;
       const int rows = sp.rows - c * kChunk;
       const size_t head = ((size_t(b) * a.T + t0) * a.Hv + h) * a.dv;
@@ -384,16 +464,9 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
       stash(lds[(c + 1) % Lds::kBufs]);
     }
   }
-  if (a.h_out && mine)
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * m + 4 * g + i;
-        if (r < a.dk) a.h_out[state + size_t(r) * a.dv] = S[m][i];
-      }
+  last_state<DKP>(a, column, g, S);
   // rows behind the last sequence
-  if (a.offsets && a.zero_tail && seq == a.nseq - 1 && mine)
+  if (!MAP && a.offsets && a.zero_tail && sp.seq == a.nseq - 1 && sp.last && mine)
     for (int t = sp.row + sp.rows + g; t < a.T; t += 4) put(static_cast<T*>(a.y) + (size_t(t) * a.Hv + h) * a.dv + col, 0.0f);
 }
 
@@ -408,7 +481,7 @@ struct PairLds {
 // The same for bfloat16 by two kinds of waves, a pair for 16 columns on each SIMD: the first carries the state, the second
 // brings the chunks' rows to LDS and makes y of the chunk before, from S and U that the first leaves in LDS.  A step is
 // then as long as the state's own chain of products, with the second wave's work in its gaps: PLACEHOLDER
-template <int DKP, bool WIDE, bool KEEP>
+template <int DKP, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
   using T = Bf16;
   using Lds = PairLds<DKP>;
@@ -417,27 +490,20 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % 4, g = lane / 16;
   const bool carries = __builtin_amdgcn_readfirstlane(threadIdx.x / 256) == 0;
   const int tid = threadIdx.x % 256;
-  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
-  const int b = a.offsets ? 0 : seq;
-  const Span sp = span_of(a, seq);
-  const int chunks = chunks_of(sp.rows);
-  const int col = blockIdx.y * kWalkColumns + wave * 16 + lane % 16;
-  const bool mine = col < a.dv;
-  const size_t state = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
+  const int part = blockIdx.x / a.Hv, h = blockIdx.x - part * a.Hv, hk = h / (a.Hv / a.Hk);
+  Part sp;
+  Column column;
+  if (!part_of(a, part, sp) || !column_of<DKP, MAP>(a, sp, part, h, blockIdx.y, wave * 16 + lane % 16, kWalkColumns, column)) return;
+  const int b = a.offsets ? 0 : sp.seq, chunks = chunks_of(sp.rows), col = column.col;
+  const bool mine = column.mine;
   const int y_row = a.Hv * a.dv;
 
   if (carries) {
     f32x4_t S[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * m + 4 * g + i;
-        S[m][i] = a.h0 && mine && r < a.dk ? a.h0[state + size_t(r) * a.dv] : 0.0f;
-      }
+    first_state<DKP>(a, column, g, S);
     uint32_t v[8];
     const auto fetch = [&](int c) {
-      const Rows vv(row_at<T>(a.v, b, sp.row + (long long)c * kChunk) + h * a.dv, a.v.row, sp.rows - c * kChunk, a.dv);
+      const Rows vv(row_at<T>(a.v, b, sp.row + (long long)c * kChunk) + h * a.dv, a.v.row, MAP && column.unit ? 0 : sp.rows - c * kChunk, a.dv);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
     };
@@ -465,8 +531,10 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
                             S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
         Unit u[3];
         split<3>(x, u);
-        lds.s[o][wave][(2 * s) * 64 + lane] = __builtin_bit_cast(uint4, u[0]);
-        lds.s[o][wave][(2 * s + 1) * 64 + lane] = __builtin_bit_cast(uint4, u[1]);
+        if constexpr (!MAP) {
+          lds.s[o][wave][(2 * s) * 64 + lane] = __builtin_bit_cast(uint4, u[0]);
+          lds.s[o][wave][(2 * s + 1) * 64 + lane] = __builtin_bit_cast(uint4, u[1]);
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           Unit w[1];
@@ -493,10 +561,12 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
       {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = bt[i] * E[i];
-        Unit u[2];
-        split<2>(x, u);
-        lds.u[o][wave][lane] = __builtin_bit_cast(uint4, u[0]);
-        lds.u[o][wave][64 + lane] = __builtin_bit_cast(uint4, u[1]);
+        if constexpr (!MAP) {
+          Unit u[2];
+          split<2>(x, u);
+          lds.u[o][wave][lane] = __builtin_bit_cast(uint4, u[0]);
+          lds.u[o][wave][64 + lane] = __builtin_bit_cast(uint4, u[1]);
+        }
       }
       if constexpr (KEEP) {
         const Rows ee(a.errors + ((size_t(b) * a.T + sp.row + (long long)c * kChunk) * a.Hv + h) * a.dv, y_row, sp.rows - c * kChunk, a.dv);
@@ -518,16 +588,9 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
       }
     }
     __syncthreads();
-    if (a.h_out && mine)
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 16 * m + 4 * g + i;
-          if (r < a.dk) a.h_out[state + size_t(r) * a.dv] = S[m][i];
-        }
+    last_state<DKP>(a, column, g, S);
     // rows behind the last sequence
-    if (a.offsets && a.zero_tail && seq == a.nseq - 1 && mine)
+    if (!MAP && a.offsets && a.zero_tail && sp.seq == a.nseq - 1 && sp.last && mine)
       for (int t = sp.row + sp.rows + g; t < a.T; t += 4) put(static_cast<T*>(a.y) + (size_t(t) * a.Hv + h) * a.dv + col, 0.0f);
     return;
   }
@@ -575,15 +638,15 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
     fetch_keys(0);
     stash_keys(0);
     if (chunks > 1) fetch_keys(1);
-    fetch_queries(0);
+    if (!MAP) fetch_queries(0);
   }
   for (int c = 0; c <= chunks; ++c) {
     __syncthreads();
     if (c + 1 < chunks) stash_keys(c + 1);
-    if (c < chunks) stash_queries(c);
+    if (!MAP && c < chunks) stash_queries(c);
     if (c + 2 < chunks) fetch_keys(c + 2);
-    if (c + 1 < chunks) fetch_queries(c + 1);
-    if (c == 0) continue;
+    if (!MAP && c + 1 < chunks) fetch_queries(c + 1);
+    if (MAP || c == 0) continue;
     const int o = (c - 1) % 2;
     const float* gains = lds.gains[(c - 1) % 4];
     f32x4_t qs[2] = {};
@@ -610,9 +673,85 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
       take(lds.p[o] + t * 64 + lane, 128, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) qs[t][i] *= a.scale * gm[4 * t + i];
-      qs[t] = product(w, u, qs[t]);
+      // all four products of the parts: with keys alike, the terms are several times y
+      qs[t] = product(w, u, mfma16(w[1], u[1], qs[t]));
 #pragma unroll
       for (int i = 0; i < 4; ++i) store_element<T>(yy, yy.at<T, true>(16 * t + 4 * g + i, col, a.dv), qs[t][i]);
+    }
+  }
+}
+
+// The state behind each part of a sequence but its last, from the one before: ends[i] <- maps[i] ends[i - 1] + ends[i], the
+// first being right already.  A wave 16 columns; a part's map, 64 KB, goes to LDS in three bfloat16 parts while the next is
+// on its way to registers.
+template <int DKP>
+__global__ __launch_bounds__(256, 1) void delta_join(DeltaRule a) {
+  constexpr int KS = DKP / 32, MT = DKP / 16, PLANE = MT * KS * 64, PIECES = DKP / 32;
+  __shared__ uint4 s_map[3 * PLANE];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
+  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, col = blockIdx.y * kWalkColumns + wave * 16 + lane % 16;
+  const bool mine = col < a.dv;
+  const Span sp = span_of(a, seq);
+  const int parts = sp.rows <= a.fold ? 1 : (sp.rows - 1) / a.fold + 1;
+  const int part0 = a.offsets ? sp.row / a.fold + seq : seq * (a.T / a.fold + (a.T % a.fold != 0));
+  if (parts <= 2) return;
+  const auto end_of = [&](int i) { return a.ends + ((size_t(part0) + i) * a.Hv + h) * a.dk * a.dv + col; };
+  const auto load = [&](int i, f32x4_t (&S)[MT]) {
+    const float* p = end_of(i);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 16 * m + 4 * g + e;
+        S[m][e] = mine && r < a.dk ? p[size_t(r) * a.dv] : 0.0f;
+      }
+  };
+  // a thread's pieces of a map: rows p_row + 32 n
+  const int p_row = tid % 8 + tid / (8 * 2 * KS) * 8, p_at = tid / 8 % (2 * KS);
+  const bool p_on = KS == 4 || tid < 64 * KS;
+  const int p_col = p_at / 2 * 32 + p_at % 2 * 8;
+  Piece<float, true> piece[PIECES];
+  const auto fetch = [&](int i) {
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n)
+      if (p_on) {
+        const Rows mm(a.maps + ((size_t(part0) + i) * a.Hv + h) * DKP * DKP + n * 32 * DKP, DKP, kChunk, DKP);
+        piece[n].load(mm, p_row, p_col, DKP);
+      }
+  };
+  f32x4_t S[MT], next[MT];
+  load(0, S);
+  fetch(1);
+  for (int i = 1; i < parts - 1; ++i) {
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < PIECES; ++n)
+      if (p_on) piece[n].store(s_map + ((p_at / 2 * MT + 2 * n + p_row / 16) * 4 + p_at % 2 * 2) * 16 + p_row % 16, PLANE);
+    __syncthreads();
+    if (i + 1 < parts - 1) fetch(i + 1);
+    load(i, next);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
+                          S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
+      Unit u[3];
+      split<3>(x, u);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        Unit w[3];
+        take(s_map + (s * MT + m) * 64 + lane, PLANE, w);
+        next[m] = product(w, u, next[m]);
+      }
+    }
+    float* p = end_of(i);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      S[m] = next[m];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 16 * m + 4 * g + e;
+        if (mine && r < a.dk) p[size_t(r) * a.dv] = S[m][e];
+      }
     }
   }
 }
@@ -701,22 +840,54 @@ __global__ __launch_bounds__(256) void delta_step(DeltaRule a) {
   }
 }
 
+int delta_rule_parts(int fold, int B, int T, int nseq, bool packed) {
+  return packed ? T / fold + nseq : B * (T / fold + (T % fold != 0));
+}
+
+// Rows of the parts that sequences are walked in, or 0.  Few heads of long sequences leave most CUs without work: P parts are
+// walked once for what they do to the state (0.75 of a walk's time, for their values' and their keys' columns) and once with
+// the state before them, with a product for each between (64 rows' time); a CU walks one workgroup's 64 columns at a time.
+int delta_rule_fold(int B, int T, int Hv, int dk, int dv, int nseq, bool packed) {
+  const long long n = packed ? nseq : B, blocks = (dv + kWalkColumns - 1) / kWalkColumns, units = dk <= 64 ? 1 : 2;
+  if (n < 1 || n * Hv * blocks > 128) return 0;
+  const int rows = int(T / n);
+  const auto rounds = [](long long groups) { return (groups + 255) / 256; };
+  int best = 0;
+  long long least = 4LL * rows;
+  for (int parts = 2; parts <= 32; parts *= 2) {
+    const int fold = (rows / parts + kSegment) / kSegment * kSegment;
+    if (fold < 2 * kSegment || fold >= rows) continue;
+    const long long walks = n * Hv * parts;
+    const long long cost = fold * (4 * rounds(walks * blocks) + 3 * rounds(walks * (blocks + units))) + 4 * 64LL * (parts - 2);
+    if (cost < least) least = cost, best = fold;
+  }
+  return best;
+}
+
+template <int DKP, typename T, bool WIDE, bool KEEP, bool MAP>
+void walk(const DeltaRule& a, int blocks, int columns, hipStream_t s) {
+  const dim3 grid(blocks, columns);
+  if constexpr (sizeof(T) == 2) delta_walk_pairs<DKP, WIDE, KEEP, MAP><<<grid, 512, 0, s>>>(a);
+  else delta_walk<DKP, T, WIDE, KEEP, MAP><<<grid, 256, 0, s>>>(a);
+}
+
+template <int DKP, typename T, bool WIDE>
+void walk_all(const DeltaRule& a, hipStream_t s) {
+  const int n = a.offsets ? a.nseq : a.B, columns = (a.dv + kWalkColumns - 1) / kWalkColumns;
+  const int parts = a.fold ? delta_rule_parts(a.fold, a.B, a.T, a.nseq, a.offsets != nullptr) : n;
+  if (a.fold) {
+    walk<DKP, T, WIDE, false, true>(a, parts * a.Hv, columns + DKP / kWalkColumns, s);
+    delta_join<DKP><<<dim3(n * a.Hv, columns), 256, 0, s>>>(a);
+  }
+  if (a.errors) walk<DKP, T, WIDE, true, false>(a, parts * a.Hv, columns, s);
+  else walk<DKP, T, WIDE, false, false>(a, parts * a.Hv, columns, s);
+}
+
 template <typename T, bool WIDE>
 void run_as(const DeltaRule& a, hipStream_t s) {
-  const int n = a.offsets ? a.nseq : a.B;
   launch_delta_prepare<T, false>(a, WIDE, s);
-  const dim3 grid(n * a.Hv, (a.dv + kWalkColumns - 1) / kWalkColumns);
-  if constexpr (sizeof(T) == 2) {
-    if (a.errors && a.dk <= 64) delta_walk_pairs<64, WIDE, true><<<grid, 512, 0, s>>>(a);
-    else if (a.errors) delta_walk_pairs<128, WIDE, true><<<grid, 512, 0, s>>>(a);
-    else if (a.dk <= 64) delta_walk_pairs<64, WIDE, false><<<grid, 512, 0, s>>>(a);
-    else delta_walk_pairs<128, WIDE, false><<<grid, 512, 0, s>>>(a);
-    return;
-  }
-  if (a.errors && a.dk <= 64) delta_walk<64, T, WIDE, true><<<grid, 256, 0, s>>>(a);
-  else if (a.errors) delta_walk<128, T, WIDE, true><<<grid, 256, 0, s>>>(a);
-  else if (a.dk <= 64) delta_walk<64, T, WIDE, false><<<grid, 256, 0, s>>>(a);
-  else delta_walk<128, T, WIDE, false><<<grid, 256, 0, s>>>(a);
+  if (a.dk <= 64) walk_all<64, T, WIDE>(a, s);
+  else walk_all<128, T, WIDE>(a, s);
 }
 
 template <typename T>
@@ -751,14 +922,24 @@ int delta_rule_slots(int B, int T, int nseq, bool packed) { return packed ? T / 
 
 int delta_rule_segments(int B, int T, int nseq, bool packed) { return packed ? T / kSegment + nseq : B * segments_of(T); }
 
-size_t delta_rule_workspace(int B, int T, int Hv, int nseq, bool packed) {
-  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float, false> * sizeof(uint4) + 96 * sizeof(float)) + 256 * sizeof(uint4);
+size_t delta_rule_workspace(int B, int T, int Hv, int dk, int dv, int nseq, bool packed) {
+  const int fold = delta_rule_fold(B, T, Hv, dk, dv, nseq, packed), wide = dk <= 64 ? 64 : 128;
+  const size_t parts = fold ? size_t(delta_rule_parts(fold, B, T, nseq, packed)) * Hv : 0;
+  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float, false> * sizeof(uint4) + 96 * sizeof(float)) +
+         256 * sizeof(uint4) + parts * (size_t(wide) * wide + size_t(dk) * dv) * sizeof(float);
 }
 
 hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s) {
-  const size_t heads = size_t(delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr)) * a.Hv;
+  const bool packed = a.offsets != nullptr;
+  const size_t heads = size_t(delta_rule_slots(a.B, a.T, a.nseq, packed)) * a.Hv, wide = a.dk <= 64 ? 64 : 128;
   a.units = static_cast<uint4*>(workspace);
-  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float, false> : kUnits<Bf16, false>));   // 160 more behind the last
+  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float, false> : kUnits<Bf16, false>));
+  float* at = a.gains + heads * 96 + 256;   // 160 more behind the last are read
+  a.fold = delta_rule_fold(a.B, a.T, a.Hv, a.dk, a.dv, a.nseq, packed);
+  if (a.fold) {
+    a.maps = at;
+    a.ends = at + size_t(delta_rule_parts(a.fold, a.B, a.T, a.nseq, packed)) * a.Hv * wide * wide;
+  }
   if (dtype == 0) run<float>(a, s);
   else run<Bf16>(a, s);
   return hipGetLastError();

@@ -392,6 +392,9 @@ struct DeltaRule {
   float* states;           // (segments, Hv, dk, dv) out, for the adjoint: S before every 128th row of a sequence; or null
   uint4* units;            // workspace: each chunk's and head's L and P (csrc/delta_rule.h)
   float* gains;            // workspace: (slots, Hv, 96) gamma, d and beta of a chunk's rows
+  int fold;                // rows of a part of a sequence that is walked by itself; 0: sequences are walked whole
+  float* ends;             // workspace: (parts, Hv, dk, dv) the state behind each part
+  float* maps;             // workspace: (parts, Hv, DKP, DKP) what a part does to the state, DKP = 64 or 128
   // adjoint (errors and states as the forward wrote them)
   TokenRows dy;            // (B, T, Hv x dv)
   const float* dh;         // (n, Hv, dk, dv) or null: zeros
@@ -405,7 +408,7 @@ struct DeltaRule {
 };
 int delta_rule_slots(int B, int T, int nseq, bool packed);     // chunks that the workspace has room for
 int delta_rule_segments(int B, int T, int nseq, bool packed);
-size_t delta_rule_workspace(int B, int T, int Hv, int nseq, bool packed);
+size_t delta_rule_workspace(int B, int T, int Hv, int dk, int dv, int nseq, bool packed);
 hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s);
 size_t delta_rule_bwd_workspace(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, bool packed);
 hipError_t launch_delta_rule_bwd(DeltaRule a, int dtype, void* workspace, hipStream_t s);

@@ -467,7 +467,7 @@ def delta_forward(q, k, v, beta, decay=None, state=None, offsets=None, out=None,
         states = torch.empty((lib.cssm_delta_rule_segments(d.B, d.T, d.nseq, int(packed)), d.Hv, d.dk, d.dv),
                              dtype=torch.float32, device=v.device)
     if d.n:
-        need = lib.cssm_delta_rule_workspace_size(d.B, d.T, d.Hv, d.nseq, int(packed))
+        need = lib.cssm_delta_rule_workspace_size(d.B, d.T, d.Hv, d.dk, d.dv, d.nseq, int(packed))
         work = torch.empty(need, dtype=torch.uint8, device=v.device)
         _call(d.dev, "cssm_delta_rule", _ref(d.q), _ref(d.k), _ref(d.v), d.dtype, _ref(d.beta), _ref(d.decay), d.B, d.T,
               d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), _ptr(state), _ptr(offsets), d.nseq,

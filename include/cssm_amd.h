@@ -1015,7 +1015,7 @@ int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const
  */
 #define CSSM_DELTA_SEGMENT 128
 int cssm_delta_rule_segments(int B, int T, int nseq, int packed);
-size_t cssm_delta_rule_workspace_size(int B, int T, int Hv, int nseq, int packed);
+size_t cssm_delta_rule_workspace_size(int B, int T, int Hv, int dk, int dv, int nseq, int packed);
 int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cssm_token_rows* v, int dtype,
                     const cssm_token_rows* beta, const cssm_token_rows* decay, int B, int T, int Hk, int Hv, int dk, int dv,
                     float scale, const float* h0, const int* offsets, int nseq, void* y, int zero_tail, float* h_out,

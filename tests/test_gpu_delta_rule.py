@@ -110,6 +110,42 @@ def test_packed_as_alone(Q):
         assert torch.equal(yi[0], y[r]) and torch.equal(fi[0], final[i])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,T,Hk,Hv,dk,dv", [(1, 1400, 1, 1, 64, 48), (1, 3000, 1, 2, 128, 128), (2, 2049, 1, 1, 100, 72),
+                                             (1, 6001, 1, 1, 32, 16)])
+def test_long(Q, B, T, Hk, Hv, dk, dv, dtype):
+    """few heads of long sequences, which are walked in parts"""
+    print_case(test="delta rule long", B=B, T=T, Hk=Hk, Hv=Hv, dk=dk, dv=dv, dtype=str(dtype))
+    q, k, v, beta, decay, state = R.inputs(B, T, Hk, Hv, dk, dv, dtype, T, correlated=True)
+    want = R.whole(q, k, v, beta, decay, state)
+    y, final = Q.delta_rule(q, k, v, beta, decay, state)
+    assert R.off(y, want["y"]) <= 1 and R.off(final, want["final"]) <= 1
+    again = Q.delta_rule(q, k, v, beta, decay, state)
+    assert torch.equal(y, again[0]) and torch.equal(final, again[1])
+    y, final = Q.delta_rule(q, k, v, beta)
+    want = R.whole(q, k, v, beta)
+    assert R.off(y, want["y"]) <= 1 and R.off(final, want["final"]) <= 1
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("offsets,tail", [([0, 700, 700, 1800, 3100], 13), ([0, 0, 2100, 2101], 0), ([0, 5, 3000], 200),
+                                          ([0, 2048], 900)])
+def test_long_packed(Q, offsets, tail, dtype):
+    T, n = offsets[-1] + tail, len(offsets) - 1
+    print_case(test="delta rule long packed", offsets=offsets, tail=tail, dtype=str(dtype))
+    q, k, v, beta, decay, state = R.inputs(1, T, 1, 2, 40, 24, dtype, T + n, n=n)
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    for t in (q, k, v, beta, decay):
+        t[offsets[-1]:] = float("nan")
+    want = R.whole(q, k, v, beta, decay, state, off)
+    y, final = Q.delta_rule(q, k, v, beta, decay, state, offsets=off)
+    assert R.off(y, want["y"]) <= 1 and R.off(final, want["final"]) <= 1
+    assert not y[offsets[-1]:].any()
+    for bad in ([0, 1 << 30], [-5, 50], [0, 1 << 30, 20], [900, 10, 3000]):
+        Q.delta_rule(q, k, v, beta, decay, offsets=torch.tensor(bad, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+
+
 def test_no_sequences(Q):
     q, k, v, beta, decay, state = R.inputs(1, 9, 1, 2, 16, 8, BF16, 9, n=0)
     off = torch.zeros(1, dtype=torch.int32, device="cuda")

@@ -51,6 +51,12 @@ def test_sequences(T, B, T_, Hk, Hv, dk, dv, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long(T, dtype):
+    """few heads of a long sequence, which the forward walks in parts"""
+    check(T, R.inputs(1, 1500, 1, 2, 48, 32, dtype, 5))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("dy,dfinal", [(True, False), (False, True)])
 def test_one_gradient(T, dy, dfinal, dtype):
     """no decay, no state, another scale; one of the two outputs used"""
