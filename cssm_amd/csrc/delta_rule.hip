@@ -84,8 +84,8 @@ __device__ __forceinline__ bool chunk_at(const DeltaRule& a, int slot, int& b, i
 // half of the wave, a column of its 32 x 32 a lane: decays, L row by row, and both written as first operands (TURNED: their
 // transposes, which the adjoint takes).  What bounds it is the 500 multiplications in a row behind L and the traffic through
 // LDS between the layouts; four waves a SIMD hide most of their latencies.
-template <typename T, bool WIDE, bool TURNED>
-__global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
+template <int DKP, typename T, bool WIDE, bool TURNED>
+__global__ __launch_bounds__(64, sizeof(T) == 2 ? 4 : 2) void delta_prepare(DeltaRule a) {
   __shared__ __attribute__((aligned(16))) float s_m[2][kChunk * kPad];
   __shared__ float s_alpha[2][kChunk];
   const int lane = threadIdx.x, j = lane % 32, half = lane / 32, G = a.Hv / a.Hk, h0 = 2 * blockIdx.y, h = h0 + half;
@@ -101,35 +101,43 @@ __global__ __launch_bounds__(64) void delta_prepare(DeltaRule a) {
   }
   s_alpha[half][j] = alpha;
   float A[kChunk], P[kChunk];
+  const Rows k[2] = {Rows(row_at<T>(a.k, b, row) + hk[0] * a.dk, a.k.row, rows, a.dk), Rows(row_at<T>(a.k, b, row) + hk[1] * a.dk, a.k.row, rows, a.dk)};
+  const Rows q[2] = {Rows(row_at<T>(a.q, b, row) + hk[0] * a.dk, a.q.row, rows, a.dk), Rows(row_at<T>(a.q, b, row) + hk[1] * a.dk, a.q.row, rows, a.dk)};
   {
-    f32x16_t kk[2] = {}, qk[2] = {};
+    f32x16_t qk[2];
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
-      if (o == 1 && hk[1] == hk[0]) {
-        kk[1] = kk[0], qk[1] = qk[0];
-        break;
-      }
-      const Rows k(row_at<T>(a.k, b, row) + hk[o] * a.dk, a.k.row, rows, a.dk);
-      const Rows q(row_at<T>(a.q, b, row) + hk[o] * a.dk, a.q.row, rows, a.dk);
-      for (int at = 0; at < a.dk; at += 16) {
-        Unit uk[PartsOf<T>::n], uq[PartsOf<T>::n];
-        load_unit<T, WIDE>(k, j, at + 8 * half, a.dk, uk);
-        load_unit<T, WIDE>(q, j, at + 8 * half, a.dk, uq);
-        kk[o] = product32(uk, uk, kk[o]);
-        qk[o] = product32(uq, uk, qk[o]);
+      f32x16_t kk = {}, x = {};
+      if (o == 0 || hk[1] != hk[0]) {
+        // all of a head's loads at once: one after the other they would take longer than everything else
+        Unit uk[DKP / 16][PartsOf<T>::n], uq[DKP / 16][PartsOf<T>::n];
+#pragma unroll
+        for (int i = 0; i < DKP / 16; ++i) load_unit<T, WIDE>(k[o], j, 16 * i + 8 * half, a.dk, uk[i]), load_unit<T, WIDE>(q[o], j, 16 * i + 8 * half, a.dk, uq[i]);
+#pragma unroll
+        for (int i = 0; i < DKP / 16; ++i) kk = product32(uk[i], uk[i], kk), x = product32(uq[i], uk[i], x);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = (8 * (i / 4) + 4 * half + i % 4) * kPad + j;
+          s_m[o][at] = kk[i];
+          if (o == 0) s_m[1][at] = kk[i];   // of the second head too, unless it is of another key
+        }
+        qk[o] = x;
+      } else {
+        qk[1] = qk[0];
       }
     }
+    __syncthreads();
 #pragma unroll
-    for (int what = 0; what < 2; ++what) {
+    for (int i = 0; i < kChunk; ++i) A[i] = s_m[half][i * kPad + j];
+    __syncthreads();
 #pragma unroll
-      for (int o = 0; o < 2; ++o)
+    for (int o = 0; o < 2; ++o)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_m[o][(8 * (i / 4) + 4 * half + i % 4) * kPad + j] = what ? qk[o][i] : kk[o][i];
-      __syncthreads();
+      for (int i = 0; i < 16; ++i) s_m[o][(8 * (i / 4) + 4 * half + i % 4) * kPad + j] = qk[o][i];
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) (what ? P : A)[i] = s_m[half][i * kPad + j];
-      __syncthreads();
-    }
+    for (int i = 0; i < kChunk; ++i) P[i] = s_m[half][i * kPad + j];
+    __syncthreads();
   }
   float d = 0.0f;
 #pragma unroll
@@ -846,7 +854,7 @@ int delta_rule_parts(int fold, int B, int T, int nseq, bool packed) {
 
 // Rows of the parts that sequences are walked in, or 0.  Few heads of long sequences leave most CUs without work: P parts are
 // walked once for what they do to the state (0.75 of a walk's time, for their values' and their keys' columns) and once with
-// the state before them, with a product for each between (64 rows' time); a CU walks one workgroup's 64 columns at a time.
+// the state before them, with a product for each between (128 rows' time); a CU walks one workgroup's 64 columns at a time.
 int delta_rule_fold(int B, int T, int Hv, int dk, int dv, int nseq, bool packed) {
   const long long n = packed ? nseq : B, blocks = (dv + kWalkColumns - 1) / kWalkColumns, units = dk <= 64 ? 1 : 2;
   if (n < 1 || n * Hv * blocks > 128) return 0;
@@ -858,7 +866,7 @@ int delta_rule_fold(int B, int T, int Hv, int dk, int dv, int nseq, bool packed)
     const int fold = (rows / parts + kSegment) / kSegment * kSegment;
     if (fold < 2 * kSegment || fold >= rows) continue;
     const long long walks = n * Hv * parts;
-    const long long cost = fold * (4 * rounds(walks * blocks) + 3 * rounds(walks * (blocks + units))) + 4 * 64LL * (parts - 2);
+    const long long cost = fold * (4 * rounds(walks * blocks) + 3 * rounds(walks * (blocks + units))) + 4 * 128LL * (parts - 2);
     if (cost < least) least = cost, best = fold;
   }
   return best;
@@ -912,8 +920,10 @@ void launch_delta_prepare(const DeltaRule& a, bool wide, hipStream_t s) {
   const int slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
   if (!slots) return;
   const dim3 grid(slots, (a.Hv + 1) / 2);
-  if (wide) delta_prepare<T, true, TURNED><<<grid, 64, 0, s>>>(a);
-  else delta_prepare<T, false, TURNED><<<grid, 64, 0, s>>>(a);
+  if (wide && a.dk <= 64) delta_prepare<64, T, true, TURNED><<<grid, 64, 0, s>>>(a);
+  else if (wide) delta_prepare<128, T, true, TURNED><<<grid, 64, 0, s>>>(a);
+  else if (a.dk <= 64) delta_prepare<64, T, false, TURNED><<<grid, 64, 0, s>>>(a);
+  else delta_prepare<128, T, false, TURNED><<<grid, 64, 0, s>>>(a);
 }
 template void launch_delta_prepare<float, true>(const DeltaRule&, bool, hipStream_t);
 template void launch_delta_prepare<Bf16, true>(const DeltaRule&, bool, hipStream_t);
