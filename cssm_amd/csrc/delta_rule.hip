@@ -301,8 +301,9 @@ struct WalkLds {
   float gains[256];   // gamma, d, beta; the rest takes what threads without a value write
 };
 
-// One workgroup carries 64 columns of one sequence's and head's state through the chunks.  While a chunk is computed
-// from LDS, the next one's rows are on their way into registers.
+// One workgroup carries 64 columns of one sequence's and head's state through the chunks (float32: in LDS there is no room
+// for the second kind of waves below).  While a chunk is computed from LDS, the next one's rows are on their way into
+// registers.  3 x 197 x 3 heads of 40 and 50: 25 us, 3.5 a chunk.
 template <int DKP, typename T, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
   using Lds = WalkLds<DKP, T>;
@@ -487,8 +488,10 @@ struct PairLds {
 };
 
 // The same for bfloat16 by two kinds of waves, a pair for 16 columns on each SIMD: the first carries the state, the second
-// brings the chunks' rows to LDS and makes y of the chunk before, from S and U that the first leaves in LDS.  A step is
-// then as long as the state's own chain of products, with the second wave's work in its gaps: PLACEHOLDER
+// brings the chunks' rows to LDS and makes y of the chunk before, from S and U that the first leaves in LDS.  A step then
+// takes the state's own chain of products, 2.3 us a chunk on a full chip and 1.8 with few workgroups, where one kind of
+// wave for all of it took 3.4 and 2.6 (8 x 2048 and 1 x 65536 rows).  What bounds it: the 560 instructions that the first wave
+// issues a step, 60 products and some 370 to split and combine, one behind the other.
 template <int DKP, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
   using T = Bf16;
@@ -691,7 +694,7 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
 
 // The state behind each part of a sequence but its last, from the one before: ends[i] <- maps[i] ends[i - 1] + ends[i], the
 // first being right already.  A wave 16 columns; a part's map, 64 KB, goes to LDS in three bfloat16 parts while the next is
-// on its way to registers.
+// on its way to registers: 7.5 us a part.
 template <int DKP>
 __global__ __launch_bounds__(256, 1) void delta_join(DeltaRule a) {
   constexpr int KS = DKP / 32, MT = DKP / 16, PLANE = MT * KS * 64, PIECES = DKP / 32;
@@ -766,7 +769,8 @@ __global__ __launch_bounds__(256, 1) void delta_join(DeltaRule a) {
 
 // One token: 32 columns of a head's state to a workgroup, 8 threads of 4 columns side by side and 32 rows, or with
 // element loads 32 threads of one column and 8 rows, at a time.  The state is read once, kept in registers between
-// the two sums over its rows, and written once.
+// the two sums over its rows, and written once: HBM bounds it.  128 x 16 heads of 128 x 128: 268 MB in 49 to 62 us, 4.3 to
+// 5.5 TB/s.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void delta_step(DeltaRule a) {
   constexpr int X = 32 / V, RG = 256 / X, R = 128 / RG, W = RG * X / 64;   // rows side by side, rows a thread, waves
@@ -852,7 +856,7 @@ int delta_rule_parts(int fold, int B, int T, int nseq, bool packed) {
   return packed ? T / fold + nseq : B * (T / fold + (T % fold != 0));
 }
 
-// Rows of the parts that sequences are walked in, or 0.  Few heads of long sequences leave most CUs without work: P parts are
+// Rows of the parts that sequences are walked in, or 0.  1 x 65536 x 8 heads: whole 3760 us, in 16 parts 430 + 105 + 300.  Few heads of long sequences leave most CUs without work: P parts are
 // walked once for what they do to the state (0.75 of a walk's time, for their values' and their keys' columns) and once with
 // the state before them, with a product for each between (128 rows' time); a CU walks one workgroup's 64 columns at a time.
 int delta_rule_fold(int B, int T, int Hv, int dk, int dv, int nseq, bool packed) {

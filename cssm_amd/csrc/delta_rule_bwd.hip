@@ -9,7 +9,9 @@
 //   ddecay_l = <S, dS>_end + sum over i >= l of (q_i.dq_i + k_i.read_i - k_i.write_i)
 // delta_walk_back carries dS from chunk to chunk, as the forward does S, and keeps it behind every 128th row; then
 // delta_grads takes each 128 rows by themselves, forwards with S and backwards with dS, a wave 16 of the keys' columns, so
-// that the sums over dv lie within a wave.
+// that the sums over dv lie within a wave.  Training 4 x 4096 x 16 heads of 128: delta_walk_back 410 us (3.2 a chunk, a chain
+// of products as the forward's), delta_grads 670 us (2048 workgroups of 8 waves, two a SIMD: 450 products a chunk and pair of
+// waves and the splitting of their operands; 32 columns a wave halve what is read from LDS, but leave one wave a SIMD: 880).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -201,7 +203,8 @@ __device__ __forceinline__ float value_of(const Unit (&u)[N], int i) {
   return v;
 }
 
-// P: dk and dv up to it.  One workgroup for 128 rows of one value head, P / 16 waves.
+// P: dk and dv up to it.  One workgroup for 128 rows of one value head, P / 16 waves.  Y, Z and their transposes take the place
+// of U's rows in LDS once those are read.
 template <int P, typename T, bool WIDE>
 __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
   constexpr int N = PartsOf<T>::n, W = P / 16, KS = P / 32, MT = P / 16, PLANE = P * 4, TASKS = (6 + W - 1) / W;
