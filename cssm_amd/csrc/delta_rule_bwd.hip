@@ -194,6 +194,198 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
       }
 }
 
+template <int DKP>
+struct BackPairLds {
+  static constexpr int kPlane = DKP * 4;
+  uint4 k[2][kPlane], kt[2][kPlane], qt[2][kPlane], l[2][3 * 128];
+  uint4 py[2][4][2 * 64], gy[2][4][3 * 64], x[2][4][2 * 64];   // for 16 columns each: P^T dY, three parts of scale gamma dY, X
+  float gains[4][96];
+};
+
+// The same for bfloat16 by two kinds of waves, as the forward's: the first carries the state's gradient, the second brings
+// the chunks' rows to LDS, makes what dY alone decides, and writes X and dV of the chunk before.
+template <int DKP, bool WIDE>
+__global__ __launch_bounds__(512, 1) void delta_back_pairs(DeltaRule a) {
+  using T = Bf16;
+  constexpr int PLANE = DKP * 4, KS = DKP / 32, MT = DKP / 16;
+  __shared__ BackPairLds<DKP> lds;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % 4, g = lane / 16;
+  const bool carries = __builtin_amdgcn_readfirstlane(threadIdx.x / 256) == 0;
+  const int tid = threadIdx.x % 256;
+  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int b = a.offsets ? 0 : seq;
+  const Span sp = span_of(a, seq);
+  const int chunks = chunks_of(sp.rows);
+  const int col = blockIdx.y * kBackColumns + wave * 16 + lane % 16;
+  const bool mine = col < a.dv;
+  const size_t state = (size_t(seq) * a.Hv + h) * a.dk * a.dv + col;
+
+  // step n is of chunk chunks - 1 - n
+  if (carries) {
+    f32x4_t S[MT];   // the state's gradient
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * m + 4 * g + i;
+        S[m][i] = a.dh && mine && r < a.dk ? a.dh[state + size_t(r) * a.dv] : 0.0f;
+      }
+    for (int n = 0; n < chunks; ++n) {
+      const int c = chunks - 1 - n, o = n % 2;
+      __syncthreads();
+      const float* gains = lds.gains[n % 4];
+      if ((c % kChunks == kChunks - 1 || n == 0) && mine) {
+        float* st = a.dstates + (size_t(sp.segment + c / kChunks) * a.Hv + h) * a.dk * a.dv + col;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * m + 4 * g + i < a.dk) st[size_t(16 * m + 4 * g + i) * a.dv] = S[m][i];
+      }
+      f32x4_t ks[2] = {};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
+                            S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
+        Unit u[3];
+        split<3>(x, u);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Unit w[1];
+          take(lds.k[o] + (s * 2 + t) * 64 + lane, PLANE, w);
+          ks[t] = product(w, u, ks[t]);
+        }
+      }
+      float gm[8], dd[8], bt[8], x[8], dU[8];
+      take_rows(gains, g, gm), take_rows(gains + 32, g, dd), take_rows(gains + 64, g, bt);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f32x4_t py = __builtin_bit_cast(f32x4_t, lds.py[o][wave][t * 64 + lane]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dU[4 * t + i] = py[i] + dd[4 * t + i] * ks[t][i], x[4 * t + i] = bt[4 * t + i] * dU[4 * t + i];
+      }
+      {
+        Unit u[3];
+        split<3>(x, u);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          Unit w[3];
+          take(lds.l[o] + t * 64 + lane, 128, w);
+          const f32x4_t le = product(w, u, f32x4_t{});
+          f32x4_t X;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) X[i] = dU[4 * t + i] - le[i], x[4 * t + i] = -gm[4 * t + i] * bt[4 * t + i] * X[i];
+          lds.x[o][wave][t * 64 + lane] = __builtin_bit_cast(uint4, X);
+        }
+      }
+      {
+        Unit u[3], v[3];
+        take(lds.gy[o][wave] + lane, 64, u);
+        split<3>(x, v);
+        const float all = gains[31];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          Unit w[1];
+          S[m] *= all;
+          take(lds.qt[o] + m * 64 + lane, PLANE, w);
+          S[m] = product(w, u, S[m]);
+          take(lds.kt[o] + m * 64 + lane, PLANE, w);
+          S[m] = product(w, v, S[m]);
+        }
+      }
+    }
+    __syncthreads();
+    if (a.dh0 && mine)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * m + 4 * g + i;
+          if (r < a.dk) a.dh0[state + size_t(r) * a.dv] = S[m][i];
+        }
+    return;
+  }
+
+  const int p_tok = tid % 8 + tid / (8 * 2 * KS) * 8, p_at = tid / 8 % (2 * KS);
+  const bool p_on = KS == 4 || tid < 64 * KS;
+  const int p_col = p_at / 2 * 32 + p_at % 2 * 8;
+  const int p_unit = ((p_at / 2 * 2 + p_tok / 16) * 4 + p_at % 2 * 2) * 16 + p_tok % 16;
+  const int c_g = tid / (DKP / 2), c_col = tid % (DKP / 2) * 2;
+  const bool c_on = DKP == 128 || tid < 2 * DKP;
+  const int c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
+  Piece<T, WIDE> pk;
+  Columns<T, WIDE> ck, cq;
+  u32x4_t l[2], p[6];
+  f32x4_t gm[2];
+  float gain;
+  uint32_t dy[8];
+  const auto fetch = [&](int n) {
+    const int c = chunks - 1 - n, rows = sp.rows - c * kChunk;
+    const long long t = sp.row + (long long)c * kChunk;
+    const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
+    const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
+    const size_t head = size_t(sp.slot + c) * a.Hv + h;
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T, true>;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dy[i] = load_element<T>(y, y.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
+    if (p_on) pk.load(k, p_tok, p_col, a.dk);
+    if (c_on) ck.load(k, 4 * c_g, c_col, a.dk), cq.load(q, 4 * c_g, c_col, a.dk);
+    l[0] = units[tid], l[1] = units[256 + tid % 128];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) p[i] = units[3 * 128 + 64 * i + lane];
+    const float* gains = a.gains + head * 96;
+    gain = gains[tid % 96];
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) gm[t2] = *reinterpret_cast<const f32x4_t*>(gains + 16 * t2 + 4 * g);
+  };
+  const auto stash = [&](int n) {   // what step n takes
+    const int o = n % 2;
+    if (p_on) pk.store(lds.k[o] + p_unit, PLANE);
+    if (c_on) ck.store(lds.kt[o] + c_unit, PLANE), cq.store(lds.qt[o] + c_unit, PLANE);
+    lds.l[o][tid] = __builtin_bit_cast(uint4, l[0]);
+    if (tid < 128) lds.l[o][256 + tid] = __builtin_bit_cast(uint4, l[1]);
+    if (tid < 96) lds.gains[n % 4][tid] = gain;
+    float dY[8], x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dY[i] = element<T>(dy[i]), x[i] = a.scale * gm[i / 4][i % 4] * dY[i];
+    Unit u[1], v[3];
+    split<1>(dY, u), split<3>(x, v);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Unit w[3] = {__builtin_bit_cast(Unit, p[t]), __builtin_bit_cast(Unit, p[2 + t]), __builtin_bit_cast(Unit, p[4 + t])};
+      lds.py[o][wave][t * 64 + lane] = __builtin_bit_cast(uint4, product(w, u, f32x4_t{}));
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) lds.gy[o][wave][i * 64 + lane] = __builtin_bit_cast(uint4, v[i]);
+  };
+  if (chunks) {
+    fetch(0);
+    stash(0);
+    if (chunks > 1) fetch(1);
+  }
+  // step n: step n + 1's operands come in, X and dV of step n - 1 go out
+  for (int n = 0; n <= chunks; ++n) {
+    __syncthreads();
+    if (n + 1 < chunks) stash(n + 1);
+    if (n + 2 < chunks) fetch(n + 2);
+    if (n == 0) continue;
+    const int c = chunks - n, rows = sp.rows - c * kChunk, o = (n - 1) % 2;
+    float bt[8];
+    take_rows(lds.gains[(n - 1) % 4] + 64, g, bt);
+    const size_t head = ((size_t(b) * a.T + sp.row + (long long)c * kChunk) * a.Hv + h) * a.dv;
+    const Rows dv(static_cast<T*>(a.dv_out) + head, a.Hv * a.dv, rows, a.dv), xx(a.duals + head, a.Hv * a.dv, rows, a.dv);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const f32x4_t X = __builtin_bit_cast(f32x4_t, lds.x[o][wave][t * 64 + lane]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        store_element<T>(dv, dv.at<T, true>(16 * t + 4 * g + i, col, a.dv), bt[4 * t + i] * X[i]);
+        store_element<float>(xx, xx.at<float, true>(16 * t + 4 * g + i, col, a.dv), X[i]);
+      }
+    }
+  }
+}
+
 // the value of element i of a lane's unit, all parts together
 template <int N>
 __device__ __forceinline__ float value_of(const Unit (&u)[N], int i) {
@@ -588,8 +780,13 @@ void run_as(const DeltaRule& a, hipStream_t s) {
   const int n = a.offsets ? a.nseq : a.B, segments = delta_rule_segments(a.B, a.T, a.nseq, a.offsets != nullptr);
   launch_delta_prepare<T, true>(a, WIDE, s);
   const dim3 grid(n * a.Hv, (a.dv + kBackColumns - 1) / kBackColumns);
-  if (a.dk <= 64) delta_walk_back<64, T, WIDE><<<grid, 256, 0, s>>>(a);
-  else delta_walk_back<128, T, WIDE><<<grid, 256, 0, s>>>(a);
+  if constexpr (sizeof(T) == 2) {
+    if (a.dk <= 64) delta_back_pairs<64, WIDE><<<grid, 512, 0, s>>>(a);
+    else delta_back_pairs<128, WIDE><<<grid, 512, 0, s>>>(a);
+  } else {
+    if (a.dk <= 64) delta_walk_back<64, T, WIDE><<<grid, 256, 0, s>>>(a);
+    else delta_walk_back<128, T, WIDE><<<grid, 256, 0, s>>>(a);
+  }
   if (!a.T) return;
   if (a.dk <= 64 && a.dv <= 64) delta_grads<64, T, WIDE><<<dim3(segments, a.Hv), 256, 0, s>>>(a);
   else delta_grads<128, T, WIDE><<<dim3(segments, a.Hv), 512, 0, s>>>(a);
