@@ -395,6 +395,16 @@ __device__ __forceinline__ float value_of(const Unit (&u)[N], int i) {
   return v;
 }
 
+// sum over 16 lanes side by side, by rotations within them
+template <int BY>
+__device__ __forceinline__ float rotated(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + BY, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum16(float x) {
+  x += rotated<8>(x), x += rotated<4>(x), x += rotated<2>(x);
+  return x + rotated<1>(x);
+}
+
 // P: dk and dv up to it.  One workgroup for 128 rows of one value head, P / 16 waves.  Y, Z and their transposes take the place
 // of U's rows in LDS once those are read.
 template <int P, typename T, bool WIDE>
@@ -616,8 +626,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         else store_element<T>(dqo, dqo.at<T, true>(r, col, a.dk), dq[i]);
         const float kv = value_of(kb, i);
         float x = fmaf(value_of(qb, i), dq[i], kv * rd[i]), y = kv * wr[i];
-#pragma unroll
-        for (int o = 1; o < 16; o *= 2) x += __shfl_xor(x, o), y += __shfl_xor(y, o);
+        x = sum16(x), y = sum16(y);
         if (lane % 16 == 0) s_read[wave][c * kChunk + r] = x, s_write[wave][c * kChunk + r] = y;
       }
     }
@@ -712,8 +721,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         if (shared) store_element<float>(dkh, dkh.at<float, true>(r, col, a.dk), before[i] + w);
         else store_element<T>(dko, dko.at<T, true>(r, col, a.dk), before[i] + w);
         float y = value_of(kb, i) * w;
-#pragma unroll
-        for (int o = 1; o < 16; o *= 2) y += __shfl_xor(y, o);
+        y = sum16(y);
         if (lane % 16 == 0) s_write[wave][c * kChunk + r] += y;
       }
     }
