@@ -1482,7 +1482,9 @@ int delta_workspace_check(const char* who, size_t need, const void* workspace, s
 extern "C" {
 
 int cssm_delta_rule_segments(int B, int T, int nseq, int packed) {
-  return B <= 0 || T < 0 || nseq < 0 ? 0 : cssm::delta_rule_segments(B, T, nseq, packed != 0);
+  if (B <= 0 || T < 0 || nseq < 0) return 0;
+  const long long n = cssm::delta_rule_segments(B, T, nseq, packed != 0);
+  return n > 0x7fffffff ? 0x7fffffff : int(n);   // more than any call takes
 }
 
 size_t cssm_delta_rule_workspace_size(int B, int T, int Hv, int dk, int dv, int nseq, int packed) {

@@ -852,8 +852,8 @@ __global__ __launch_bounds__(256) void delta_step(DeltaRule a) {
   }
 }
 
-int delta_rule_parts(int fold, int B, int T, int nseq, bool packed) {
-  return packed ? T / fold + nseq : B * (T / fold + (T % fold != 0));
+long long delta_rule_parts(int fold, int B, int T, int nseq, bool packed) {
+  return packed ? T / fold + (long long)nseq : (long long)B * (T / fold + (T % fold != 0));
 }
 
 // Rows of the parts that sequences are walked in, or 0.  1 x 65536 x 8 heads: whole 3760 us, in 16 parts 430 + 105 + 300.  Few heads of long sequences leave most CUs without work: P parts are
@@ -886,7 +886,7 @@ void walk(const DeltaRule& a, int blocks, int columns, hipStream_t s) {
 template <int DKP, typename T, bool WIDE>
 void walk_all(const DeltaRule& a, hipStream_t s) {
   const int n = a.offsets ? a.nseq : a.B, columns = (a.dv + kWalkColumns - 1) / kWalkColumns;
-  const int parts = a.fold ? delta_rule_parts(a.fold, a.B, a.T, a.nseq, a.offsets != nullptr) : n;
+  const int parts = a.fold ? int(delta_rule_parts(a.fold, a.B, a.T, a.nseq, a.offsets != nullptr)) : n;
   if (a.fold) {
     walk<DKP, T, WIDE, false, true>(a, parts * a.Hv, columns + DKP / kWalkColumns, s);
     delta_join<DKP><<<dim3(n * a.Hv, columns), 256, 0, s>>>(a);
@@ -921,7 +921,7 @@ void step(DeltaRule& a, hipStream_t s) {
 
 template <typename T, bool TURNED>
 void launch_delta_prepare(const DeltaRule& a, bool wide, hipStream_t s) {
-  const int slots = delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr);
+  const int slots = int(delta_rule_slots(a.B, a.T, a.nseq, a.offsets != nullptr));   // times Hv below 2^23
   if (!slots) return;
   const dim3 grid(slots, (a.Hv + 1) / 2);
   if (wide && a.dk <= 64) delta_prepare<64, T, true, TURNED><<<grid, 64, 0, s>>>(a);
@@ -932,9 +932,13 @@ void launch_delta_prepare(const DeltaRule& a, bool wide, hipStream_t s) {
 template void launch_delta_prepare<float, true>(const DeltaRule&, bool, hipStream_t);
 template void launch_delta_prepare<Bf16, true>(const DeltaRule&, bool, hipStream_t);
 
-int delta_rule_slots(int B, int T, int nseq, bool packed) { return packed ? T / kChunk + nseq : B * chunks_of(T); }
+long long delta_rule_slots(int B, int T, int nseq, bool packed) {
+  return packed ? T / kChunk + (long long)nseq : (long long)B * chunks_of(T);
+}
 
-int delta_rule_segments(int B, int T, int nseq, bool packed) { return packed ? T / kSegment + nseq : B * segments_of(T); }
+long long delta_rule_segments(int B, int T, int nseq, bool packed) {
+  return packed ? T / kSegment + (long long)nseq : (long long)B * segments_of(T);
+}
 
 size_t delta_rule_workspace(int B, int T, int Hv, int dk, int dv, int nseq, bool packed) {
   const int fold = delta_rule_fold(B, T, Hv, dk, dv, nseq, packed), wide = dk <= 64 ? 64 : 128;

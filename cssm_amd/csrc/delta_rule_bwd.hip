@@ -785,7 +785,7 @@ __global__ __launch_bounds__(256) void delta_tail(DeltaRule a) {
 
 template <typename T, bool WIDE>
 void run_as(const DeltaRule& a, hipStream_t s) {
-  const int n = a.offsets ? a.nseq : a.B, segments = delta_rule_segments(a.B, a.T, a.nseq, a.offsets != nullptr);
+  const int n = a.offsets ? a.nseq : a.B, segments = int(delta_rule_segments(a.B, a.T, a.nseq, a.offsets != nullptr));
   launch_delta_prepare<T, true>(a, WIDE, s);
   const dim3 grid(n * a.Hv, (a.dv + kBackColumns - 1) / kBackColumns);
   if constexpr (sizeof(T) == 2) {

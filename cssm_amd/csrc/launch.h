@@ -406,8 +406,8 @@ struct DeltaRule {
   float* dstates;          // workspace: (segments, Hv, dk, dv) the state's gradient behind each segment
   float *dq_heads, *dk_heads;   // workspace: (B, T, Hv, dk) each value head's share (dq_heads only where heads are shared)
 };
-int delta_rule_slots(int B, int T, int nseq, bool packed);     // chunks that the workspace has room for
-int delta_rule_segments(int B, int T, int nseq, bool packed);
+long long delta_rule_slots(int B, int T, int nseq, bool packed);     // chunks that the workspace has room for
+long long delta_rule_segments(int B, int T, int nseq, bool packed);
 size_t delta_rule_workspace(int B, int T, int Hv, int dk, int dv, int nseq, bool packed);
 hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s);
 size_t delta_rule_bwd_workspace(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, bool packed);

@@ -387,6 +387,7 @@ def _gate_rows(t, name: str, lead, H: int, dev: int, like: str) -> _lib.TokenRow
 
 _Rows5, _Rows2 = ctypes.c_longlong * 15, ctypes.c_longlong * 6     # cssm_token_rows one behind the other
 _ROWS = ctypes.sizeof(_lib.TokenRows)
+_MOST = 0x7fffffff
 
 
 def _fine(t, shape, dtype, dev: int) -> bool:
@@ -400,13 +401,14 @@ def _new(t: torch.Tensor) -> torch.Tensor:
 
 
 class _Delta(NamedTuple):
-    """Checked arguments of the delta rule: GPU, rows, sizes."""
+    """Checked arguments of the delta rule: GPU, rows (addresses in ``rows``), sizes."""
     dev: int
-    q: _lib.TokenRows
-    k: _lib.TokenRows
-    v: _lib.TokenRows
-    beta: _lib.TokenRows
-    decay: Optional[_lib.TokenRows]
+    rows: object
+    q: int
+    k: int
+    v: int
+    beta: int
+    decay: Optional[int]
     dtype: int
     B: int
     T: int
@@ -418,7 +420,51 @@ class _Delta(NamedTuple):
     nseq: int       # with offsets, else 0
 
 
-def _delta(q, k, v, beta, decay, state, offsets, step: bool = False, need_state: bool = False) -> _Delta:
+def _plain_delta(q, k, v, beta, decay, state, offsets, step: bool) -> Optional[_Delta]:
+    """:func:`_delta` of contiguous tensors that go together: the usual call, without the checks that name what is wrong.
+    None for any other."""
+    try:
+        dev, dt, f32, sv, sk, gate = v.get_device(), v.dtype, torch.float32, v.shape, k.shape, beta.shape
+        if len(sv) == 4 and offsets is None and not step:
+            B, T, Hv, dv = sv
+            n, nseq = B, 0
+            same = sk[0] == B and sk[1] == T and gate == (B, T, Hv)
+        elif len(sv) == 3 and step:
+            B, Hv, dv = sv
+            T, n, nseq = 1, B, 0
+            same = sk[0] == B and gate == (B, Hv)
+        elif len(sv) == 3 and offsets is not None:
+            T, Hv, dv = sv
+            B, n = 1, offsets.numel() - 1
+            nseq = n
+            same = (sk[0] == T and gate == (T, Hv) and n >= 0 and offsets.dim() == 1 and offsets.dtype is torch.int32
+                    and offsets.get_device() == dev and offsets.is_contiguous())
+        else:
+            return None
+        Hk, dk = sk[-2], sk[-1]
+        if not (same and dev >= 0 and dt in _DTYPES and k.dtype is dt and q.dtype is dt and beta.dtype is f32 and q.shape == sk
+                and len(sk) == len(sv) and 0 < dk <= 128 and 0 < dv <= 128 and Hk > 0 and 0 < Hv <= _MOST and Hv % Hk == 0
+                and B <= _MOST and T <= _MOST
+                and q.get_device() == dev and k.get_device() == dev and beta.get_device() == dev
+                and v.is_contiguous() and q.is_contiguous() and k.is_contiguous() and beta.is_contiguous()
+                and (decay is None or (decay.dtype is f32 and decay.shape == gate and decay.get_device() == dev
+                                       and decay.is_contiguous()))
+                and ((state is None and not step) or _fine(state, (n, Hv, dk, dv), f32, dev))):
+            return None
+    except (AttributeError, ValueError, IndexError):
+        return None
+    rk, rv = Hk * dk, Hv * dv
+    rows = _Rows5(q.data_ptr(), T * rk, rk, k.data_ptr(), T * rk, rk, v.data_ptr(), T * rv, rv, beta.data_ptr(), T * Hv, Hv,
+                  0 if decay is None else decay.data_ptr(), T * Hv, Hv)
+    at = ctypes.addressof(rows)
+    return _Delta(dev, rows, at, at + _ROWS, at + 2 * _ROWS, at + 3 * _ROWS, None if decay is None else at + 4 * _ROWS,
+                  _DTYPES[dt], B, T, Hk, Hv, dk, dv, n, nseq)
+
+
+def _delta(q, k, v, beta, decay, state, offsets, step: bool = False) -> _Delta:
+    d = _plain_delta(q, k, v, beta, decay, state, offsets, step)
+    if d is not None:
+        return d
     dev = _gpu(v, "v")
     if v.dtype not in _DTYPES:
         raise ValueError(f"v: unsupported dtype {v.dtype}")
@@ -446,9 +492,10 @@ def _delta(q, k, v, beta, decay, state, offsets, step: bool = False, need_state:
             raise ValueError("offsets must be a tensor of n + 1 row numbers")
         _check(offsets, "offsets", offsets.shape, torch.int32, dev)
         n = nseq = offsets.numel() - 1
-    if state is not None or need_state:
+    if state is not None or step:
         _check(state, "state", (n, Hv, dk, dv), torch.float32, dev)
-    return _Delta(dev, rq, rk, rv, rb, rd, _DTYPES[v.dtype], B, T, Hk, Hv, dk, dv, n, nseq)
+    rows = rq, rk, rv, rb, rd
+    return _Delta(dev, rows, *(_ref(r) for r in rows), _DTYPES[v.dtype], B, T, Hk, Hv, dk, dv, n, nseq)
 
 
 def delta_forward(q, k, v, beta, decay=None, state=None, offsets=None, out=None, scale=None, keep=False):
@@ -459,19 +506,17 @@ def delta_forward(q, k, v, beta, decay=None, state=None, offsets=None, out=None,
         y = _new(v)
     else:
         y = _check(out, "out", v.shape, v.dtype, d.dev)
-    final = torch.empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32, device=v.device)
+    final = v.new_empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32)
     lib = _lib.load()
     errors = states = None
     if keep:
-        errors = torch.empty(v.shape, dtype=torch.float32, device=v.device)
-        states = torch.empty((lib.cssm_delta_rule_segments(d.B, d.T, d.nseq, int(packed)), d.Hv, d.dk, d.dv),
-                             dtype=torch.float32, device=v.device)
+        errors = v.new_empty(v.shape, dtype=torch.float32)
+        states = v.new_empty((lib.cssm_delta_rule_segments(d.B, d.T, d.nseq, int(packed)), d.Hv, d.dk, d.dv), dtype=torch.float32)
     if d.n:
         need = lib.cssm_delta_rule_workspace_size(d.B, d.T, d.Hv, d.dk, d.dv, d.nseq, int(packed))
-        work = torch.empty(need, dtype=torch.uint8, device=v.device)
-        _call(d.dev, "cssm_delta_rule", _ref(d.q), _ref(d.k), _ref(d.v), d.dtype, _ref(d.beta), _ref(d.decay), d.B, d.T,
-              d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), _ptr(state), _ptr(offsets), d.nseq,
-              y.data_ptr(), int(packed and out is None), final.data_ptr(), _ptr(errors), _ptr(states), work.data_ptr(), need)
+        work = v.new_empty(need, dtype=torch.uint8)
+        _call(d.dev, "cssm_delta_rule", d.q, d.k, d.v, d.dtype, d.beta, d.decay, d.B, d.T, d.Hk, d.Hv, d.dk, d.dv,
+              d.dk ** -0.5 if scale is None else float(scale), _ptr(state), _ptr(offsets), d.nseq, y.data_ptr(), int(packed and out is None), final.data_ptr(), _ptr(errors), _ptr(states), work.data_ptr(), need)
     elif packed and out is None:
         y.zero_()
     return y, final, errors, states
@@ -484,15 +529,13 @@ def delta_backward(q, k, beta, decay, offsets, errors, states, dy, dfinal, scale
     lib = _lib.load()
     _check(errors, "errors", dy.shape, torch.float32, d.dev)
     _check(states, "states", (lib.cssm_delta_rule_segments(d.B, d.T, d.nseq, int(packed)), d.Hv, d.dk, d.dv), torch.float32, d.dev)
-
     dq, dk, dv, db, dg = _new(q), _new(k), _new(dy), _new(beta), None if decay is None else _new(decay)
-    dh0 = torch.empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32, device=dy.device)
+    dh0 = dy.new_empty((d.n, d.Hv, d.dk, d.dv), dtype=torch.float32)
     if d.n:
         need = lib.cssm_delta_rule_bwd_workspace_size(d.B, d.T, d.Hk, d.Hv, d.dk, d.dv, d.nseq, int(packed))
-        work = torch.empty(need, dtype=torch.uint8, device=dy.device)
-        _call(d.dev, "cssm_delta_rule_bwd", _ref(d.q), _ref(d.k), d.dtype, _ref(d.beta), _ref(d.decay), _ref(d.v), d.B, d.T,
-              d.Hk, d.Hv, d.dk, d.dv, d.dk ** -0.5 if scale is None else float(scale), _ptr(offsets), d.nseq,
-              errors.data_ptr(), states.data_ptr(), _ptr(dfinal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        work = dy.new_empty(need, dtype=torch.uint8)
+        _call(d.dev, "cssm_delta_rule_bwd", d.q, d.k, d.dtype, d.beta, d.decay, d.v, d.B, d.T, d.Hk, d.Hv, d.dk, d.dv,
+              d.dk ** -0.5 if scale is None else float(scale), _ptr(offsets), d.nseq, errors.data_ptr(), states.data_ptr(), _ptr(dfinal), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
               db.data_ptr(), _ptr(dg), dh0.data_ptr(), work.data_ptr(), need)
     else:
         for t in (dq, dk, dv, db) if dg is None else (dq, dk, dv, db, dg):
@@ -510,7 +553,8 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Te
     ``q``, ``k`` (B, T, Hk, dk) and ``v`` (B, T, Hv, dv), float32 or bfloat16 and alike, widths to 128, the heads side by
     side (slices of one projection's output will do); Hv / Hk value heads next to each other share a query and key head.
     ``beta``, ``decay`` (B, T, Hv) float32, decay <= 0 (None: 0, no decay; -inf clears the state).  The rule is stable for
-    keys of at most unit length and 0 <= beta <= 2; nothing checks that.  ``state`` (B, Hv, dk, dv) float32 before the first
+    keys of at most unit length and 0 <= beta <= 2; nothing checks that.  A row with beta = 0 and decay = 0 leaves the state:
+    that masks it, its values being finite.  ``state`` (B, Hv, dk, dv) float32 before the first
     row (None: zeros); ``scale`` dk^-0.5 unless given.  ``offsets`` and ``out`` as in :func:`token_scan`: packed rows
     (T, H, width), states (n, Hv, dk, dv).  Rows are taken 32 at a time, and a value that is not finite spoils its sequence
     from the 32 rows on in which it stands.  Not differentiable: see :func:`cssm_amd.training.delta_rule_train`.
@@ -518,52 +562,20 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Te
     return delta_forward(q, k, v, beta, decay, state, offsets, out, scale)[:2]
 
 
-def _plain_tokens(q, k, v, beta, decay, state):
-    """(GPU, B, Hk, Hv, dk, dv) of contiguous tokens that go together: the usual call, without the checks that name what is
-    wrong.  None for any other."""
-    try:
-        dev, dt, f32 = v.get_device(), v.dtype, torch.float32
-        B, Hv, dv = v.shape
-        _, Hk, dk = sk = k.shape
-        gate = beta.shape
-        if (dev >= 0 and dt in _DTYPES and k.dtype is dt and q.dtype is dt and beta.dtype is f32 and state.dtype is f32
-                and q.shape == sk and sk[0] == B and gate == (B, Hv) and state.shape == (B, Hv, dk, dv)
-                and 0 < dk <= 128 and 0 < dv <= 128 and Hk > 0 and Hv > 0 and Hv % Hk == 0
-                and q.get_device() == dev and k.get_device() == dev and beta.get_device() == dev and state.get_device() == dev
-                and v.is_contiguous() and q.is_contiguous() and k.is_contiguous() and beta.is_contiguous()
-                and state.is_contiguous()
-                and (decay is None or (decay.dtype is f32 and decay.shape == gate and decay.get_device() == dev
-                                       and decay.is_contiguous()))):
-            return dev, B, Hk, Hv, dk, dv
-    except (AttributeError, ValueError):
-        pass
-    return None
-
-
 def delta_rule_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor, state: torch.Tensor,
                     decay: Optional[torch.Tensor] = None, out_state: Optional[torch.Tensor] = None,
                     scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """One token for each sequence: (y, state) from ``q``, ``k`` (B, Hk, dk), ``v`` (B, Hv, dv), ``beta``, ``decay`` (B, Hv)
     and ``state`` (B, Hv, dk, dv) float32, which ``out_state=state`` updates in place."""
-    sizes = _plain_tokens(q, k, v, beta, decay, state)
-    if sizes is not None:
-        dev, B, Hk, Hv, dk, dv = sizes
-        rows = _Rows5(q.data_ptr(), Hk * dk, 0, k.data_ptr(), Hk * dk, 0, v.data_ptr(), Hv * dv, 0, beta.data_ptr(), Hv, 0,
-                      0 if decay is None else decay.data_ptr(), Hv, 0)
-        at = ctypes.addressof(rows)
-        refs = at, at + _ROWS, at + 2 * _ROWS, at + 3 * _ROWS, None if decay is None else at + 4 * _ROWS
-    else:
-        d = _delta(q, k, v, beta, decay, state, None, step=True, need_state=True)
-        dev, B, Hk, Hv, dk, dv = d.dev, d.B, d.Hk, d.Hv, d.dk, d.dv
-        refs = _ref(d.q), _ref(d.k), _ref(d.v), _ref(d.beta), _ref(d.decay)
+    d = _delta(q, k, v, beta, decay, state, None, step=True)
     if out_state is None:
         out_state = torch.empty_like(state)
     elif out_state is not state:
-        _check(out_state, "out_state", state.shape, torch.float32, dev)
+        _check(out_state, "out_state", state.shape, torch.float32, d.dev)
     y = _new(v)
-    if B:
-        _call(dev, "cssm_delta_rule_step", refs[0], refs[1], refs[2], _DTYPES[v.dtype], refs[3], refs[4], B, Hk, Hv, dk, dv,
-              dk ** -0.5 if scale is None else float(scale), state.data_ptr(), y.data_ptr(), out_state.data_ptr())
+    if d.B:
+        _call(d.dev, "cssm_delta_rule_step", d.q, d.k, d.v, d.dtype, d.beta, d.decay, d.B, d.Hk, d.Hv, d.dk, d.dv,
+              d.dk ** -0.5 if scale is None else float(scale), state.data_ptr(), y.data_ptr(), out_state.data_ptr())
     return y, out_state
 
 
@@ -679,19 +691,25 @@ def rotate_heads(q: torch.Tensor, k: Optional[torch.Tensor], positions: Optional
 def rotate_heads_backward(q, k, dq_out, dk_out, positions, table, q_weight, k_weight, norm, eps, pairs):
     """Adjoint of :func:`rotate_heads` (cssm_rotate_heads_bwd): (dq, dk, dq_weight, dk_weight), None where there is none."""
     r = _rotary(q, k, positions, table, q_weight, k_weight, norm, eps, pairs)
-    like = "batch" if q.dim() == 4 else "packed"
-    gq, _ = _heads(dq_out, "dq_out", q.shape[:-2], q.shape[-1], q.dtype, r.dev, like)
-    gk = None if k is None else _heads(dk_out, "dk_out", q.shape[:-2], q.shape[-1], q.dtype, r.dev, like)[0]
-    if dq_out.shape != q.shape or (k is not None and dk_out.shape != k.shape):
-        raise ValueError("the outputs' gradients have the outputs' shapes")
+    if _fine(dq_out, q.shape, q.dtype, r.dev) and (k is None or _fine(dk_out, k.shape, q.dtype, r.dev)):
+        _, _, T, Hq, Hk, D = r.head     # contiguous, as usual
+        rows = _Rows2(dq_out.data_ptr(), T * Hq * D, Hq * D, 0 if k is None else dk_out.data_ptr(), T * Hk * D, Hk * D)
+        gq, gk = ctypes.addressof(rows), None if k is None else ctypes.addressof(rows) + _ROWS
+    else:
+        like = "batch" if q.dim() == 4 else "packed"
+        tq, _ = _heads(dq_out, "dq_out", q.shape[:-2], q.shape[-1], q.dtype, r.dev, like)
+        tk = None if k is None else _heads(dk_out, "dk_out", q.shape[:-2], q.shape[-1], q.dtype, r.dev, like)[0]
+        if dq_out.shape != q.shape or (k is not None and dk_out.shape != k.shape):
+            raise ValueError("the outputs' gradients have the outputs' shapes")
+        gq, gk = _ref(tq), _ref(tk)
     dq, dk = _new(q), None if k is None else _new(k)
     dwq, dwk = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
     if q.numel():
         work, need = None, 0
         if dwq is not None or dwk is not None:
             need = _lib.load().cssm_rotate_heads_bwd_workspace_size(q.shape[-1])
-            work = torch.empty(need // 4, dtype=torch.float32, device=q.device)
-        _call(r.dev, "cssm_rotate_heads_bwd", r.q, r.k, _ref(gq), _ref(gk), *r.head, *r.rest, dq.data_ptr(),
+            work = q.new_empty(need // 4, dtype=torch.float32)
+        _call(r.dev, "cssm_rotate_heads_bwd", r.q, r.k, gq, gk, *r.head, *r.rest, dq.data_ptr(),
               _ptr(dk), _ptr(dwq), _ptr(dwk), _ptr(work), need)
     else:
         for t in (dwq, dwk):

@@ -106,7 +106,9 @@ def test_sizes(lib):
     assert lib.cssm_delta_rule_segments(0, 5, 0, 0) == lib.cssm_delta_rule_segments(1, -1, 0, 0) == 0
     for a in ((0, 5, 1, 1, 1, 0, 0), (1, -1, 1, 1, 1, 0, 0), (1, 5, 0, 1, 1, 0, 0), (1, 5, 1, 0, 1, 0, 0)):
         assert lib.cssm_delta_rule_workspace_size(*a) == 0
+    assert lib.cssm_delta_rule_segments(1 << 30, 1 << 30, 0, 0) == (1 << 31) - 1
     # sizes past 32 bits
+    assert lib.cssm_delta_rule_workspace_size(1 << 20, 1 << 20, 1, 8, 8, 0, 0) > 1 << 45
     assert lib.cssm_delta_rule_workspace_size(64, 1 << 16, 32, 128, 128, 0, 0) > 1 << 32
     assert lib.cssm_delta_rule_bwd_workspace_size(64, 1 << 16, 32, 32, 128, 128, 0, 0) > 1 << 34
 
