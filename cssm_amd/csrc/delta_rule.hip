@@ -217,8 +217,9 @@ struct Part {
 // part x of the launch; false for a number that no part takes
 __device__ __forceinline__ bool part_of(const DeltaRule& a, int x, Part& p) {
   if (!a.fold) {
-    const Span sp = span_of(a, x);
-    p = {x, sp.row, sp.rows, sp.slot, sp.segment, true, true};
+    const int seq = __builtin_amdgcn_readfirstlane(longest_first(a, x));
+    const Span sp = span_of(a, seq);
+    p = {seq, sp.row, sp.rows, sp.slot, sp.segment, true, true};
     return true;
   }
   int seq, i;

@@ -39,7 +39,8 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
   constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, LP = kUnits<T, true> / 256;
   __shared__ Lds lds[Lds::kBufs];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
-  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int x = blockIdx.x / a.Hv, h = blockIdx.x - x * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int seq = __builtin_amdgcn_readfirstlane(longest_first(a, x));
   const int b = a.offsets ? 0 : seq;
   const Span sp = span_of(a, seq);
   const int chunks = chunks_of(sp.rows);
@@ -212,7 +213,8 @@ __global__ __launch_bounds__(512, 1) void delta_back_pairs(DeltaRule a) {
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64) % 4, g = lane / 16;
   const bool carries = __builtin_amdgcn_readfirstlane(threadIdx.x / 256) == 0;
   const int tid = threadIdx.x % 256;
-  const int seq = blockIdx.x / a.Hv, h = blockIdx.x - seq * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int x = blockIdx.x / a.Hv, h = blockIdx.x - x * a.Hv, hk = h / (a.Hv / a.Hk);
+  const int seq = __builtin_amdgcn_readfirstlane(longest_first(a, x));
   const int b = a.offsets ? 0 : seq;
   const Span sp = span_of(a, seq);
   const int chunks = chunks_of(sp.rows);

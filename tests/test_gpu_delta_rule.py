@@ -98,6 +98,18 @@ def test_packed(Q, offsets, tail, dtype):
     assert y2 is out and torch.equal(out[:offsets[-1]], y[:offsets[-1]]) and bool((out[offsets[-1]:] == 7).all())
 
 
+@pytest.mark.parametrize("n", [63, 64, 65, 200])
+def test_many_packed(Q, n):
+    """sequences taken by their length up to 64 of them, in their order from there"""
+    gen = torch.Generator().manual_seed(n)
+    cuts = torch.randint(0, 700, (n - 1,), generator=gen).sort().values.tolist()
+    off = torch.tensor([0] + cuts + [700], dtype=torch.int32, device="cuda")
+    q, k, v, beta, decay, state = R.inputs(1, 705, 1, 2, 16, 8, F32, n, n=n)
+    want = R.whole(q, k, v, beta, decay, state, off)
+    y, final = Q.delta_rule(q, k, v, beta, decay, state, offsets=off)
+    assert R.off(y, want["y"]) <= 1 and R.off(final, want["final"]) <= 1
+
+
 def test_packed_as_alone(Q):
     """each packed sequence as it is by itself, bit for bit"""
     q, k, v, beta, decay, state = R.inputs(1, 300, 1, 2, 64, 64, BF16, 8, n=4)
