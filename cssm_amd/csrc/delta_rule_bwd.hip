@@ -437,31 +437,25 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
   const int left = sp.rows - seg * kSegment, rows_all = left < kSegment ? left : kSegment, chunks = chunks_of(rows_all);
   const size_t slot0 = size_t(sp.slot) + size_t(seg) * kChunks;
   const int col = wave * 16 + lane % 16;   // of the keys
-  const bool mine = col < a.dk;
   const int v_row = a.Hv * a.dv;
   for (int i = tid; i < chunks * 96; i += 4 * P) s_gains[i / 96][i % 96] = a.gains[((slot0 + i / 96) * a.Hv + h) * 96 + i % 96];
 
   // S^T, or its gradient's: rows of dv, a lane one column of dk
   f32x4_t S[MT];
-  const auto load_state = [&](const float* from) {
-    const float* p = from + (size_t(sp.segment + seg) * a.Hv + h) * a.dk * a.dv + size_t(col) * a.dv;
-    f32x4_t r[MT];
+  const auto load_state = [&](const float* from, f32x4_t (&to)[MT]) {
+    const Rows p(from + ((size_t(sp.segment + seg) * a.Hv + h) * a.dk + wave * 16) * a.dv, a.dv, a.dk - wave * 16, a.dv);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
+      if constexpr (WIDE) {
+        to[m] = __builtin_bit_cast(f32x4_t, load16(p, p.at<float, true>(lane % 16, 16 * m + 4 * g, a.dv)));
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[m][i] = mine && 16 * m + 4 * g + i < a.dv ? p[16 * m + 4 * g + i] : 0.0f;
-    float with = 0.0f;   // <S, r>
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) with = fmaf(S[m][i], r[m][i], with), S[m][i] = r[m][i];
-    return with;
+        for (int i = 0; i < 4; ++i) to[m][i] = element<float>(load_element<float>(p, p.at<float, false>(lane % 16, 16 * m + 4 * g + i, a.dv)));
+      }
   };
-#pragma unroll
-  for (int m = 0; m < MT; ++m) S[m] = f32x4_t{};
-  load_state(a.states);
+  load_state(a.states, S);
 
-  // the first half of the threads takes E and X, the second dy, k and q
+  // each half of the threads takes about half of the splitting
   const bool first = tid < 2 * P;
   const int id = first ? tid : tid - 2 * P;
   const int p_tok = id % 8 + id / (8 * 2 * KS) * 8, p_at = id / 8 % (2 * KS), p_col = p_at / 2 * 32 + p_at % 2 * 8;
@@ -480,12 +474,15 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
       if (first) {
         const Rows x(a.duals + head_of(c), v_row, rows, a.dv), e(a.errors + head_of(c), v_row, rows, a.dv);
         px.load(x, p_tok, p_col, a.dv), pe.load(e, p_tok, p_col, a.dv);
-        ce.load(e, 4 * c_g, c_col, a.dv);
+        const Rows q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
+        cq.load(q, 4 * c_g, c_col, a.dk);
+        asm volatile("");   // the halves' ends stay apart: joined, their values lie in scratch
       } else {
-        const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
-        const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
+        const Rows e(a.errors + head_of(c), v_row, rows, a.dv), y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
+        const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk);
+        ce.load(e, 4 * c_g, c_col, a.dv);
         py.load(y, p_tok, p_col, a.dv);
-        ck.load(k, 4 * c_g, c_col, a.dk), cq.load(q, 4 * c_g, c_col, a.dk);
+        ck.load(k, 4 * c_g, c_col, a.dk);
       }
     };
     fetch(0);
@@ -497,10 +494,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         const float beta = gains[64 + p_tok];
         px.template store_by<3>(beta, s_x + p_unit, PLANE);
         pe.template store_by<3>(beta, s_u + p_unit, PLANE);
-        float by[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) by[j] = gains[64 + unit_row(4 * c_g, j)] * gains[32 + unit_row(4 * c_g, j)];
-        ce.template store_by<3>(by, s_ut + c_unit, PLANE);
+        cq.store(s_qt + c_unit, PLANE);
         float dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) dot = fmaf(px.get(i), pe.get(i), dot);
@@ -508,8 +502,12 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         for (int o = 8; o < 16 * KS; o *= 2) dot += __shfl_xor(dot, o);
         if (p_at == 0 && p_tok < rows) a.dbeta[(size_t(b) * a.T + row0 + c * kChunk + p_tok) * a.Hv + h] = dot;
       } else {
+        float by[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) by[j] = gains[64 + unit_row(4 * c_g, j)] * gains[32 + unit_row(4 * c_g, j)];
+        ce.template store_by<3>(by, s_ut + c_unit, PLANE);
         py.store(s_y + p_unit, PLANE);
-        ck.store(s_kt + c_unit, PLANE), cq.store(s_qt + c_unit, PLANE);
+        ck.store(s_kt + c_unit, PLANE);
       }
       __syncthreads();
       if (c + 1 < chunks) fetch(c + 1);
@@ -634,10 +632,6 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
     }
   }
 
-  float with = load_state(a.dstates);
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) with += __shfl_xor(with, o);
-  if (lane == 0) s_sum[wave] = with;
   {
     Piece<float, WIDE> pe;
     Columns<float, WIDE> cx;
@@ -651,33 +645,43 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) part[i] = element<float>(load_element<float>(dkh, dkh.at<float, true>(unit_row(4 * g, i), col, a.dk)));
       if (first) {
-        const Rows x(a.duals + head_of(c), v_row, rows, a.dv), e(a.errors + head_of(c), v_row, rows, a.dv);
-        pe.load(e, p_tok, p_col, a.dv);
-        cx.load(x, 4 * c_g, c_col, a.dv);
-      } else {
-        const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
+        const Rows e(a.errors + head_of(c), v_row, rows, a.dv);
         const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
-        cy.load(y, 4 * c_g, c_col, a.dv);
+        pe.load(e, p_tok, p_col, a.dv);
         ck.load(k, 4 * c_g, c_col, a.dk), cq.load(q, 4 * c_g, c_col, a.dk);
+        asm volatile("");
+      } else {
+        const Rows x(a.duals + head_of(c), v_row, rows, a.dv), y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
+        cx.load(x, 4 * c_g, c_col, a.dv);
+        cy.load(y, 4 * c_g, c_col, a.dv);
       }
     };
     fetch(chunks - 1);
+    {
+      f32x4_t end[MT];
+      load_state(a.dstates, end);
+      float with = 0.0f;   // <S, dS>
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) with = fmaf(S[m][i], end[m][i], with), S[m][i] = end[m][i];
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) with += __shfl_xor(with, o);
+      if (lane == 0) s_sum[wave] = with;
+    }
     for (int c = chunks - 1; c >= 0; --c) {
       const int rows = rows_all - c * kChunk;
       __syncthreads();
       const float* gains = s_gains[c];
       if (first) {
         pe.template store_by<3>(gains[64 + p_tok], s_u + p_unit, PLANE);
+        ck.store(s_kt + c_unit, PLANE), cq.store(s_qt + c_unit, PLANE);
+      } else {
         float by[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) by[j] = -gains[64 + unit_row(4 * c_g, j)] * gains[unit_row(4 * c_g, j)];
         cx.template store_by<3>(by, s_ut + c_unit, PLANE);
-      } else {
-        float by[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) by[j] = a.scale * gains[unit_row(4 * c_g, j)];
-        cy.template store_by<3>(by, s_x + c_unit, PLANE);
-        ck.store(s_kt + c_unit, PLANE), cq.store(s_qt + c_unit, PLANE);
+        cy.store(s_y + c_unit, PLANE);
       }
       float before[8];
 #pragma unroll
@@ -701,13 +705,19 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
       Unit kb[N], qb[N];
       take(s_kt + wave * 64 + lane, PLANE, kb);
       take(s_qt + wave * 64 + lane, PLANE, qb);
+      float gm[8];
+      take_rows(gains, g, gm);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) gm[i] *= a.scale * value_of(qb, i);
+      Unit qg[3];   // scale gamma q: a wave's 16 columns of q to split, not all columns of dy
+      split<3>(gm, qg);
       const float all = gains[31];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        Unit w[3];
+        Unit w[3], y[N];
         S[m] *= all;
-        take(s_x + m * 64 + lane, PLANE, w);
-        S[m] = product(w, qb, S[m]);
+        take(s_y + m * 64 + lane, PLANE, y);
+        S[m] = product(y, qg, S[m]);
         take(s_ut + m * 64 + lane, PLANE, w);
         S[m] = product(w, kb, S[m]);
       }
