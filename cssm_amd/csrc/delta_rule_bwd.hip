@@ -7,11 +7,12 @@
 // A decay enters through products over the rows between a reader and a writer, so its gradient is what the rows from it on
 // read, less what they write, down to the end, where the rest of the sequence enters as one number:
 //   ddecay_l = <S, dS>_end + sum over i >= l of (q_i.dq_i + k_i.read_i - k_i.write_i)
-// delta_walk_back carries dS from chunk to chunk, as the forward does S, and keeps it behind every 128th row; then
-// delta_grads takes each 128 rows by themselves, forwards with S and backwards with dS, a wave 16 of the keys' columns, so
-// that the sums over dv lie within a wave.  Training 4 x 4096 x 16 heads of 128: delta_walk_back 410 us (3.2 a chunk, a chain
-// of products as the forward's), delta_grads 670 us (2048 workgroups of 8 waves, two a SIMD: 450 products a chunk and pair of
-// waves and the splitting of their operands; 32 columns a wave halve what is read from LDS, but leave one wave a SIMD: 880).
+// delta_back_pairs (bfloat16; float32: delta_walk_back) carries dS from chunk to chunk, as the forward does S, and keeps it
+// behind every 128th row; then delta_grads takes each 128 rows by themselves, forwards with S and backwards with dS, a wave 16
+// of the keys' columns, so that the sums over dv lie within a wave.  Training 4 x 4096 x 16 heads of 128: delta_back_pairs
+// 342 us (2.7 a chunk, a chain of products as the forward's; one kind of wave for all of it 410), delta_grads 575 us (2048
+// workgroups of 8 waves, two a SIMD, of which the loads of states were 120 with 4 bytes each and are 80 with 16; 32 columns a
+// wave halve what is read from LDS, but leave one wave a SIMD: 880).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -408,14 +409,16 @@ __device__ __forceinline__ float sum16(float x) {
 }
 
 // P: dk and dv up to it.  One workgroup for 128 rows of one value head, P / 16 waves.  Y, Z and their transposes take the place
-// of U's rows in LDS once those are read.
+// of U's rows in LDS once those are read, and the columns of d U that of X's rows.
+// 64 wide two workgroups share a CU, in 256 registers a thread (training 4 x 4096 x 16 heads of 64: bfloat16 383 -> 233 us,
+// float32 446 -> 379); 128 wide that leaves 128 registers, which spill (1280 us in place of 575).
 template <int P, typename T, bool WIDE>
-__global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
+__global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(DeltaRule a) {
   constexpr int N = PartsOf<T>::n, W = P / 16, KS = P / 32, MT = P / 16, PLANE = P * 4, TASKS = (6 + W - 1) / W;
   constexpr int UROOM = 3 * PLANE > 12 * 128 ? 3 * PLANE : 12 * 128;
-  __shared__ uint4 s_y[N * PLANE], s_x[3 * PLANE], s_u[UROOM], s_ut[3 * PLANE], s_kt[N * PLANE], s_qt[N * PLANE];
+  __shared__ uint4 s_y[N * PLANE], s_x[3 * PLANE], s_u[UROOM], s_kt[N * PLANE], s_qt[N * PLANE];
   __shared__ __attribute__((aligned(16))) float s_gains[kChunks][96];
-  __shared__ float s_read[W][kSegment], s_write[W][kSegment], s_sum[W];
+  __shared__ float s_net[W][kSegment], s_sum[W];   // what a row reads less what it writes
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, h = blockIdx.y, hk = h / (a.Hv / a.Hk);
   const bool shared = a.Hv != a.Hk;
   int seq, seg, b = 0;
@@ -502,15 +505,10 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         for (int o = 8; o < 16 * KS; o *= 2) dot += __shfl_xor(dot, o);
         if (p_at == 0 && p_tok < rows) a.dbeta[(size_t(b) * a.T + row0 + c * kChunk + p_tok) * a.Hv + h] = dot;
       } else {
-        float by[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) by[j] = gains[64 + unit_row(4 * c_g, j)] * gains[32 + unit_row(4 * c_g, j)];
-        ce.template store_by<3>(by, s_ut + c_unit, PLANE);
         py.store(s_y + p_unit, PLANE);
         ck.store(s_kt + c_unit, PLANE);
       }
       __syncthreads();
-      if (c + 1 < chunks) fetch(c + 1);
 
       // Y and Z, a 16 x 16 tile a wave: (0, 0), (1, 0) and (1, 1) of both
       f32x4_t tile[TASKS];
@@ -557,7 +555,13 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
           xs[t] = product(w3, u, xs[t]);
         }
       }
-      __syncthreads();   // U's rows are read: Y, Z, Y^T and Z^T take their place, 3 parts of 128 units each
+      __syncthreads();   // U's rows are read: Y, Z, Y^T and Z^T take their place, 3 parts of 128 units each; X's: d U's columns
+      if (!first) {
+        float by[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) by[j] = gains[64 + unit_row(4 * c_g, j)] * gains[32 + unit_row(4 * c_g, j)];
+        ce.template store_by<3>(by, s_x + c_unit, PLANE);
+      }
 #pragma unroll
       for (int n = 0; n < TASKS; ++n) {
         const int task = wave + n * W, z = task / 3, ti = task % 3 > 0, tj = task % 3 == 2;
@@ -585,6 +589,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         }
       }
       __syncthreads();
+      if (c + 1 < chunks) fetch(c + 1);
       Unit kb[N], qb[N];
       take(s_kt + wave * 64 + lane, PLANE, kb);
       take(s_qt + wave * 64 + lane, PLANE, qb);
@@ -611,7 +616,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         Unit w[3];
-        take(s_ut + m * 64 + lane, PLANE, w);
+        take(s_x + m * 64 + lane, PLANE, w);
         S[m] = product(w, kb, S[m] * all);
       }
       const size_t at_row = size_t(b) * a.T + row0 + c * kChunk;
@@ -625,9 +630,8 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         if (shared) store_element<float>(dqh, dqh.at<float, true>(r, col, a.dk), dq[i]);
         else store_element<T>(dqo, dqo.at<T, true>(r, col, a.dk), dq[i]);
         const float kv = value_of(kb, i);
-        float x = fmaf(value_of(qb, i), dq[i], kv * rd[i]), y = kv * wr[i];
-        x = sum16(x), y = sum16(y);
-        if (lane % 16 == 0) s_read[wave][c * kChunk + r] = x, s_write[wave][c * kChunk + r] = y;
+        const float net = sum16(fmaf(value_of(qb, i), dq[i], kv * rd[i]) - kv * wr[i]);
+        if (lane % 16 == 0) s_net[wave][c * kChunk + r] = net;
       }
     }
   }
@@ -680,7 +684,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         float by[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) by[j] = -gains[64 + unit_row(4 * c_g, j)] * gains[unit_row(4 * c_g, j)];
-        cx.template store_by<3>(by, s_ut + c_unit, PLANE);
+        cx.template store_by<3>(by, s_x + c_unit, PLANE);
         cy.store(s_y + c_unit, PLANE);
       }
       float before[8];
@@ -718,7 +722,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         S[m] *= all;
         take(s_y + m * 64 + lane, PLANE, y);
         S[m] = product(y, qg, S[m]);
-        take(s_ut + m * 64 + lane, PLANE, w);
+        take(s_x + m * 64 + lane, PLANE, w);
         S[m] = product(w, kb, S[m]);
       }
       float dd[8];
@@ -732,9 +736,8 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
         const float w = dd[i] * us[i / 4][i % 4];
         if (shared) store_element<float>(dkh, dkh.at<float, true>(r, col, a.dk), before[i] + w);
         else store_element<T>(dko, dko.at<T, true>(r, col, a.dk), before[i] + w);
-        float y = value_of(kb, i) * w;
-        y = sum16(y);
-        if (lane % 16 == 0) s_write[wave][c * kChunk + r] += y;
+        const float net = sum16(value_of(kb, i) * w);
+        if (lane % 16 == 0) s_net[wave][c * kChunk + r] -= net;
       }
     }
   }
@@ -747,7 +750,7 @@ __global__ __launch_bounds__(4 * P, 1) void delta_grads(DeltaRule a) {
       v[i] = 0.0f;
       if (r < rows_all)
 #pragma unroll
-        for (int w = 0; w < W; ++w) v[i] += s_read[w][r] - s_write[w][r];
+        for (int w = 0; w < W; ++w) v[i] += s_net[w][r];
     }
     float all = v[0] + v[1], rest = 0.0f;
 #pragma unroll
