@@ -252,11 +252,7 @@ __device__ __forceinline__ void take_rows(const float* s, int g, float (&v)[8]) 
   }
 }
 
-// parts of P: those that y's type shows; its transpose has all, since the gates' gradients are float32
-template <typename T, bool TURNED>
-constexpr int kPParts = sizeof(T) == 2 && !TURNED ? 2 : 3;
-template <typename T, bool TURNED>
-constexpr int kUnits = (3 + kPParts<T, TURNED>) * 128;   // units of L and P of one chunk and head
+constexpr int kUnits = 6 * 128;   // units of L and P of one chunk and head, three parts each
 
 // ---- sequences and their chunks
 

@@ -8,8 +8,8 @@
 //   R = V - gamma K S,  E = R - L beta R,  Y = scale gamma Q S + P beta E,  S <- gamma_31 S + K^T (d beta E)
 // delta_prepare computes L and P of all chunks at once; delta_walk then carries S from chunk to chunk, a wave 16 of
 // the state's columns, which lie in its registers as the result of one product and the operand of the next.
-// The state is float32 and enters its products in three bfloat16 parts (csrc/delta_rule.h); y's own products take two
-// where y is bfloat16.
+// The state is float32 and enters its products in three bfloat16 parts (csrc/delta_rule.h), as do L, P, R and U: y is rounded
+// once, where it is stored.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,6 +24,12 @@ namespace {
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kPad = kChunk + 4;
+
+// two results above each other as the parts of the next product's second operand
+__device__ __forceinline__ void split_pair(f32x4_t above, f32x4_t below, Unit (&u)[3]) {
+  const float x[8] = {above[0], above[1], above[2], above[3], below[0], below[1], below[2], below[3]};
+  split<3>(x, u);
+}
 
 // the 8 values of a row from `at` on, in their parts
 template <typename T, bool WIDE>
@@ -182,7 +188,7 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 4 : 2) void delta_prepare(Delt
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
       if (o == 1 && !two) break;
-      uint4* u = a.units + (size_t(slot) * a.Hv + h0 + o) * kUnits<T, TURNED> + (what ? 3 * 128 : 0);
+      uint4* u = a.units + (size_t(slot) * a.Hv + h0 + o) * kUnits + (what ? 3 * 128 : 0);
 #pragma unroll
       for (int tile = 0; tile < 2; ++tile) {
         const int r = 16 * tile + lane % 16, c = lane / 16 * 4;
@@ -192,17 +198,10 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 4 : 2) void delta_prepare(Delt
           const int cc = unit_row(c, i);
           v[i] = TURNED ? s_m[o][cc * kPad + r] : s_m[o][r * kPad + cc];
         }
-        if (what) {
-          Unit w[kPParts<T, TURNED>];
-          split<kPParts<T, TURNED>>(v, w);
+        Unit w[3];
+        split<3>(v, w);
 #pragma unroll
-          for (int n = 0; n < kPParts<T, TURNED>; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
-        } else {
-          Unit w[3];
-          split<3>(v, w);
-#pragma unroll
-          for (int n = 0; n < 3; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
-        }
+        for (int n = 0; n < 3; ++n) u[(n * 2 + tile) * 64 + lane] = __builtin_bit_cast(uint4, w[n]);
       }
     }
   }
@@ -298,7 +297,7 @@ constexpr int kWalkColumns = 64;   // of a workgroup: 16 for each of its four wa
 template <int DKP, typename T>
 struct WalkLds {
   static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
-  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[(kUnits<T, false> + 255) / 256 * 256];
+  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[(kUnits + 255) / 256 * 256];
   float gains[256];   // gamma, d, beta; the rest takes what threads without a value write
 };
 
@@ -308,8 +307,8 @@ struct WalkLds {
 template <int DKP, typename T, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
   using Lds = WalkLds<DKP, T>;
-  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, PP = kPParts<T, false>;
-  constexpr int LP = (kUnits<T, false> + 255) / 256;
+  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16;
+  constexpr int LP = (kUnits + 255) / 256;
   __shared__ Lds lds[Lds::kBufs];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
   const int part = blockIdx.x / a.Hv, h = blockIdx.x - part * a.Hv, hk = h / (a.Hv / a.Hk);
@@ -342,7 +341,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
     const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
     const Rows vv(row_at<T>(a.v, b, t) + h * a.dv, a.v.row, MAP && column.unit ? 0 : rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
-    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T, false> + tid;   // the last ones past this chunk's: into the next, or the end's room
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits + tid;   // the last ones past this chunk's: into the next, or the end's room
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
     if (p_on) pk.load(k, p_tok, p_col, a.dk);
@@ -395,12 +394,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
         ks[t] = product(w, u, ks[t]);
         if constexpr (MAP) continue;
         take(in.q + (s * 2 + t) * 64 + lane, PLANE, w);
-        if constexpr (PP == 3) {
-          qs[t] = product(w, u, qs[t]);
-        } else {
-          const Unit u2[2] = {u[0], u[1]};
-          qs[t] = product(w, u2, qs[t]);
-        }
+        qs[t] = product(w, u, qs[t]);
       }
     }
     float R[8], E[8], x[8], gm[8], dd[8], bt[8];
@@ -436,11 +430,11 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
       for (int i = 0; i < 8; ++i) x[i] = bt[i] * E[i];
     }
     if constexpr (!MAP) {
-      Unit u[PP];
-      split<PP>(x, u);
+      Unit u[3];
+      split<3>(x, u);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        Unit w[PP];
+        Unit w[3];
         take(in.lp + 3 * 128 + t * 64 + lane, 128, w);
         qs[t] = product(w, u, qs[t]);
       }
@@ -483,16 +477,16 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
 template <int DKP>
 struct PairLds {
   static constexpr int kPlane = DKP * 4;
-  uint4 k[2][kPlane], kt[2][kPlane], l[2][3 * 128], q[2][kPlane], p[2][2 * 128];
-  uint4 s[2][4][DKP / 32 * 2 * 64], u[2][4][2 * 64];   // two parts of S and U, a wave's columns each
+  uint4 k[2][kPlane], kt[2][kPlane], l[2][3 * 128], q[2][kPlane], p[2][3 * 128];
+  f32x4_t qs[2][4][2 * 64], u[2][4][2 * 64];   // Q S and U, a wave's columns each
   float gains[4][96];
 };
 
-// The same for bfloat16 by two kinds of waves, a pair for 16 columns on each SIMD: the first carries the state, the second
-// brings the chunks' rows to LDS and makes y of the chunk before, from S and U that the first leaves in LDS.  A step then
-// takes the state's own chain of products, 2.3 us a chunk on a full chip and 1.8 with few workgroups, where one kind of
-// wave for all of it took 3.4 and 2.6 (8 x 2048 and 1 x 65536 rows).  What bounds it: the 560 instructions that the first wave
-// issues a step, 60 products and some 370 to split and combine, one behind the other.
+// The same for bfloat16 by two kinds of waves, a pair for 16 columns on each SIMD: the first carries the state and takes Q S from
+// its parts while it has them, the second brings the chunks' rows to LDS and makes y of the chunk before, from Q S and U that the
+// first leaves in LDS.  One kind of wave for all of it took 3.4 us a chunk on a full chip; Q S by the second wave, which
+// splits the state once more, 3.1 (8 x 2048 rows: 243 us a call, 200 so).  What bounds it: the instructions that the first wave
+// issues a step, 80 products and those that split and combine, one behind the other.
 template <int DKP, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
   using T = Bf16;
@@ -536,24 +530,22 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
           for (int i = 0; i < 4; ++i)
             if (16 * m + 4 * g + i < a.dk) st[size_t(16 * m + 4 * g + i) * a.dv] = S[m][i];
       }
-      f32x4_t ks[2] = {};
+      f32x4_t ks[2] = {}, qs[2] = {};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const float x[8] = {S[2 * s][0], S[2 * s][1], S[2 * s][2], S[2 * s][3],
-                            S[2 * s + 1][0], S[2 * s + 1][1], S[2 * s + 1][2], S[2 * s + 1][3]};
         Unit u[3];
-        split<3>(x, u);
-        if constexpr (!MAP) {
-          lds.s[o][wave][(2 * s) * 64 + lane] = __builtin_bit_cast(uint4, u[0]);
-          lds.s[o][wave][(2 * s + 1) * 64 + lane] = __builtin_bit_cast(uint4, u[1]);
-        }
+        split_pair(S[2 * s], S[2 * s + 1], u);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           Unit w[1];
           take(lds.k[o] + (s * 2 + t) * 64 + lane, PLANE, w);
           ks[t] = product(w, u, ks[t]);
+          if constexpr (MAP) continue;
+          take(lds.q[o] + (s * 2 + t) * 64 + lane, PLANE, w);
+          qs[t] = product(w, u, qs[t]);
         }
       }
+      if constexpr (!MAP) lds.qs[o][wave][lane] = qs[0], lds.qs[o][wave][64 + lane] = qs[1];
       float R[8], E[8], x[8], gm[8], dd[8], bt[8];
       take_rows(gains, g, gm), take_rows(gains + 32, g, dd), take_rows(gains + 64, g, bt);
 #pragma unroll
@@ -573,12 +565,7 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
       {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = bt[i] * E[i];
-        if constexpr (!MAP) {
-          Unit u[2];
-          split<2>(x, u);
-          lds.u[o][wave][lane] = __builtin_bit_cast(uint4, u[0]);
-          lds.u[o][wave][64 + lane] = __builtin_bit_cast(uint4, u[1]);
-        }
+        if constexpr (!MAP) lds.u[o][wave][lane] = f32x4_t{x[0], x[1], x[2], x[3]}, lds.u[o][wave][64 + lane] = f32x4_t{x[4], x[5], x[6], x[7]};
       }
       if constexpr (KEEP) {
         const Rows ee(a.errors + ((size_t(b) * a.T + sp.row + (long long)c * kChunk) * a.Hv + h) * a.dv, y_row, sp.rows - c * kChunk, a.dv);
@@ -617,76 +604,67 @@ __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
   const int c_unit = (c_col / 16 * 4 + c_g) * 16 + c_col % 16;
   Piece<T, WIDE> pk, pq;
   Columns<T, WIDE> ck;
-  u32x4_t l[2], p;
+  u32x4_t l[2], p[2];
   float gain;
   const auto units_of = [&](int c) {
-    return reinterpret_cast<const u32x4_t*>(a.units) + (size_t(sp.slot + c) * a.Hv + h) * kUnits<T, false>;
+    return reinterpret_cast<const u32x4_t*>(a.units) + (size_t(sp.slot + c) * a.Hv + h) * kUnits;
   };
-  const auto fetch_keys = [&](int c) {   // what the state takes
+  const auto fetch_rows = [&](int c) {   // what the state takes
     const Rows k(row_at<T>(a.k, b, sp.row + (long long)c * kChunk) + hk * a.dk, a.k.row, sp.rows - c * kChunk, a.dk);
     if (p_on) pk.load(k, p_tok, p_col, a.dk);
     if (c_on) ck.load(k, 4 * c_g, c_col, a.dk);
+    if (!MAP) {
+      const Rows q(row_at<T>(a.q, b, sp.row + (long long)c * kChunk) + hk * a.dk, a.q.row, sp.rows - c * kChunk, a.dk);
+      if (p_on) pq.load(q, p_tok, p_col, a.dk);
+    }
     l[0] = units_of(c)[tid], l[1] = units_of(c)[256 + tid % 128];
     gain = a.gains[(size_t(sp.slot + c) * a.Hv + h) * 96 + tid % 96];
   };
-  const auto stash_keys = [&](int c) {
+  const auto stash_rows = [&](int c) {
     if (p_on) pk.store(lds.k[c % 2] + p_unit, PLANE);
     if (c_on) ck.store(lds.kt[c % 2] + c_unit, PLANE);
+    if (p_on && !MAP) pq.store(lds.q[c % 2] + p_unit, PLANE);
     lds.l[c % 2][tid] = __builtin_bit_cast(uint4, l[0]);
     if (tid < 128) lds.l[c % 2][256 + tid] = __builtin_bit_cast(uint4, l[1]);
     if (tid < 96) lds.gains[c % 4][tid] = gain;
   };
-  const auto fetch_queries = [&](int c) {   // what y takes
-    const Rows q(row_at<T>(a.q, b, sp.row + (long long)c * kChunk) + hk * a.dk, a.q.row, sp.rows - c * kChunk, a.dk);
-    if (p_on) pq.load(q, p_tok, p_col, a.dk);
-    p = units_of(c)[3 * 128 + tid];
+  const auto fetch_pairs = [&](int c) {   // what y takes
+    p[0] = units_of(c)[3 * 128 + tid], p[1] = units_of(c)[3 * 128 + 256 + tid % 128];
   };
-  const auto stash_queries = [&](int c) {
-    if (p_on) pq.store(lds.q[c % 2] + p_unit, PLANE);
-    lds.p[c % 2][tid] = __builtin_bit_cast(uint4, p);
+  const auto stash_pairs = [&](int c) {
+    lds.p[c % 2][tid] = __builtin_bit_cast(uint4, p[0]);
+    if (tid < 128) lds.p[c % 2][256 + tid] = __builtin_bit_cast(uint4, p[1]);
   };
-  // step c: chunk c + 1's keys and chunk c's queries come in, chunk c - 1's y goes out
+  // step c: chunk c + 1's rows and chunk c's P come in, chunk c - 1's y goes out
   if (chunks) {
-    fetch_keys(0);
-    stash_keys(0);
-    if (chunks > 1) fetch_keys(1);
-    if (!MAP) fetch_queries(0);
+    fetch_rows(0);
+    stash_rows(0);
+    if (chunks > 1) fetch_rows(1);
+    if (!MAP) fetch_pairs(0);
   }
   for (int c = 0; c <= chunks; ++c) {
     __syncthreads();
-    if (c + 1 < chunks) stash_keys(c + 1);
-    if (!MAP && c < chunks) stash_queries(c);
-    if (c + 2 < chunks) fetch_keys(c + 2);
-    if (!MAP && c + 1 < chunks) fetch_queries(c + 1);
+    if (c + 1 < chunks) stash_rows(c + 1);
+    if (!MAP && c < chunks) stash_pairs(c);
+    if (c + 2 < chunks) fetch_rows(c + 2);
+    if (!MAP && c + 1 < chunks) fetch_pairs(c + 1);
     if (MAP || c == 0) continue;
     const int o = (c - 1) % 2;
     const float* gains = lds.gains[(c - 1) % 4];
-    f32x4_t qs[2] = {};
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      Unit u[2];
-      take(lds.s[o][wave] + 2 * s * 64 + lane, 64, u);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        Unit w[1];
-        take(lds.q[o] + (s * 2 + t) * 64 + lane, PLANE, w);
-        qs[t] = product(w, u, qs[t]);
-      }
-    }
+    f32x4_t qs[2] = {lds.qs[o][wave][lane], lds.qs[o][wave][64 + lane]};
     float gm[8];
     take_rows(gains, g, gm);
-    Unit u[2];
-    take(lds.u[o][wave] + lane, 64, u);
+    Unit u[3];
+    split_pair(lds.u[o][wave][lane], lds.u[o][wave][64 + lane], u);
     const Rows yy(static_cast<T*>(a.y) + ((size_t(b) * a.T + sp.row + (long long)(c - 1) * kChunk) * a.Hv + h) * a.dv, y_row,
                   sp.rows - (c - 1) * kChunk, a.dv);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      Unit w[2];
+      Unit w[3];
       take(lds.p[o] + t * 64 + lane, 128, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) qs[t][i] *= a.scale * gm[4 * t + i];
-      // all four products of the parts: with keys alike, the terms are several times y
-      qs[t] = product(w, u, mfma16(w[1], u[1], qs[t]));
+      qs[t] = product(w, u, qs[t]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) store_element<T>(yy, yy.at<T, true>(16 * t + 4 * g + i, col, a.dv), qs[t][i]);
     }
@@ -944,7 +922,7 @@ long long delta_rule_segments(int B, int T, int nseq, bool packed) {
 size_t delta_rule_workspace(int B, int T, int Hv, int dk, int dv, int nseq, bool packed) {
   const int fold = delta_rule_fold(B, T, Hv, dk, dv, nseq, packed), wide = dk <= 64 ? 64 : 128;
   const size_t parts = fold ? size_t(delta_rule_parts(fold, B, T, nseq, packed)) * Hv : 0;
-  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits<float, false> * sizeof(uint4) + 96 * sizeof(float)) +
+  return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits * sizeof(uint4) + 96 * sizeof(float)) +
          256 * sizeof(uint4) + parts * (size_t(wide) * wide + size_t(dk) * dv) * sizeof(float);
 }
 
@@ -952,7 +930,7 @@ hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_
   const bool packed = a.offsets != nullptr;
   const size_t heads = size_t(delta_rule_slots(a.B, a.T, a.nseq, packed)) * a.Hv, wide = a.dk <= 64 ? 64 : 128;
   a.units = static_cast<uint4*>(workspace);
-  a.gains = reinterpret_cast<float*>(a.units + heads * (dtype == 0 ? kUnits<float, false> : kUnits<Bf16, false>));
+  a.gains = reinterpret_cast<float*>(a.units + heads * kUnits);
   float* at = a.gains + heads * 96 + 256;   // 160 more behind the last are read
   a.fold = delta_rule_fold(a.B, a.T, a.Hv, a.dk, a.dv, a.nseq, packed);
   if (a.fold) {

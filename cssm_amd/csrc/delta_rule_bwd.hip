@@ -30,14 +30,14 @@ constexpr int kChunks = kSegment / kChunk;
 template <int DKP, typename T>
 struct BackLds {
   static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
-  uint4 k[kN * kPlane], kt[kN * kPlane], qt[kN * kPlane], lp[kUnits<T, true>];
+  uint4 k[kN * kPlane], kt[kN * kPlane], qt[kN * kPlane], lp[kUnits];
   float gains[256];
 };
 
 template <int DKP, typename T, bool WIDE>
 __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
   using Lds = BackLds<DKP, T>;
-  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, LP = kUnits<T, true> / 256;
+  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, LP = kUnits / 256;
   __shared__ Lds lds[Lds::kBufs];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
   const int x = blockIdx.x / a.Hv, h = blockIdx.x - x * a.Hv, hk = h / (a.Hv / a.Hk);
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
     const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
     const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
-    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T, true> + tid;
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits + tid;
 #pragma unroll
     for (int i = 0; i < 8; ++i) dy[i] = load_element<T>(y, y.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
     if (p_on) pk.load(k, p_tok, p_col, a.dk);
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(512, 1) void delta_back_pairs(DeltaRule a) {
     const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
     const Rows y(row_at<T>(a.dy, b, t) + h * a.dv, a.dy.row, rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
-    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits<T, true>;
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits;
 #pragma unroll
     for (int i = 0; i < 8; ++i) dy[i] = load_element<T>(y, y.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
     if (p_on) pk.load(k, p_tok, p_col, a.dk);
@@ -834,7 +834,7 @@ size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 size_t delta_rule_bwd_workspace(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, bool packed) {
   const size_t heads = size_t(delta_rule_slots(B, T, nseq, packed)) * Hv, rows = size_t(B) * T * Hv;
-  return heads * (kUnits<float, true> * sizeof(uint4) + (96 + kChunk * kChunk) * sizeof(float)) + 256 * sizeof(float) +
+  return heads * (kUnits * sizeof(uint4) + (96 + kChunk * kChunk) * sizeof(float)) + 256 * sizeof(float) +
          up16(rows * dv * sizeof(float)) + up16(size_t(delta_rule_segments(B, T, nseq, packed)) * Hv * dk * dv * sizeof(float)) +
          up16(rows * dk * sizeof(float)) * (Hv != Hk ? 2 : 1);
 }
@@ -848,7 +848,7 @@ hipError_t launch_delta_rule_bwd(DeltaRule a, int dtype, void* workspace, hipStr
     at += up16(bytes);
     return p;
   };
-  a.units = reinterpret_cast<uint4*>(room(heads * kUnits<float, true> * sizeof(uint4)));
+  a.units = reinterpret_cast<uint4*>(room(heads * kUnits * sizeof(uint4)));
   a.gains = reinterpret_cast<float*>(room((heads * 96 + 256) * sizeof(float)));   // 160 more behind the last are read
   a.decays = reinterpret_cast<float*>(room(heads * kChunk * kChunk * sizeof(float)));
   a.duals = reinterpret_cast<float*>(room(rows * a.dv * sizeof(float)));
