@@ -252,6 +252,7 @@ __device__ __forceinline__ void take_rows(const float* s, int g, float (&v)[8]) 
   }
 }
 
+constexpr int kDecays = 3 * kChunk * kChunk;   // D, and with decays P and A, of one chunk and head for the adjoint
 constexpr int kUnits = 6 * 128;   // units of L and P of one chunk and head, three parts each
 
 // ---- sequences and their chunks

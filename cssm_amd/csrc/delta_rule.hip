@@ -150,9 +150,13 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 4 : 2) void delta_prepare(Delt
   for (int i = 0; i < kChunk; ++i) {
     const bool at = i == j;
     d = at ? 1.0f : d * s_alpha[half][i];   // 0 above the diagonal
-    if (TURNED && on) a.decays[(size_t(slot) * a.Hv + h) * (kChunk * kChunk) + i * kChunk + j] = d;
     A[i] = at ? 0.0f : d * A[i];
     P[i] *= d * a.scale;
+    if (TURNED && on) {
+      float* to = a.decays + (size_t(slot) * a.Hv + h) * kDecays + i * kChunk + j;
+      to[0] = d;
+      if (a.decay.p) to[kChunk * kChunk] = P[i], to[2 * kChunk * kChunk] = A[i];
+    }
     s_m[half][i * kPad + j] = A[i] * beta;
   }
   float gamma = alpha;   // of this row and those before it in the chunk

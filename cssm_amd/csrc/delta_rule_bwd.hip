@@ -4,15 +4,20 @@
 //   dS <- gamma_31 dS' + scale Q^T gamma dY - K^T gamma beta X
 //   Y_ij = scale D_ij dY_i.U_j (i >= j),  Z_ij = D_ij beta_i X_i.U_j (i > j)
 //   dQ = Y K + scale gamma dY S^T,  read = -Z K - gamma beta X S^T,  write = Y^T Q - Z^T K + d U dS'^T,  dK = read + write
-// A decay enters through products over the rows between a reader and a writer, so its gradient is what the rows from it on
-// read, less what they write, down to the end, where the rest of the sequence enters as one number:
-//   ddecay_l = <S, dS>_end + sum over i >= l of (q_i.dq_i + k_i.read_i - k_i.write_i)
+// A decay is a factor of whatever crosses it, from a writer before it or the chunk's first state to a reader from it on or the
+// chunk's last state, and its gradient is the sum of just that:
+//   ddecay_l = sum over i >= l > j of W_ij + sum over i >= l of r_i + sum over j < l of c_j + gamma_31 <S, dS'>
+//   W_ij = P_ij dY_i.U_j - A_ij beta_i X_i.U_j,  r_i = q_i.(scale gamma_i S dY_i) - k_i.(gamma_i beta_i S X_i),  c_j = d_j k_j.(dS' U_j)
+// Every term has the factor a_l: nothing cancels that is larger than it, and a_l = 0 gives 0.  What the rows from l on read
+// less what they write, the shorter sum, is the same by cancellation: at a = exp(-8) nothing of it was right.
 // delta_back_pairs (bfloat16; float32: delta_walk_back) carries dS from chunk to chunk, as the forward does S, and keeps it
 // behind every 128th row; then delta_grads takes each 128 rows by themselves, forwards with S and backwards with dS, a wave 16
-// of the keys' columns, so that the sums over dv lie within a wave.  Training 4 x 4096 x 16 heads of 128: delta_back_pairs
-// 342 us (2.7 a chunk, a chain of products as the forward's; one kind of wave for all of it 410), delta_grads 575 us (2048
-// workgroups of 8 waves, two a SIMD, of which the loads of states were 120 with 4 bytes each and are 80 with 16; 32 columns a
-// wave halve what is read from LDS, but leave one wave a SIMD: 880).
+// of the keys' columns, so that the sums over dv lie within a wave.  The states between a segment's chunks go to the workspace
+// on the way forwards and are read again by the same threads on the way back, where dS' is at hand, for <S, dS'>.
+// Training 4 x 4096 x 16 heads of 128: delta_back_pairs 350 us (2.7 a chunk, a chain of products as the forward's; one kind of
+// wave for all of it 410), delta_grads 700 us (2048 workgroups of 8 waves, two a SIMD), of which ddecay is some 130: the states
+// between the chunks 75 (one of the two in LDS changed nothing, nor did loading them a barrier earlier), the sums of W 37, r and c
+// 22.  32 columns a wave halve what is read from LDS, but leave one wave a SIMD (880 in place of 575, both without ddecay's).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -412,13 +417,36 @@ __device__ __forceinline__ float sum16(float x) {
 // of U's rows in LDS once those are read, and the columns of d U that of X's rows.
 // 64 wide two workgroups share a CU, in 256 registers a thread (training 4 x 4096 x 16 heads of 64: bfloat16 383 -> 233 us,
 // float32 446 -> 379); 128 wide that leaves 128 registers, which spill (1280 us in place of 575).
+// the value `BY` lanes before or behind within 16, 0 beyond them
+template <int BY>
+__device__ __forceinline__ float lane_before(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x110 + BY, 0xf, 0xf, true));
+}
+template <int BY>
+__device__ __forceinline__ float lane_behind(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x100 + BY, 0xf, 0xf, true));
+}
+// the sum of the lanes before, or behind, within 16
+__device__ __forceinline__ float sum_before(float x) {
+  x = lane_before<1>(x);
+  x += lane_before<1>(x), x += lane_before<2>(x), x += lane_before<4>(x);
+  return x + lane_before<8>(x);
+}
+__device__ __forceinline__ float sum_behind(float x) {
+  x = lane_behind<1>(x);
+  x += lane_behind<1>(x), x += lane_behind<2>(x), x += lane_behind<4>(x);
+  return x + lane_behind<8>(x);
+}
+
 template <int P, typename T, bool WIDE>
 __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(DeltaRule a) {
   constexpr int N = PartsOf<T>::n, W = P / 16, KS = P / 32, MT = P / 16, PLANE = P * 4, TASKS = (6 + W - 1) / W;
   constexpr int UROOM = 3 * PLANE > 12 * 128 ? 3 * PLANE : 12 * 128;
   __shared__ uint4 s_y[N * PLANE], s_x[3 * PLANE], s_u[UROOM], s_kt[N * PLANE], s_qt[N * PLANE];
   __shared__ __attribute__((aligned(16))) float s_gains[kChunks][96];
-  __shared__ float s_net[W][kSegment], s_sum[W];   // what a row reads less what it writes
+  constexpr int PAIRS = W < 6 ? W : 6;   // waves that have tiles of Y and Z
+  // ddecay's terms, by waves: W_ij that cross each row, r, c and gamma_31 <S, dS'>
+  __shared__ float s_pairs[PAIRS][kSegment], s_read[W][kSegment], s_write[W][kSegment], s_whole[W][kChunks];
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16, h = blockIdx.y, hk = h / (a.Hv / a.Hk);
   const bool shared = a.Hv != a.Hk;
   int seq, seg, b = 0;
@@ -457,6 +485,7 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
       }
   };
   load_state(a.states, S);
+  f32x4_t* passed = reinterpret_cast<f32x4_t*>(a.passed) + ((size_t(sp.segment + seg) * a.Hv + h) * 2 * W + wave) * MT * 64 + lane;
 
   // each half of the threads takes about half of the splitting
   const bool first = tid < 2 * P;
@@ -510,8 +539,12 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
       }
       __syncthreads();
 
+      if (a.ddecay && c > 0 && c + 1 < chunks)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) passed[((c - 1) * W * MT + m) * 64] = S[m];
       // Y and Z, a 16 x 16 tile a wave: (0, 0), (1, 0) and (1, 1) of both
       f32x4_t tile[TASKS];
+      float across[2] = {0.0f, 0.0f};   // W's sums for l = lane % 16 and 16 more
 #pragma unroll
       for (int n = 0; n < TASKS; ++n) {
         const int task = wave + n * W, z = task / 3, ti = task % 3 > 0, tj = task % 3 == 2;
@@ -531,12 +564,45 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
               tile[n] = product(w, u, tile[n]);
             }
           }
-          const float* D = a.decays + ((slot0 + c) * a.Hv + h) * (kChunk * kChunk) + 16 * tj + lane % 16;
+          const float* D = a.decays + ((slot0 + c) * a.Hv + h) * kDecays + 16 * tj + lane % 16;
+          if (a.ddecay) {
+            const float* M = D + (z ? 2 : 1) * kChunk * kChunk;
+            const int l = lane % 16;
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = (z ? -tile[n][i] : tile[n][i]) * M[(16 * ti + 4 * g + i) * kChunk];
+            if (ti == tj) {   // rows from l on, columns before l
+              float sum = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float before = sum_before(e[i]);
+                sum += 4 * g + i >= l ? before : 0.0f;
+              }
+              if (ti) across[1] += sum;
+              else across[0] += sum;
+            } else {   // all rows and columns before l; rows from l on and all columns
+              across[0] += sum_before((e[0] + e[1]) + (e[2] + e[3]));
+              float sum = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float row = sum16(e[i]);
+                sum += 4 * g + i >= l ? row : 0.0f;
+              }
+              across[1] += sum;
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = 16 * ti + 4 * g + i;
             tile[n][i] *= z ? (r == 16 * tj + lane % 16 ? 0.0f : D[r * kChunk]) : a.scale * D[r * kChunk];
           }
+        }
+      }
+      if (a.ddecay && wave < PAIRS) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          across[i] += __shfl_xor(across[i], 16), across[i] += __shfl_xor(across[i], 32);
+          if (g == i) s_pairs[wave][c * kChunk + lane] = across[i];
         }
       }
       f32x4_t ys[2] = {}, xs[2] = {};
@@ -600,6 +666,13 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
         Unit w[3];
 #pragma unroll
         for (int i = 0; i < 4; ++i) ys[t][i] *= a.scale * gm[4 * t + i], xs[t][i] *= gm[4 * t + i];
+        if (a.ddecay) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float read = sum16(fmaf(value_of(qb, 4 * t + i), ys[t][i], -value_of(kb, 4 * t + i) * xs[t][i]));
+            if (lane % 16 == 0) s_read[wave][c * kChunk + 16 * t + 4 * g + i] = read;
+          }
+        }
         f32x4_t yq = {}, zk = {};
         take(s_u + t * 64 + lane, 128, w);
         ys[t] = product(w, kb, ys[t]);
@@ -613,11 +686,13 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
         for (int i = 0; i < 4; ++i) dq[4 * t + i] = ys[t][i], rd[4 * t + i] = -xs[t][i], wr[4 * t + i] = yq[i] - zk[i];
       }
       const float all = gains[31];
+      if (c + 1 < chunks) {   // the state before the last chunk stays
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        Unit w[3];
-        take(s_x + m * 64 + lane, PLANE, w);
-        S[m] = product(w, kb, S[m] * all);
+        for (int m = 0; m < MT; ++m) {
+          Unit w[3];
+          take(s_x + m * 64 + lane, PLANE, w);
+          S[m] = product(w, kb, S[m] * all);
+        }
       }
       const size_t at_row = size_t(b) * a.T + row0 + c * kChunk;
       const Rows dkh(a.dk_heads + (at_row * a.Hv + h) * a.dk, a.Hv * a.dk, rows, a.dk);
@@ -629,9 +704,6 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
         store_element<float>(dkh, dkh.at<float, true>(r, col, a.dk), rd[i] + wr[i]);
         if (shared) store_element<float>(dqh, dqh.at<float, true>(r, col, a.dk), dq[i]);
         else store_element<T>(dqo, dqo.at<T, true>(r, col, a.dk), dq[i]);
-        const float kv = value_of(kb, i);
-        const float net = sum16(fmaf(value_of(qb, i), dq[i], kv * rd[i]) - kv * wr[i]);
-        if (lane % 16 == 0) s_net[wave][c * kChunk + r] = net;
       }
     }
   }
@@ -661,17 +733,22 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
       }
     };
     fetch(chunks - 1);
-    {
-      f32x4_t end[MT];
-      load_state(a.dstates, end);
-      float with = 0.0f;   // <S, dS>
+    const auto whole = [&](int c, const f32x4_t (&x)[MT], const f32x4_t (&y)[MT]) {   // gamma_31 <x, y>
+      float with = 0.0f;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) with = fmaf(S[m][i], end[m][i], with), S[m][i] = end[m][i];
+        for (int i = 0; i < 4; ++i) with = fmaf(x[m][i], y[m][i], with);
 #pragma unroll
       for (int o = 1; o < 64; o *= 2) with += __shfl_xor(with, o);
-      if (lane == 0) s_sum[wave] = with;
+      if (lane == 0) s_whole[wave][c] = s_gains[c][31] * with;
+    };
+    {
+      f32x4_t end[MT];
+      load_state(a.dstates, end);
+      if (a.ddecay) whole(chunks - 1, S, end);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) S[m] = end[m];
     }
     for (int c = chunks - 1; c >= 0; --c) {
       const int rows = rows_all - c * kChunk;
@@ -692,6 +769,16 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
       for (int i = 0; i < 8; ++i) before[i] = part[i];
       __syncthreads();
       if (c > 0) fetch(c - 1);
+      if (a.ddecay && c + 1 < chunks) {   // with the state before this chunk
+        f32x4_t start[MT];
+        if (c == 0) {
+          load_state(a.states, start);
+        } else {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) start[m] = passed[((c - 1) * W * MT + m) * 64];
+        }
+        whole(c, start, S);
+      }
       f32x4_t us[2] = {};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -736,35 +823,34 @@ __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(De
         const float w = dd[i] * us[i / 4][i % 4];
         if (shared) store_element<float>(dkh, dkh.at<float, true>(r, col, a.dk), before[i] + w);
         else store_element<T>(dko, dko.at<T, true>(r, col, a.dk), before[i] + w);
-        const float net = sum16(value_of(kb, i) * w);
-        if (lane % 16 == 0) s_net[wave][c * kChunk + r] -= net;
+        if (a.ddecay) {
+          const float write = sum16(value_of(kb, i) * w);
+          if (lane % 16 == 0) s_write[wave][c * kChunk + r] = write;
+        }
       }
     }
   }
   __syncthreads();
   if (a.ddecay && wave == 0) {
-    float v[2];   // rows 2 l and 2 l + 1: what they read less what they write, then summed from the end
+    float pairs[2], read[2], write[2], over = 0.0f;   // of rows 2 l and 2 l + 1, 16 lanes a chunk
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = 2 * lane + i;
-      v[i] = 0.0f;
-      if (r < rows_all)
+      pairs[i] = read[i] = write[i] = 0.0f;
+      if (r < rows_all) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) v[i] += s_net[w][r];
+        for (int w = 0; w < PAIRS; ++w) pairs[i] += s_pairs[w][r];
+#pragma unroll
+        for (int w = 0; w < W; ++w) read[i] += s_read[w][r], write[i] += s_write[w][r];
+      }
     }
-    float all = v[0] + v[1], rest = 0.0f;
+    if (lane / 16 < chunks)
 #pragma unroll
-    for (int w = 0; w < W; ++w) rest += s_sum[w];
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-      const float after = __shfl_down(all, o);
-      if (lane + o < 64) all += after;
-    }
-    float behind = __shfl_down(all, 1);
-    behind = lane == 63 ? rest : behind + rest;
+      for (int w = 0; w < W; ++w) over += s_whole[w][lane / 16];
+    const float behind = sum_behind(read[0] + read[1]) + over, before = sum_before(write[0] + write[1]);
     float* out = a.ddecay + (size_t(b) * a.T + row0) * a.Hv + h;
-    if (2 * lane + 1 < rows_all) out[size_t(2 * lane + 1) * a.Hv] = behind + v[1];
-    if (2 * lane < rows_all) out[size_t(2 * lane) * a.Hv] = behind + v[1] + v[0];
+    if (2 * lane < rows_all) out[size_t(2 * lane) * a.Hv] = pairs[0] + (behind + read[0] + read[1]) + before;
+    if (2 * lane + 1 < rows_all) out[size_t(2 * lane + 1) * a.Hv] = pairs[1] + (behind + read[1]) + (before + write[0]);
   }
 }
 
@@ -834,8 +920,9 @@ size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 
 size_t delta_rule_bwd_workspace(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, bool packed) {
   const size_t heads = size_t(delta_rule_slots(B, T, nseq, packed)) * Hv, rows = size_t(B) * T * Hv;
-  return heads * (kUnits * sizeof(uint4) + (96 + kChunk * kChunk) * sizeof(float)) + 256 * sizeof(float) +
-         up16(rows * dv * sizeof(float)) + up16(size_t(delta_rule_segments(B, T, nseq, packed)) * Hv * dk * dv * sizeof(float)) +
+  const size_t segments = size_t(delta_rule_segments(B, T, nseq, packed)) * Hv, wide = dk <= 64 && dv <= 64 ? 64 : 128;
+  return heads * (kUnits * sizeof(uint4) + (96 + kDecays) * sizeof(float)) + 256 * sizeof(float) +
+         up16(rows * dv * sizeof(float)) + up16(segments * dk * dv * sizeof(float)) + segments * 2 * wide * wide * sizeof(float) +
          up16(rows * dk * sizeof(float)) * (Hv != Hk ? 2 : 1);
 }
 
@@ -850,9 +937,11 @@ hipError_t launch_delta_rule_bwd(DeltaRule a, int dtype, void* workspace, hipStr
   };
   a.units = reinterpret_cast<uint4*>(room(heads * kUnits * sizeof(uint4)));
   a.gains = reinterpret_cast<float*>(room((heads * 96 + 256) * sizeof(float)));   // 160 more behind the last are read
-  a.decays = reinterpret_cast<float*>(room(heads * kChunk * kChunk * sizeof(float)));
+  a.decays = reinterpret_cast<float*>(room(heads * kDecays * sizeof(float)));
   a.duals = reinterpret_cast<float*>(room(rows * a.dv * sizeof(float)));
-  a.dstates = reinterpret_cast<float*>(room(size_t(delta_rule_segments(a.B, a.T, a.nseq, packed)) * a.Hv * a.dk * a.dv * sizeof(float)));
+  const size_t segments = size_t(delta_rule_segments(a.B, a.T, a.nseq, packed)) * a.Hv, wide = a.dk <= 64 && a.dv <= 64 ? 64 : 128;
+  a.dstates = reinterpret_cast<float*>(room(segments * a.dk * a.dv * sizeof(float)));
+  a.passed = reinterpret_cast<float*>(room(segments * 2 * wide * wide * sizeof(float)));
   a.dk_heads = reinterpret_cast<float*>(room(rows * a.dk * sizeof(float)));
   a.dq_heads = a.Hv != a.Hk ? reinterpret_cast<float*>(room(rows * a.dk * sizeof(float))) : nullptr;
   if (dtype == 0) run<float>(a, s);

@@ -401,9 +401,10 @@ struct DeltaRule {
   void *dq, *dkey, *dv_out;   // (B, T, heads, width) of the inputs' type
   float *dbeta, *ddecay;   // (B, T, Hv); ddecay null without decay
   float* dh0;              // (n, Hv, dk, dv) or null
-  float* decays;           // workspace: (slots, Hv, 32, 32) D
+  float* decays;           // workspace: (slots, Hv, 3, 32, 32) D, P and A
   float* duals;            // workspace: (B, T, Hv, dv) X
   float* dstates;          // workspace: (segments, Hv, dk, dv) the state's gradient behind each segment
+  float* passed;           // workspace: (segments, Hv, 2, P, P) the state before a segment's second and third chunk, P = 64 or 128
   float *dq_heads, *dk_heads;   // workspace: (B, T, Hv, dk) each value head's share (dq_heads only where heads are shared)
 };
 long long delta_rule_slots(int B, int T, int nseq, bool packed);     // chunks that the workspace has room for

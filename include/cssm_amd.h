@@ -1031,7 +1031,7 @@ int cssm_delta_rule(const cssm_token_rows* q, const cssm_token_rows* k, const cs
  *   dbeta, ddecay  (B, T, Hv) float32 out, ddecay NULL without decay; all zero behind the last sequence
  *   dh0          (n, Hv, dk, dv) float32 out, or NULL
  *   workspace    cssm_delta_rule_bwd_workspace_size bytes, 16-byte aligned
- * decay's gradient is what a change of it does; where decay is -inf that is none, up to rounding.
+ * decay's gradient is what a change of it does, summed without cancellation; where decay is -inf that is 0.
  */
 size_t cssm_delta_rule_bwd_workspace_size(int B, int T, int Hk, int Hv, int dk, int dv, int nseq, int packed);
 int cssm_delta_rule_bwd(const cssm_token_rows* q, const cssm_token_rows* k, int dtype, const cssm_token_rows* beta,
