@@ -1467,6 +1467,7 @@ int delta_rule_args(const char* who, DeltaRule& a, const cssm_token_rows* q, con
       if (has(r) && r->row_stride > 1 << 24) return fail(CSSM_ERR_UNSUPPORTED, "%s: row_stride=%lld", who, r->row_stride);
   if ((long long)Hv * dv > 1 << 24) return fail(CSSM_ERR_UNSUPPORTED, "%s: Hv=%d dv=%d", who, Hv, dv);
   a.q = rows_of(q), a.k = rows_of(k), a.v = rows_of(v), a.beta = rows_of(beta), a.decay = rows_of(decay);
+  if (T <= 1) a.q.row = a.k.row = (long long)Hk * dk, a.v.row = (long long)Hv * dv;   // of one row, not used; the kernels' offsets have 32 bits
   a.B = B, a.T = T, a.Hk = Hk, a.Hv = Hv, a.dk = dk, a.dv = dv, a.scale = scale, a.offsets = offsets, a.nseq = nseq;
   return token_align_check(who, dtype, {a.q.p, a.k.p, a.v.p}, {a.beta.p, a.decay.p, offsets});
 }
