@@ -191,14 +191,15 @@ __global__ __launch_bounds__(256) void rotate_heads(Rotary a, int lanes, int sli
       }
     } else {
       float ga[NV][V], gb[NV][V], dot = 0.0f;
+      const float rw = on ? rs : 0.0f;   // without a head and eps r has no value
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         unpack<T, V>(qa[n], ga[n]), unpack<T, V>(qb[n], gb[n]);
         pairs.template turn<true>(ga[n], gb[n], n);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          dw[i][n][0][v] = fmaf(ga[n][v], fa[n][v] * rs, dw[i][n][0][v]);
-          dw[i][n][1][v] = fmaf(gb[n][v], fb[n][v] * rs, dw[i][n][1][v]);
+          dw[i][n][0][v] = fmaf(ga[n][v], fa[n][v] * rw, dw[i][n][0][v]);
+          dw[i][n][1][v] = fmaf(gb[n][v], fb[n][v] * rw, dw[i][n][1][v]);
           ga[n][v] *= w[i][n][0][v], gb[n][v] *= w[i][n][1][v];
           dot = fmaf(ga[n][v], fa[n][v], dot), dot = fmaf(gb[n][v], fb[n][v], dot);
         }
