@@ -298,22 +298,21 @@ __device__ __forceinline__ void last_state(const DeltaRule& a, const Column& c, 
 
 constexpr int kWalkColumns = 64;   // of a workgroup: 16 for each of its four waves
 
-template <int DKP, typename T>
+template <int DKP>
 struct WalkLds {
-  static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
-  uint4 k[kN * kPlane], q[kN * kPlane], kt[kN * kPlane], lp[(kUnits + 255) / 256 * 256];
+  uint4 k[3 * DKP * 4], q[3 * DKP * 4], kt[3 * DKP * 4], lp[kUnits];
   float gains[256];   // gamma, d, beta; the rest takes what threads without a value write
 };
 
-// One workgroup carries 64 columns of one sequence's and head's state through the chunks (float32: in LDS there is no room
-// for the second kind of waves below).  While a chunk is computed from LDS, the next one's rows are on their way into
-// registers.  3 x 197 x 3 heads of 40 and 50: 25 us, 3.5 a chunk.
-template <int DKP, typename T, bool WIDE, bool KEEP, bool MAP>
+// float32: one workgroup carries 64 columns of one sequence's and head's state through the chunks, one kind of wave for all of
+// it.  While a chunk is computed from LDS, the next one's rows are on their way into registers; they take its place between
+// two barriers (two buffers would fit 64 wide, 100 KB, and save one of them; 128 wide, 87 KB each, they do not).
+// 3 x 197 x 3 heads of 40 and 50: 25 us, 3.5 a chunk.
+template <int DKP, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
-  using Lds = WalkLds<DKP, T>;
-  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16;
-  constexpr int LP = (kUnits + 255) / 256;
-  __shared__ Lds lds[Lds::kBufs];
+  using T = float;
+  constexpr int N = 3, PLANE = DKP * 4, KS = DKP / 32, MT = DKP / 16, LP = kUnits / 256;
+  __shared__ WalkLds<DKP> lds;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
   const int part = blockIdx.x / a.Hv, h = blockIdx.x - part * a.Hv, hk = h / (a.Hv / a.Hk);
   Part sp;
@@ -345,7 +344,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
     const Rows k(row_at<T>(a.k, b, t) + hk * a.dk, a.k.row, rows, a.dk), q(row_at<T>(a.q, b, t) + hk * a.dk, a.q.row, rows, a.dk);
     const Rows vv(row_at<T>(a.v, b, t) + h * a.dv, a.v.row, MAP && column.unit ? 0 : rows, a.dv);
     const size_t head = size_t(sp.slot + c) * a.Hv + h;
-    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits + tid;   // the last ones past this chunk's: into the next, or the end's room
+    const u32x4_t* units = reinterpret_cast<const u32x4_t*>(a.units) + head * kUnits + tid;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = load_element<T>(vv, vv.at<T, WIDE>(unit_row(4 * g, i), col, a.dv));
     if (p_on) pk.load(k, p_tok, p_col, a.dk);
@@ -353,24 +352,23 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
     if (c_on) ck.load(k, 4 * c_g, c_col, a.dk);
 #pragma unroll
     for (int i = 0; i < LP; ++i) lp[i] = units[256 * i];
-    gain = a.gains[head * 96 + tid];
+    gain = a.gains[head * 96 + tid];   // past the 96: the next ones, or the room behind the last
   };
-  const auto stash = [&](Lds& to) {
-    if (p_on) pk.store(to.k + p_unit, PLANE);
-    if (p_on && !MAP) pq.store(to.q + p_unit, PLANE);
-    if (c_on) ck.store(to.kt + c_unit, PLANE);
+  const auto stash = [&] {
+    if (p_on) pk.store(lds.k + p_unit, PLANE);
+    if (p_on && !MAP) pq.store(lds.q + p_unit, PLANE);
+    if (c_on) ck.store(lds.kt + c_unit, PLANE);
 #pragma unroll
-    for (int i = 0; i < LP; ++i) to.lp[tid + 256 * i] = __builtin_bit_cast(uint4, lp[i]);
-    to.gains[tid] = gain;
+    for (int i = 0; i < LP; ++i) lds.lp[tid + 256 * i] = __builtin_bit_cast(uint4, lp[i]);
+    lds.gains[tid] = gain;
   };
 
   if (chunks) {
     fetch(0);
-    stash(lds[0]);
+    stash();
   }
   for (int c = 0; c < chunks; ++c) {
     __syncthreads();
-    const Lds& in = lds[c % Lds::kBufs];
     float V[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) V[i] = element<T>(v[i]);
@@ -394,19 +392,19 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Unit w[N];
-        take(in.k + (s * 2 + t) * 64 + lane, PLANE, w);
+        take(lds.k + (s * 2 + t) * 64 + lane, PLANE, w);
         ks[t] = product(w, u, ks[t]);
         if constexpr (MAP) continue;
-        take(in.q + (s * 2 + t) * 64 + lane, PLANE, w);
+        take(lds.q + (s * 2 + t) * 64 + lane, PLANE, w);
         qs[t] = product(w, u, qs[t]);
       }
     }
     float R[8], E[8], x[8], gm[8], dd[8], bt[8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const float4 g4 = *reinterpret_cast<const float4*>(&in.gains[16 * t + 4 * g]);
-      const float4 d4 = *reinterpret_cast<const float4*>(&in.gains[32 + 16 * t + 4 * g]);
-      const float4 b4 = *reinterpret_cast<const float4*>(&in.gains[64 + 16 * t + 4 * g]);
+      const float4 g4 = *reinterpret_cast<const float4*>(&lds.gains[16 * t + 4 * g]);
+      const float4 d4 = *reinterpret_cast<const float4*>(&lds.gains[32 + 16 * t + 4 * g]);
+      const float4 b4 = *reinterpret_cast<const float4*>(&lds.gains[64 + 16 * t + 4 * g]);
       gm[4 * t] = g4.x, gm[4 * t + 1] = g4.y, gm[4 * t + 2] = g4.z, gm[4 * t + 3] = g4.w;
       dd[4 * t] = d4.x, dd[4 * t + 1] = d4.y, dd[4 * t + 2] = d4.z, dd[4 * t + 3] = d4.w;
       bt[4 * t] = b4.x, bt[4 * t + 1] = b4.y, bt[4 * t + 2] = b4.z, bt[4 * t + 3] = b4.w;
@@ -423,7 +421,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Unit w[3];
-        take(in.lp + t * 64 + lane, 128, w);
+        take(lds.lp + t * 64 + lane, 128, w);
         const f32x4_t le = product(w, u, f32x4_t{});
 #pragma unroll
         for (int i = 0; i < 4; ++i) E[4 * t + i] = R[4 * t + i] - le[i];
@@ -439,7 +437,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Unit w[3];
-        take(in.lp + 3 * 128 + t * 64 + lane, 128, w);
+        take(lds.lp + 3 * 128 + t * 64 + lane, 128, w);
         qs[t] = product(w, u, qs[t]);
       }
       const long long t0 = sp.row + (long long)c * kChunk;
@@ -459,17 +457,17 @@ __global__ __launch_bounds__(256, 1) void delta_walk(DeltaRule a) {
       for (int i = 0; i < 8; ++i) x[i] *= dd[i];
       Unit u[3];
       split<3>(x, u);
-      const float all = in.gains[31];
+      const float all = lds.gains[31];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         Unit w[N];
-        take(in.kt + m * 64 + lane, PLANE, w);
+        take(lds.kt + m * 64 + lane, PLANE, w);
         S[m] = product(w, u, S[m] * all);
       }
     }
     if (c + 1 < chunks) {
-      if (Lds::kBufs == 1) __syncthreads();
-      stash(lds[(c + 1) % Lds::kBufs]);
+      __syncthreads();
+      stash();
     }
   }
   last_state<DKP>(a, column, g, S);
@@ -863,7 +861,7 @@ template <int DKP, typename T, bool WIDE, bool KEEP, bool MAP>
 void walk(const DeltaRule& a, int blocks, int columns, hipStream_t s) {
   const dim3 grid(blocks, columns);
   if constexpr (sizeof(T) == 2) delta_walk_pairs<DKP, WIDE, KEEP, MAP><<<grid, 512, 0, s>>>(a);
-  else delta_walk<DKP, T, WIDE, KEEP, MAP><<<grid, 256, 0, s>>>(a);
+  else delta_walk<DKP, WIDE, KEEP, MAP><<<grid, 256, 0, s>>>(a);
 }
 
 template <int DKP, typename T, bool WIDE>
@@ -927,7 +925,7 @@ size_t delta_rule_workspace(int B, int T, int Hv, int dk, int dv, int nseq, bool
   const int fold = delta_rule_fold(B, T, Hv, dk, dv, nseq, packed), wide = dk <= 64 ? 64 : 128;
   const size_t parts = fold ? size_t(delta_rule_parts(fold, B, T, nseq, packed)) * Hv : 0;
   return size_t(delta_rule_slots(B, T, nseq, packed)) * Hv * (kUnits * sizeof(uint4) + 96 * sizeof(float)) +
-         256 * sizeof(uint4) + parts * (size_t(wide) * wide + size_t(dk) * dv) * sizeof(float);
+         256 * sizeof(float) + parts * (size_t(wide) * wide + size_t(dk) * dv) * sizeof(float);
 }
 
 hipError_t launch_delta_rule(DeltaRule a, int dtype, void* workspace, hipStream_t s) {

@@ -32,18 +32,18 @@ namespace {
 constexpr int kBackColumns = 64;   // of a workgroup: 16 for each of its four waves
 constexpr int kChunks = kSegment / kChunk;
 
-template <int DKP, typename T>
+template <int DKP>
 struct BackLds {
-  static constexpr int kN = PartsOf<T>::n, kPlane = DKP * 4, kBufs = sizeof(T) == 2 ? 2 : 1;
-  uint4 k[kN * kPlane], kt[kN * kPlane], qt[kN * kPlane], lp[kUnits];
+  uint4 k[3 * DKP * 4], kt[3 * DKP * 4], qt[3 * DKP * 4], lp[kUnits];
   float gains[256];
 };
 
-template <int DKP, typename T, bool WIDE>
+// float32: one kind of wave for all of it, as the forward's
+template <int DKP, bool WIDE>
 __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
-  using Lds = BackLds<DKP, T>;
-  constexpr int N = Lds::kN, PLANE = Lds::kPlane, KS = DKP / 32, MT = DKP / 16, LP = kUnits / 256;
-  __shared__ Lds lds[Lds::kBufs];
+  using T = float;
+  constexpr int N = 3, PLANE = DKP * 4, KS = DKP / 32, MT = DKP / 16, LP = kUnits / 256;
+  __shared__ BackLds<DKP> lds;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, g = lane / 16;
   const int x = blockIdx.x / a.Hv, h = blockIdx.x - x * a.Hv, hk = h / (a.Hv / a.Hk);
   const int seq = __builtin_amdgcn_readfirstlane(longest_first(a, x));
@@ -91,21 +91,20 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
     for (int i = 0; i < LP; ++i) lp[i] = units[256 * i];
     gain = a.gains[head * 96 + tid];   // past the 96: the next ones, or the room behind the last
   };
-  const auto stash = [&](Lds& to) {
-    if (p_on) pk.store(to.k + p_unit, PLANE);
-    if (c_on) ck.store(to.kt + c_unit, PLANE), cq.store(to.qt + c_unit, PLANE);
+  const auto stash = [&] {
+    if (p_on) pk.store(lds.k + p_unit, PLANE);
+    if (c_on) ck.store(lds.kt + c_unit, PLANE), cq.store(lds.qt + c_unit, PLANE);
 #pragma unroll
-    for (int i = 0; i < LP; ++i) to.lp[tid + 256 * i] = __builtin_bit_cast(uint4, lp[i]);
-    to.gains[tid] = gain;
+    for (int i = 0; i < LP; ++i) lds.lp[tid + 256 * i] = __builtin_bit_cast(uint4, lp[i]);
+    lds.gains[tid] = gain;
   };
 
   if (chunks) {
     fetch(chunks - 1);
-    stash(lds[(chunks - 1) % Lds::kBufs]);
+    stash();
   }
   for (int c = chunks - 1; c >= 0; --c) {
     __syncthreads();
-    const Lds& in = lds[c % Lds::kBufs];
     float dY[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) dY[i] = element<T>(dy[i]);
@@ -129,19 +128,19 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Unit w[N];
-        take(in.k + (s * 2 + t) * 64 + lane, PLANE, w);
+        take(lds.k + (s * 2 + t) * 64 + lane, PLANE, w);
         ks[t] = product(w, u, ks[t]);
       }
     }
     float gm[8], dd[8], bt[8], x[8], dU[8], X[8];
-    take_rows(in.gains, g, gm), take_rows(in.gains + 32, g, dd), take_rows(in.gains + 64, g, bt);
+    take_rows(lds.gains, g, gm), take_rows(lds.gains + 32, g, dd), take_rows(lds.gains + 64, g, bt);
     {
       Unit u[N];
       split<N>(dY, u);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Unit w[3];
-        take(in.lp + 3 * 128 + t * 64 + lane, 128, w);
+        take(lds.lp + 3 * 128 + t * 64 + lane, 128, w);
         const f32x4_t py = product(w, u, f32x4_t{});
 #pragma unroll
         for (int i = 0; i < 4; ++i) dU[4 * t + i] = py[i] + dd[4 * t + i] * ks[t][i], x[4 * t + i] = bt[4 * t + i] * dU[4 * t + i];
@@ -153,7 +152,7 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         Unit w[3];
-        take(in.lp + t * 64 + lane, 128, w);
+        take(lds.lp + t * 64 + lane, 128, w);
         const f32x4_t le = product(w, u, f32x4_t{});
 #pragma unroll
         for (int i = 0; i < 4; ++i) X[4 * t + i] = dU[4 * t + i] - le[i];
@@ -175,20 +174,20 @@ __global__ __launch_bounds__(256, 1) void delta_walk_back(DeltaRule a) {
       for (int i = 0; i < 8; ++i) x[i] = a.scale * gm[i] * dY[i], z[i] = -gm[i] * bt[i] * X[i];
       Unit u[3], v[3];
       split<3>(x, u), split<3>(z, v);
-      const float all = in.gains[31];
+      const float all = lds.gains[31];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         Unit w[N];
         S[m] *= all;
-        take(in.qt + m * 64 + lane, PLANE, w);
+        take(lds.qt + m * 64 + lane, PLANE, w);
         S[m] = product(w, u, S[m]);
-        take(in.kt + m * 64 + lane, PLANE, w);
+        take(lds.kt + m * 64 + lane, PLANE, w);
         S[m] = product(w, v, S[m]);
       }
     }
     if (c > 0) {
-      if (Lds::kBufs == 1) __syncthreads();
-      stash(lds[(c - 1) % Lds::kBufs]);
+      __syncthreads();
+      stash();
     }
   }
   if (a.dh0 && mine)
@@ -893,8 +892,8 @@ void run_as(const DeltaRule& a, hipStream_t s) {
     if (a.dk <= 64) delta_back_pairs<64, WIDE><<<grid, 512, 0, s>>>(a);
     else delta_back_pairs<128, WIDE><<<grid, 512, 0, s>>>(a);
   } else {
-    if (a.dk <= 64) delta_walk_back<64, T, WIDE><<<grid, 256, 0, s>>>(a);
-    else delta_walk_back<128, T, WIDE><<<grid, 256, 0, s>>>(a);
+    if (a.dk <= 64) delta_walk_back<64, WIDE><<<grid, 256, 0, s>>>(a);
+    else delta_walk_back<128, WIDE><<<grid, 256, 0, s>>>(a);
   }
   if (!a.T) return;
   if (a.dk <= 64 && a.dv <= 64) delta_grads<64, T, WIDE><<<dim3(segments, a.Hv), 256, 0, s>>>(a);

@@ -18,7 +18,7 @@ namespace cssm {
 
 namespace {
 
-constexpr int kAxes = 4, kRotaryGroups = 1024;   // workgroups of the adjoint, at most
+constexpr int kAxes = 4, kRotaryGroups = 1024;   // workgroups of a launch, at most
 
 __device__ __forceinline__ const char* head_row(const TokenRows& x, long long m, int T, size_t size) {
   const int b = int(m) / T, t = int(m) - b * T;   // M is at most 2^31 - 1
@@ -300,7 +300,7 @@ void launch(const Rotary& a, int lanes, hipStream_t s) {
   int slices = (most + heads - 1) / heads;
   while (slices > 1 && a.M * slices > 4096) slices = (slices + 1) / 2;
   const long long units = a.M * slices, groups = (units + 3) / 4;   // at most 2^31 - 1, or 4096
-  const int grid = int(BACK ? (groups < kRotaryGroups ? groups : kRotaryGroups) : groups < kRotaryGroups ? groups : kRotaryGroups);
+  const int grid = int(groups < kRotaryGroups ? groups : kRotaryGroups);
   const size_t lds = BACK && a.parts ? size_t(8) * a.D * sizeof(float) : 0;
   if (a.halves) rotate_heads<T, V, NV, true, BACK><<<grid, 256, lds, s>>>(a, lanes, slices, uint32_t(units));
   else rotate_heads<T, V, NV, false, BACK><<<grid, 256, lds, s>>>(a, lanes, slices, uint32_t(units));
