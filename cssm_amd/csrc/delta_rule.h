@@ -273,7 +273,7 @@ __device__ __forceinline__ Span span_of(const DeltaRule& a, int i) {
 
 // The x-th longest of up to 64 packed sequences (the first of equals first), x itself of more or of a batch: workgroups begin in
 // order, and the longest sequence, begun last, would be walked by a chip that has nothing else left (23 sequences in 16001
-// rows x 16 heads, twelve draws: 256 us in their order, 232 so).  All lanes take part.
+// rows x 16 heads, twelve draws: 266 us in their order, 241 so).  All lanes take part.
 __device__ __forceinline__ int longest_first(const DeltaRule& a, int x) {
   if (!a.offsets || a.nseq > 64) return x;
   const int lane = threadIdx.x % 64, mine = lane < a.nseq ? span_of(a, lane).rows : -1;

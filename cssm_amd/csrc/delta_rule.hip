@@ -486,9 +486,9 @@ struct PairLds {
 
 // The same for bfloat16 by two kinds of waves, a pair for 16 columns on each SIMD: the first carries the state and takes Q S from
 // its parts while it has them, the second brings the chunks' rows to LDS and makes y of the chunk before, from Q S and U that the
-// first leaves in LDS.  One kind of wave for all of it took 3.4 us a chunk on a full chip; Q S by the second wave, which
-// splits the state once more, 3.1 (8 x 2048 rows: 243 us a call, 200 so).  What bounds it: the instructions that the first wave
-// issues a step, 80 products and those that split and combine, one behind the other.
+// first leaves in LDS: 2.4 us a chunk on a full chip (8 x 2048 x 16 heads of 128: 154 us) and 1.9 with few workgroups.  One kind
+// of wave for all of it took 3.4 and 2.6; Q S by the second wave, which splits the state once more, 3.1.  What bounds it: the 600
+// instructions that the first wave issues a step, 84 products and those that split and combine, one behind the other.
 template <int DKP, bool WIDE, bool KEEP, bool MAP>
 __global__ __launch_bounds__(512, 1) void delta_walk_pairs(DeltaRule a) {
   using T = Bf16;
@@ -837,9 +837,11 @@ long long delta_rule_parts(int fold, int B, int T, int nseq, bool packed) {
   return packed ? T / fold + (long long)nseq : (long long)B * (T / fold + (T % fold != 0));
 }
 
-// Rows of the parts that sequences are walked in, or 0.  1 x 65536 x 8 heads: whole 3760 us, in 16 parts 430 + 105 + 300.  Few heads of long sequences leave most CUs without work: P parts are
+// Rows of the parts that sequences are walked in, or 0.  Few heads of long sequences leave most CUs without work: P parts are
 // walked once for what they do to the state (0.75 of a walk's time, for their values' and their keys' columns) and once with
 // the state before them, with a product for each between (128 rows' time); a CU walks one workgroup's 64 columns at a time.
+// More than 128 workgroups: two parts of each would not run at once any more.
+// 1 x 65536 x 8 heads: whole 3810 us, in 16 parts of 4224 rows 435 + 107 + 310.
 int delta_rule_fold(int B, int T, int Hv, int dk, int dv, int nseq, bool packed) {
   const long long n = packed ? nseq : B, blocks = (dv + kWalkColumns - 1) / kWalkColumns, units = dk <= 64 ? 1 : 2;
   if (n < 1 || n * Hv * blocks > 128) return 0;

@@ -412,10 +412,6 @@ __device__ __forceinline__ float sum16(float x) {
   return x + rotated<1>(x);
 }
 
-// P: dk and dv up to it.  One workgroup for 128 rows of one value head, P / 16 waves.  Y, Z and their transposes take the place
-// of U's rows in LDS once those are read, and the columns of d U that of X's rows.
-// 64 wide two workgroups share a CU, in 256 registers a thread (training 4 x 4096 x 16 heads of 64: bfloat16 383 -> 233 us,
-// float32 446 -> 379); 128 wide that leaves 128 registers, which spill (1280 us in place of 575).
 // the value `BY` lanes before or behind within 16, 0 beyond them
 template <int BY>
 __device__ __forceinline__ float lane_before(float x) {
@@ -437,6 +433,11 @@ __device__ __forceinline__ float sum_behind(float x) {
   return x + lane_behind<8>(x);
 }
 
+// P: dk and dv up to it.  One workgroup for 128 rows of one value head, P / 16 waves.  Y, Z and their transposes take the place
+// of U's rows in LDS once those are read, and the columns of d U that of X's rows.
+// 64 wide two workgroups share a CU, in 256 registers a thread (training 4 x 4096 x 16 heads of 64: bfloat16 452 -> 281 us,
+// float32 519 -> 444); 128 wide that leaves 128 registers, which spill (1280 us in place of 575, without ddecay's terms).  As it
+// is it spills too: bfloat16 10 and 17 registers (64 and 128 wide), float32 53 and 63, 128 wide off the vector width 144 and 172.
 template <int P, typename T, bool WIDE>
 __global__ __launch_bounds__(4 * P, P == 64 && WIDE ? 2 : 1) void delta_grads(DeltaRule a) {
   constexpr int N = PartsOf<T>::n, W = P / 16, KS = P / 32, MT = P / 16, PLANE = P * 4, TASKS = (6 + W - 1) / W;

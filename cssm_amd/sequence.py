@@ -554,7 +554,8 @@ def delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Te
     side (slices of one projection's output will do); Hv / Hk value heads next to each other share a query and key head.
     ``beta``, ``decay`` (B, T, Hv) float32, decay <= 0 (None: 0, no decay; -inf clears the state).  The rule is stable for
     keys of at most unit length and 0 <= beta <= 2; nothing checks that.  A row with beta = 0 and decay = 0 leaves the state:
-    that masks it, its values being finite.  ``state`` (B, Hv, dk, dv) float32 before the first
+    that masks it, its values and the products of its key and query with others being finite (zeros, not the type's lowest
+    value).  ``state`` (B, Hv, dk, dv) float32 before the first
     row (None: zeros); ``scale`` dk^-0.5 unless given.  ``offsets`` and ``out`` as in :func:`token_scan`: packed rows
     (T, H, width), states (n, Hv, dk, dv).  Rows are taken 32 at a time, and a value that is not finite spoils its sequence
     from the 32 rows on in which it stands.  Not differentiable: see :func:`cssm_amd.training.delta_rule_train`.

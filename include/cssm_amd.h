@@ -1011,8 +1011,8 @@ int cssm_scaled_matmul(const void* a, const void* a_scales, const void* w, const
  *   workspace    cssm_delta_rule_workspace_size bytes, 16-byte aligned
  * dk and dv to 128, rows of q, k and v at most 2^24 elements apart (with T = 1 row_stride is not used), fewer than 2^23 chunks of 32 rows times Hv and 2^20
  * sequences times Hv (CSSM_ERR_UNSUPPORTED otherwise).  The outputs do not overlap the inputs.  Sums and states are float32.
- * Rows are taken 32 at a time: a value that is not finite, in a masked row too, spoils its sequence from the 32 rows on in
- * which it stands.
+ * Rows are taken 32 at a time: a value, or a product of two rows, that is not finite, in a masked row too, spoils its sequence
+ * from the 32 rows on in which it stands.
  * The same call gives the same bits.
  */
 #define CSSM_DELTA_SEGMENT 128
